@@ -1,4 +1,4 @@
-"""ctypes binding of libhq.so, the gfx950 quantized matmul path (C ABI: include/hq.h, hq_llama.h).
+"""ctypes binding of libhq.so, the gfx950 quantized matmul path and the serving operators (C ABI: include/*.h).
 
 Python is plumbing here: it moves numpy arrays in and out of device buffers and calls the C ABI.
 There is no fallback: if libhq.so is not built, or a call fails, an exception is raised.
@@ -16,7 +16,7 @@ DT_GGML = 3
 BLOCK_VALUES = {Q8_0: 32, Q2_K: 256, Q3_K: 256, Q4_K: 256, Q5_K: 256, Q6_K: 256}
 BLOCK_BYTES = {Q8_0: 34, Q2_K: 84, Q3_K: 110, Q4_K: 144, Q5_K: 176, Q6_K: 210}
 
-# Every function declared in include/hq.h and include/hq_llama.h.
+# Every function declared in the headers but include/hq_backend.h.
 EXPORTS = (
     "hq_last_error", "hq_device_init", "hq_device_count", "hq_device_name", "hq_mat_upload", "hq_mat_free",
     "hq_mat_shape", "hq_mat_device_bytes", "hq_mat_download", "hq_dequant_f32", "hq_gemm", "hq_gemv",
@@ -26,6 +26,8 @@ EXPORTS = (
     "hq_embed_f32", "hq_gemm_kernel", "hq_gemm_noalloc", "hq_gemm_workspace_bytes", "hq_gemv_swiglu",
     "hq_gguf_open", "hq_gguf_close", "hq_gguf_n_tensors", "hq_gguf_tensor_info", "hq_gguf_find", "hq_gguf_get_uint",
     "hq_gguf_wmat", "hq_mat_upload_pair", "hq_gemm_swiglu", "hq_time_gemm_swiglu", "hq_time_read",
+    # include/hq_serve.h
+    "hq_batch_create", "hq_batch_free", "hq_batch_set", "hq_rope_table", "hq_rope_append", "hq_attention", "hq_logprobs",
 )
 # include/hq_backend.h (no hq_ prefix: the names of the reference entry points they replace)
 BACKEND_EXPORTS = ("hip_backend_create", "hip_selftest")
@@ -90,6 +92,30 @@ RefBackend._fields_ = [
     ("last_hidden", C.CFUNCTYPE(C.c_int, _BP, C.c_void_p))]
 
 
+KV_F16, KV_Q8 = 0, 1  # hq_kv_t types
+
+
+class Kv(C.Structure):
+    """hq_kv_t: one layer's paged cache."""
+    _fields_ = [("type", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("n_pages", C.c_uint32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("page_stride", C.c_int64), ("pos_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Rope(C.Structure):
+    """hq_rope_t."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("f32", C.c_int), ("q_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("kv_stride", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("norm_offset", C.c_float), ("eps", C.c_float), ("table", C.c_void_p), ("n_table", C.c_int), ("rot_dim", C.c_int),
+                ("positions", C.c_void_p), ("axis", C.c_void_p), ("n_axes", C.c_int), ("q_out", C.c_void_p)]
+
+
+class Attn(C.Structure):
+    """hq_attn_t."""
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("scale", C.c_float), ("gate", C.c_void_p), ("gate_f32", C.c_int),
+                ("gate_stride", C.c_int64), ("gate_head_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
 class HQError(RuntimeError):
     pass
 
@@ -145,6 +171,13 @@ def load(path=LIB_PATH):
         "hq_mat_upload_pair": (i, [C.POINTER(WMat), C.POINTER(WMat), i, C.POINTER(vp)]),
         "hq_gemm_swiglu": (i, [vp, vp, i, vp, vp]),
         "hq_time_gemm_swiglu": (i, [C.POINTER(vp), i, vp, i, vp, i, i, vp, C.POINTER(C.c_float)]),
+        "hq_batch_create": (i, [i, i, i, i, C.POINTER(vp)]),
+        "hq_batch_free": (None, [vp]),
+        "hq_batch_set": (i, [vp, C.POINTER(Kv), i, i, vp, vp, vp, i, vp]),
+        "hq_rope_table": (i, [vp, i, i, vp, vp]),
+        "hq_rope_append": (i, [vp, C.POINTER(Kv), C.POINTER(Rope), vp]),
+        "hq_attention": (i, [vp, C.POINTER(Kv), C.POINTER(Attn), vp]),
+        "hq_logprobs": (i, [vp, i, i, u32, C.c_int64, vp, i, i, vp, vp, vp, vp, vp]),
         "hq_gguf_open": (i, [C.c_char_p, C.POINTER(vp)]),
         "hq_gguf_close": (None, [vp]),
         "hq_gguf_n_tensors": (sz, [vp]),
@@ -463,6 +496,84 @@ def time_gather(mats, H, ids_dev, n_sets, B, k, out, iters, reps, stream):
     _check(_lib.hq_time_gather(arr, len(mats), H.ptr, ids_dev.ptr, n_sets, B, k, out.ptr, iters, reps, stream.ptr,
                                C.byref(ms)))
     return ms.value
+
+
+def _dev(p):
+    return p.ptr if isinstance(p, DevBuf) else p
+
+
+class KvCache:
+    """A layer's paged cache (hq_kv_t) over device memory: k, v and the scales are DevBuf or raw pointers; strides: elements
+    between pages, positions and heads."""
+
+    def __init__(self, type, n_pages, page_size, n_kv_heads, head_dim, k, v, strides, k_scale=None, v_scale=None):
+        self.keep = (k, v, k_scale, v_scale)
+        self.s = Kv(type, page_size, n_kv_heads, head_dim, n_pages, _dev(k), _dev(v), _dev(k_scale), _dev(v_scale), *strides)
+
+
+class Batch:
+    """hq_batch: one serving step's sequences (hq_batch_create, hq_batch_set)."""
+
+    def __init__(self, max_seqs, max_tokens, max_pages, device=0):
+        self.h = None
+        h = C.c_void_p()
+        _check(load().hq_batch_create(device, max_seqs, max_tokens, max_pages, C.byref(h)))
+        self.h = h.value
+
+    def set(self, kv, n_heads, n_new, n_pos, pages, stream=None):
+        """The step: sequence i's last n_new[i] of n_pos[i] positions are new tokens; pages: its row of [sequences, n]."""
+        n_new, n_pos = np.ascontiguousarray(n_new, np.int32), np.ascontiguousarray(n_pos, np.int32)
+        pages = np.ascontiguousarray(pages, np.uint32)
+        if n_new.ndim != 1 or n_pos.shape != n_new.shape or pages.ndim != 2 or len(pages) != len(n_new):
+            raise HQError(f"Batch.set: n_new {n_new.shape}, n_pos {n_pos.shape}, pages {pages.shape}")
+        self.n_heads = n_heads
+        _check(_lib.hq_batch_set(self.h, C.byref(kv.s), n_heads, len(n_new), _ptr(n_new), _ptr(n_pos), _ptr(pages), pages.shape[1], stream))
+
+    def free(self):
+        if self.h:
+            _lib.hq_batch_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def rope_table(inv_freq, n, table, stream=None):
+    """hq_rope_table: (cos, sin) of n positions into device memory [n, len(inv_freq), 2]."""
+    inv_freq = np.ascontiguousarray(inv_freq, np.float32)
+    _check(load().hq_rope_table(_ptr(inv_freq), 2 * len(inv_freq), n, _dev(table), stream))
+
+
+def rope_append(batch, kv, q, k, v, q_out, table, n_table, rot_dim, *, f32, q_stride, kv_stride, q_head_stride=None, positions=None,
+                axis=None, q_norm=None, k_norm=None, norm_offset=0.0, eps=1e-6, stream=None):
+    """hq_rope_append on device memory (DevBuf or raw pointers); axis: the axis of each frequency, with positions."""
+    if axis is not None:
+        axis = np.ascontiguousarray(axis, np.uint8)
+        if len(axis) != rot_dim // 2:
+            raise HQError(f"rope_append: axis has {len(axis)} frequencies, rot_dim {rot_dim}")
+    r = Rope(_dev(q), _dev(k), _dev(v), int(f32), q_stride, q_head_stride or kv.s.head_dim, kv_stride, _dev(q_norm), _dev(k_norm),
+             norm_offset, eps, _dev(table), n_table, rot_dim, _dev(positions), None if axis is None else axis.ctypes.data,
+             0 if axis is None or not len(axis) else int(axis.max()) + 1, _dev(q_out))
+    _check(_lib.hq_rope_append(batch.h, C.byref(kv.s), C.byref(r), stream))
+
+
+def attention(batch, kv, q, out, scale, *, q_stride=None, out_stride=None, gate=None, gate_f32=False, gate_stride=0,
+              gate_head_stride=0, stream=None):
+    """hq_attention on device memory (DevBuf or raw pointers); rows of q and out are contiguous unless strides are given."""
+    if q_stride is None or out_stride is None:
+        row = batch.n_heads * kv.s.head_dim
+        q_stride, out_stride = row if q_stride is None else q_stride, row if out_stride is None else out_stride
+    a = Attn(_dev(q), q_stride, scale, _dev(gate), int(gate_f32), gate_stride, gate_head_stride, _dev(out), out_stride)
+    _check(_lib.hq_attention(batch.h, C.byref(kv.s), C.byref(a), stream))
+
+
+def logprobs(logits, M, V, *, f32, stride=None, ids=None, n_ids=0, top_k=0, logp=None, entropy=None, top_ids=None, top_logp=None, stream=None):
+    """hq_logprobs on device memory (DevBuf or raw pointers)."""
+    _check(load().hq_logprobs(_dev(logits), int(f32), M, V, V if stride is None else stride, _dev(ids), n_ids, top_k, _dev(logp),
+                              _dev(entropy), _dev(top_ids), _dev(top_logp), stream))
 
 
 class LlamaModel:
