@@ -8,11 +8,23 @@
 #include "hq_internal.h"
 #include "hq_serve.h"
 
-// One sequence: its new tokens tok0 .. tok0 + n_new - 1, of which the last n_new stand at positions n_pos - n_new ..
-// n_pos - 1 (negative: padding), and its pages, pages[page0 ..].
-struct HqSeq {
-    int tok0, n_new, n_pos, page0;
+// One workgroup's work in hq_attention: rows row0 .. of kv head kvh of a sequence (row t rep + e: its new token t, query head
+// kvh rep + e; R rows in all) over positions k0 .. k1 - 1; part `part` of the n_parts that its block of rows is cut into.
+struct HqItem {
+    int kvh;        // -1: nothing
+    int tok0;       // the sequence's first new token
+    int base;       // the position of it
+    int R, row0;
+    int k0, k1;
+    int page0;      // its pages
+    int part, n_parts;
+    int block;        // the block's counter, where n_parts > 1
+    uint32_t part_at; // its parts, in units of 16 bytes of hq_batch::parts
 };
+// Kernel bodies of hq_attention by the rows a workgroup takes.
+enum { HQ_STREAM16, HQ_STREAM32, HQ_ROWS128, HQ_ROWS256, HQ_BODIES };
+// Floats of a part's row for a head_dim.
+int hq_attn_part_floats(int head_dim);
 
 struct hq_batch {
     int device, n_cu;
@@ -24,9 +36,12 @@ struct hq_batch {
     // device arrays, parts of `dev`
     const int *tok_pos;   // position of token t in its sequence
     const int *tok_slot;  // page * page_size + slot, or -1: not stored
-    const int *tok_seq;
-    const HqSeq *seqs;
     const uint32_t *pages;
+    const HqItem *items[HQ_BODIES];
+    int n_items[HQ_BODIES];
+    int *counters;      // one per block cut into parts; zero between calls
+    float *parts;       // rows of such blocks
+    size_t part_bytes;  // allocated
     // storage: one pinned copy of `dev`, which the next set waits for
     int *host, *dev;
     size_t words;  // of each

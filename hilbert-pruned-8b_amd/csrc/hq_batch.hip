@@ -5,7 +5,9 @@
 #include <algorithm>
 #include <math.h>
 #include <new>
+#include <queue>
 #include <string.h>
+#include <vector>
 
 #include "hq_batch.h"
 #include "hq_device.h"
@@ -34,6 +36,118 @@ int check_geometry(const char *who, const hq_kv_t *kv) {
     return 0;
 }
 
+// ------------------------------------------------------------------------------------ hq_attention's work
+struct Block {
+    HqItem it;
+    int len;  // positions, of its last row
+};
+
+// Blocks of rows become items (see HqItem). Cutting a long block's positions fills the chip where blocks are few or uneven,
+// at the price of a part's way through memory, about `over` positions' time for each item. The length of a piece is the one
+// of a few whose items, dealt longest first to `slots` workgroups at a time, end first; none is shorter than `least`.
+int piece_length(const std::vector<Block> &bl, int unit, int slots, int over, int least) {
+    int64_t total = 0;
+    int longest = 0;
+    for (const Block &b : bl) total += b.len, longest = std::max(longest, b.len);
+    int best = longest;
+    double best_end = 1e300;
+    std::vector<int> cost;
+    for (int f = 0; f <= 4; f++) {
+        const int L = f ? (int)std::max<int64_t>((total / (slots * f) + unit - 1) / unit * unit, least) : std::max(longest, unit);
+        if (f && L >= longest) continue;
+        cost.clear();
+        for (const Block &b : bl) {
+            const int n = std::max(1, (b.len + L / 2) / L), each = (b.len + n - 1) / n;
+            for (int i = 0; i < n; i++) cost.push_back(each + (n > 1 ? 2 * over : over));
+        }
+        std::sort(cost.begin(), cost.end(), [](int a, int b) { return a > b; });
+        std::priority_queue<double, std::vector<double>, std::greater<double>> q;
+        for (int i = 0; i < slots; i++) q.push(0);
+        double end = 0;
+        for (int c : cost) {
+            const double e = q.top() + c;
+            q.pop(), q.push(e);
+            end = std::max(end, e);
+        }
+        if (end < best_end) best_end = end, best = L;
+    }
+    return best;
+}
+
+struct Plan {
+    std::vector<HqItem> items[HQ_BODIES];
+    int blocks = 0;          // counters
+    uint64_t part_units = 0; // of 16 bytes
+};
+
+constexpr int XCDS = 8;
+
+void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const int32_t *n_new, const int32_t *n_pos, Plan *out) {
+    const int rep = n_heads / kv.n_kv_heads, rows_of[HQ_BODIES] = {16, 32, 128, 256};
+    std::vector<Block> bl[HQ_BODIES];
+    int tok0 = 0, page0 = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        const int R = n_new[i] * rep, base = n_pos[i] - n_new[i];
+        const int body = R <= 16 ? HQ_STREAM16 : R <= 32 && kv.head_dim <= 128 ? HQ_STREAM32 : R <= 128 || kv.head_dim > 128 ? HQ_ROWS128 : HQ_ROWS256;
+        for (int h = 0; h < kv.n_kv_heads && R; h++)
+            for (int row0 = (R - 1) / rows_of[body] * rows_of[body]; row0 >= 0; row0 -= rows_of[body]) {
+                const int n = std::max(0, base + (std::min(R, row0 + rows_of[body]) - 1) / rep + 1);
+                bl[body].push_back({{h, tok0, base, R, row0, 0, n, page0, 0, 1, 0, 0}, n});
+            }
+        tok0 += n_new[i];
+        page0 += (n_pos[i] + kv.page_size - 1) / kv.page_size;
+    }
+    for (int body = 0; body < HQ_BODIES; body++) {
+        if (bl[body].empty()) continue;
+        const bool stream = body <= HQ_STREAM32;
+        const int unit = stream ? 128 : 64;
+        const int slots = n_cu * (stream || body == HQ_ROWS128 ? 2 : 1);
+        const int L = piece_length(bl[body], unit, slots, stream ? 128 : 192, 256);
+        std::vector<HqItem> all;
+        for (const Block &b : bl[body]) {
+            const int units = (b.len + unit - 1) / unit, n = std::max(1, std::min((b.len + L / 2) / L, units));
+            HqItem it = b.it;
+            it.n_parts = n;
+            if (n > 1) {
+                it.block = out->blocks++;
+                it.part_at = (uint32_t)out->part_units;
+                out->part_units += (uint64_t)n * rows_of[body] * hq_attn_part_floats(kv.head_dim) / 4;
+            }
+            for (int p = 0; p < n; p++) {
+                it.part = p;
+                it.k0 = (int)((int64_t)units * p / n) * unit;
+                it.k1 = p == n - 1 ? b.len : (int)((int64_t)units * (p + 1) / n) * unit;
+                all.push_back(it);
+            }
+        }
+        const auto longer = [](const HqItem &a, const HqItem &b) { return a.k1 - a.k0 > b.k1 - b.k0; };
+        std::vector<HqItem> &to = out->items[body];
+        if (stream) {
+            std::stable_sort(all.begin(), all.end(), longer);
+            to = all;
+            continue;
+        }
+        // blocks of one sequence and kv head read the same keys and values: items go to the XCDs (workgroup i runs on XCD
+        // i % 8) in eight runs of equal work, each run longest first
+        int64_t total = 0, run = 0;
+        for (const HqItem &it : all) total += it.k1 - it.k0 + unit;
+        std::vector<HqItem> q[XCDS];
+        for (const HqItem &it : all) {
+            const int64_t mid = run + (it.k1 - it.k0 + unit) / 2;
+            q[std::min<int64_t>(mid * XCDS / total, XCDS - 1)].push_back(it);
+            run += it.k1 - it.k0 + unit;
+        }
+        size_t most = 0;
+        for (auto &v : q) std::stable_sort(v.begin(), v.end(), longer), most = std::max(most, v.size());
+        for (size_t j = 0; j < most; j++)
+            for (auto &v : q) {
+                HqItem none = {};
+                none.kvh = -1;
+                to.push_back(j < v.size() ? v[j] : none);
+            }
+    }
+}
+
 }  // namespace
 
 int hq_kv_check(const char *who, const hq_kv_t *kv, const hq_batch *b) {
@@ -47,6 +161,7 @@ int hq_kv_check(const char *who, const hq_kv_t *kv, const hq_batch *b) {
     if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return hq_internal_fail("%s: k and v must be 16-byte aligned", who);
     if (kv->type == HQ_KV_Q8 && (!kv->k_scale || !kv->v_scale || !aligned(kv->k_scale, 16) || !aligned(kv->v_scale, 16)))
         return hq_internal_fail("%s: a Q8 cache needs 16-byte aligned scales", who);
+    if (kv->pos_stride >= ((int64_t)1 << 30) / kv->page_size) return hq_internal_fail("%s: a page's positions span 2^30 elements or more", who);
     for (int64_t s : {kv->page_stride, kv->pos_stride, kv->head_stride})
         if (s < 0 || s % 16 || s > ((int64_t)1 << 40)) return hq_internal_fail("%s: cache stride %lld (a multiple of 16)", who, (long long)s);
     return 0;
@@ -78,6 +193,7 @@ extern "C" void hq_batch_free(hq_batch *b) {
     (void)use_device(b->device);
     (void)hipDeviceSynchronize();
     if (b->dev) (void)hipFree(b->dev);
+    if (b->parts) (void)hipFree(b->parts);
     if (b->host) (void)hipHostFree(b->host);
     if (b->sent) (void)hipEventDestroy(b->sent);
     delete b;
@@ -105,6 +221,7 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
                 return hq_internal_fail("%s: page %lld of sequence %d is %u (the cache has %u)", who, (long long)p, i, pages[(size_t)i * (size_t)pages_ld + (size_t)p], kv->n_pages);
         P += need;
     }
+    if (T * n_heads >= (1ll << 31)) return hq_internal_fail("%s: %lld tokens of %d heads", who, (long long)T, n_heads);
     if (T > b->max_tokens) return hq_internal_fail("%s: %lld new tokens (the batch takes %d)", who, (long long)T, b->max_tokens);
     if (P >= (1ll << 30)) return hq_internal_fail("%s: %lld pages in all", who, (long long)P);
     if (use_device(b->device)) return -1;
@@ -113,7 +230,16 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
         SCK(hipEventSynchronize(b->sent));
         b->sending = false;
     }
-    const size_t words = 3 * (size_t)T + 4 * (size_t)n_seqs + (size_t)P + 16;
+    Plan plan;
+    try {
+        plan_attention(*kv, n_heads, b->n_cu, n_seqs, n_new, n_pos, &plan);
+    } catch (const std::exception &) {
+        return hq_internal_fail("%s: out of memory", who);
+    }
+    if (plan.part_units >> 32) return hq_internal_fail("%s: %llu MiB of workspace", who, (unsigned long long)(plan.part_units >> 16));
+    size_t n_items = 0;
+    for (auto &v : plan.items) n_items += v.size();
+    const size_t words = n_items * (sizeof(HqItem) / 4) + 2 * (size_t)T + (size_t)plan.blocks + (size_t)P + 16;
     if (words > b->words) {
         const size_t want = std::max(words, words + words / 2);
         SCK(hipDeviceSynchronize());
@@ -126,29 +252,46 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
         SCK(hipHostMalloc((void **)&b->host, want * 4, hipHostMallocDefault));
         b->words = want;
     }
-    int *seq = b->host, *pos = seq + 4 * n_seqs, *slot = pos + T, *of = slot + T, *pg = of + T;
-    int t = 0, at = 0;
+    if (plan.part_units * 16 > b->part_bytes) {
+        SCK(hipDeviceSynchronize());
+        if (b->parts) SCK(hipFree(b->parts));
+        b->parts = nullptr;
+        b->part_bytes = 0;
+        SCK(hipMalloc((void **)&b->parts, plan.part_units * 16));
+        b->part_bytes = plan.part_units * 16;
+    }
+    int *w = b->host;
+    const auto dev = [&]() { return b->dev + (w - b->host); };
+    for (int i = 0; i < HQ_BODIES; i++) {
+        b->items[i] = (const HqItem *)dev();
+        b->n_items[i] = (int)plan.items[i].size();
+        if (!plan.items[i].empty()) memcpy(w, plan.items[i].data(), plan.items[i].size() * sizeof(HqItem));
+        w += plan.items[i].size() * (sizeof(HqItem) / 4);
+    }
+    b->counters = dev();
+    if (plan.blocks) memset(w, 0, (size_t)plan.blocks * 4);
+    w += plan.blocks;
+    b->pages = (const uint32_t *)dev();
     for (int i = 0; i < n_seqs; i++) {
-        const HqSeq s = {t, n_new[i], n_pos[i], at};
-        memcpy(seq + 4 * i, &s, sizeof s);
-        const uint32_t *const row = pages ? pages + (size_t)i * (size_t)pages_ld : nullptr;
+        const int need = (n_pos[i] + ps - 1) / ps;
+        if (need) memcpy(w, pages + (size_t)i * (size_t)pages_ld, (size_t)need * 4);
+        w += need;
+    }
+    b->tok_pos = dev(), b->tok_slot = b->tok_pos + T;
+    int *const slot = w + T;
+    for (int i = 0, t = 0; i < n_seqs; i++)
         for (int j = 0; j < n_new[i]; j++, t++) {
             const int p = n_pos[i] - n_new[i] + j;
-            pos[t] = p, of[t] = i;
-            slot[t] = p < 0 ? -1 : (int)(row[p / ps] * (uint32_t)ps + (uint32_t)(p % ps));
+            w[t] = p;
+            slot[t] = p < 0 ? -1 : (int)(pages[(size_t)i * (size_t)pages_ld + (size_t)(p / ps)] * (uint32_t)ps + (uint32_t)(p % ps));
         }
-        const int need = (n_pos[i] + ps - 1) / ps;
-        if (need) memcpy(pg + at, row, (size_t)need * 4);
-        at += need;
-    }
-    const size_t used = (size_t)(pg + at - b->host);
+    w = slot + T;
+    const size_t used = (size_t)(w - b->host);
     if (used) {
         SCK(hipMemcpyAsync(b->dev, b->host, used * 4, hipMemcpyHostToDevice, (hipStream_t)stream));
         SCK(hipEventRecord(b->sent, (hipStream_t)stream));
         b->sending = true;
     }
-    const auto dev = [&](const int *p) { return b->dev + (p - b->host); };
-    b->seqs = (const HqSeq *)dev(seq), b->tok_pos = dev(pos), b->tok_slot = dev(slot), b->tok_seq = dev(of), b->pages = (const uint32_t *)dev(pg);
     b->n_seqs = n_seqs, b->n_tokens = (int)T, b->n_heads = n_heads;
     b->geom = *kv;
     b->set = true;

@@ -1,6 +1,23 @@
 // hq_paged_attention.hip - attention of a step's new tokens over the paged cache (hq_attention, include/hq_serve.h).
+//
+// The queries that share a kv head are one matrix: row r = t rep + e of a sequence is its new token t in query head g rep +
+// e of kv head g (rep = heads / kv heads), so grouped heads and neighbouring tokens read each key and value once. hq_batch.hip
+// cuts a step into items: a block of rows of one kv head over a range of positions. Two bodies do them:
+//   k_rows    blocks of 32 rows per wave: a workgroup's waves share tiles of positions in LDS (prompts, chunks)
+//   k_stream  16 or 32 rows: each wave streams tiles of its own straight into operand registers (single tokens)
+// Both form everything transposed, so that nothing moves between lanes from scores to outputs: S^T = K Q^T leaves row li in
+// every lane and positions in its registers, which is the B operand of O^T = V^T P^T. Both run the online softmax: a running
+// maximum and sum per row, outputs scaled when the maximum grows.
+//
+// Precision: fp16 operands, fp32 products, sums, maxima and outputs. Rounded to 16 bits are the weights p (2^-11 of each;
+// the sum takes them unrounded) and, of a Q8 cache, the decoded values (2^-11; scores of k_stream meet the exact codes).
+//
+// Places that a row does not see weigh 0, and 0 times an infinity or NaN would be NaN: in a tile that some row sees only part
+// of, values that are not finite (`odd` below) enter the product as 0, and are added to the outputs of the rows that do see
+// them afterwards.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <math.h>
 
 #include "hq_batch.h"
@@ -8,84 +25,681 @@
 
 namespace {
 
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
 struct Args {
     hq_kv_t kv;
     hq_attn_t a;
-    const int *tok_pos, *tok_seq;
-    const HqSeq *seqs;
+    const HqItem *items;
     const uint32_t *pages;
-    int nh, rep;
+    float *parts;
+    int *counters;
+    int nh, rep, shift;  // shift: log2 of the page size
+    float sc, slack;     // |scale| log2(e); how far (in raw scores) a maximum may grow before the outputs are rescaled
 };
 
-template <bool Q8>
-DEV float kv_at(const void *p, size_t at) {
-    return Q8 ? (float)((const int8_t *)p)[at] : (float)((const _Float16 *)p)[at];
-}
+DEV f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-DEV float wave_max(float v) {
+// the maximum / sum of a lane's value and that of the lane 32 away
+DEV float max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+DEV float sum_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+DEV float max_lg(float v) { return max_halves(fmaxf(v, __shfl_xor(v, 16, 64))); }
+DEV float sum_lg(float v) { return sum_halves(v + __shfl_xor(v, 16, 64)); }
+
+DEV float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+// 2^(x - m) of a part's maximum x (log2 units) against the row's m; a part that saw nothing has x = -inf
+DEV float part_scale(float x, float m) { return x == -INFINITY ? 0.f : ex2(x - m); }
+
+// fp16 pairs of the 16-bit words of x that are infinities or NaN
+DEV bool odd2(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
+DEV bool odd16(u4v x) { return odd2(x.x) || odd2(x.y) || odd2(x.z) || odd2(x.w); }
+DEV bool odd(_Float16 x) { return odd2(__builtin_bit_cast(uint16_t, x)); }
+// v with 0 for infinities and NaN; the 0/1 pattern of +inf and NaN (up), of -inf and NaN (down)
+DEV h8 finite8(h8 v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    for (int e = 0; e < 8; e++) v[e] = odd(v[e]) ? (_Float16)0.f : v[e];
     return v;
 }
-DEV float wave_sum(float v) {
+DEV u4v finite16(u4v v) { return __builtin_bit_cast(u4v, finite8(__builtin_bit_cast(h8, v))); }
+DEV h8 pattern8(h8 v, bool up) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int e = 0; e < 8; e++) v[e] = odd(v[e]) && !(up ? v[e] < (_Float16)0.f : v[e] > (_Float16)0.f) ? (_Float16)1.f : (_Float16)0.f;
     return v;
 }
+// an output that saw `up` and `down` such values (counts)
+DEV float add_odd(float o, float up, float down) {
+    if (up > 0.f) o += INFINITY;
+    if (down > 0.f) o -= INFINITY;
+    return o;
+}
 
-// One wave per token and head: 64 positions at a time, a lane a score, then a lane every 64th dim of the output, with a
-// running maximum and sum.
-template <bool Q8>
-__global__ void __launch_bounds__(64) k_attn_paged(Args g) {
-    __shared__ float q[256], ps[64];
-    __shared__ uint32_t row[64];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hd = g.kv.head_dim, kvh = h / g.rep;
-    const HqSeq s = g.seqs[g.tok_seq[t]];
-    const int n = g.tok_pos[t] + 1, ps_ = g.kv.page_size;
-    for (int d = lane; d < hd; d += 64) q[d] = (float)((const _Float16 *)g.a.q)[(size_t)t * g.a.q_stride + (size_t)h * hd + d] * g.a.scale;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < n; p0 += 64) {
-        __syncthreads();
-        const int p = p0 + lane;
-        float x = -INFINITY;
-        if (p < n) {
-            const uint32_t page = g.pages[s.page0 + p / ps_], in = (uint32_t)p % (uint32_t)ps_;
-            row[lane] = page * (uint32_t)ps_ + in;
-            const size_t at = (size_t)page * g.kv.page_stride + (size_t)in * g.kv.pos_stride + (size_t)kvh * g.kv.head_stride;
-            x = 0.f;
-            for (int d = 0; d < hd; d++) x += q[d] * kv_at<Q8>(g.kv.k, at + d);
-            if (Q8) x *= h2f(g.kv.k_scale[((size_t)page * g.kv.n_kv_heads + kvh) * ps_ + in]);
-        }
-        const float mn = fmaxf(m, wave_max(x)), m0 = mn == -INFINITY ? 0.f : mn;
-        const float e = p < n ? expf(x - m0) : 0.f, f = expf(m - m0);
-        ps[lane] = e;
-        l = l * f + wave_sum(e);
-        m = mn;
-        __syncthreads();
-        for (int i = 0; i < 4; i++) o[i] *= f;
-        for (int j = 0; j < 64 && p0 + j < n; j++) {
-            const uint32_t page = row[j] / (uint32_t)ps_, in = row[j] % (uint32_t)ps_;
-            const size_t at = (size_t)page * g.kv.page_stride + (size_t)in * g.kv.pos_stride + (size_t)kvh * g.kv.head_stride;
-            const float w = Q8 ? ps[j] * h2f(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + kvh) * ps_ + in]) : ps[j];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (lane + 64 * i < hd) o[i] += w * kv_at<Q8>(g.kv.v, at + lane + 64 * i);
-        }
-    }
+// Q8 codes as fp16: bytes q ^ 0x80 under 0x64 are 1024 + q + 128
+DEV h2 codes2(uint32_t w) {
+    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    return as_h2(w) - bias;
+}
+// 16 codes times their position's scale: one rounding to fp16
+DEV void decode16(u4v c, _Float16 d, h8 &lo, h8 &hi) {
+    const h2 dd = {d, d};
+    h2 o[8];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int d = lane + 64 * i;
-        if (d >= hd) continue;
-        float y = n > 0 ? o[i] / l : 0.f;
-        if (g.a.gate) {
-            const size_t at = (size_t)t * g.a.gate_stride + (size_t)h * g.a.gate_head_stride + d;
-            y *= 1.0f / (1.0f + expf(-(g.a.gate_f32 ? ((const float *)g.a.gate)[at] : (float)((const _Float16 *)g.a.gate)[at])));
-        }
-        ((_Float16 *)g.a.out)[(size_t)t * g.a.out_stride + (size_t)h * hd + d] = (_Float16)y;
+        const uint32_t w = c[i] ^ 0x80808080u;
+        o[2 * i] = codes2(perm_lo(w)) * dd;
+        o[2 * i + 1] = codes2(perm_hi(w)) * dd;
     }
+    lo = h8{o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
+    hi = h8{o[4].x, o[4].y, o[5].x, o[5].y, o[6].x, o[6].y, o[7].x, o[7].y};
+}
+
+// four outputs d .. d + 3 of row r, v / l, gated
+DEV void finish(const Args &g, const HqItem &it, int r, int d, f4 v, float l) {
+    const int hd = g.kv.head_dim;
+    if (r >= it.R || d >= hd) return;
+    const int t = r / g.rep, h = it.kvh * g.rep + r - t * g.rep;
+    const size_t tok = (size_t)(it.tok0 + t);
+    if (it.base + t < 0) v = f4{0.f, 0.f, 0.f, 0.f}, l = 1.f;  // padding: sees nothing
+    h4 y;
+    f4 gate = {0.f, 0.f, 0.f, 0.f};
+    if (g.a.gate) {
+        const size_t at = tok * g.a.gate_stride + (size_t)h * g.a.gate_head_stride + d;
+        if (g.a.gate_f32) gate = *(const f4 *)((const float *)g.a.gate + at);
+        else {
+            const h4 x = *(const h4 *)((const _Float16 *)g.a.gate + at);
+            gate = f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        float x = v[e] / l;
+        if (g.a.gate) x *= 1.0f / (1.0f + expf(-gate[e]));
+        y[e] = (_Float16)x;
+    }
+    *(h4 *)((_Float16 *)g.a.out + tok * g.a.out_stride + (size_t)h * hd + d) = y;
+}
+
+// A part's row: its sums [HDP], then (maximum in log2 units, sum). Parts are written and read at device scope; the last of
+// a block's items to arrive adds them in part order, so the result does not depend on the order of arrival.
+template <int HDP>
+constexpr int PARTF = HDP + 4;
+
+template <int HDP, int ROWS, int NT>
+DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = atomicAdd(&g.counters[it.block], 1) == it.n_parts - 1;
+        if (last) atomicExch(&g.counters[it.block], 0);
+        *flag = last;
+    }
+    __syncthreads();
+    if (!*flag) return;
+    constexpr int C = HDP / 4;
+    for (int x = threadIdx.x; x < ROWS * C; x += NT) {
+        const int row = x / C, d = 4 * (x % C);
+        if (it.row0 + row >= it.R) continue;
+        float m = -INFINITY, l = 0.f;
+        f4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < it.n_parts; p0 += 4) {
+            f4 y[4], ml[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t at = (uint32_t)((std::min(p0 + e, it.n_parts - 1) * ROWS + row) * PARTF<HDP>) * 4u;
+                ml[e] = buf_load16_sc1(rp, at + HDP * 4u, 0);
+                y[e] = buf_load16_sc1(rp, at + (uint32_t)d * 4u, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (p0 + e >= it.n_parts) continue;
+                const float mn = fmaxf(m, ml[e].x), a = part_scale(m, mn), b = part_scale(ml[e].x, mn);
+                v = v * a + y[e] * b;
+                l = l * a + ml[e].y * b;
+                m = mn;
+            }
+        }
+        finish(g, it, it.row0 + row, d, v, l);
+    }
+}
+
+DEV const uint32_t *page_of(const Args &g, const HqItem &it, int p) { return g.pages + it.page0 + (p >> g.shift); }
+
+// ------------------------------------------------------------------------------------ rows
+// Row pitch of an LDS tile and the XOR of its 16-byte pieces: 16 rows that follow each other put a piece on 16 different
+// places of the 256 bytes the LDS reads in a clock (operand K), and four rows put 64 bytes on its four quarters (operand V).
+template <int HDP>
+constexpr int PITCH = HDP <= 64 ? 128 : HDP <= 128 ? 256 : 512;
+template <int HDP>
+DEV int swizzle(int row) {
+    return HDP <= 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+template <int HDP>
+constexpr int KT = HDP <= 128 ? 64 : 32;  // positions per tile
+
+// A workgroup of NW waves takes 32 NW rows. Tiles of KT positions go through registers into LDS (Q8 decoded on the way), two
+// buffers deep: while a tile is multiplied the next one is on its way from memory. A wave holds its queries, S^T [KT x 32]
+// and O^T [HDP x 32] in registers; V's operand is read transposed from LDS, its key order that of S^T's registers.
+template <int HDP, bool Q8, int NW>
+__global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
+    constexpr int P = PITCH<HDP>, T = KT<HDP>, KB = T / 32, NJ = HDP / 16, ND = HDP / 32, TILE = T * P;
+    constexpr int LPR = P / (Q8 ? 32 : 16), RPI = 64 / LPR, UNITS = T / RPI, NI = 2 * UNITS / NW;
+    static_assert(RPI <= 16 && NI * NW == 2 * UNITS, "whole loads per wave, each in one page");
+    __shared__ __align__(1024) char lds[4 * TILE];
+    __shared__ int flags[2], last;
+    const HqItem it = g.items[blockIdx.x];
+    if (it.kvh < 0) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hf = lane >> 5;
+    const int hd = g.kv.head_dim, rep = g.rep;
+    const int r0 = it.row0 + 32 * w, r = r0 + li;
+    const int n = it.base + (std::min(it.R, it.row0 + 32 * NW) - 1) / rep + 1;  // positions some row of the block sees
+    const int n_blk = it.base + it.row0 / rep + 1;                              // positions every row of the block sees
+    const int wn = r0 < it.R ? it.base + (std::min(it.R, r0 + 32) - 1) / rep + 1 : 0, wn_all = it.base + r0 / rep + 1;
+    const int lim = it.base + std::min(r, it.R - 1) / rep + 1;
+    if (threadIdx.x < 2) flags[threadIdx.x] = -1;
+
+    h8 q[NJ];
+    {
+        const int rr = std::min(r, it.R - 1), t = rr / rep, h = it.kvh * rep + rr - t * rep;
+        const _Float16 *p = (const _Float16 *)g.a.q + (size_t)(it.tok0 + t) * g.a.q_stride + (size_t)h * hd;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int d = 16 * j + 8 * hf;
+            q[j] = d < hd ? *(const h8 *)(p + d) : h8{};
+            if (g.a.scale < 0.f) q[j] = -q[j];
+        }
+    }
+
+    // staging: wave w's loads u = w NI + i of a tile: matrix u / UNITS, rows RPI (u % UNITS) + lane / LPR, a 16-byte piece each
+    const int lrow = lane / LPR, piece = lane % LPR;
+    const bool on = piece * (Q8 ? 16 : 8) < hd;
+    const size_t es = Q8 ? 1 : 2;
+    const char *const kb0 = (const char *)g.kv.k + (size_t)it.kvh * g.kv.head_stride * es, *const vb0 = (const char *)g.kv.v + (size_t)it.kvh * g.kv.head_stride * es;
+    const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es);
+    u4v st[NI];
+    _Float16 sd[NI];
+    uint32_t pg[NI];
+    int wat[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int u = w * NI + i, row = RPI * (u % UNITS) + lrow;
+        wat[i] = (u / UNITS) * TILE + row * P + (((Q8 ? 2 * piece : piece) ^ swizzle<HDP>(row)) << 4);
+        st[i] = u4v{0, 0, 0, 0}, sd[i] = (_Float16)0.f;
+    }
+    auto fetch_pages = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) pg[i] = *page_of(g, it, std::min(s0 + RPI * ((w * NI + i) % UNITS), n - 1));
+    };
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int u = w * NI + i, in = std::min(s0 + RPI * (u % UNITS) + lrow, n - 1) & (g.kv.page_size - 1);
+            const char *base = (u < UNITS ? kb0 : vb0) + (size_t)pg[i] * (size_t)g.kv.page_stride * es;
+            if (on) st[i] = *(const u4v *)(base + ((uint32_t)in * pos_b + (uint32_t)piece * 16u));
+            if (Q8) sd[i] = ((const _Float16 *)(u < UNITS ? g.kv.k_scale : g.kv.v_scale))[((size_t)pg[i] * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in];
+        }
+    };
+    auto store = [&](int buf, int s0) {
+        char *const to = lds + buf * 2 * TILE;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const bool look = s0 + T > n_blk && w * NI + i >= UNITS;
+            if (Q8) {
+                h8 lo, hi;
+                decode16(st[i], sd[i], lo, hi);
+                if (!on) lo = hi = h8{};
+                if (look && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi)))) lo = finite8(lo), hi = finite8(hi), flags[buf] = s0;
+                *(h8 *)(to + wat[i]) = lo;
+                *(h8 *)(to + (wat[i] ^ 16)) = hi;
+            } else {
+                u4v x = st[i];
+                if (look && odd16(x)) x = finite16(x), flags[buf] = s0;
+                *(u4v *)(to + wat[i]) = x;
+            }
+        }
+    };
+
+    float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores), what the exponents are taken against, the sum
+    f16v o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.f;
+
+    const int end = std::min(it.k1, n);
+    const uint32_t kx = (uint32_t)(li * P + ((hf ^ swizzle<HDP>(li)) << 4));
+    const int i16 = lane & 15, vrow = 4 * hf + (i16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+    const uint32_t vx = (uint32_t)(TILE + vrow * P + ((vc ^ swizzle<HDP>(vrow)) << 4) + 8 * (i16 & 1));
+    if (it.k0 < end) {
+        fetch_pages(it.k0);
+        load(it.k0);
+        if (it.k0 + T < end) fetch_pages(it.k0 + T);
+        __syncthreads();  // the flags are set
+        store(0, it.k0);
+        if (it.k0 + T < end) load(it.k0 + T);
+        if (it.k0 + 2 * T < end) fetch_pages(it.k0 + 2 * T);
+        __syncthreads();
+    }
+    int buf = 0;
+    for (int s0 = it.k0; s0 < end; s0 += T, buf ^= 1) {
+        if (s0 < wn) {
+            const char *const tile = lds + buf * 2 * TILE;
+            f16v s[KB];
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[b][e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int b = 0; b < KB; b++) s[b] = mfma32(*(const h8 *)(tile + ((kx ^ (32u * j)) + 32 * P * b)), q[j], s[b]);
+            if (s0 + T > wn_all) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[b][e] = s0 + 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[b][e] : -INFINITY;
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][e]);
+            if (__any(mx > m + g.slack)) {
+                const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : mn * g.sc;
+                const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
+                m = mn, mref = nref;
+                l *= a;
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] *= a;
+            }
+            h8 p[2 * KB];
+            float add = 0.f;
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float x = ex2(fmaf(s[b][e], g.sc, -mref));
+                    add += x;
+                    p[2 * b + (e >> 3)][e & 7] = (_Float16)x;
+                }
+            l += add;
+            auto operand = [&](int d, int k) {
+                typedef __attribute__((address_space(3))) s4 lds_s4;
+                const uint32_t at = (uint32_t)(uintptr_t)tile + ((vx ^ (64u * d)) + 16 * P * k);
+                const uint32_t at8 = (uint32_t)(uintptr_t)tile + ((vx ^ (64u * d) ^ 32u) + 16 * P * k + 8 * P);
+                const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)at));
+                const h4 c = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)at8));
+                return h8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+            };
+#pragma unroll
+            for (int k = 0; k < 2 * KB; k++)
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] = mfma32(operand(d, k), p[k], o[d]);
+            if (flags[buf] == s0) {  // the tile's odd values, position by position
+#pragma clang loop unroll(disable)
+                for (int at = s0; at < std::min(s0 + T, wn); at++) {
+                    const uint32_t page = *page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
+                    const char *const v = vb0 + ((size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
+                    const _Float16 d8 = Q8 ? ((const _Float16 *)g.kv.v_scale)[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in] : (_Float16)0.f;
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int dim = 32 * d + 8 * c + 4 * hf;
+                            if (at >= lim || dim >= hd) continue;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const _Float16 x = Q8 ? (_Float16)(float)((const int8_t *)v)[dim + e] * d8 : ((const _Float16 *)v)[dim + e];
+                                if (odd(x)) o[d][4 * c + e] += (float)x;
+                            }
+                        }
+                }
+            }
+        }
+        if (s0 + T < end) {
+            store(buf ^ 1, s0 + T);
+            if (s0 + 2 * T < end) load(s0 + 2 * T);
+            if (s0 + 3 * T < end) fetch_pages(s0 + 3 * T);
+        }
+        __syncthreads();
+    }
+    const float lt = sum_halves(l);
+    if (it.n_parts == 1) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) finish(g, it, r, 32 * d + 8 * c + 4 * hf, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]}, lt);
+        return;
+    }
+    constexpr int ROWS = 32 * NW;
+    const rsrc_t rp = make_rsrc(g.parts + (size_t)it.part_at * 4, (uint32_t)it.n_parts * ROWS * PARTF<HDP> * 4u);
+    const uint32_t at = (uint32_t)((it.part * ROWS + 32 * w + li) * PARTF<HDP>) * 4u;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            buf_store16(rp, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]}, at + (uint32_t)(32 * d + 8 * c + 4 * hf) * 4u);
+    if (hf == 0) buf_store16(rp, f4{m == -INFINITY ? -INFINITY : mref, lt, 0.f, 0.f}, at + HDP * 4u);
+    join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last);
+}
+
+// ------------------------------------------------------------------------------------ stream
+// A workgroup of NW waves takes 16 QB rows; the waves take tiles of 32 positions in turn, each with a softmax of its own, and
+// the waves' (maximum, sum, output) are added in wave order at the end. A lane (li = lane % 16, lg = lane / 16) loads keys
+// straight into the operand (key li, 16 bytes of dims), and of V the DPL dims DPL li .. of the eight positions 4 lg + r and
+// 16 + 4 lg + r, which are the positions of its score registers; pairs of positions are put together by v_perm into the
+// operand of block b, whose row li is dim DPL li + b.
+template <int HDP, bool Q8, int QB, int NW>
+__global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
+    constexpr int DPL = HDP / 16, NJ = HDP / 32, ROWS = 16 * QB, VW = Q8 ? DPL / 4 : DPL / 2, LDO = HDP + 4;
+    constexpr int KL = Q8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a key
+    __shared__ __align__(16) float os[NW > 4 ? 4 : NW][ROWS][LDO];
+    __shared__ float ms[NW][ROWS], ls[NW][ROWS];
+    __shared__ int last;
+    const HqItem it = g.items[blockIdx.x];
+    if (it.kvh < 0) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
+    const int hd = g.kv.head_dim, rep = g.rep;
+    const int n = it.base + (std::min(it.R, it.row0 + ROWS) - 1) / rep + 1, n_all = it.base + it.row0 / rep + 1;
+    const int end = std::min(it.k1, n);
+
+    h8 q[QB][NJ];
+    int lim[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const int r = std::min(it.row0 + 16 * b + li, it.R - 1), t = r / rep, h = it.kvh * rep + r - t * rep;
+        lim[b] = it.base + t + 1;
+        const _Float16 *p = (const _Float16 *)g.a.q + (size_t)(it.tok0 + t) * g.a.q_stride + (size_t)h * hd;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int d = Q8 ? 64 * (j / 2) + 16 * lg + 8 * (j % 2) : 32 * j + 8 * lg;
+            q[b][j] = d < hd ? *(const h8 *)(p + d) : h8{};
+            if (g.a.scale < 0.f) q[b][j] = -q[b][j];
+        }
+    }
+    const size_t es = Q8 ? 1 : 2;
+    const char *const kb0 = (const char *)g.kv.k + (size_t)it.kvh * g.kv.head_stride * es, *const vb0 = (const char *)g.kv.v + (size_t)it.kvh * g.kv.head_stride * es;
+    const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es), pmask = (uint32_t)g.kv.page_size - 1;
+    const size_t page_b = (size_t)g.kv.page_stride * es;
+
+    u4v kf[2][KL];
+    uint32_t vf[2][4][VW];
+    u2v ksc[2], vsc[2];
+    uint32_t pgk[2], pgn[2];  // pages of the tile whose keys are loaded next, of the one whose values are
+    auto fetch = [&](int s0, uint32_t (&pg)[2]) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) pg[b] = *page_of(g, it, std::min(s0 + 16 * b, n - 1));
+    };
+    auto load_k = [&](int s0, const uint32_t (&pg)[2]) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const uint32_t in = (uint32_t)std::min(s0 + 16 * b + li, n - 1) & pmask;
+            const char *p = kb0 + (size_t)pg[b] * page_b;
+#pragma unroll
+            for (int j = 0; j < KL; j++) {
+                const int d = (Q8 ? 64 * j + 16 * lg : 32 * j + 8 * lg);
+                kf[b][j] = d < hd ? *(const u4v *)(p + (in * pos_b + (uint32_t)d * (uint32_t)es)) : u4v{0, 0, 0, 0};
+            }
+            if (Q8) ksc[b] = *(const u2v *)(g.kv.k_scale + ((size_t)pg[b] * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + ((uint32_t)(s0 + 16 * b + 4 * lg) & pmask));
+        }
+    };
+    auto load_v = [&](int s0, const uint32_t (&pg)[2]) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const char *p = vb0 + (size_t)pg[b] * page_b;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t in = (uint32_t)std::min(s0 + 16 * b + 4 * lg + r, n - 1) & pmask;
+                // dims past head_dim: the last ones again (dropped)
+                const int d = std::min(DPL * li, hd - DPL);
+                const char *at = p + (in * pos_b + (uint32_t)d * (uint32_t)es);
+                if constexpr (VW == 1) vf[b][r][0] = *(const uint32_t *)at;
+                else if constexpr (VW == 2) {
+                    const u2v x = *(const u2v *)at;
+                    vf[b][r][0] = x.x, vf[b][r][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < VW / 4; c++) {
+                        const u4v x = *(const u4v *)(at + 16 * c);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) vf[b][r][4 * c + e] = x[e];
+                    }
+                }
+            }
+            if (Q8) vsc[b] = *(const u2v *)(g.kv.v_scale + ((size_t)pg[b] * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + ((uint32_t)(s0 + 16 * b + 4 * lg) & pmask));
+        }
+    };
+
+    float m[QB], mref[QB], l[QB];
+    f4 o[QB][DPL];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        m[b] = -INFINITY, mref[b] = 0.f, l[b] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DPL; c++) o[b][c] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    constexpr int STEP = 32 * NW;
+    int s0 = it.k0 + 32 * w;
+    if (s0 < end) {
+        fetch(s0, pgk);
+        load_k(s0, pgk);
+    }
+    for (; s0 < end; s0 += STEP) {
+        load_v(s0, pgk);
+        if (s0 + STEP < end) fetch(s0 + STEP, pgn);
+        f4 s[QB][2];
+#pragma unroll
+        for (int b = 0; b < QB; b++) s[b][0] = s[b][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                h8 kk;
+                if (Q8) {
+                    const uint32_t w0 = kf[p][j / 2][2 * (j % 2)] ^ 0x80808080u, w1 = kf[p][j / 2][2 * (j % 2) + 1] ^ 0x80808080u;
+                    const h2 a0 = codes2(perm_lo(w0)), a1 = codes2(perm_hi(w0)), a2 = codes2(perm_lo(w1)), a3 = codes2(perm_hi(w1));
+                    kk = h8{a0.x, a0.y, a1.x, a1.y, a2.x, a2.y, a3.x, a3.y};
+                } else {
+                    kk = __builtin_bit_cast(h8, kf[p][Q8 ? 0 : j]);
+                }
+#pragma unroll
+                for (int b = 0; b < QB; b++) s[b][p] = mfma(kk, q[b][j], s[b][p]);
+            }
+        if (Q8) {
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float d = h2f((uint16_t)(ksc[p][r / 2] >> (16 * (r % 2))));
+#pragma unroll
+                    for (int b = 0; b < QB; b++) s[b][p][r] *= d;
+                }
+        }
+        if (s0 + STEP < end) load_k(s0 + STEP, pgn);
+        const bool cut = s0 + 32 > n_all;  // some row does not see all of the tile
+        if (Q8 && s0 + 32 > n) {  // nothing is known of scales behind the last position
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (s0 + 16 * p + 4 * lg + r >= n) vsc[p][r / 2] &= r % 2 ? 0x0000ffffu : 0xffff0000u;
+        }
+        h8 pr[QB];
+#pragma unroll
+        for (int b = 0; b < QB; b++) {
+            if (cut)
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[b][p][r] = s0 + 16 * p + 4 * lg + r < lim[b] ? s[b][p][r] : -INFINITY;
+            float mx = s[b][0][0];
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[b][p][r]);
+            if (__any(mx > m[b] + g.slack)) {
+                const float mn = fmaxf(m[b], max_lg(mx)), nref = mn == -INFINITY ? 0.f : mn * g.sc;
+                const float a = m[b] == -INFINITY ? 0.f : ex2(mref[b] - nref);
+                m[b] = mn, mref[b] = nref;
+                l[b] *= a;
+#pragma unroll
+                for (int c = 0; c < DPL; c++) o[b][c] *= a;
+            }
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float x = ex2(fmaf(s[b][p][r], g.sc, -mref[b]));
+                    l[b] += x;
+                    pr[b][4 * p + r] = (_Float16)x;
+                }
+        }
+        // operand of block c: dim DPL li + c of the eight positions
+        auto operand = [&](int c) {
+            uint32_t x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int p = k / 2, r = 2 * (k % 2);
+                if (Q8) {
+                    // byte c of two positions' words
+                    const uint32_t sel = 0x0c000c00u | (uint32_t)((c & 3) + 4) << 16 | (uint32_t)(c & 3);
+                    const uint32_t y = __builtin_amdgcn_perm(vf[p][r + 1][c / 4] ^ 0x80808080u, vf[p][r][c / 4] ^ 0x80808080u, sel) | 0x64006400u;
+                    x[k] = __builtin_bit_cast(uint32_t, codes2(y) * as_h2(vsc[p][r / 2]));
+                } else {
+                    x[k] = __builtin_amdgcn_perm(vf[p][r + 1][c / 2], vf[p][r][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                }
+            }
+            return __builtin_bit_cast(h8, u4v{x[0], x[1], x[2], x[3]});
+        };
+        bool bad = false;
+        if (cut) {
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                // Q8: scales from 512 on (their products may pass fp16), infinities and NaN
+                if (Q8) bad |= ((vsc[p].x | vsc[p].x >> 16 | vsc[p].y | vsc[p].y >> 16) & 0x6000u) == 0x6000u;
+                else
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int c = 0; c < VW; c++) bad |= odd2(vf[p][r][c]);
+            }
+        }
+        if (cut && __any(bad)) {
+#pragma unroll
+            for (int b = 0; b < QB; b++) {
+                h8 seen;
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) seen[4 * p + r] = (_Float16)(s0 + 16 * p + 4 * lg + r < lim[b] ? 1.f : 0.f);
+#pragma unroll
+                for (int c = 0; c < DPL; c++) {
+                    const h8 v = operand(c);
+                    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+                    o[b][c] = mfma(finite8(v), pr[b], o[b][c]);
+                    const f4 up = mfma(pattern8(v, true), seen, zero), down = mfma(pattern8(v, false), seen, zero);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[b][c][e] = add_odd(o[b][c][e], up[e], down[e]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < DPL; c++) {
+                const h8 v = operand(c);
+#pragma unroll
+                for (int b = 0; b < QB; b++) o[b][c] = mfma(v, pr[b], o[b][c]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++) pgk[b] = pgn[b];
+    }
+
+    // the waves' parts, in wave order
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const float lt = sum_lg(l[b]);
+        if (lg == 0) ms[w][16 * b + li] = m[b] == -INFINITY ? -INFINITY : mref[b], ls[w][16 * b + li] = lt;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        float mm = ms[0][16 * b + li];
+#pragma unroll
+        for (int v = 1; v < NW; v++) mm = fmaxf(mm, ms[v][16 * b + li]);
+        const float f = part_scale(ms[w][16 * b + li], mm);
+#pragma unroll
+        for (int c = 0; c < DPL; c++) o[b][c] *= f;
+    }
+    static_assert(NW == 4, "one round of the waves' outputs through LDS");
+#pragma unroll
+    for (int b = 0; b < QB; b++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int c = 0; c < DPL; c += 4)
+                *(f4 *)&os[w][16 * b + li][DPL * (4 * lg + r) + c] = f4{o[b][c][r], o[b][c + 1][r], o[b][c + 2][r], o[b][c + 3][r]};
+    __syncthreads();
+    const rsrc_t rp = make_rsrc(g.parts + (size_t)it.part_at * 4, it.n_parts > 1 ? (uint32_t)it.n_parts * ROWS * PARTF<HDP> * 4u : 0u);
+    for (int x = threadIdx.x; x < ROWS * (HDP / 4); x += 64 * NW) {
+        const int row = x / (HDP / 4), d = 4 * (x % (HDP / 4));
+        f4 v = *(const f4 *)&os[0][row][d];
+        float mm = ms[0][row];
+#pragma unroll
+        for (int u = 1; u < NW; u++) {
+            v += *(const f4 *)&os[u][row][d];
+            mm = fmaxf(mm, ms[u][row]);
+        }
+        float lt = 0.f;
+#pragma unroll
+        for (int u = 0; u < NW; u++) lt += ls[u][row] * part_scale(ms[u][row], mm);
+        if (it.n_parts == 1) {
+            finish(g, it, it.row0 + row, d, v, lt);
+        } else {
+            const uint32_t at = (uint32_t)((it.part * ROWS + row) * PARTF<HDP>) * 4u;
+            buf_store16(rp, v, at + (uint32_t)d * 4u);
+            if (d == 0) buf_store16(rp, f4{mm, lt, 0.f, 0.f}, at + HDP * 4u);
+        }
+    }
+    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last);
+}
+
+template <bool Q8>
+void launch(int body, int hd, const Args &g, unsigned grid, hipStream_t st) {
+#define HQ_ROWS(H, NW) k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g)
+#define HQ_STREAM(H, QB) k_stream<H, Q8, QB, 4><<<grid, 256, 0, st>>>(g)
+    const int p = hd <= 64 ? 0 : hd <= 96 ? 1 : hd <= 128 ? 2 : hd <= 192 ? 3 : 4;
+    switch (body * 5 + p) {
+    case 5 * HQ_STREAM16 + 0: HQ_STREAM(64, 1); break;
+    case 5 * HQ_STREAM16 + 1: case 5 * HQ_STREAM16 + 2: HQ_STREAM(128, 1); break;
+    case 5 * HQ_STREAM16 + 3: case 5 * HQ_STREAM16 + 4: HQ_STREAM(256, 1); break;
+    case 5 * HQ_STREAM32 + 0: HQ_STREAM(64, 2); break;
+    case 5 * HQ_STREAM32 + 1: case 5 * HQ_STREAM32 + 2: HQ_STREAM(128, 2); break;
+    case 5 * HQ_ROWS128 + 0: HQ_ROWS(64, 4); break;
+    case 5 * HQ_ROWS128 + 1: HQ_ROWS(96, 4); break;
+    case 5 * HQ_ROWS128 + 2: HQ_ROWS(128, 4); break;
+    case 5 * HQ_ROWS128 + 3: HQ_ROWS(192, 4); break;
+    case 5 * HQ_ROWS128 + 4: HQ_ROWS(256, 4); break;
+    case 5 * HQ_ROWS256 + 0: HQ_ROWS(64, 8); break;
+    case 5 * HQ_ROWS256 + 1: HQ_ROWS(96, 8); break;
+    case 5 * HQ_ROWS256 + 2: HQ_ROWS(128, 8); break;
+    default: break;
+    }
+#undef HQ_ROWS
+#undef HQ_STREAM
 }
 
 }  // namespace
+
+int hq_attn_part_floats(int hd) { return (hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : hd <= 192 ? 192 : 256) + 4; }
 
 extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_t *a, void *stream) {
     const char *const who = "hq_attention";
@@ -99,7 +713,7 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
     if (a->q_stride < 0 || a->q_stride > most || a->q_stride % 8 || a->out_stride < row || a->out_stride > most || a->out_stride % 8)
         return hq_internal_fail("%s: strides %lld and %lld (multiples of 8; out's at least a row's %lld)", who, (long long)a->q_stride,
                                 (long long)a->out_stride, (long long)row);
-    if (!isfinite(a->scale)) return hq_internal_fail("%s: scale %g", who, (double)a->scale);
+    if (!(fabsf(a->scale) <= 1e20f)) return hq_internal_fail("%s: scale %g", who, (double)a->scale);
     if (a->gate) {
         if ((uintptr_t)a->gate % (a->gate_f32 ? 16 : 8)) return hq_internal_fail("%s: the gate must be aligned to 4 elements", who);
         if (a->gate_stride < 0 || a->gate_stride > most || a->gate_stride % 4 || a->gate_head_stride < 0 || a->gate_head_stride > most || a->gate_head_stride % 4)
@@ -108,10 +722,16 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
     int cur = -1;
     SCK(hipGetDevice(&cur));
     if (cur != b->device) SCK(hipSetDevice(b->device));
-    const Args g = {*kv, *a, b->tok_pos, b->tok_seq, b->seqs, b->pages, b->n_heads, b->n_heads / kv->n_kv_heads};
-    const dim3 grid((unsigned)b->n_tokens, (unsigned)b->n_heads);
-    if (kv->type == HQ_KV_Q8) k_attn_paged<true><<<grid, 64, 0, (hipStream_t)stream>>>(g);
-    else k_attn_paged<false><<<grid, 64, 0, (hipStream_t)stream>>>(g);
-    SCK(hipGetLastError());
+    Args g = {*kv, *a, nullptr, b->pages, b->parts, b->counters, b->n_heads, b->n_heads / kv->n_kv_heads, __builtin_ctz((unsigned)kv->page_size), 0.f, 0.f};
+    // (a smaller scale leaves every weight alike in fp32; 0 would make NaN of masked scores)
+    g.sc = std::max(fabsf(a->scale) * 1.4426950408889634f, 1e-30f);
+    g.slack = 8.0f / g.sc;  // weights up to 2^8 keep their 11 bits in fp16
+    for (int body = 0; body < HQ_BODIES; body++) {
+        if (!b->n_items[body]) continue;
+        g.items = b->items[body];
+        if (kv->type == HQ_KV_Q8) launch<true>(body, kv->head_dim, g, (unsigned)b->n_items[body], (hipStream_t)stream);
+        else launch<false>(body, kv->head_dim, g, (unsigned)b->n_items[body], (hipStream_t)stream);
+        SCK(hipGetLastError());
+    }
     return 0;
 }

@@ -29,7 +29,8 @@ enum {
  * k[p * page_stride + s * pos_stride + h * head_stride + d] (and the same in v), so both usual orders of a page, positions
  * or heads outermost, are strides. Q8 scales stand at k_scale[(p * n_kv_heads + h) * page_size + s].
  * page_size: a power of two, 16 .. 4096; head_dim: a multiple of 16, at most 256; the strides: multiples of 16; k and v
- * 16-byte aligned. There is no limit on the cache's bytes; pages * page_size is below 2^31. */
+ * 16-byte aligned. There is no limit on the cache's bytes; pages * page_size is below 2^31, page_size * pos_stride below
+ * 2^30. */
 typedef struct {
     int type, page_size, n_kv_heads, head_dim;
     uint32_t n_pages;
@@ -96,7 +97,7 @@ int hq_rope_append(const hq_batch *b, const hq_kv_t *kv, const hq_rope_t *r, voi
 typedef struct {
     const uint16_t *q; /* fp16: head h of token t at q + t * q_stride + h * head_dim; 16-byte aligned, stride a multiple of 8 */
     int64_t q_stride;
-    float scale;       /* of the scores, 1 / sqrt(head_dim) as a rule; finite */
+    float scale;       /* of the scores, 1 / sqrt(head_dim) as a rule; at most 1e20 in magnitude */
     /* optional output gate, fp16 or fp32 (gate_f32): out = o * 1 / (1 + exp(-gate)); head h of token t at gate +
      * t * gate_stride + h * gate_head_stride, aligned to 4 elements, strides multiples of 4 */
     const void *gate;
