@@ -449,9 +449,10 @@ static int aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 namespace {
 struct Staging {  // slots: 0 x fp32, 1 x fp16, 2 y fp32 (hq_matmul_host), 3 embedding ids, 4 readout ids,
                   // 5 GEMM partial tiles, 6 GEMM tile counters (kept zero), 7 activation sub-block sums,
-                  // 8 fp32 gate/up product of the unfused hq_gemm_swiglu path
-    void *buf[9] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
-    size_t cap[9] = {0, 0, 0, 0, 0, 0, 0, 0, 0};
+                  // 8 fp32 gate/up product of the unfused hq_gemm_swiglu path,
+                  // 9 sums of split rows and 10 row counters (kept zero) of hq_logprobs
+    void *buf[11] = {};
+    size_t cap[11] = {};
 };
 std::mutex g_staging_mu;
 std::map<std::pair<int, void *>, Staging> g_staging;
@@ -503,6 +504,17 @@ int device_cus(int device, int *n_cu) {
     return 0;
 }
 
+}  // namespace
+
+extern "C" int hq_internal_device(int *device, int *n_cu) {
+    HIPCK(hipGetDevice(device));
+    return device_cus(*device, n_cu);
+}
+extern "C" int hq_internal_staging(int device, void *stream, int slot, size_t bytes, void **p, int *grew) {
+    return staging(device, stream, slot, bytes, p, grew);
+}
+
+namespace {
 // GEMM workspace of an M-row hq_gemm on W's device and `stream`. A counter array that grows is
 // zeroed once here, synchronously; the kernels leave every counter back at zero.
 int gemm_work(const hq_mat *W, int M, void *stream, HqGemmWork *wk, bool swiglu = false) {

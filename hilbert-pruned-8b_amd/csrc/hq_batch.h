@@ -23,8 +23,9 @@ struct HqItem {
 };
 // Kernel bodies of hq_attention by the rows a workgroup takes.
 enum { HQ_STREAM16, HQ_STREAM32, HQ_ROWS128, HQ_ROWS256, HQ_BODIES };
-// Floats of a part's row for a head_dim.
-int hq_attn_part_floats(int head_dim);
+// The dims that a body's kernel for a head_dim holds; a part's row has HQ_PART_EXTRA floats more.
+int hq_attn_width(int body, int head_dim);
+constexpr int HQ_PART_EXTRA = 4;
 
 struct hq_batch {
     int device, n_cu;

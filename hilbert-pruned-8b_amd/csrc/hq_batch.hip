@@ -111,7 +111,7 @@ void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const 
             if (n > 1) {
                 it.block = out->blocks++;
                 it.part_at = (uint32_t)out->part_units;
-                out->part_units += (uint64_t)n * rows_of[body] * hq_attn_part_floats(kv.head_dim) / 4;
+                out->part_units += (uint64_t)n * rows_of[body] * (hq_attn_width(body, kv.head_dim) + HQ_PART_EXTRA) / 4;
             }
             for (int p = 0; p < n; p++) {
                 it.part = p;

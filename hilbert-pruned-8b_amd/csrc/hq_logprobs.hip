@@ -1,13 +1,28 @@
 // hq_logprobs.hip - log probabilities of given tokens, entropy and likeliest tokens of rows of logits (hq_logprobs,
 // include/hq_serve.h).
+//
+// One pass over the logits: each thread keeps m = max x, s = sum e^(x - m) and t = sum (x - m) e^(x - m) of what it reads,
+// rescaled when m grows, so that log p = x - m - log s and the entropy is log s - t / s; both sums have one sign, nothing
+// cancels. Few rows are split over workgroups; the last of a row's to arrive joins their sums in part order.
+//
+// The top k come from the same pass: the k-th largest of the threads' maxima, B, is no larger than the k-th largest logit, so
+// only the threads' shares whose maximum reaches B are read again (k of 512 or more, from cache), and the few logits found
+// there are ranked by counting. No share is sorted and nothing is inserted anywhere in the stream.
+//
+// Bound: the bytes of the logits; for few rows the chain of launch, loads, the row's last workgroup and its second look.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <math.h>
 
 #include "hq_batch.h"
 #include "hq_device.h"
 
 namespace {
+
+constexpr int NT = 512, WAVES = NT / 64;
+constexpr int MAX_BUCKETS = 256;   // shares of a row that the second look chooses from
+constexpr int FOUND = 1024, TIES = 256;
 
 struct LpArgs {
     const void *x;
@@ -17,12 +32,11 @@ struct LpArgs {
     int64_t stride;
     uint32_t V;
     int n_ids, k;
+    int parts, group;  // workgroups per row; neighbouring threads whose maxima make one bucket
+    uint32_t per;      // 16-byte pieces per part
+    float *work;       // [rows][parts][4 + NT / group]: m, s, t, -, then the buckets
+    int *counters;     // [rows], zero when idle
 };
-
-template <bool F32>
-DEV float logit(const void *x, size_t at) {
-    return F32 ? ((const float *)x)[at] : (float)((const _Float16 *)x)[at];
-}
 
 // Logits as unsigned integers in their order: every NaN above +inf, -0 as +0; with the token below them, lower tokens
 // first, one 64-bit key orders candidates.
@@ -35,70 +49,284 @@ DEV float from_order(uint32_t o) {
     if (o == 0xffffffffu) return NAN;
     return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-DEV uint64_t key_of(float x, uint32_t at) { return (uint64_t)order_of(x) << 32 | (uint32_t)~at; }
 
-// log p of a logit x in a row of maximum m and sum of e^(x - m) = s
+// log p of a logit x in a row of maximum m and sum of e^(x - m) = e^logs
 DEV float log_p(float x, float m, float logs) {
-    if (m == -INFINITY) return -INFINITY;
+    if (m == -INFINITY && logs == -INFINITY) return -INFINITY;
     return (x - m) - logs;
 }
 
-template <class T, class F>
-DEV T block_reduce(T v, T *red, F f) {
+constexpr float LOG2E = 1.4426950408889634f;
+DEV float ex(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }  // e^d
+
+struct Sums {
+    float m, s, t;
+    // to a maximum of mn >= m (differences past 1e30 weigh 0 and must not make NaN of t)
+    __device__ __forceinline__ void raise(float mn) {
+        const float f = m == -INFINITY ? 0.f : ex(m - mn);
+        t = m == -INFINITY ? 0.f : (t + fmaxf(m - mn, -1e30f) * s) * f;
+        s = m == -INFINITY ? s : s * f;
+        m = mn;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        const float mn = fmaxf(m, o.m);
+        raise(mn), o.raise(mn);
+        s += o.s, t += o.t;
+    }
+};
+
+template <bool F32>
+constexpr int VEC = F32 ? 4 : 8;  // logits of a 16-byte piece
+
+// Piece v of a row whose first logit is `mis` logits into piece 0: its values, -inf outside the row.
+template <bool F32>
+DEV void piece(const char *base, uint32_t v, uint32_t n_pieces, uint32_t mis, uint32_t V, float (&x)[VEC<F32>]) {
+    const u4v w = *(const u4v *)(base + (size_t)v * 16);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = f(v, (T)__shfl_xor(v, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return f(f(red[0], red[1]), f(red[2], red[3]));
+    for (int e = 0; e < VEC<F32>; e++) x[e] = F32 ? __builtin_bit_cast(float, (uint32_t)w[e % 4]) : h2f((uint16_t)(w[e / 2 % 4] >> (16 * (e % 2))));
+    if (v == 0 || v + 1 == n_pieces) {
+#pragma unroll
+        for (int e = 0; e < VEC<F32>; e++)
+            if (v * VEC<F32> + e - mis >= V) x[e] = -INFINITY;  // (unsigned: before the row too)
+    }
 }
 
-// One workgroup per row: the maximum, the sums, then each of the top tokens by a pass over the row.
+struct Shared {
+    Sums sums[WAVES];
+    uint32_t bucket[MAX_BUCKETS];
+    unsigned long long found[FOUND + TIES], out[64];
+    int n_found, n_ties, n_cand, last, count[WAVES];
+};
+
 template <bool F32>
-__global__ void __launch_bounds__(256) k_logprobs(LpArgs g) {
-    __shared__ float red[4];
-    __shared__ unsigned long long rk[4];
-    const size_t row = blockIdx.x, at = row * (size_t)g.stride;
-    const auto add = [](float a, float b) { return a + b; };
-    float m = -INFINITY, nan = 0.f;
-    for (uint32_t i = threadIdx.x; i < g.V; i += 256) {
-        const float x = logit<F32>(g.x, at + i);
-        m = fmaxf(m, x);
-        if (x != x) nan = x;
+struct Row {
+    const LpArgs &g;
+    const char *base;
+    uint32_t mis, n_pieces;
+    __device__ __forceinline__ float at(uint32_t i) const {
+        const size_t a = (size_t)mis + i;
+        return F32 ? ((const float *)base)[a] : (float)((const _Float16 *)base)[a];
     }
-    m = block_reduce(m, red, [](float a, float b) { return fmaxf(a, b); });
-    nan = block_reduce(nan, red, add);
-    float s = 0.f, t = 0.f;
-    if (m != -INFINITY)
-        for (uint32_t i = threadIdx.x; i < g.V; i += 256) {
-            const float d = logit<F32>(g.x, at + i) - m, e = expf(d);
-            s += e;
-            if (d != -INFINITY) t += d * e;
+    // f(order, token) of every logit that bucket b's threads read, by thread `tid` of `n`
+    template <class F>
+    __device__ __forceinline__ void bucket(int b, int tid, int n, F f) const {
+        const int per = NT / g.group, p = b / per, t0 = (b % per) * g.group;
+        const uint32_t v0 = (uint32_t)p * g.per, v1 = std::min(v0 + g.per, n_pieces);
+        for (uint32_t j = tid;; j += n) {
+            const uint32_t v = v0 + j / g.group * NT + t0 + j % g.group;
+            if (v0 + j / g.group * NT >= v1) break;
+            if (v >= v1) continue;
+            float x[VEC<F32>];
+            piece<F32>(base, v, n_pieces, mis, g.V, x);
+#pragma unroll
+            for (int e = 0; e < VEC<F32>; e++) {
+                const uint32_t i = v * VEC<F32> + e - mis;
+                if (i < g.V) f(order_of(x[e]), i);
+            }
         }
-    s = block_reduce(s, red, add);
-    t = block_reduce(t, red, add);
-    const float bad = nan + (m == INFINITY ? NAN : 0.f), logs = logf(s);
-    if (g.entropy && threadIdx.x == 0) g.entropy[row] = bad + (m == -INFINITY ? 0.f : logs - t / s);
+    }
+    // how many logits of the row are at least `o` in order (whole workgroup)
+    __device__ __forceinline__ int count_from(uint32_t o, Shared &sh) const {
+        int c = 0;
+        for (uint32_t i = threadIdx.x; i < g.V; i += NT) c += order_of(at(i)) >= o;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) c += __shfl_xor(c, d, 64);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = c;
+        __syncthreads();
+        c = 0;
+        for (int w = 0; w < WAVES; w++) c += sh.count[w];
+        return c;
+    }
+};
+
+// Largest B that at least k of the first n words of v reach (0 where there are fewer); every wave for itself.
+DEV uint32_t kth_largest(const uint32_t *v, int n, int k) {
+    uint32_t x[MAX_BUCKETS / 64];
+#pragma unroll
+    for (int i = 0; i < MAX_BUCKETS / 64; i++) {
+        const int at = 64 * i + (threadIdx.x & 63);
+        x[i] = at < n ? v[at] : 0u;
+    }
+    uint32_t b = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t mid = b | 1u << bit;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < MAX_BUCKETS / 64; i++)
+            if (64 * i < n) c += __popcll(__ballot(x[i] >= mid));
+        if (c >= k) b = mid;
+    }
+    return b;
+}
+
+// The row's top k to sh.out as keys, likeliest first: buckets (n of them) hold the orders of their maxima; odd: the row has
+// a NaN or +inf, whose buckets say nothing.
+template <bool F32>
+DEV void top_k(const Row<F32> &row, int n, bool odd, Shared &sh) {
+    const int k = row.g.k, tid = threadIdx.x;
+    uint32_t B = 0;
+    bool exact = odd;
+    if (!odd) B = kth_largest(sh.bucket, n, k);
+    for (;;) {
+        if (exact) {  // B: the k-th largest logit itself
+            B = 0;
+            for (int bit = 31; bit >= 0; bit--)
+                if (row.count_from(B | 1u << bit, sh) >= k) B |= 1u << bit;
+        }
+        __syncthreads();
+        if (tid == 0) sh.n_found = sh.n_ties = 0;
+        __syncthreads();
+        const auto take = [&](uint32_t o, uint32_t i) {
+            if (o < B) return;
+            const unsigned long long key = (unsigned long long)o << 32 | (uint32_t)~i;
+            if (o > B) {
+                const int at = atomicAdd(&sh.n_found, 1);
+                if (at < FOUND) sh.found[at] = key;
+            } else {
+                const int at = atomicAdd(&sh.n_ties, 1);
+                if (at < TIES) sh.found[FOUND + at] = key;
+            }
+        };
+        // a wave takes a bucket at a time
+        for (int b = tid >> 6; b < n; b += WAVES)
+            if (odd || sh.bucket[b] >= B) row.bucket(b, tid & 63, 64, take);
+        __syncthreads();
+        if (sh.n_found <= FOUND) break;
+        exact = true;  // more than FOUND logits pass the buckets' bound (a sorted row): fewer than k pass the exact one
+    }
+    int nf = sh.n_found;
+    if (nf < k && sh.n_ties > TIES) {
+        // the first k - nf logits that equal B, in the order of tokens
+        const int need = k - nf;
+        int have = 0;
+        for (uint32_t i0 = 0; i0 < row.g.V && have < need; i0 += NT) {
+            const uint32_t i = i0 + tid;
+            const bool tie = i < row.g.V && order_of(row.at(i)) == B;
+            const uint64_t mask = __ballot(tie);
+            __syncthreads();
+            if ((tid & 63) == 0) sh.count[tid >> 6] = __popcll(mask);
+            __syncthreads();
+            int at = have + __popcll(mask & ((1ull << (tid & 63)) - 1));
+            for (int w = 0; w < WAVES; w++) {
+                if (w < tid >> 6) at += sh.count[w];
+                have += sh.count[w];
+            }
+            if (tie && at < need) sh.found[FOUND + at] = (unsigned long long)B << 32 | (uint32_t)~i;
+        }
+        __syncthreads();
+        if (tid == 0) sh.n_ties = std::min(have, need);
+        __syncthreads();
+    }
+    const int nt = nf < k ? std::min(sh.n_ties, TIES) : 0, all = nf + nt;
+    for (int x = tid; x < all; x += NT) {
+        const unsigned long long key = sh.found[x < nf ? x : FOUND + x - nf];
+        int rank = 0;
+        for (int y = 0; y < nf; y++) rank += sh.found[y] > key;
+        for (int y = 0; y < nt; y++) rank += sh.found[FOUND + y] > key;
+        if (rank < k) sh.out[rank] = key;
+    }
+    __syncthreads();
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
+    __shared__ Shared sh;
+    constexpr int U = F32 ? 4 : 2;  // pieces in flight per thread: 16 logits
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const size_t r = blockIdx.x / g.parts;
+    const int part = blockIdx.x % g.parts;
+    const char *const start = (const char *)g.x + r * (size_t)g.stride * (F32 ? 4 : 2);
+    const uint32_t mis = (uint32_t)((uintptr_t)start & 15u) / (F32 ? 4 : 2);
+    const Row<F32> row = {g, start - ((uintptr_t)start & 15u), mis, (mis + g.V + VEC<F32> - 1) / VEC<F32>};
+    const uint32_t v0 = (uint32_t)part * g.per, v1 = std::min(v0 + g.per, row.n_pieces);
+    Sums a = {-INFINITY, 0.f, 0.f};
+    for (uint32_t v = v0 + tid; v < v1; v += U * NT) {
+        float x[U][VEC<F32>];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (v + u * NT < v1) piece<F32>(row.base, v + u * NT, row.n_pieces, mis, g.V, x[u]);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC<F32>; e++) x[u][e] = -INFINITY;
+        }
+        float mn = a.m;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < VEC<F32>; e++) mn = fmaxf(mn, x[u][e]);
+        a.raise(mn);
+        const float m0 = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < VEC<F32>; e++) {
+                const float d = x[u][e] - m0, p = ex(d);
+                a.s += p;
+                a.t = fmaf(fmaxf(d, -1e30f), p, a.t);
+            }
+    }
+    const bool want_top = g.top_ids || g.top_logp;
+    const int per = NT / g.group;
+    uint32_t big = 0;
+    if (want_top) {
+        float mx = a.m;
+        for (int o = 1; o < g.group; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+        big = order_of(mx);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) a.add({__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)});
+    if (lane == 0) sh.sums[w] = a;
+    __syncthreads();
+    a = sh.sums[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; i++) a.add(sh.sums[i]);
+    if (g.parts > 1) {
+        const uint32_t each = 4 + per;
+        const rsrc_t rp = make_rsrc(g.work + r * (size_t)g.parts * each, (uint32_t)g.parts * each * 4u);
+        if (tid == 0) buf_store16(rp, f4{a.m, a.s, a.t, 0.f}, (uint32_t)part * each * 4u);
+        if (want_top && tid % g.group == 0)
+            __builtin_amdgcn_raw_buffer_store_b32(big, rp, ((uint32_t)part * each + 4 + tid / g.group) * 4u, 0u, CPOL_SC1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            sh.last = atomicAdd(&g.counters[r], 1) == g.parts - 1;
+            if (sh.last) atomicExch(&g.counters[r], 0);
+        }
+        __syncthreads();
+        if (!sh.last) return;
+        a = {-INFINITY, 0.f, 0.f};
+        for (int p = 0; p < g.parts; p++) {
+            const f4 o = buf_load16_sc1(rp, (uint32_t)p * each * 4u, 0);
+            a.add({o.x, o.y, o.z});
+        }
+        if (want_top)
+            for (int b = tid; b < g.parts * per; b += NT)
+                sh.bucket[b] = __builtin_amdgcn_raw_buffer_load_b32(rp, ((uint32_t)(b / per) * each + 4 + b % per) * 4u, 0u, CPOL_SC1);
+    } else if (want_top && tid % g.group == 0) {
+        sh.bucket[tid / g.group] = big;
+    }
+    // m = +inf: e^(inf - inf) made s NaN; a NaN did too. Nothing but -inf: s = 0, its log -inf.
+    const float logs = logf(a.s);
+    const bool nothing = a.m == -INFINITY && a.s == 0.f;
+    if (g.entropy && tid == 0) g.entropy[r] = nothing ? 0.f : logs - a.t / a.s;
     if (g.logp)
-        for (int j = threadIdx.x; j < g.n_ids; j += 256) {
-            const uint32_t id = g.ids[row * g.n_ids + j];
-            g.logp[row * g.n_ids + j] = id < g.V ? bad + log_p(logit<F32>(g.x, at + id), m, logs) : NAN;
+        for (int j = tid; j < g.n_ids; j += NT) {
+            const uint32_t id = g.ids[r * g.n_ids + j];
+            g.logp[r * g.n_ids + j] = id < g.V ? log_p(row.at(id), a.m, logs) : NAN;
         }
-    if (!g.top_ids && !g.top_logp) return;
-    unsigned long long below = ~0ull;
-    for (int j = 0; j < g.k; j++) {
-        unsigned long long best = 0;
-        for (uint32_t i = threadIdx.x; i < g.V; i += 256) {
-            const unsigned long long key = key_of(logit<F32>(g.x, at + i), i);
-            if (key < below && key > best) best = key;
-        }
-        best = block_reduce(best, rk, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-        below = best;
-        if (threadIdx.x == 0) {
-            if (g.top_ids) g.top_ids[row * g.k + j] = ~(uint32_t)best;
-            if (g.top_logp) g.top_logp[row * g.k + j] = bad + log_p(from_order((uint32_t)(best >> 32)), m, logs);
-        }
+    if (!want_top) return;
+    __syncthreads();
+    top_k<F32>(row, g.parts * per, !(a.s >= 0.f), sh);
+    for (int j = tid; j < g.k; j += NT) {
+        const unsigned long long key = sh.out[j];
+        if (g.top_ids) g.top_ids[r * g.k + j] = ~(uint32_t)key;
+        if (g.top_logp) g.top_logp[r * g.k + j] = log_p(from_order((uint32_t)(key >> 32)), a.m, logs);
     }
+}
+
+__global__ void k_zero(int *p, int n) {
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0;
 }
 
 }  // namespace
@@ -116,9 +344,31 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
     if (n_ids == 0) logp = nullptr;
     if (top_k == 0) top_ids = nullptr, top_logp = nullptr;
     if (!logp && !entropy && !top_ids && !top_logp) return 0;
-    const LpArgs g = {logits, ids, logp, entropy, top_logp, top_ids, stride, V, n_ids, top_k};
-    if (f32) k_logprobs<true><<<(unsigned)M, 256, 0, (hipStream_t)stream>>>(g);
-    else k_logprobs<false><<<(unsigned)M, 256, 0, (hipStream_t)stream>>>(g);
+    LpArgs g = {logits, ids, logp, entropy, top_logp, top_ids, stride, V, n_ids, top_k, 1, 1, 0, nullptr, nullptr};
+    // Few rows: parts of at least 512 threads x 4 pieces, while the chip has workgroups to spare (two per CU). Buckets stay
+    // within MAX_BUCKETS: more parts, more threads to a bucket.
+    int device, n_cu;
+    if (hq_internal_device(&device, &n_cu)) return -1;
+    const uint32_t pieces = (V + (f32 ? 3u : 7u)) / (f32 ? 4u : 8u) + 1;
+    g.parts = (int)std::max(1u, std::min({2u * (uint32_t)n_cu / (uint32_t)M, pieces / (NT * 4), (uint32_t)MAX_BUCKETS / 8}));
+    while (g.parts * (NT / g.group) > MAX_BUCKETS) g.group *= 2;
+    g.per = (pieces + (uint32_t)g.parts - 1) / (uint32_t)g.parts;
+    if (g.parts > 1) {
+        const size_t each = 4 + NT / (size_t)g.group, sums = (size_t)M * g.parts * each * 4;
+        void *work, *cnt;
+        int grew;
+        if (hq_internal_staging(device, stream, HQ_STAGE_LOGPROBS, sums, &work, &grew) ||
+            hq_internal_staging(device, stream, HQ_STAGE_LOGPROBS_COUNT, (size_t)M * 4, &cnt, &grew))
+            return -1;
+        if (grew) {
+            k_zero<<<1, 256, 0, (hipStream_t)stream>>>((int *)cnt, M);
+            SCK(hipGetLastError());
+        }
+        g.work = (float *)work, g.counters = (int *)cnt;
+    }
+    const unsigned grid = (unsigned)M * (unsigned)g.parts;
+    if (f32) k_logprobs<true><<<grid, NT, 0, (hipStream_t)stream>>>(g);
+    else k_logprobs<false><<<grid, NT, 0, (hipStream_t)stream>>>(g);
     SCK(hipGetLastError());
     return 0;
 }

@@ -9,8 +9,10 @@
 // every lane and positions in its registers, which is the B operand of O^T = V^T P^T. Both run the online softmax: a running
 // maximum and sum per row, outputs scaled when the maximum grows.
 //
-// Precision: fp16 operands, fp32 products, sums, maxima and outputs. Rounded to 16 bits are the weights p (2^-11 of each;
-// the sum takes them unrounded) and, of a Q8 cache, the decoded values (2^-11; scores of k_stream meet the exact codes).
+// Precision: fp16 operands, fp32 products, sums, maxima and outputs. Rounded to 16 bits are the weights p alone (2^-11 of each;
+// the sum takes them unrounded). Of a Q8 cache the operands are exact: keys enter as their codes and the scores take the
+// scale in fp32; values enter as code * 2^e, the scale's power of two (exact down to fp16's last bit), and its mantissa
+// joins the weight before that is rounded. Decoding to fp16 instead doubled the error of the outputs (2.1e-4 -> 4.8e-4).
 //
 // Places that a row does not see weigh 0, and 0 times an infinity or NaN would be NaN: in a tile that some row sees only part
 // of, values that are not finite (`odd` below) enter the product as 0, and are added to the outputs of the rows that do see
@@ -37,7 +39,7 @@ struct Args {
     float *parts;
     int *counters;
     int nh, rep, shift;  // shift: log2 of the page size
-    float sc, slack;     // |scale| log2(e); how far (in raw scores) a maximum may grow before the outputs are rescaled
+    float sc, slack;     // |scale| log2(e); how far a maximum may grow before the outputs are rescaled (raw scores; Q8: in log2 units)
 };
 
 DEV f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -86,7 +88,14 @@ DEV h2 codes2(uint32_t w) {
     const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
     return as_h2(w) - bias;
 }
-// 16 codes times their position's scale: one rounding to fp16
+// A value scale as a power of two (the scale itself where it is not finite) and what remains, fp32 in [1, 2), below 1 for
+// scales under fp16's normal range; 1 where it is not finite.
+DEV uint32_t pow2_of(uint32_t d) { return (d & 0x7c00u) == 0x7c00u ? d : (d & 0x7c00u) < 0x400u ? 0x400u : d & 0x7c00u; }
+DEV float rest_of(uint32_t d) {
+    const uint32_t inverse = 0x7f000000u - __builtin_bit_cast(uint32_t, h2f((uint16_t)pow2_of(d)));  // of 2^k: 2^-k
+    return (d & 0x7c00u) == 0x7c00u ? 1.f : h2f((uint16_t)d) * __builtin_bit_cast(float, inverse);
+}
+// 16 codes times d: a power of two, or 1
 DEV void decode16(u4v c, _Float16 d, h8 &lo, h8 &hi) {
     const h2 dd = {d, d};
     h2 o[8];
@@ -129,7 +138,7 @@ DEV void finish(const Args &g, const HqItem &it, int r, int d, f4 v, float l) {
 // A part's row: its sums [HDP], then (maximum in log2 units, sum). Parts are written and read at device scope; the last of
 // a block's items to arrive adds them in part order, so the result does not depend on the order of arrival.
 template <int HDP>
-constexpr int PARTF = HDP + 4;
+constexpr int PARTF = HDP + HQ_PART_EXTRA;
 
 template <int HDP, int ROWS, int NT>
 DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
@@ -194,6 +203,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     static_assert(RPI <= 16 && NI * NW == 2 * UNITS, "whole loads per wave, each in one page");
     __shared__ __align__(1024) char lds[4 * TILE];
     __shared__ int flags[2], last;
+    __shared__ __align__(16) float fac[Q8 ? 4 * T : 4];  // Q8, two tiles: what the scores of a position take (key scale, score scale), and its weight
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hf = lane >> 5;
@@ -253,8 +263,11 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             const bool look = s0 + T > n_blk && w * NI + i >= UNITS;
             if (Q8) {
                 h8 lo, hi;
-                decode16(st[i], sd[i], lo, hi);
+                const bool val = w * NI + i >= UNITS;
+                const uint32_t db = __builtin_bit_cast(uint16_t, sd[i]);
+                decode16(st[i], val ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(db)) : (_Float16)1.f, lo, hi);
                 if (!on) lo = hi = h8{};
+                if (piece == 0) fac[(2 * buf + val) * T + RPI * ((w * NI + i) % UNITS) + lrow] = val ? rest_of(db) : (float)sd[i] * g.sc;
                 if (look && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi)))) lo = finite8(lo), hi = finite8(hi), flags[buf] = s0;
                 *(h8 *)(to + wat[i]) = lo;
                 *(h8 *)(to + (wat[i] ^ 16)) = hi;
@@ -266,7 +279,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         }
     };
 
-    float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores), what the exponents are taken against, the sum
+    float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores; Q8: in log2 units), what the exponents are taken against, the sum
     f16v o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -300,6 +313,16 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int b = 0; b < KB; b++) s[b] = mfma32(*(const h8 *)(tile + ((kx ^ (32u * j)) + 32 * P * b)), q[j], s[b]);
+            if (Q8) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const f4 f = *(const f4 *)&fac[2 * buf * T + 32 * b + 8 * c + 4 * hf];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[b][4 * c + e] *= f[e];
+                    }
+            }
             if (s0 + T > wn_all) {
 #pragma unroll
                 for (int b = 0; b < KB; b++)
@@ -312,7 +335,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][e]);
             if (__any(mx > m + g.slack)) {
-                const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : mn * g.sc;
+                const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
                 const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
                 m = mn, mref = nref;
                 l *= a;
@@ -326,10 +349,16 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
             for (int b = 0; b < KB; b++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float x = ex2(fmaf(s[b][e], g.sc, -mref));
-                    add += x;
-                    p[2 * b + (e >> 3)][e & 7] = (_Float16)x;
+                for (int c = 0; c < 4; c++) {
+                    f4 f;
+                    if (Q8) f = *(const f4 *)&fac[(2 * buf + 1) * T + 32 * b + 8 * c + 4 * hf];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int e = 4 * c + i;
+                        const float x = ex2(Q8 ? s[b][e] - mref : fmaf(s[b][e], g.sc, -mref));
+                        add += x;
+                        p[2 * b + (e >> 3)][e & 7] = (_Float16)(Q8 ? x * f[i] : x);
+                    }
                 }
             l += add;
             auto operand = [&](int d, int k) {
@@ -349,7 +378,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
                 for (int at = s0; at < std::min(s0 + T, wn); at++) {
                     const uint32_t page = *page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
                     const char *const v = vb0 + ((size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
-                    const _Float16 d8 = Q8 ? ((const _Float16 *)g.kv.v_scale)[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in] : (_Float16)0.f;
+                    const _Float16 d8 = Q8 ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in])) : (_Float16)0.f;
 #pragma unroll
                     for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -433,7 +462,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 
     u4v kf[2][KL];
     uint32_t vf[2][4][VW];
-    u2v ksc[2], vsc[2];
+    u2v ksc[2], vsc[2], pow2[2];
     uint32_t pgk[2], pgn[2];  // pages of the tile whose keys are loaded next, of the one whose values are
     auto fetch = [&](int s0, uint32_t (&pg)[2]) {
 #pragma unroll
@@ -519,7 +548,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
             for (int p = 0; p < 2; p++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float d = h2f((uint16_t)(ksc[p][r / 2] >> (16 * (r % 2))));
+                    const float d = h2f((uint16_t)(ksc[p][r / 2] >> (16 * (r % 2)))) * g.sc;
 #pragma unroll
                     for (int b = 0; b < QB; b++) s[b][p][r] *= d;
                 }
@@ -532,6 +561,17 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (s0 + 16 * p + 4 * lg + r >= n) vsc[p][r / 2] &= r % 2 ? 0x0000ffffu : 0xffff0000u;
+        }
+        float rest[2][4];
+        if (Q8) {
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t d = vsc[p][r / 2] >> (16 * (r % 2)) & 0xffffu;
+                    rest[p][r] = rest_of(d);
+                    pow2[p][r / 2] = r % 2 ? pow2[p][r / 2] | pow2_of(d) << 16 : pow2_of(d);
+                }
         }
         h8 pr[QB];
 #pragma unroll
@@ -547,7 +587,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[b][p][r]);
             if (__any(mx > m[b] + g.slack)) {
-                const float mn = fmaxf(m[b], max_lg(mx)), nref = mn == -INFINITY ? 0.f : mn * g.sc;
+                const float mn = fmaxf(m[b], max_lg(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
                 const float a = m[b] == -INFINITY ? 0.f : ex2(mref[b] - nref);
                 m[b] = mn, mref[b] = nref;
                 l[b] *= a;
@@ -558,9 +598,9 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
             for (int p = 0; p < 2; p++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float x = ex2(fmaf(s[b][p][r], g.sc, -mref[b]));
+                    const float x = ex2(Q8 ? s[b][p][r] - mref[b] : fmaf(s[b][p][r], g.sc, -mref[b]));
                     l[b] += x;
-                    pr[b][4 * p + r] = (_Float16)x;
+                    pr[b][4 * p + r] = (_Float16)(Q8 ? x * rest[p][r] : x);
                 }
         }
         // operand of block c: dim DPL li + c of the eight positions
@@ -573,7 +613,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
                     // byte c of two positions' words
                     const uint32_t sel = 0x0c000c00u | (uint32_t)((c & 3) + 4) << 16 | (uint32_t)(c & 3);
                     const uint32_t y = __builtin_amdgcn_perm(vf[p][r + 1][c / 4] ^ 0x80808080u, vf[p][r][c / 4] ^ 0x80808080u, sel) | 0x64006400u;
-                    x[k] = __builtin_bit_cast(uint32_t, codes2(y) * as_h2(vsc[p][r / 2]));
+                    x[k] = __builtin_bit_cast(uint32_t, codes2(y) * as_h2(pow2[p][r / 2]));
                 } else {
                     x[k] = __builtin_amdgcn_perm(vf[p][r + 1][c / 2], vf[p][r][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
                 }
@@ -673,33 +713,38 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 }
 
 template <bool Q8>
-void launch(int body, int hd, const Args &g, unsigned grid, hipStream_t st) {
-#define HQ_ROWS(H, NW) k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g)
-#define HQ_STREAM(H, QB) k_stream<H, Q8, QB, 4><<<grid, 256, 0, st>>>(g)
-    const int p = hd <= 64 ? 0 : hd <= 96 ? 1 : hd <= 128 ? 2 : hd <= 192 ? 3 : 4;
-    switch (body * 5 + p) {
-    case 5 * HQ_STREAM16 + 0: HQ_STREAM(64, 1); break;
-    case 5 * HQ_STREAM16 + 1: case 5 * HQ_STREAM16 + 2: HQ_STREAM(128, 1); break;
-    case 5 * HQ_STREAM16 + 3: case 5 * HQ_STREAM16 + 4: HQ_STREAM(256, 1); break;
-    case 5 * HQ_STREAM32 + 0: HQ_STREAM(64, 2); break;
-    case 5 * HQ_STREAM32 + 1: case 5 * HQ_STREAM32 + 2: HQ_STREAM(128, 2); break;
-    case 5 * HQ_ROWS128 + 0: HQ_ROWS(64, 4); break;
-    case 5 * HQ_ROWS128 + 1: HQ_ROWS(96, 4); break;
-    case 5 * HQ_ROWS128 + 2: HQ_ROWS(128, 4); break;
-    case 5 * HQ_ROWS128 + 3: HQ_ROWS(192, 4); break;
-    case 5 * HQ_ROWS128 + 4: HQ_ROWS(256, 4); break;
-    case 5 * HQ_ROWS256 + 0: HQ_ROWS(64, 8); break;
-    case 5 * HQ_ROWS256 + 1: HQ_ROWS(96, 8); break;
-    case 5 * HQ_ROWS256 + 2: HQ_ROWS(128, 8); break;
-    default: break;
+hipError_t launch(int body, int width, const Args &g, unsigned grid, hipStream_t st) {
+#define HQ_ROWS(B, H, NW) case B + H: k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g); break
+#define HQ_STREAM(B, H, QB) case B + H: k_stream<H, Q8, QB, 4><<<grid, 256, 0, st>>>(g); break
+    constexpr int B0 = 1000 * HQ_STREAM16, B1 = 1000 * HQ_STREAM32, B2 = 1000 * HQ_ROWS128, B3 = 1000 * HQ_ROWS256;
+    switch (1000 * body + width) {
+        HQ_STREAM(B0, 64, 1);
+        HQ_STREAM(B0, 128, 1);
+        HQ_STREAM(B0, 256, 1);
+        HQ_STREAM(B1, 64, 2);
+        HQ_STREAM(B1, 128, 2);
+        HQ_ROWS(B2, 64, 4);
+        HQ_ROWS(B2, 96, 4);
+        HQ_ROWS(B2, 128, 4);
+        HQ_ROWS(B2, 192, 4);
+        HQ_ROWS(B2, 256, 4);
+        HQ_ROWS(B3, 64, 8);
+        HQ_ROWS(B3, 96, 8);
+        HQ_ROWS(B3, 128, 8);
+    default: return hipErrorInvalidValue;
     }
 #undef HQ_ROWS
 #undef HQ_STREAM
+    return hipGetLastError();
 }
 
 }  // namespace
 
-int hq_attn_part_floats(int hd) { return (hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : hd <= 192 ? 192 : 256) + 4; }
+// (a part's row is PARTF<width> floats: its size in the plan and in the kernels comes from this one rule)
+int hq_attn_width(int body, int hd) {
+    if (body == HQ_STREAM16 || body == HQ_STREAM32) return hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    return hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : hd <= 192 ? 192 : 256;
+}
 
 extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_t *a, void *stream) {
     const char *const who = "hq_attention";
@@ -725,13 +770,12 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
     Args g = {*kv, *a, nullptr, b->pages, b->parts, b->counters, b->n_heads, b->n_heads / kv->n_kv_heads, __builtin_ctz((unsigned)kv->page_size), 0.f, 0.f};
     // (a smaller scale leaves every weight alike in fp32; 0 would make NaN of masked scores)
     g.sc = std::max(fabsf(a->scale) * 1.4426950408889634f, 1e-30f);
-    g.slack = 8.0f / g.sc;  // weights up to 2^8 keep their 11 bits in fp16
+    g.slack = kv->type == HQ_KV_Q8 ? 8.0f : 8.0f / g.sc;  // weights up to 2^8 (2^9 with a value scale's mantissa) keep their 11 bits in fp16
     for (int body = 0; body < HQ_BODIES; body++) {
         if (!b->n_items[body]) continue;
         g.items = b->items[body];
-        if (kv->type == HQ_KV_Q8) launch<true>(body, kv->head_dim, g, (unsigned)b->n_items[body], (hipStream_t)stream);
-        else launch<false>(body, kv->head_dim, g, (unsigned)b->n_items[body], (hipStream_t)stream);
-        SCK(hipGetLastError());
+        const int width = hq_attn_width(body, kv->head_dim);
+        SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, g, (unsigned)b->n_items[body], (hipStream_t)stream));
     }
     return 0;
 }

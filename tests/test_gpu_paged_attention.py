@@ -74,6 +74,21 @@ def test_attention(hqlib, nh, nkv, hd, page, layout, lens, q8):
     check(got, *attention(pool, q, n_new, n_pos, hd ** -0.5))
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("hd", [16, 48, 64, 80, 96, 112, 128, 160, 192, 256])
+def test_blocks_cut_into_parts(hqlib, hd, q8):
+    """Long sequences with few rows, whose positions go to several workgroups: rows of 16, of 32, of 128 and 256, every
+    width of the kernels; a part's rows must fit the workspace that the plan gave them."""
+    rng = np.random.default_rng(hd)
+    for nh, lens in ((1, [(1, 4000), (20, 3500)]), (2, [(1, 9), (1, 6000), (1, 33), (40, 3000)]), (4, [(130, 2048)])):
+        pool = Pool(rng, [t for _, t in lens], 64, 1, hd, q8)
+        fill(pool, rng, [t for _, t in lens])
+        q = rng.normal(0, 1.5, (sum(a for a, _ in lens), nh, hd)).astype(np.float16)
+        print(f"[gpu] parts: {nh} heads x {hd} {lens} q8={q8}", flush=True)
+        got = run(hqlib, pool, nh, lens, q, hd ** -0.5)
+        check(got, *attention(pool, q, [a for a, _ in lens], [t for _, t in lens], hd ** -0.5))
+
+
 @pytest.mark.parametrize("gate_f32", [False, True])
 @pytest.mark.parametrize("q8", [False, True])
 def test_gate_strides_and_stream(hqlib, q8, gate_f32):
