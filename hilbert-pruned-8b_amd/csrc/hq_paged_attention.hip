@@ -178,7 +178,9 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
     }
 }
 
-DEV const uint32_t *page_of(const Args &g, const HqItem &it, int p) { return g.pages + it.page0 + (p >> g.shift); }
+// (through the scalar cache: p is the same in every lane; the table does not change while a kernel runs)
+typedef const __attribute__((address_space(4))) uint32_t const_u32;
+DEV uint32_t page_of(const Args &g, const HqItem &it, int p) { return ((const_u32 *)(uintptr_t)g.pages)[it.page0 + (p >> g.shift)]; }
 
 // ------------------------------------------------------------------------------------ rows
 // Row pitch of an LDS tile and the XOR of its 16-byte pieces: 16 rows that follow each other put a piece on 16 different
@@ -190,20 +192,54 @@ DEV int swizzle(int row) {
     return HDP <= 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
 }
 
-template <int HDP>
-constexpr int KT = HDP <= 128 ? 64 : 32;  // positions per tile
+constexpr int KT = 32;  // positions per tile
 
-// A workgroup of NW waves takes 32 NW rows. Tiles of KT positions go through registers into LDS (Q8 decoded on the way), two
-// buffers deep: while a tile is multiplied the next one is on its way from memory. A wave holds its queries, S^T [KT x 32]
-// and O^T [HDP x 32] in registers; V's operand is read transposed from LDS, its key order that of S^T's registers.
+DEV const void *uniform(const void *p) {
+    const uint64_t x = (uint64_t)p;
+    return (const void *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x));
+}
+// LDS DMA: lane i's 16 (4) bytes at base + off land at lds + 16 i (4 i). Untracked by the compiler, which would otherwise wait
+// for all of them before every LDS read: callers wait with wait_dma. M0 is restored.
+DEV void dma16_global(const void *base, uint32_t off, uint32_t lds) {
+    uint32_t save;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(uniform(base))
+                 : "memory");
+}
+DEV void dma4_global(const void *at, uint32_t lds) {
+    uint32_t save;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at)
+                 : "memory");
+}
+template <int N>
+DEV void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory"); }
+// a workgroup barrier that leaves loads and LDS DMA in flight
+DEV void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Tiles that k_rows keeps in LDS, the ones on their way from memory among them: what fits 160 KB (two workgroups of 4 waves
+// per CU for head_dim <= 128, else one).
+template <int HDP, bool Q8, int NW>
+constexpr int DEPTH = HDP <= 128 && NW == 8 ? 6 : Q8 ? 5 : 4;
+
+// A workgroup of NW waves takes 32 NW rows. Tiles of KT positions come into a ring in LDS by DMA, DEPTH - 2 tiles ahead: the
+// time of a tile is shorter than the way from HBM. Every wave multiplies every tile: while it turns the scores of a tile into
+// weights (vector instructions), the matrix cores form the scores of the next one. It holds its queries, two S^T [KT x 32] and
+// O^T [HDP x 32] in registers; V's operand is read transposed from LDS, its key order that of S^T's registers. Q8 tiles are
+// decoded a tile ahead from the ring into two more buffers of each matrix, once for all waves.
 template <int HDP, bool Q8, int NW>
 __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
-    constexpr int P = PITCH<HDP>, T = KT<HDP>, KB = T / 32, NJ = HDP / 16, ND = HDP / 32, TILE = T * P;
-    constexpr int LPR = P / (Q8 ? 32 : 16), RPI = 64 / LPR, UNITS = T / RPI, NI = 2 * UNITS / NW;
-    static_assert(RPI <= 16 && NI * NW == 2 * UNITS, "whole loads per wave, each in one page");
-    __shared__ __align__(1024) char lds[4 * TILE];
+    constexpr int P = PITCH<HDP>, T = KT, KB = T / 32, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
+    constexpr int RAWP = Q8 ? P / 2 : P, RAW = T * RAWP;  // a ring tile's pitch and bytes
+    constexpr int LPR = RAWP / 16, RPI = 64 / LPR, UNITS = T / RPI, NI = (2 * UNITS + NW - 1) / NW;
+    static_assert(RPI <= 16, "a load stays in a page");
+    static_assert(NI * NW == 2 * UNITS || NI == 1, "every wave that loads has NI loads per tile");
+    constexpr int RING = Q8 ? 4 * TILE : 0, SCALES = RING + D * 2 * RAW;  // Q8: K, K, V, V decoded; the ring; its scales
+    __shared__ __align__(1024) char lds[SCALES + (Q8 ? D * 128 : 0)];
     __shared__ int flags[2], last;
-    __shared__ __align__(16) float fac[Q8 ? 4 * T : 4];  // Q8, two tiles: what the scores of a position take (key scale, score scale), and its weight
+    __shared__ __align__(16) float fac[Q8 ? 4 * T : 4];  // Q8, as lds: what a position's scores take (key scale, score scale), and its weight
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hf = lane >> 5;
@@ -211,7 +247,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const int r0 = it.row0 + 32 * w, r = r0 + li;
     const int n = it.base + (std::min(it.R, it.row0 + 32 * NW) - 1) / rep + 1;  // positions some row of the block sees
     const int n_blk = it.base + it.row0 / rep + 1;                              // positions every row of the block sees
-    const int wn = r0 < it.R ? it.base + (std::min(it.R, r0 + 32) - 1) / rep + 1 : 0, wn_all = it.base + r0 / rep + 1;
+    const int end = std::min(it.k1, n), tiles = end > it.k0 ? (end - it.k0 + T - 1) / T : 0;
+    const int wn = std::min(end, r0 < it.R ? it.base + (std::min(it.R, r0 + 32) - 1) / rep + 1 : 0), wn_all = it.base + r0 / rep + 1;
     const int lim = it.base + std::min(r, it.R - 1) / rep + 1;
     if (threadIdx.x < 2) flags[threadIdx.x] = -1;
 
@@ -227,180 +264,267 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         }
     }
 
-    // staging: wave w's loads u = w NI + i of a tile: matrix u / UNITS, rows RPI (u % UNITS) + lane / LPR, a 16-byte piece each
-    const int lrow = lane / LPR, piece = lane % LPR;
-    const bool on = piece * (Q8 ? 16 : 8) < hd;
+    // The ring: wave w's loads u = w NI + i of a tile: matrix u / UNITS, rows RPI (u % UNITS) + lane / LPR, a 16-byte piece each.
+    // A piece's place in LDS is the lane's, so the lane takes the piece that belongs there. Pieces past head_dim stay 0.
+    const uint32_t at0 = (uint32_t)(uintptr_t)lds;
+    const int lrow = lane / LPR, place = lane % LPR;
     const size_t es = Q8 ? 1 : 2;
     const char *const kb0 = (const char *)g.kv.k + (size_t)it.kvh * g.kv.head_stride * es, *const vb0 = (const char *)g.kv.v + (size_t)it.kvh * g.kv.head_stride * es;
-    const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es);
-    u4v st[NI];
-    _Float16 sd[NI];
-    uint32_t pg[NI];
-    int wat[NI];
+    const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es), pmask = (uint32_t)g.kv.page_size - 1;
+    uint32_t pg[NI], pgs[2];
+    auto fetch_pages = [&](int i) {  // of tile i
+        if (Q8)
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        const int u = w * NI + i, row = RPI * (u % UNITS) + lrow;
-        wat[i] = (u / UNITS) * TILE + row * P + (((Q8 ? 2 * piece : piece) ^ swizzle<HDP>(row)) << 4);
-        st[i] = u4v{0, 0, 0, 0}, sd[i] = (_Float16)0.f;
-    }
-    auto fetch_pages = [&](int s0) {
+            for (int x = 0; x < 2; x++) pgs[x] = page_of(g, it, std::min(it.k0 + i * T + 16 * x, n - 1));
 #pragma unroll
-        for (int i = 0; i < NI; i++) pg[i] = *page_of(g, it, std::min(s0 + RPI * ((w * NI + i) % UNITS), n - 1));
+        for (int x = 0; x < NI; x++) pg[x] = page_of(g, it, std::min(it.k0 + i * T + RPI * ((w * NI + x) % UNITS), n - 1));
     };
-    auto load = [&](int s0) {
+    auto issue = [&](int i, int slot) {
+        if (i >= tiles) return;
+        const int s0 = it.k0 + i * T;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int u = w * NI + i, in = std::min(s0 + RPI * (u % UNITS) + lrow, n - 1) & (g.kv.page_size - 1);
-            const char *base = (u < UNITS ? kb0 : vb0) + (size_t)pg[i] * (size_t)g.kv.page_stride * es;
-            if (on) st[i] = *(const u4v *)(base + ((uint32_t)in * pos_b + (uint32_t)piece * 16u));
-            if (Q8) sd[i] = ((const _Float16 *)(u < UNITS ? g.kv.k_scale : g.kv.v_scale))[((size_t)pg[i] * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in];
+        for (int x = 0; x < NI; x++) {
+            const int u = w * NI + x, row = RPI * (u % UNITS) + lrow;
+            if (u >= 2 * UNITS) continue;
+            const uint32_t in = (uint32_t)std::min(s0 + row, n - 1) & pmask;
+            const int piece = Q8 ? place : place ^ swizzle<HDP>(row);
+            const char *base = (u < UNITS ? kb0 : vb0) + (size_t)pg[x] * (size_t)g.kv.page_stride * es;
+            const uint32_t to = at0 + RING + slot * 2 * RAW + (u / UNITS) * RAW + RPI * (u % UNITS) * RAWP;
+            if (piece * (Q8 ? 16 : 8) < hd) dma16_global(base, in * pos_b + (uint32_t)piece * 16u, to);
+        }
+        if (Q8 && w == 0 && lane < 32) {
+            // scales, two positions a lane: lanes 0 .. 15 keys', 16 .. 31 values'; whole runs of 16 (what lies behind the last
+            // position is not used)
+            const int p = s0 + 2 * (lane & 15);
+            const uint32_t page = lane & 8 ? pgs[1] : pgs[0];
+            const uint16_t *const sc = lane < 16 ? g.kv.k_scale : g.kv.v_scale;
+            dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + ((uint32_t)p & pmask), at0 + SCALES + slot * 128);
         }
     };
-    auto store = [&](int buf, int s0) {
-        char *const to = lds + buf * 2 * TILE;
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const bool look = s0 + T > n_blk && w * NI + i >= UNITS;
-            if (Q8) {
-                h8 lo, hi;
-                const bool val = w * NI + i >= UNITS;
-                const uint32_t db = __builtin_bit_cast(uint16_t, sd[i]);
-                decode16(st[i], val ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(db)) : (_Float16)1.f, lo, hi);
-                if (!on) lo = hi = h8{};
-                if (piece == 0) fac[(2 * buf + val) * T + RPI * ((w * NI + i) % UNITS) + lrow] = val ? rest_of(db) : (float)sd[i] * g.sc;
-                if (look && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi)))) lo = finite8(lo), hi = finite8(hi), flags[buf] = s0;
-                *(h8 *)(to + wat[i]) = lo;
-                *(h8 *)(to + (wat[i] ^ 16)) = hi;
-            } else {
-                u4v x = st[i];
-                if (look && odd16(x)) x = finite16(x), flags[buf] = s0;
-                *(u4v *)(to + wat[i]) = x;
-            }
+    // until tile i of the `issued` that are on their way or here is here, at most AFTER tiles behind it
+    auto wait_tile = [&](int i, int issued, auto after) {
+        constexpr int AFTER = decltype(after)::value;
+        if (issued - 1 - i < AFTER) wait_dma<0>();
+        else if (Q8 && w == 0) wait_dma<AFTER * (NI + 1)>();
+        else wait_dma<AFTER * NI>();
+    };
+    // Q8: tile i's keys (values) out of the ring, decoded, by the whole workgroup: a piece of 16 codes a thread
+    auto decode = [&](int i, bool val) {
+        if (i >= tiles) return;
+        constexpr int PIECES = T * P / 32;
+        const int s0 = it.k0 + i * T, slot = i % D, buf = i & 1;
+        const uint16_t *const sc = (const uint16_t *)(lds + SCALES + slot * 128) + (val ? 32 : 0);
+        for (int x = threadIdx.x; x < PIECES; x += 64 * NW) {
+            const int row = x / LPR, piece = x % LPR;
+            const u4v c = *(const u4v *)(lds + RING + slot * 2 * RAW + (val ? RAW : 0) + row * RAWP + piece * 16);
+            const uint32_t d = s0 + row < n ? sc[row] : 0u;
+            h8 lo, hi;
+            decode16(c, val ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(d)) : (_Float16)1.f, lo, hi);
+            if (piece * 16 >= hd) lo = hi = h8{};
+            if (piece == 0) fac[(2 * val + buf) * T + row] = val ? rest_of(d) : h2f((uint16_t)d) * g.sc;
+            if (val && s0 + T > n_blk && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi))))
+                lo = finite8(lo), hi = finite8(hi), flags[buf] = i;
+            char *const to = lds + (2 * val + buf) * TILE + row * P;
+            const int at = (2 * piece) ^ swizzle<HDP>(row);
+            *(h8 *)(to + at * 16) = lo;
+            *(h8 *)(to + (at ^ 1) * 16) = hi;
+        }
+    };
+    // fp16: the odd values of tile i, which some row sees only part of, become 0
+    auto look = [&](int i) {
+        if (i >= tiles || it.k0 + i * T + T <= n_blk) return;
+        for (int x = threadIdx.x; x < TILE / 16; x += 64 * NW) {
+            u4v *const at = (u4v *)(lds + (i % D) * 2 * RAW + RAW + x * 16);
+            const u4v v = *at;
+            if (odd16(v)) *at = finite16(v), flags[i & 1] = i;
         }
     };
 
     float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores; Q8: in log2 units), what the exponents are taken against, the sum
-    f16v o[ND];
+    f16v o[ND], s[KB];
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[d][e] = 0.f;
 
-    const int end = std::min(it.k1, n);
-    const uint32_t kx = (uint32_t)(li * P + ((hf ^ swizzle<HDP>(li)) << 4));
+    const uint32_t kx = at0 + (uint32_t)(li * P + ((hf ^ swizzle<HDP>(li)) << 4));
     const int i16 = lane & 15, vrow = 4 * hf + (i16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-    const uint32_t vx = (uint32_t)(TILE + vrow * P + ((vc ^ swizzle<HDP>(vrow)) << 4) + 8 * (i16 & 1));
-    if (it.k0 < end) {
-        fetch_pages(it.k0);
-        load(it.k0);
-        if (it.k0 + T < end) fetch_pages(it.k0 + T);
-        __syncthreads();  // the flags are set
-        store(0, it.k0);
-        if (it.k0 + T < end) load(it.k0 + T);
-        if (it.k0 + 2 * T < end) fetch_pages(it.k0 + 2 * T);
-        __syncthreads();
-    }
-    int buf = 0;
-    for (int s0 = it.k0; s0 < end; s0 += T, buf ^= 1) {
-        if (s0 < wn) {
-            const char *const tile = lds + buf * 2 * TILE;
-            f16v s[KB];
+    const uint32_t vx = at0 + (uint32_t)((Q8 ? 2 * TILE : RAW) + vrow * P + ((vc ^ swizzle<HDP>(vrow)) << 4) + 8 * (i16 & 1));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    typedef const __attribute__((address_space(3))) h8 lds_h8;
+    // operands of the tile at `buf` (bytes): keys 32 b .. by dims 16 j ..; dims 32 d .. by positions 16 k ..
+    auto key_operand = [&](uint32_t buf, int j, int b) { return *(lds_h8 *)(uintptr_t)(((kx + buf) ^ (32u * j)) + 32 * P * b); };
+    auto value_operand = [&](uint32_t buf, int d, int k) {
+        const uint32_t x = (vx + buf) ^ (64u * d);
+        const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)(x + 16 * P * k)));
+        const h4 c = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)((x ^ 32u) + 16 * P * k + 8 * P)));
+        return h8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+    };
+    // y times the key scales of the tile in buffer `buf`
+    auto scale_scores = [&](f16v (&y)[KB], int buf) {
+        if (!Q8) return;
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const f4 f = *(const f4 *)&fac[buf * T + 32 * b + 8 * c + 4 * hf];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[b][4 * c + e] *= f[e];
+            }
+    };
+    auto zero_scores = [&](f16v (&y)[KB]) {
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) y[b][e] = 0.f;
+    };
+    // scores s of the tile at s0 to weights, and its values' product; the scores of the tile after it (of whatever the buffer
+    // holds, behind the last)
+    auto step = [&](int s0, int buf, uint32_t k_at, uint32_t v_at) {
+        h8 kf[NJ][KB], vf[KB][ND];
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) kf[j][b] = key_operand(k_at, j, b);
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int d = 0; d < ND; d++) vf[k][d] = value_operand(v_at, d, k);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s0 + T > wn_all) {
 #pragma unroll
             for (int b = 0; b < KB; b++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) s[b][e] = 0.f;
+                for (int e = 0; e < 16; e++) s[b][e] = s0 + 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[b][e] : -INFINITY;
+        }
+        float mx = s[0][0];
 #pragma unroll
-            for (int j = 0; j < NJ; j++)
+        for (int b = 0; b < KB; b++)
 #pragma unroll
-                for (int b = 0; b < KB; b++) s[b] = mfma32(*(const h8 *)(tile + ((kx ^ (32u * j)) + 32 * P * b)), q[j], s[b]);
-            if (Q8) {
+            for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][e]);
+        if (__any(mx > m + g.slack)) {
+            const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
+            const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
+            m = mn, mref = nref;
+            l *= a;
 #pragma unroll
-                for (int b = 0; b < KB; b++)
+            for (int d = 0; d < ND; d++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const f4 f = *(const f4 *)&fac[2 * buf * T + 32 * b + 8 * c + 4 * hf];
+                for (int e = 0; e < 16; e++) o[d][e] *= a;
+        }
+        f16v y[KB];
+        zero_scores(y);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[b][4 * c + e] *= f[e];
-                    }
-            }
-            if (s0 + T > wn_all) {
+        for (int j = 0; j < NJ; j++)
 #pragma unroll
-                for (int b = 0; b < KB; b++)
+            for (int b = 0; b < KB; b++) y[b] = mfma32(kf[j][b], q[j], y[b]);
+        h8 p[2 * KB];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[b][e] = s0 + 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[b][e] : -INFINITY;
-            }
-            float mx = s[0][0];
+        for (int b = 0; b < KB; b++)
 #pragma unroll
-            for (int b = 0; b < KB; b++)
+            for (int c = 0; c < 4; c++) {
+                f4 f;
+                if (Q8) f = *(const f4 *)&fac[(2 + buf) * T + 32 * b + 8 * c + 4 * hf];
 #pragma unroll
-                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][e]);
-            if (__any(mx > m + g.slack)) {
-                const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
-                const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
-                m = mn, mref = nref;
-                l *= a;
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] *= a;
-            }
-            h8 p[2 * KB];
-            float add = 0.f;
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    f4 f;
-                    if (Q8) f = *(const f4 *)&fac[(2 * buf + 1) * T + 32 * b + 8 * c + 4 * hf];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int e = 4 * c + i;
-                        const float x = ex2(Q8 ? s[b][e] - mref : fmaf(s[b][e], g.sc, -mref));
-                        add += x;
-                        p[2 * b + (e >> 3)][e & 7] = (_Float16)(Q8 ? x * f[i] : x);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const int e = 4 * c + i;
+                    const float x = ex2(Q8 ? s[b][e] - mref : fmaf(s[b][e], g.sc, -mref));
+                    if (Q8) l += x;
+                    p[2 * b + (e >> 3)][e & 7] = (_Float16)(Q8 ? x * f[i] : x);
                 }
-            l += add;
-            auto operand = [&](int d, int k) {
-                typedef __attribute__((address_space(3))) s4 lds_s4;
-                const uint32_t at = (uint32_t)(uintptr_t)tile + ((vx ^ (64u * d)) + 16 * P * k);
-                const uint32_t at8 = (uint32_t)(uintptr_t)tile + ((vx ^ (64u * d) ^ 32u) + 16 * P * k + 8 * P);
-                const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)at));
-                const h4 c = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)at8));
-                return h8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
-            };
+            }
+        if (!Q8) {  // (the sum of the weights as they are multiplied)
+            const h2 one = {(_Float16)1.f, (_Float16)1.f};
 #pragma unroll
             for (int k = 0; k < 2 * KB; k++)
 #pragma unroll
-                for (int d = 0; d < ND; d++) o[d] = mfma32(operand(d, k), p[k], o[d]);
-            if (flags[buf] == s0) {  // the tile's odd values, position by position
+                for (int e = 0; e < 8; e += 2) l = __builtin_amdgcn_fdot2(h2{p[k][e], p[k][e + 1]}, one, l, false);
+        }
+        // the score products go out between the exponentials
+#pragma unroll
+        for (int i = 0; i < NJ * KB; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        h8 vg[KB][ND];
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int d = 0; d < ND; d++) vg[k][d] = value_operand(v_at, d, KB + k);
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] = mfma32(vf[k][d], p[k], o[d]);
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] = mfma32(vg[k][d], p[KB + k], o[d]);
+        scale_scores(y, buf ^ 1);
+#pragma unroll
+        for (int b = 0; b < KB; b++) s[b] = y[b];
+    };
+    // the odd values of the tile at s0, position by position
+    auto odd_values = [&](int s0) {
 #pragma clang loop unroll(disable)
-                for (int at = s0; at < std::min(s0 + T, wn); at++) {
-                    const uint32_t page = *page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
-                    const char *const v = vb0 + ((size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
-                    const _Float16 d8 = Q8 ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in])) : (_Float16)0.f;
+        for (int at = s0; at < std::min(s0 + T, wn); at++) {
+            const uint32_t page = page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
+            const char *const v = vb0 + ((size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
+            const _Float16 d8 = Q8 ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in])) : (_Float16)0.f;
 #pragma unroll
-                    for (int d = 0; d < ND; d++)
+            for (int d = 0; d < ND; d++)
 #pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const int dim = 32 * d + 8 * c + 4 * hf;
-                            if (at >= lim || dim >= hd) continue;
+                for (int c = 0; c < 4; c++) {
+                    const int dim = 32 * d + 8 * c + 4 * hf;
+                    if (at >= lim || dim >= hd) continue;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const _Float16 x = Q8 ? (_Float16)(float)((const int8_t *)v)[dim + e] * d8 : ((const _Float16 *)v)[dim + e];
-                                if (odd(x)) o[d][4 * c + e] += (float)x;
-                            }
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        const _Float16 x = Q8 ? (_Float16)(float)((const int8_t *)v)[dim + e] * d8 : ((const _Float16 *)v)[dim + e];
+                        if (odd(x)) o[d][4 * c + e] += (float)x;
+                    }
                 }
-            }
         }
-        if (s0 + T < end) {
-            store(buf ^ 1, s0 + T);
-            if (s0 + 2 * T < end) load(s0 + 2 * T);
-            if (s0 + 3 * T < end) fetch_pages(s0 + 3 * T);
+    };
+
+    if (tiles) {
+        if (!Q8 && hd < HDP)  // (decode() writes zeros itself)
+            for (int x = threadIdx.x; x < D * 2 * RAW / 16; x += 64 * NW) *(u4v *)(lds + x * 16) = u4v{0, 0, 0, 0};
+        barrier();
+#pragma unroll
+        for (int i = 0; i < D - 1; i++) {
+            fetch_pages(std::min(i, tiles - 1));
+            issue(i, i);
         }
-        __syncthreads();
+        fetch_pages(std::min(D - 1, tiles - 1));
+        wait_tile(Q8 ? 1 : 0, std::min(D - 1, tiles), std::integral_constant<int, Q8 ? D - 3 : D - 2>());
+        barrier();
+        if constexpr (Q8) decode(0, false), decode(1, false), decode(0, true);
+        else look(0);
+        barrier();
+        zero_scores(s);
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) s[b] = mfma32(key_operand(0, j, b), q[j], s[b]);
+        scale_scores(s, 0);
     }
+    int slot = 0;  // i % D
+    for (int i = 0; i < tiles; i++) {
+        const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1;
+        // tile i + 1 (Q8: i + 2) is there, D - 3 (D - 4) tiles after it may still be on their way
+        wait_tile(Q8 ? i + 2 : i + 1, std::min(i + D - 1, tiles), std::integral_constant<int, Q8 ? D - 4 : D - 3>());
+        barrier();
+        issue(i + D - 1, before);
+        fetch_pages(std::min(i + D, tiles - 1));
+        if (s0 < wn) {
+            if (Q8) step(s0, i & 1, ((i & 1) ^ 1) * TILE, (i & 1) * TILE);
+            else step(s0, i & 1, after * 2 * RAW, slot * 2 * RAW);
+            if (flags[i & 1] == i) odd_values(s0);
+        }
+        if constexpr (Q8) decode(i + 2, false), decode(i + 1, true);
+        else look(i + 1);
+        slot = after;
+    }
+    wait_dma<0>();
     const float lt = sum_halves(l);
     if (it.n_parts == 1) {
 #pragma unroll
@@ -466,7 +590,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
     uint32_t pgk[2], pgn[2];  // pages of the tile whose keys are loaded next, of the one whose values are
     auto fetch = [&](int s0, uint32_t (&pg)[2]) {
 #pragma unroll
-        for (int b = 0; b < 2; b++) pg[b] = *page_of(g, it, std::min(s0 + 16 * b, n - 1));
+        for (int b = 0; b < 2; b++) pg[b] = page_of(g, it, std::min(s0 + 16 * b, n - 1));
     };
     auto load_k = [&](int s0, const uint32_t (&pg)[2]) {
 #pragma unroll
