@@ -109,31 +109,36 @@ DEV void decode16(u4v c, _Float16 d, h8 &lo, h8 &hi) {
     hi = h8{o[4].x, o[4].y, o[5].x, o[5].y, o[6].x, o[6].y, o[7].x, o[7].y};
 }
 
-// four outputs d .. d + 3 of row r, v / l, gated
-DEV void finish(const Args &g, const HqItem &it, int r, int d, f4 v, float l) {
-    const int hd = g.kv.head_dim;
-    if (r >= it.R || d >= hd) return;
-    const int t = r / g.rep, h = it.kvh * g.rep + r - t * g.rep;
-    const size_t tok = (size_t)(it.tok0 + t);
-    if (it.base + t < 0) v = f4{0.f, 0.f, 0.f, 0.f}, l = 1.f;  // padding: sees nothing
-    h4 y;
-    f4 gate = {0.f, 0.f, 0.f, 0.f};
-    if (g.a.gate) {
-        const size_t at = tok * g.a.gate_stride + (size_t)h * g.a.gate_head_stride + d;
-        if (g.a.gate_f32) gate = *(const f4 *)((const float *)g.a.gate + at);
-        else {
-            const h4 x = *(const h4 *)((const _Float16 *)g.a.gate + at);
-            gate = f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-        }
+// Where row r of an item goes: its outputs v / l, gated, four dims at a time.
+struct OutRow {
+    _Float16 *out;  // null: not a row
+    const char *gate;
+    float inv;
+    int hd, gate_f32;
+    __device__ __forceinline__ OutRow(const Args &g, const HqItem &it, int r, float l) : out(nullptr), gate(nullptr), inv(1.0f / l), hd(g.kv.head_dim), gate_f32(g.a.gate_f32) {
+        if (r >= it.R) return;
+        const int t = r / g.rep, h = it.kvh * g.rep + r - t * g.rep;
+        const size_t tok = (size_t)(it.tok0 + t);
+        out = (_Float16 *)g.a.out + tok * g.a.out_stride + (size_t)h * hd;
+        if (g.a.gate) gate = (const char *)g.a.gate + (tok * g.a.gate_stride + (size_t)h * g.a.gate_head_stride) * (gate_f32 ? 4 : 2);
+        if (it.base + t < 0) inv = 0.f;  // padding: sees nothing, its sums are 0
     }
+    __device__ __forceinline__ void put(int d, f4 v) const {
+        if (!out || d >= hd) return;
+        v *= inv;
+        if (gate) {
+            f4 x;
+            if (gate_f32) x = *(const f4 *)(gate + 4 * d);
+            else {
+                const h4 y = *(const h4 *)(gate + 2 * d);
+                x = f4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+            }
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        float x = v[e] / l;
-        if (g.a.gate) x *= 1.0f / (1.0f + expf(-gate[e]));
-        y[e] = (_Float16)x;
+            for (int e = 0; e < 4; e++) v[e] *= 1.0f / (1.0f + expf(-x[e]));
+        }
+        *(h4 *)(out + d) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
     }
-    *(h4 *)((_Float16 *)g.a.out + tok * g.a.out_stride + (size_t)h * hd + d) = y;
-}
+};
 
 // A part's row: its sums [HDP], then (maximum in log2 units, sum). Parts are written and read at device scope; the last of
 // a block's items to arrive adds them in part order, so the result does not depend on the order of arrival.
@@ -174,7 +179,7 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
                 m = mn;
             }
         }
-        finish(g, it, it.row0 + row, d, v, l);
+        OutRow(g, it, it.row0 + row, l).put(d, v);
     }
 }
 
@@ -233,13 +238,15 @@ template <int HDP, bool Q8, int NW>
 __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     constexpr int P = PITCH<HDP>, T = KT, KB = T / 32, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
     constexpr int RAWP = Q8 ? P / 2 : P, RAW = T * RAWP;  // a ring tile's pitch and bytes
-    constexpr int LPR = RAWP / 16, RPI = 64 / LPR, UNITS = T / RPI, NI = (2 * UNITS + NW - 1) / NW;
-    static_assert(RPI <= 16, "a load stays in a page");
-    static_assert(NI * NW == 2 * UNITS || NI == 1, "every wave that loads has NI loads per tile");
+    constexpr int LPR = RAWP / 16, RPI = 64 / LPR, UNITS = T / RPI, NI = 2 * UNITS > NW ? 2 * UNITS / NW : 1;
+    // With PRE a wave reads a tile's first operands before the barrier in front of it: K's, and for fp16 half of V's. The ring
+    // must be a tile deeper.
+    constexpr bool PRE = D >= 6, PREV = PRE && !Q8;
+    constexpr int LEAD = (Q8 ? 2 : 1) + (PRE ? 1 : 0);  // tile i + LEAD is in LDS when tile i's turn comes
     constexpr int RING = Q8 ? 4 * TILE : 0, SCALES = RING + D * 2 * RAW;  // Q8: K, K, V, V decoded; the ring; its scales
     __shared__ __align__(1024) char lds[SCALES + (Q8 ? D * 128 : 0)];
-    __shared__ int flags[2], last;
-    __shared__ __align__(16) float fac[Q8 ? 4 * T : 4];  // Q8, as lds: what a position's scores take (key scale, score scale), and its weight
+    __shared__ int flags[4], last;
+    __shared__ __align__(16) float fac[Q8 ? 6 * T : 4];  // Q8: what a position's scores take (key scale, score scale), four tiles; its weight, two
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hf = lane >> 5;
@@ -250,7 +257,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const int end = std::min(it.k1, n), tiles = end > it.k0 ? (end - it.k0 + T - 1) / T : 0;
     const int wn = std::min(end, r0 < it.R ? it.base + (std::min(it.R, r0 + 32) - 1) / rep + 1 : 0), wn_all = it.base + r0 / rep + 1;
     const int lim = it.base + std::min(r, it.R - 1) / rep + 1;
-    if (threadIdx.x < 2) flags[threadIdx.x] = -1;
+    if (threadIdx.x < 4) flags[threadIdx.x] = -1;
 
     h8 q[NJ];
     {
@@ -260,46 +267,60 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         for (int j = 0; j < NJ; j++) {
             const int d = 16 * j + 8 * hf;
             q[j] = d < hd ? *(const h8 *)(p + d) : h8{};
-            if (g.a.scale < 0.f) q[j] = -q[j];
         }
     }
 
-    // The ring: wave w's loads u = w NI + i of a tile: matrix u / UNITS, rows RPI (u % UNITS) + lane / LPR, a 16-byte piece each.
-    // A piece's place in LDS is the lane's, so the lane takes the piece that belongs there. Pieces past head_dim stay 0.
+    // The ring: wave w takes rows RPI NI (w % WM) .. of one matrix, a run within 16 rows and so within a page, 16-byte pieces in
+    // NI loads. A piece's place in LDS is the lane's, so the lane takes the piece that belongs there. Pieces past head_dim stay 0.
+    constexpr int WM = UNITS / NI;  // waves per matrix
+    static_assert(RPI * NI <= 16, "a wave's rows stay in a page");
     const uint32_t at0 = (uint32_t)(uintptr_t)lds;
-    const int lrow = lane / LPR, place = lane % LPR;
     const size_t es = Q8 ? 1 : 2;
-    const char *const kb0 = (const char *)g.kv.k + (size_t)it.kvh * g.kv.head_stride * es, *const vb0 = (const char *)g.kv.v + (size_t)it.kvh * g.kv.head_stride * es;
+    const bool loads = w < 2 * WM, values = w >= WM;
+    const int row_w = RPI * NI * (w % WM), in_w = row_w & 15;
+    const char *const kv0 = (const char *)(values ? g.kv.v : g.kv.k) + (size_t)it.kvh * g.kv.head_stride * es;
+    const size_t page_b = (size_t)g.kv.page_stride * es;
     const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es), pmask = (uint32_t)g.kv.page_size - 1;
-    uint32_t pg[NI], pgs[2];
-    auto fetch_pages = [&](int i) {  // of tile i
-        if (Q8)
+    const uint32_t to_w = at0 + RING + (values ? RAW : 0) + row_w * RAWP;
+    uint32_t piece_at[NI];  // byte of the lane's piece in a row
+    bool on[NI];
 #pragma unroll
-            for (int x = 0; x < 2; x++) pgs[x] = page_of(g, it, std::min(it.k0 + i * T + 16 * x, n - 1));
+    for (int x = 0; x < NI; x++) {
+        const int row = row_w + RPI * x + lane / LPR, place = lane % LPR, piece = Q8 ? place : place ^ swizzle<HDP>(row);
+        on[x] = piece * (Q8 ? 16 : 8) < hd;
+        piece_at[x] = (uint32_t)piece * 16u;
+    }
+    // Pages: lane t holds those of the wave's rows (Q8: of both runs of 16) of tile 64 c + t; read again every 64 tiles. (A scalar
+    // load per tile would be waited for at every barrier.)
+    uint32_t pages[Q8 ? 2 : 1];
+    auto fetch_pages = [&](int i) {
 #pragma unroll
-        for (int x = 0; x < NI; x++) pg[x] = page_of(g, it, std::min(it.k0 + i * T + RPI * ((w * NI + x) % UNITS), n - 1));
+        for (int x = 0; x < (Q8 ? 2 : 1); x++) {
+            pages[x] = g.pages[it.page0 + (std::min(it.k0 + (i + lane) * T + (Q8 ? 16 * x : row_w & ~15), n - 1) >> g.shift)];
+            asm volatile("" : "+v"(pages[x]));  // here, not where they are used
+        }
     };
-    auto issue = [&](int i, int slot) {
-        if (i >= tiles) return;
-        const int s0 = it.k0 + i * T;
-#pragma unroll
-        for (int x = 0; x < NI; x++) {
-            const int u = w * NI + x, row = RPI * (u % UNITS) + lrow;
-            if (u >= 2 * UNITS) continue;
-            const uint32_t in = (uint32_t)std::min(s0 + row, n - 1) & pmask;
-            const int piece = Q8 ? place : place ^ swizzle<HDP>(row);
-            const char *base = (u < UNITS ? kb0 : vb0) + (size_t)pg[x] * (size_t)g.kv.page_stride * es;
-            const uint32_t to = at0 + RING + slot * 2 * RAW + (u / UNITS) * RAW + RPI * (u % UNITS) * RAWP;
-            if (piece * (Q8 ? 16 : 8) < hd) dma16_global(base, in * pos_b + (uint32_t)piece * 16u, to);
-        }
-        if (Q8 && w == 0 && lane < 32) {
-            // scales, two positions a lane: lanes 0 .. 15 keys', 16 .. 31 values'; whole runs of 16 (what lies behind the last
-            // position is not used)
-            const int p = s0 + 2 * (lane & 15);
-            const uint32_t page = lane & 8 ? pgs[1] : pgs[0];
-            const uint16_t *const sc = lane < 16 ? g.kv.k_scale : g.kv.v_scale;
-            dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + ((uint32_t)p & pmask), at0 + SCALES + slot * 128);
-        }
+    auto page_in = [&](int i, int x) { return (uint32_t)__builtin_amdgcn_readlane((int)pages[x], i & 63); };
+    // load x of tile i (the caller has checked that there is one), which goes to `slot`
+    auto load_piece = [&](int i, int slot, int x) {
+        if (!loads) return;
+        // (rows behind the last position: the last one's again, their weight is 0)
+        const uint32_t in = (uint32_t)std::min(it.k0 + i * T + row_w + RPI * x + lane / LPR, n - 1) & pmask;
+        const char *const base = kv0 + (size_t)page_in(i, Q8 ? row_w >> 4 : 0) * page_b;
+        const uint32_t at = in * pos_b + piece_at[x], to = to_w + slot * 2 * RAW + RPI * x * RAWP;
+        if (hd == HDP) dma16_global(base, at, to);
+        else if (on[x]) dma16_global(base, at, to);
+    };
+    auto load_scales = [&](int i, int slot) {
+        if (!Q8 || w != 0) return;
+        const uint32_t page0 = page_in(i, 0), page1 = page_in(i, Q8 ? 1 : 0);
+        if (lane >= 32) return;
+        // two positions a lane: lanes 0 .. 15 keys', 16 .. 31 values'; whole runs of 16 (what lies behind the last position is
+        // not used)
+        const int p = it.k0 + i * T + 2 * (lane & 15);
+        const uint32_t page = lane & 8 ? page1 : page0;
+        const uint16_t *const sc = lane < 16 ? g.kv.k_scale : g.kv.v_scale;
+        dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + ((uint32_t)p & pmask), at0 + SCALES + slot * 128);
     };
     // until tile i of the `issued` that are on their way or here is here, at most AFTER tiles behind it
     auto wait_tile = [&](int i, int issued, auto after) {
@@ -321,9 +342,9 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             h8 lo, hi;
             decode16(c, val ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(d)) : (_Float16)1.f, lo, hi);
             if (piece * 16 >= hd) lo = hi = h8{};
-            if (piece == 0) fac[(2 * val + buf) * T + row] = val ? rest_of(d) : h2f((uint16_t)d) * g.sc;
+            if (piece == 0) fac[(val ? 4 + buf : i & 3) * T + row] = val ? rest_of(d) : h2f((uint16_t)d) * g.sc;
             if (val && s0 + T > n_blk && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi))))
-                lo = finite8(lo), hi = finite8(hi), flags[buf] = i;
+                lo = finite8(lo), hi = finite8(hi), flags[i & 3] = i;
             char *const to = lds + (2 * val + buf) * TILE + row * P;
             const int at = (2 * piece) ^ swizzle<HDP>(row);
             *(h8 *)(to + at * 16) = lo;
@@ -336,12 +357,13 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         for (int x = threadIdx.x; x < TILE / 16; x += 64 * NW) {
             u4v *const at = (u4v *)(lds + (i % D) * 2 * RAW + RAW + x * 16);
             const u4v v = *at;
-            if (odd16(v)) *at = finite16(v), flags[i & 1] = i;
+            if (odd16(v)) *at = finite16(v), flags[i & 3] = i;
         }
     };
 
+    float mx = -INFINITY;                      // of the lane's scores of the tile whose turn it is
     float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores; Q8: in log2 units), what the exponents are taken against, the sum
-    f16v o[ND], s[KB];
+    f16v o[ND], sa[KB], sb[KB];  // outputs; scores of a tile and of the next
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -360,14 +382,14 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         const h4 c = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)((x ^ 32u) + 16 * P * k + 8 * P)));
         return h8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
     };
-    // y times the key scales of the tile in buffer `buf`
-    auto scale_scores = [&](f16v (&y)[KB], int buf) {
+    // y times the key scales of tile i
+    auto scale_scores = [&](f16v (&y)[KB], int i) {
         if (!Q8) return;
 #pragma unroll
         for (int b = 0; b < KB; b++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const f4 f = *(const f4 *)&fac[buf * T + 32 * b + 8 * c + 4 * hf];
+                const f4 f = *(const f4 *)&fac[(i & 3) * T + 32 * b + 8 * c + 4 * hf];
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[b][4 * c + e] *= f[e];
             }
@@ -378,30 +400,31 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
             for (int e = 0; e < 16; e++) y[b][e] = 0.f;
     };
-    // scores s of the tile at s0 to weights, and its values' product; the scores of the tile after it (of whatever the buffer
-    // holds, behind the last)
-    auto step = [&](int s0, int buf, uint32_t k_at, uint32_t v_at) {
-        h8 kf[NJ][KB], vf[KB][ND];
+    h8 kf[NJ], vf[ND];
+    auto read_keys = [&](uint32_t buf) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
+        for (int j = 0; j < NJ; j++) kf[j] = key_operand(buf, j, 0);
+    };
+    auto read_values = [&](uint32_t buf) {
 #pragma unroll
-            for (int b = 0; b < KB; b++) kf[j][b] = key_operand(k_at, j, b);
-#pragma unroll
-        for (int k = 0; k < KB; k++)
-#pragma unroll
-            for (int d = 0; d < ND; d++) vf[k][d] = value_operand(v_at, d, k);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < ND; d++) vf[d] = value_operand(buf, d, 0);
+    };
+    static_assert(KB == 1, "one block of scores a tile");
+    // Scores s of tile i to weights, and its values' product; y: the scores of the tile after it (of whatever the buffer holds,
+    // behind the last). k_at, v_at: the next tile's keys and this one's values in LDS; k_pre, v_pre: what the next step starts
+    // with. Written out in the order of issue: a score product, its share of the exponentials and a load; then a product of
+    // values beside the maxima of the new scores.
+    auto step = [&](int i, uint32_t k_at, uint32_t v_at, uint32_t k_pre, uint32_t v_pre, int to, f16v (&s)[KB], f16v (&y)[KB]) {
+        const int s0 = it.k0 + i * T;
+        if (!PRE) read_keys(k_at);
+        if (!PREV) read_values(v_at);
         if (s0 + T > wn_all) {
 #pragma unroll
-            for (int b = 0; b < KB; b++)
+            for (int e = 0; e < 16; e++) s[0][e] = s0 + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[0][e] : -INFINITY;
+            mx = s[0][0];
 #pragma unroll
-                for (int e = 0; e < 16; e++) s[b][e] = s0 + 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[b][e] : -INFINITY;
+            for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[0][e]);
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][e]);
         if (__any(mx > m + g.slack)) {
             const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
             const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
@@ -412,63 +435,76 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= a;
         }
-        f16v y[KB];
+        const bool more = i + D - 1 < tiles;
         zero_scores(y);
+        float x[16];
+        h8 p[2], vg[ND];
+        f4 f[Q8 ? 4 : 1];
+        if (Q8)
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
+            for (int c = 0; c < 4; c++) f[c] = *(const f4 *)&fac[(4 + (i & 1)) * T + 8 * c + 4 * hf];
+        // weights 2 c and 2 c + 1: their exponentials; later, as fp16 (and summed)
+        auto weigh = [&](int c) {
 #pragma unroll
-            for (int b = 0; b < KB; b++) y[b] = mfma32(kf[j][b], q[j], y[b]);
-        h8 p[2 * KB];
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                f4 f;
-                if (Q8) f = *(const f4 *)&fac[(2 + buf) * T + 32 * b + 8 * c + 4 * hf];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int e = 4 * c + i;
-                    const float x = ex2(Q8 ? s[b][e] - mref : fmaf(s[b][e], g.sc, -mref));
-                    if (Q8) l += x;
-                    p[2 * b + (e >> 3)][e & 7] = (_Float16)(Q8 ? x * f[i] : x);
-                }
+            for (int e = 2 * c; e < 2 * c + 2; e++) x[e] = ex2(Q8 ? s[0][e] - mref : fmaf(s[0][e], g.sc, -mref));
+        };
+        auto round = [&](int c) {
+            const int e = 2 * c;
+            if (Q8) {
+                l += x[e] + x[e + 1];
+                x[e] *= f[e / 4][e % 4], x[e + 1] *= f[e / 4][e % 4 + 1];
             }
-        if (!Q8) {  // (the sum of the weights as they are multiplied)
-            const h2 one = {(_Float16)1.f, (_Float16)1.f};
+            const h2 y2 = {(_Float16)x[e], (_Float16)x[e + 1]};
+            p[e / 8][e % 8] = y2.x, p[e / 8][e % 8 + 1] = y2.y;
+            if (!Q8) l = __builtin_amdgcn_fdot2(y2, h2{(_Float16)1.f, (_Float16)1.f}, l, false);  // (the weights as they are multiplied)
+        };
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 2 * KB; k++)
+        for (int j = 0; j < NJ; j++) {
+            y[0] = mfma32(kf[j], q[j], y[0]);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) l = __builtin_amdgcn_fdot2(h2{p[k][e], p[k][e + 1]}, one, l, false);
+            for (int c = 8 * j / NJ; c < 8 * (j + 1) / NJ; c++) {
+                weigh(c);
+                if (c) round(c - 1);
+            }
+            if (j < ND) vg[j] = value_operand(v_at, j, 1);
+            if (more) {
+#pragma unroll
+                for (int x = NI * j / NJ; x < NI * (j + 1) / NJ; x++) load_piece(i + D - 1, to, x);
+                if (j == NJ - 1) load_scales(i + D - 1, to);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // the score products go out between the exponentials
+        round(7);
+        float my = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NJ * KB; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        for (int d = 0; d < ND; d++) {
+            o[d] = mfma32(vf[d], p[0], o[d]);
+            if (PRE)
+#pragma unroll
+                for (int j = NJ * d / (2 * ND); j < NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        h8 vg[KB][ND];
+        scale_scores(y, i + 1);
 #pragma unroll
-        for (int k = 0; k < KB; k++)
+        for (int d = 0; d < ND; d++) {
+            o[d] = mfma32(vg[d], p[1], o[d]);
+            if (PRE)
 #pragma unroll
-            for (int d = 0; d < ND; d++) vg[k][d] = value_operand(v_at, d, KB + k);
+                for (int j = NJ / 2 + NJ * d / (2 * ND); j < NJ / 2 + NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
+            if (PREV) vf[d] = value_operand(v_pre, d, 0);
 #pragma unroll
-        for (int k = 0; k < KB; k++)
-#pragma unroll
-            for (int d = 0; d < ND; d++) o[d] = mfma32(vf[k][d], p[k], o[d]);
-#pragma unroll
-        for (int k = 0; k < KB; k++)
-#pragma unroll
-            for (int d = 0; d < ND; d++) o[d] = mfma32(vg[k][d], p[KB + k], o[d]);
-        scale_scores(y, buf ^ 1);
-#pragma unroll
-        for (int b = 0; b < KB; b++) s[b] = y[b];
+            for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        mx = my;
     };
     // the odd values of the tile at s0, position by position
     auto odd_values = [&](int s0) {
 #pragma clang loop unroll(disable)
         for (int at = s0; at < std::min(s0 + T, wn); at++) {
             const uint32_t page = page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
-            const char *const v = vb0 + ((size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
+            const char *const v = (const char *)g.kv.v + ((size_t)it.kvh * (size_t)g.kv.head_stride + (size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
             const _Float16 d8 = Q8 ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in])) : (_Float16)0.f;
 #pragma unroll
             for (int d = 0; d < ND; d++)
@@ -488,49 +524,74 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     if (tiles) {
         if (!Q8 && hd < HDP)  // (decode() writes zeros itself)
             for (int x = threadIdx.x; x < D * 2 * RAW / 16; x += 64 * NW) *(u4v *)(lds + x * 16) = u4v{0, 0, 0, 0};
+        fetch_pages(0);
         barrier();
 #pragma unroll
         for (int i = 0; i < D - 1; i++) {
-            fetch_pages(std::min(i, tiles - 1));
-            issue(i, i);
+            if (i < tiles) {
+#pragma unroll
+                for (int x = 0; x < NI; x++) load_piece(i, i, x);
+                load_scales(i, i);
+            }
         }
-        fetch_pages(std::min(D - 1, tiles - 1));
-        wait_tile(Q8 ? 1 : 0, std::min(D - 1, tiles), std::integral_constant<int, Q8 ? D - 3 : D - 2>());
+        wait_tile(LEAD - 1, std::min(D - 1, tiles), std::integral_constant<int, D - 1 - LEAD>());
         barrier();
-        if constexpr (Q8) decode(0, false), decode(1, false), decode(0, true);
-        else look(0);
+        if constexpr (Q8) {
+            decode(0, false), decode(1, false), decode(0, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LEAD; i++) look(i);
+        }
         barrier();
-        zero_scores(s);
+        if (g.a.scale < 0.f)
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
+            for (int j = 0; j < NJ; j++) q[j] = -q[j];
+        zero_scores(sa);
+        read_keys(0);
 #pragma unroll
-            for (int b = 0; b < KB; b++) s[b] = mfma32(key_operand(0, j, b), q[j], s[b]);
-        scale_scores(s, 0);
+        for (int j = 0; j < NJ; j++) sa[0] = mfma32(kf[j], q[j], sa[0]);
+        scale_scores(sa, 0);
+#pragma unroll
+        for (int e = 0; e < 16; e++) mx = fmaxf(mx, sa[0][e]);
+        if (PRE) read_keys(Q8 ? TILE : 2 * RAW);
+        if (PREV) read_values(0);
+        if constexpr (Q8 && PRE) {
+            barrier();  // the first tile's keys have been read
+            decode(2, false);
+        }
     }
     int slot = 0;  // i % D
-    for (int i = 0; i < tiles; i++) {
-        const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1;
-        // tile i + 1 (Q8: i + 2) is there, D - 3 (D - 4) tiles after it may still be on their way
-        wait_tile(Q8 ? i + 2 : i + 1, std::min(i + D - 1, tiles), std::integral_constant<int, Q8 ? D - 4 : D - 3>());
+    auto tile = [&](int i, f16v (&s)[KB], f16v (&y)[KB]) {
+        const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1, after2 = after == D - 1 ? 0 : after + 1;
+        // tile i + LEAD is there, the tiles behind it may still be on their way
+        wait_tile(i + LEAD, std::min(i + D - 1, tiles), std::integral_constant<int, D - 2 - LEAD>());
         barrier();
-        issue(i + D - 1, before);
-        fetch_pages(std::min(i + D, tiles - 1));
         if (s0 < wn) {
-            if (Q8) step(s0, i & 1, ((i & 1) ^ 1) * TILE, (i & 1) * TILE);
-            else step(s0, i & 1, after * 2 * RAW, slot * 2 * RAW);
-            if (flags[i & 1] == i) odd_values(s0);
+            if (Q8) step(i, (~i & 1) * TILE, (i & 1) * TILE, (i & 1) * TILE, 0, before, s, y);
+            else step(i, after * 2 * RAW, slot * 2 * RAW, after2 * 2 * RAW, after * 2 * RAW, before, s, y);
+            if (s0 + T > n_blk && flags[i & 3] == i) odd_values(s0);
+        } else if (i + D - 1 < tiles) {
+#pragma unroll
+            for (int x = 0; x < NI; x++) load_piece(i + D - 1, before, x);
+            load_scales(i + D - 1, before);
         }
-        if constexpr (Q8) decode(i + 2, false), decode(i + 1, true);
-        else look(i + 1);
+        if (((i + D) & 63) == 0) fetch_pages(i + D);
+        if constexpr (Q8) decode(i + LEAD, false), decode(i + 1, true);
+        else look(i + LEAD);
         slot = after;
+    };
+    for (int i = 0; i < tiles; i += 2) {
+        tile(i, sa, sb);
+        if (i + 1 < tiles) tile(i + 1, sb, sa);
     }
     wait_dma<0>();
     const float lt = sum_halves(l);
     if (it.n_parts == 1) {
+        const OutRow out(g, it, r, lt);
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) finish(g, it, r, 32 * d + 8 * c + 4 * hf, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]}, lt);
+            for (int c = 0; c < 4; c++) out.put(32 * d + 8 * c + 4 * hf, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]});
         return;
     }
     constexpr int ROWS = 32 * NW;
@@ -826,7 +887,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 #pragma unroll
         for (int u = 0; u < NW; u++) lt += ls[u][row] * part_scale(ms[u][row], mm);
         if (it.n_parts == 1) {
-            finish(g, it, it.row0 + row, d, v, lt);
+            OutRow(g, it, it.row0 + row, lt).put(d, v);
         } else {
             const uint32_t at = (uint32_t)((it.part * ROWS + row) * PARTF<HDP>) * 4u;
             buf_store16(rp, v, at + (uint32_t)d * 4u);
