@@ -101,7 +101,7 @@ void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const 
         if (bl[body].empty()) continue;
         const bool stream = body <= HQ_STREAM32;
         const int unit = stream ? 128 : 64;
-        const int slots = n_cu * (stream || body == HQ_ROWS128 ? 2 : 1);
+        const int slots = n_cu * (stream || (body == HQ_ROWS128 && kv.head_dim <= 128) ? 2 : 1);  // workgroups at a time
         const int L = piece_length(bl[body], unit, slots, stream ? 128 : 192, 256);
         std::vector<HqItem> all;
         for (const Block &b : bl[body]) {

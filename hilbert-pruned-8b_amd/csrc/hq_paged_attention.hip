@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 
 #include "hq_batch.h"
 #include "hq_device.h"
@@ -145,8 +146,10 @@ struct OutRow {
 template <int HDP>
 constexpr int PARTF = HDP + HQ_PART_EXTRA;
 
+// scratch: LDS for 2 ROWS JOIN floats, which the workgroup is done with.
+constexpr int JOIN = 16;  // parts whose (maximum, sum) are in LDS at a time
 template <int HDP, int ROWS, int NT>
-DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
+DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float *scratch) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -156,36 +159,75 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
     }
     __syncthreads();
     if (!*flag) return;
-    constexpr int C = HDP / 4;
-    for (int x = threadIdx.x; x < ROWS * C; x += NT) {
-        const int row = x / C, d = 4 * (x % C);
-        if (it.row0 + row >= it.R) continue;
-        float m = -INFINITY, l = 0.f;
-        f4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int p0 = 0; p0 < it.n_parts; p0 += 4) {
-            f4 y[4], ml[4];
+    // a thread takes four dims of every (NT / C)-th row, RU rows and PU parts at a time
+    constexpr int C = HDP / 4, STEP = NT / C;
+    constexpr bool FEW = ROWS <= 32;  // a (maximum, sum) is then read by each thread, in the same round trip
+    constexpr int RU = FEW ? (ROWS + STEP - 1) / STEP : 8, PU = 4;
+    static_assert(NT % C == 0 || HDP == 96 || HDP == 192, "whole rows per pass");
+    f2 *const ml = (f2 *)scratch;
+    const int d = 4 * (threadIdx.x % C), first = threadIdx.x / C;
+    const int rows = std::min(ROWS, it.R - it.row0);
+    for (int r0 = 0; r0 < rows; r0 += STEP * RU) {
+        float m[RU], l[RU];
+        f4 v[RU];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t at = (uint32_t)((std::min(p0 + e, it.n_parts - 1) * ROWS + row) * PARTF<HDP>) * 4u;
-                ml[e] = buf_load16_sc1(rp, at + HDP * 4u, 0);
-                y[e] = buf_load16_sc1(rp, at + (uint32_t)d * 4u, 0);
+        for (int u = 0; u < RU; u++) m[u] = -INFINITY, l[u] = 0.f, v[u] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < it.n_parts; p0 += JOIN) {
+            if (!FEW && (r0 == 0 || it.n_parts > JOIN)) {
+                __syncthreads();
+                for (int x = threadIdx.x; x < ROWS * std::min(JOIN, it.n_parts - p0); x += NT) {
+                    const f4 y = buf_load16_sc1(rp, (uint32_t)((p0 * ROWS + x) * PARTF<HDP> + HDP) * 4u, 0);
+                    ml[x] = f2{y.x, y.y};
+                }
+                __syncthreads();
             }
+            if (first >= STEP) continue;
+            for (int p1 = p0; p1 < std::min(p0 + JOIN, it.n_parts); p1 += PU) {
+                f4 y[RU][PU], zz[RU][PU];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (p0 + e >= it.n_parts) continue;
-                const float mn = fmaxf(m, ml[e].x), a = part_scale(m, mn), b = part_scale(ml[e].x, mn);
-                v = v * a + y[e] * b;
-                l = l * a + ml[e].y * b;
-                m = mn;
+                for (int u = 0; u < RU; u++)
+#pragma unroll
+                    for (int e = 0; e < PU; e++) {
+                        const int row = std::min(r0 + first + u * STEP, ROWS - 1), p = std::min(p1 + e, it.n_parts - 1);
+                        y[u][e] = buf_load16_sc1(rp, (uint32_t)((p * ROWS + row) * PARTF<HDP> + d) * 4u, 0);
+                        if (FEW) zz[u][e] = buf_load16_sc1(rp, (uint32_t)((p * ROWS + row) * PARTF<HDP> + HDP) * 4u, 0);
+                    }
+#pragma unroll
+                for (int u = 0; u < RU; u++)
+#pragma unroll
+                    for (int e = 0; e < PU; e++) {
+                        if (p1 + e >= it.n_parts) continue;
+                        f2 z;
+                        if (FEW) z = f2{zz[u][e].x, zz[u][e].y};
+                        else z = ml[(p1 + e - p0) * ROWS + std::min(r0 + first + u * STEP, ROWS - 1)];
+                        const float mn = fmaxf(m[u], z.x), a = part_scale(m[u], mn), b = part_scale(z.x, mn);
+                        v[u] = v[u] * a + y[u][e] * b;
+                        l[u] = l[u] * a + z.y * b;
+                        m[u] = mn;
+                    }
             }
         }
-        OutRow(g, it, it.row0 + row, l).put(d, v);
+        if (first < STEP)
+#pragma unroll
+            for (int u = 0; u < RU; u++) {
+                const int row = r0 + first + u * STEP;
+                if (row < rows) OutRow(g, it, it.row0 + row, l[u]).put(d, v[u]);
+            }
     }
 }
 
 // (through the scalar cache: p is the same in every lane; the table does not change while a kernel runs)
 typedef const __attribute__((address_space(4))) uint32_t const_u32;
 DEV uint32_t page_of(const Args &g, const HqItem &it, int p) { return ((const_u32 *)(uintptr_t)g.pages)[it.page0 + (p >> g.shift)]; }
+
+// f(0) .. f(N - 1), each index a constant
+template <int N, class F>
+DEV void unrolled(F f) {
+    if constexpr (N > 0) {
+        unrolled<N - 1>(f);
+        f(std::integral_constant<int, N - 1>());
+    }
+}
 
 // ------------------------------------------------------------------------------------ rows
 // Row pitch of an LDS tile and the XOR of its 16-byte pieces: 16 rows that follow each other put a piece on 16 different
@@ -204,19 +246,24 @@ DEV const void *uniform(const void *p) {
     return (const void *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x));
 }
 // LDS DMA: lane i's 16 (4) bytes at base + off land at lds + 16 i (4 i). Untracked by the compiler, which would otherwise wait
-// for all of them before every LDS read: callers wait with wait_dma. M0 is restored.
-DEV void dma16_global(const void *base, uint32_t off, uint32_t lds) {
+// for all of them before every LDS read: callers wait with wait_dma.
+// `lanes`: which take part; as data, so that a conditional load is no branch. m0 and exec are restored.
+DEV void dma16_global(const void *base, uint32_t off, uint32_t lds, uint64_t lanes) {
     uint32_t save;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(save)
-                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(uniform(base))
+    uint64_t all;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b64 %1, exec\n\ts_mov_b32 m0, %2\n\ts_mov_b64 exec, %5\n\ts_nop 1\n\t"
+                 "global_load_lds_dwordx4 %3, %4\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save), "=&s"(all)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(uniform(base)), "s"(lanes)
                  : "memory");
 }
-DEV void dma4_global(const void *at, uint32_t lds) {
+DEV void dma4_global(const void *at, uint32_t lds, uint64_t lanes) {
     uint32_t save;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(save)
-                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at)
+    uint64_t all;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b64 %1, exec\n\ts_mov_b32 m0, %2\n\ts_mov_b64 exec, %4\n\ts_nop 1\n\t"
+                 "global_load_lds_dword %3, off\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save), "=&s"(all)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at), "s"(lanes)
                  : "memory");
 }
 template <int N>
@@ -245,7 +292,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     constexpr int LEAD = (Q8 ? 2 : 1) + (PRE ? 1 : 0);  // tile i + LEAD is in LDS when tile i's turn comes
     constexpr int RING = Q8 ? 4 * TILE : 0, SCALES = RING + D * 2 * RAW;  // Q8: K, K, V, V decoded; the ring; its scales
     __shared__ __align__(1024) char lds[SCALES + (Q8 ? D * 128 : 0)];
-    __shared__ int flags[4], last;
+    __shared__ int found_odd, last;
     __shared__ __align__(16) float fac[Q8 ? 6 * T : 4];  // Q8: what a position's scores take (key scale, score scale), four tiles; its weight, two
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
@@ -257,18 +304,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const int end = std::min(it.k1, n), tiles = end > it.k0 ? (end - it.k0 + T - 1) / T : 0;
     const int wn = std::min(end, r0 < it.R ? it.base + (std::min(it.R, r0 + 32) - 1) / rep + 1 : 0), wn_all = it.base + r0 / rep + 1;
     const int lim = it.base + std::min(r, it.R - 1) / rep + 1;
-    if (threadIdx.x < 4) flags[threadIdx.x] = -1;
-
-    h8 q[NJ];
-    {
-        const int rr = std::min(r, it.R - 1), t = rr / rep, h = it.kvh * rep + rr - t * rep;
-        const _Float16 *p = (const _Float16 *)g.a.q + (size_t)(it.tok0 + t) * g.a.q_stride + (size_t)h * hd;
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            const int d = 16 * j + 8 * hf;
-            q[j] = d < hd ? *(const h8 *)(p + d) : h8{};
-        }
-    }
+    if (threadIdx.x == 0) found_odd = 0;
 
     // The ring: wave w takes rows RPI NI (w % WM) .. of one matrix, a run within 16 rows and so within a page, 16-byte pieces in
     // NI loads. A piece's place in LDS is the lane's, so the lane takes the piece that belongs there. Pieces past head_dim stay 0.
@@ -282,13 +318,14 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const size_t page_b = (size_t)g.kv.page_stride * es;
     const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es), pmask = (uint32_t)g.kv.page_size - 1;
     const uint32_t to_w = at0 + RING + (values ? RAW : 0) + row_w * RAWP;
-    uint32_t piece_at[NI];  // byte of the lane's piece in a row
-    bool on[NI];
+    uint32_t piece_at[NI];  // byte of the lane's piece in its row
+    int row_at[NI];         // its row in the run
+    uint64_t on[NI];        // lanes whose piece is one
 #pragma unroll
     for (int x = 0; x < NI; x++) {
         const int row = row_w + RPI * x + lane / LPR, place = lane % LPR, piece = Q8 ? place : place ^ swizzle<HDP>(row);
-        on[x] = piece * (Q8 ? 16 : 8) < hd;
-        piece_at[x] = (uint32_t)piece * 16u;
+        on[x] = loads ? __ballot(piece * (Q8 ? 16 : 8) < hd) : 0;
+        piece_at[x] = (uint32_t)piece * 16u, row_at[x] = row & 15;
     }
     // Pages: lane t holds those of the wave's rows (Q8: of both runs of 16) of tile 64 c + t; read again every 64 tiles. (A scalar
     // load per tile would be waited for at every barrier.)
@@ -300,27 +337,30 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             asm volatile("" : "+v"(pages[x]));  // here, not where they are used
         }
     };
-    auto page_in = [&](int i, int x) { return (uint32_t)__builtin_amdgcn_readlane((int)pages[x], i & 63); };
-    // load x of tile i (the caller has checked that there is one), which goes to `slot`
-    auto load_piece = [&](int i, int slot, int x) {
-        if (!loads) return;
-        // (rows behind the last position: the last one's again, their weight is 0)
-        const uint32_t in = (uint32_t)std::min(it.k0 + i * T + row_w + RPI * x + lane / LPR, n - 1) & pmask;
-        const char *const base = kv0 + (size_t)page_in(i, Q8 ? row_w >> 4 : 0) * page_b;
-        const uint32_t at = in * pos_b + piece_at[x], to = to_w + slot * 2 * RAW + RPI * x * RAWP;
-        if (hd == HDP) dma16_global(base, at, to);
-        else if (on[x]) dma16_global(base, at, to);
+    auto page_in = [&](int i, bool second) { return (uint32_t)__builtin_amdgcn_readlane((int)(second ? pages[Q8 ? 1 : 0] : pages[0]), i & 63); };
+    // The wave's rows of tile i in memory: their run of 16, its last row that is to be read (behind the last position: that one
+    // again, its weight is 0), and whether there is such a tile. The load of piece x to `slot`.
+    struct Run {
+        const char *at;
+        int last;
+        bool is;
+    };
+    auto run_of = [&](int i) {
+        const int first = std::min(it.k0 + i * T + (row_w & ~15), (n - 1) & ~15);
+        return Run{kv0 + (size_t)page_in(i, Q8 && row_w >= 16) * page_b + (size_t)((uint32_t)first & pmask) * pos_b, n - 1 - first, i < tiles};
+    };
+    auto load_piece = [&](const Run &run, int slot, int x) {
+        const uint32_t at = (uint32_t)std::min(row_at[x], run.last) * pos_b + piece_at[x];
+        dma16_global(run.at, at, to_w + slot * 2 * RAW + RPI * x * RAWP, run.is ? on[x] : 0);
     };
     auto load_scales = [&](int i, int slot) {
-        if (!Q8 || w != 0) return;
-        const uint32_t page0 = page_in(i, 0), page1 = page_in(i, Q8 ? 1 : 0);
-        if (lane >= 32) return;
+        if (!Q8) return;
         // two positions a lane: lanes 0 .. 15 keys', 16 .. 31 values'; whole runs of 16 (what lies behind the last position is
         // not used)
-        const int p = it.k0 + i * T + 2 * (lane & 15);
-        const uint32_t page = lane & 8 ? page1 : page0;
-        const uint16_t *const sc = lane < 16 ? g.kv.k_scale : g.kv.v_scale;
-        dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + ((uint32_t)p & pmask), at0 + SCALES + slot * 128);
+        const uint32_t p = (uint32_t)(it.k0 + i * T + 2 * (lane & 15));
+        const uint32_t page = lane & 8 ? page_in(i, true) : page_in(i, false);
+        const uint16_t *const sc = lane & 16 ? g.kv.v_scale : g.kv.k_scale;
+        dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + (p & pmask), at0 + SCALES + slot * 128, w == 0 && i < tiles ? 0xffffffffull : 0);
     };
     // until tile i of the `issued` that are on their way or here is here, at most AFTER tiles behind it
     auto wait_tile = [&](int i, int issued, auto after) {
@@ -344,7 +384,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             if (piece * 16 >= hd) lo = hi = h8{};
             if (piece == 0) fac[(val ? 4 + buf : i & 3) * T + row] = val ? rest_of(d) : h2f((uint16_t)d) * g.sc;
             if (val && s0 + T > n_blk && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi))))
-                lo = finite8(lo), hi = finite8(hi), flags[i & 3] = i;
+                lo = finite8(lo), hi = finite8(hi), found_odd = 1;
             char *const to = lds + (2 * val + buf) * TILE + row * P;
             const int at = (2 * piece) ^ swizzle<HDP>(row);
             *(h8 *)(to + at * 16) = lo;
@@ -357,11 +397,12 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         for (int x = threadIdx.x; x < TILE / 16; x += 64 * NW) {
             u4v *const at = (u4v *)(lds + (i % D) * 2 * RAW + RAW + x * 16);
             const u4v v = *at;
-            if (odd16(v)) *at = finite16(v), flags[i & 3] = i;
+            if (odd16(v)) *at = finite16(v), found_odd = 1;
         }
     };
 
     float mx = -INFINITY;                      // of the lane's scores of the tile whose turn it is
+    h8 q[NJ];
     float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores; Q8: in log2 units), what the exponents are taken against, the sum
     f16v o[ND], sa[KB], sb[KB];  // outputs; scores of a tile and of the next
 #pragma unroll
@@ -416,8 +457,13 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     // values beside the maxima of the new scores.
     auto step = [&](int i, uint32_t k_at, uint32_t v_at, uint32_t k_pre, uint32_t v_pre, int to, f16v (&s)[KB], f16v (&y)[KB]) {
         const int s0 = it.k0 + i * T;
-        if (!PRE) read_keys(k_at);
-        if (!PREV) read_values(v_at);
+        // (without PRE operands are read AHEAD products before theirs)
+        constexpr int AHEAD = 4;
+        h8 kr[AHEAD], vr[AHEAD];
+        if (!PRE)
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) kr[j] = key_operand(k_at, j, 0);
+        if (PRE && !PREV) read_values(v_at);
         if (s0 + T > wn_all) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[0][e] = s0 + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[0][e] : -INFINITY;
@@ -435,7 +481,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= a;
         }
-        const bool more = i + D - 1 < tiles;
+        const Run run = run_of(i + D - 1);
         zero_scores(y);
         float x[16];
         h8 p[2], vg[ND];
@@ -459,68 +505,63 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             if (!Q8) l = __builtin_amdgcn_fdot2(y2, h2{(_Float16)1.f, (_Float16)1.f}, l, false);  // (the weights as they are multiplied)
         };
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            y[0] = mfma32(kf[j], q[j], y[0]);
+        unrolled<NJ>([&](auto index) {
+            constexpr int j = decltype(index)::value;
+            if constexpr (PRE) {
+                y[0] = mfma32(kf[j], q[j], y[0]);
+            } else {
+                y[0] = mfma32(kr[j % AHEAD], q[j], y[0]);
+                if constexpr (j + AHEAD < NJ) kr[j % AHEAD] = key_operand(k_at, j + AHEAD, 0);
+                else vr[j + AHEAD - NJ] = value_operand(v_at, (j + AHEAD - NJ) % ND, (j + AHEAD - NJ) / ND);
+            }
 #pragma unroll
             for (int c = 8 * j / NJ; c < 8 * (j + 1) / NJ; c++) {
                 weigh(c);
                 if (c) round(c - 1);
             }
-            if (j < ND) vg[j] = value_operand(v_at, j, 1);
-            if (more) {
+            if constexpr (PRE && j < ND) vg[j] = value_operand(v_at, j, 1);
 #pragma unroll
-                for (int x = NI * j / NJ; x < NI * (j + 1) / NJ; x++) load_piece(i + D - 1, to, x);
-                if (j == NJ - 1) load_scales(i + D - 1, to);
-            }
+            for (int x = NI * j / NJ; x < NI * (j + 1) / NJ; x++) load_piece(run, to, x);
+            if constexpr (j == NJ - 1) load_scales(i + D - 1, to);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
         round(7);
         float my = -INFINITY;
+        if constexpr (!PRE) {
+            unrolled<2 * ND>([&](auto index) {
+                constexpr int t = decltype(index)::value, d = t % ND;
+                o[d] = mfma32(vr[t % AHEAD], p[t / ND], o[d]);
+                if constexpr (t + AHEAD < 2 * ND) vr[t % AHEAD] = value_operand(v_at, (t + AHEAD) % ND, (t + AHEAD) / ND);
+                if constexpr (t + 1 == ND) scale_scores(y, i + 1);
+                if constexpr (t >= ND)
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            o[d] = mfma32(vf[d], p[0], o[d]);
-            if (PRE)
+                    for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        } else {
 #pragma unroll
-                for (int j = NJ * d / (2 * ND); j < NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        scale_scores(y, i + 1);
+            for (int d = 0; d < ND; d++) {
+                o[d] = mfma32(vf[d], p[0], o[d]);
+                if (PRE)
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            o[d] = mfma32(vg[d], p[1], o[d]);
-            if (PRE)
+                    for (int j = NJ * d / (2 * ND); j < NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            scale_scores(y, i + 1);
 #pragma unroll
-                for (int j = NJ / 2 + NJ * d / (2 * ND); j < NJ / 2 + NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
-            if (PREV) vf[d] = value_operand(v_pre, d, 0);
+            for (int d = 0; d < ND; d++) {
+                o[d] = mfma32(vg[d], p[1], o[d]);
+                if (PRE)
 #pragma unroll
-            for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int j = NJ / 2 + NJ * d / (2 * ND); j < NJ / 2 + NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
+                if (PREV) vf[d] = value_operand(v_pre, d, 0);
+#pragma unroll
+                for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         mx = my;
     };
-    // the odd values of the tile at s0, position by position
-    auto odd_values = [&](int s0) {
-#pragma clang loop unroll(disable)
-        for (int at = s0; at < std::min(s0 + T, wn); at++) {
-            const uint32_t page = page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
-            const char *const v = (const char *)g.kv.v + ((size_t)it.kvh * (size_t)g.kv.head_stride + (size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
-            const _Float16 d8 = Q8 ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in])) : (_Float16)0.f;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int dim = 32 * d + 8 * c + 4 * hf;
-                    if (at >= lim || dim >= hd) continue;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const _Float16 x = Q8 ? (_Float16)(float)((const int8_t *)v)[dim + e] * d8 : ((const _Float16 *)v)[dim + e];
-                        if (odd(x)) o[d][4 * c + e] += (float)x;
-                    }
-                }
-        }
-    };
-
     if (tiles) {
         if (!Q8 && hd < HDP)  // (decode() writes zeros itself)
             for (int x = threadIdx.x; x < D * 2 * RAW / 16; x += 64 * NW) *(u4v *)(lds + x * 16) = u4v{0, 0, 0, 0};
@@ -528,10 +569,19 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         barrier();
 #pragma unroll
         for (int i = 0; i < D - 1; i++) {
-            if (i < tiles) {
+            const Run run = run_of(i);
 #pragma unroll
-                for (int x = 0; x < NI; x++) load_piece(i, i, x);
-                load_scales(i, i);
+            for (int x = 0; x < NI; x++) load_piece(run, i, x);
+            load_scales(i, i);
+        }
+        // (after the loads: what waits for the pages must not wait for the queries)
+        {
+            const int rr = std::min(r, it.R - 1), t = rr / rep, h = it.kvh * rep + rr - t * rep;
+            const _Float16 *p = (const _Float16 *)g.a.q + (size_t)(it.tok0 + t) * g.a.q_stride + (size_t)h * hd;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const int d = 16 * j + 8 * hf;
+                q[j] = d < hd ? *(const h8 *)(p + d) : h8{};
             }
         }
         wait_tile(LEAD - 1, std::min(D - 1, tiles), std::integral_constant<int, D - 1 - LEAD>());
@@ -569,10 +619,10 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         if (s0 < wn) {
             if (Q8) step(i, (~i & 1) * TILE, (i & 1) * TILE, (i & 1) * TILE, 0, before, s, y);
             else step(i, after * 2 * RAW, slot * 2 * RAW, after2 * 2 * RAW, after * 2 * RAW, before, s, y);
-            if (s0 + T > n_blk && flags[i & 3] == i) odd_values(s0);
-        } else if (i + D - 1 < tiles) {
+        } else {
+            const Run run = run_of(i + D - 1);
 #pragma unroll
-            for (int x = 0; x < NI; x++) load_piece(i + D - 1, before, x);
+            for (int x = 0; x < NI; x++) load_piece(run, before, x);
             load_scales(i + D - 1, before);
         }
         if (((i + D) & 63) == 0) fetch_pages(i + D);
@@ -585,6 +635,38 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         if (i + 1 < tiles) tile(i + 1, sb, sa);
     }
     wait_dma<0>();
+    __syncthreads();
+    if (found_odd) {
+        // the odd values of the tiles that some row sees only part of, position by position
+#pragma clang loop unroll(disable)
+        for (int at = it.k0 + (std::max(n_blk, it.k0) - it.k0) / T * T; at < wn; at++) {
+            const uint32_t page = page_of(g, it, at), in = (uint32_t)at & (uint32_t)(g.kv.page_size - 1);
+            const char *const v = (const char *)g.kv.v + ((size_t)it.kvh * (size_t)g.kv.head_stride + (size_t)page * (size_t)g.kv.page_stride + (size_t)in * (size_t)g.kv.pos_stride) * es;
+            const _Float16 d8 = Q8 ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(g.kv.v_scale[((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + in])) : (_Float16)0.f;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int dim = 32 * d + 8 * c + 4 * hf;
+                    h4 x = {};
+                    if (dim < hd) {
+                        if (Q8) {
+                            const uint32_t q4 = *(const uint32_t *)(v + dim);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[e] = (_Float16)(float)(int8_t)byte_of(q4, e) * d8;
+                        } else {
+                            x = *(const h4 *)(v + 2 * dim);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y = (float)x[e], rest = y - fminf(fmaxf(y, -65504.f), 65504.f);  // 0, or what is odd of it
+                        o[d][4 * c + e] += at < lim ? rest : 0.f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    }
     const float lt = sum_halves(l);
     if (it.n_parts == 1) {
         const OutRow out(g, it, r, lt);
@@ -603,7 +685,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         for (int c = 0; c < 4; c++)
             buf_store16(rp, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]}, at + (uint32_t)(32 * d + 8 * c + 4 * hf) * 4u);
     if (hf == 0) buf_store16(rp, f4{m == -INFINITY ? -INFINITY : mref, lt, 0.f, 0.f}, at + HDP * 4u);
-    join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last);
+    static_assert(2 * 4 * ROWS * JOIN <= sizeof lds, "the parts' maxima and sums in the ring");
+    join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last, (float *)lds);
 }
 
 // ------------------------------------------------------------------------------------ stream
@@ -894,7 +977,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
             if (d == 0) buf_store16(rp, f4{mm, lt, 0.f, 0.f}, at + HDP * 4u);
         }
     }
-    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last);
+    static_assert(2 * 4 * ROWS * JOIN <= sizeof os, "the parts' maxima and sums in the waves' arena");
+    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last, &os[0][0][0]);
 }
 
 template <bool Q8>
