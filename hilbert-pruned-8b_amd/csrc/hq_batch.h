@@ -15,6 +15,8 @@ struct HqItem {
     int tok0;       // the sequence's first new token
     int base;       // the position of it
     int R, row0;
+    int t0, e0;     // row0 / rep and row0 % rep
+    int n;          // positions that the block's last row sees
     int k0, k1;
     int page0;      // its pages
     int part, n_parts;

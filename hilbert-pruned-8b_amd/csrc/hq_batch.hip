@@ -91,8 +91,8 @@ void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const 
         const int body = R <= 16 ? HQ_STREAM16 : R <= 32 && kv.head_dim <= 128 ? HQ_STREAM32 : R <= 128 || kv.head_dim > 128 ? HQ_ROWS128 : HQ_ROWS256;
         for (int h = 0; h < kv.n_kv_heads && R; h++)
             for (int row0 = (R - 1) / rows_of[body] * rows_of[body]; row0 >= 0; row0 -= rows_of[body]) {
-                const int n = std::max(0, base + (std::min(R, row0 + rows_of[body]) - 1) / rep + 1);
-                bl[body].push_back({{h, tok0, base, R, row0, 0, n, page0, 0, 1, 0, 0}, n});
+                const int see = base + (std::min(R, row0 + rows_of[body]) - 1) / rep + 1, n = std::max(0, see);
+                bl[body].push_back({{h, tok0, base, R, row0, row0 / rep, row0 % rep, see, 0, n, page0, 0, 1, 0, 0}, n});
             }
         tok0 += n_new[i];
         page0 += (n_pos[i] + kv.page_size - 1) / kv.page_size;
@@ -204,7 +204,7 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
     const char *const who = "hq_batch_set";
     if (!b || !kv) return hq_internal_fail("%s: null argument", who);
     if (check_geometry(who, kv)) return -1;
-    if (n_heads < 1 || n_heads % kv->n_kv_heads || n_heads > 65536)
+    if (n_heads < 1 || n_heads % kv->n_kv_heads || n_heads > 32768)
         return hq_internal_fail("%s: %d heads over %d kv heads", who, n_heads, kv->n_kv_heads);
     if (n_seqs < 0 || n_seqs > b->max_seqs) return hq_internal_fail("%s: %d sequences (the batch takes %d)", who, n_seqs, b->max_seqs);
     if (n_seqs && (!n_new || !n_pos)) return hq_internal_fail("%s: null argument", who);

@@ -40,8 +40,16 @@ struct Args {
     float *parts;
     int *counters;
     int nh, rep, shift;  // shift: log2 of the page size
+    uint32_t inverse;    // 2^32 / rep, rounded up; 0 for rep = 1
     float sc, slack;     // |scale| log2(e); how far a maximum may grow before the outputs are rescaled (raw scores; Q8: in log2 units)
 };
+
+// The new token that row `row0 + local` of an item's block is of (local and the remainder e0 together below 2^16 + 256, rep at
+// most 2^15: the product is exact).
+DEV int token_of(const Args &g, const HqItem &it, int local) {
+    const uint32_t x = (uint32_t)(it.e0 + local);
+    return it.t0 + (int)(g.inverse ? __umulhi(x, g.inverse) : x);
+}
 
 DEV f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
@@ -110,15 +118,15 @@ DEV void decode16(u4v c, _Float16 d, h8 &lo, h8 &hi) {
     hi = h8{o[4].x, o[4].y, o[5].x, o[5].y, o[6].x, o[6].y, o[7].x, o[7].y};
 }
 
-// Where row r of an item goes: its outputs v / l, gated, four dims at a time.
+// Where row `row0 + local` of an item goes: its outputs v / l, gated, four dims at a time.
 struct OutRow {
     _Float16 *out;  // null: not a row
     const char *gate;
     float inv;
     int hd, gate_f32;
-    __device__ __forceinline__ OutRow(const Args &g, const HqItem &it, int r, float l) : out(nullptr), gate(nullptr), inv(1.0f / l), hd(g.kv.head_dim), gate_f32(g.a.gate_f32) {
-        if (r >= it.R) return;
-        const int t = r / g.rep, h = it.kvh * g.rep + r - t * g.rep;
+    __device__ __forceinline__ OutRow(const Args &g, const HqItem &it, int local, float l) : out(nullptr), gate(nullptr), inv(1.0f / l), hd(g.kv.head_dim), gate_f32(g.a.gate_f32) {
+        if (it.row0 + local >= it.R) return;
+        const int t = token_of(g, it, local), h = it.kvh * g.rep + it.row0 + local - t * g.rep;
         const size_t tok = (size_t)(it.tok0 + t);
         out = (_Float16 *)g.a.out + tok * g.a.out_stride + (size_t)h * hd;
         if (g.a.gate) gate = (const char *)g.a.gate + (tok * g.a.gate_stride + (size_t)h * g.a.gate_head_stride) * (gate_f32 ? 4 : 2);
@@ -162,7 +170,7 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float
     // a thread takes four dims of every (NT / C)-th row, RU rows and PU parts at a time
     constexpr int C = HDP / 4, STEP = NT / C;
     constexpr bool FEW = ROWS <= 32;  // a (maximum, sum) is then read by each thread, in the same round trip
-    constexpr int RU = FEW ? (ROWS + STEP - 1) / STEP : 8, PU = 4;
+    constexpr int RU = FEW ? (ROWS + STEP - 1) / STEP : 8, PU = FEW || HDP > 128 ? 4 : 2;
     static_assert(NT % C == 0 || HDP == 96 || HDP == 192, "whole rows per pass");
     f2 *const ml = (f2 *)scratch;
     const int d = 4 * (threadIdx.x % C), first = threadIdx.x / C;
@@ -211,7 +219,7 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float
 #pragma unroll
             for (int u = 0; u < RU; u++) {
                 const int row = r0 + first + u * STEP;
-                if (row < rows) OutRow(g, it, it.row0 + row, l[u]).put(d, v[u]);
+                if (row < rows) OutRow(g, it, row, l[u]).put(d, v[u]);
             }
     }
 }
@@ -286,24 +294,20 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     constexpr int P = PITCH<HDP>, T = KT, KB = T / 32, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
     constexpr int RAWP = Q8 ? P / 2 : P, RAW = T * RAWP;  // a ring tile's pitch and bytes
     constexpr int LPR = RAWP / 16, RPI = 64 / LPR, UNITS = T / RPI, NI = 2 * UNITS > NW ? 2 * UNITS / NW : 1;
-    // With PRE a wave reads a tile's first operands before the barrier in front of it: K's, and for fp16 half of V's. The ring
-    // must be a tile deeper.
-    constexpr bool PRE = D >= 6, PREV = PRE && !Q8;
-    constexpr int LEAD = (Q8 ? 2 : 1) + (PRE ? 1 : 0);  // tile i + LEAD is in LDS when tile i's turn comes
+    constexpr int LEAD = Q8 ? 2 : 1;  // tile i + LEAD is in LDS when tile i's turn comes
     constexpr int RING = Q8 ? 4 * TILE : 0, SCALES = RING + D * 2 * RAW;  // Q8: K, K, V, V decoded; the ring; its scales
     __shared__ __align__(1024) char lds[SCALES + (Q8 ? D * 128 : 0)];
     __shared__ int found_odd, last;
-    __shared__ __align__(16) float fac[Q8 ? 6 * T : 4];  // Q8: what a position's scores take (key scale, score scale), four tiles; its weight, two
+    __shared__ __align__(16) float fac[Q8 ? 4 * T : 4];  // Q8, two tiles: what a position's scores take (key scale, score scale); its weight
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hf = lane >> 5;
-    const int hd = g.kv.head_dim, rep = g.rep;
-    const int r0 = it.row0 + 32 * w, r = r0 + li;
-    const int n = it.base + (std::min(it.R, it.row0 + 32 * NW) - 1) / rep + 1;  // positions some row of the block sees
-    const int n_blk = it.base + it.row0 / rep + 1;                              // positions every row of the block sees
+    const int hd = g.kv.head_dim, n = it.n;
+    const int r0 = it.row0 + 32 * w, mine = std::min(32 * w + li, it.R - 1 - it.row0);  // (rows past the last: that one again)
+    const int n_blk = it.base + it.t0 + 1;  // positions every row of the block sees
     const int end = std::min(it.k1, n), tiles = end > it.k0 ? (end - it.k0 + T - 1) / T : 0;
-    const int wn = std::min(end, r0 < it.R ? it.base + (std::min(it.R, r0 + 32) - 1) / rep + 1 : 0), wn_all = it.base + r0 / rep + 1;
-    const int lim = it.base + std::min(r, it.R - 1) / rep + 1;
+    const int wn = std::min(end, r0 < it.R ? it.base + token_of(g, it, std::min(32 * w + 31, it.R - 1 - it.row0)) + 1 : 0);
+    const int wn_all = it.base + token_of(g, it, 32 * w) + 1, lim = it.base + token_of(g, it, mine) + 1;
     if (threadIdx.x == 0) found_odd = 0;
 
     // The ring: wave w takes rows RPI NI (w % WM) .. of one matrix, a run within 16 rows and so within a page, 16-byte pieces in
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             h8 lo, hi;
             decode16(c, val ? __builtin_bit_cast(_Float16, (uint16_t)pow2_of(d)) : (_Float16)1.f, lo, hi);
             if (piece * 16 >= hd) lo = hi = h8{};
-            if (piece == 0) fac[(val ? 4 + buf : i & 3) * T + row] = val ? rest_of(d) : h2f((uint16_t)d) * g.sc;
+            if (piece == 0) fac[(2 * val + buf) * T + row] = val ? rest_of(d) : h2f((uint16_t)d) * g.sc;
             if (val && s0 + T > n_blk && (odd16(__builtin_bit_cast(u4v, lo)) || odd16(__builtin_bit_cast(u4v, hi))))
                 lo = finite8(lo), hi = finite8(hi), found_odd = 1;
             char *const to = lds + (2 * val + buf) * TILE + row * P;
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         for (int b = 0; b < KB; b++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const f4 f = *(const f4 *)&fac[(i & 3) * T + 32 * b + 8 * c + 4 * hf];
+                const f4 f = *(const f4 *)&fac[(i & 1) * T + 32 * b + 8 * c + 4 * hf];
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[b][4 * c + e] *= f[e];
             }
@@ -441,29 +445,17 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
             for (int e = 0; e < 16; e++) y[b][e] = 0.f;
     };
-    h8 kf[NJ], vf[ND];
-    auto read_keys = [&](uint32_t buf) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) kf[j] = key_operand(buf, j, 0);
-    };
-    auto read_values = [&](uint32_t buf) {
-#pragma unroll
-        for (int d = 0; d < ND; d++) vf[d] = value_operand(buf, d, 0);
-    };
     static_assert(KB == 1, "one block of scores a tile");
     // Scores s of tile i to weights, and its values' product; y: the scores of the tile after it (of whatever the buffer holds,
-    // behind the last). k_at, v_at: the next tile's keys and this one's values in LDS; k_pre, v_pre: what the next step starts
-    // with. Written out in the order of issue: a score product, its share of the exponentials and a load; then a product of
-    // values beside the maxima of the new scores.
-    auto step = [&](int i, uint32_t k_at, uint32_t v_at, uint32_t k_pre, uint32_t v_pre, int to, f16v (&s)[KB], f16v (&y)[KB]) {
+    // behind the last). k_at, v_at: the next tile's keys and this one's values in LDS. Written out in the
+    // order of issue: a score product, its share of the exponentials and a load; then a product of values beside the maxima of
+    // the new scores; operands are read AHEAD products before theirs.
+    auto step = [&](int i, uint32_t k_at, uint32_t v_at, int to, f16v (&s)[KB], f16v (&y)[KB]) {
         const int s0 = it.k0 + i * T;
-        // (without PRE operands are read AHEAD products before theirs)
         constexpr int AHEAD = 4;
         h8 kr[AHEAD], vr[AHEAD];
-        if (!PRE)
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++) kr[j] = key_operand(k_at, j, 0);
-        if (PRE && !PREV) read_values(v_at);
+        for (int j = 0; j < AHEAD; j++) kr[j] = key_operand(k_at, j, 0);
         if (s0 + T > wn_all) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[0][e] = s0 + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[0][e] : -INFINITY;
@@ -484,11 +476,11 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         const Run run = run_of(i + D - 1);
         zero_scores(y);
         float x[16];
-        h8 p[2], vg[ND];
+        h8 p[2];
         f4 f[Q8 ? 4 : 1];
         if (Q8)
 #pragma unroll
-            for (int c = 0; c < 4; c++) f[c] = *(const f4 *)&fac[(4 + (i & 1)) * T + 8 * c + 4 * hf];
+            for (int c = 0; c < 4; c++) f[c] = *(const f4 *)&fac[(2 + (i & 1)) * T + 8 * c + 4 * hf];
         // weights 2 c and 2 c + 1: their exponentials; later, as fp16 (and summed)
         auto weigh = [&](int c) {
 #pragma unroll
@@ -507,19 +499,14 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         __builtin_amdgcn_sched_barrier(0);
         unrolled<NJ>([&](auto index) {
             constexpr int j = decltype(index)::value;
-            if constexpr (PRE) {
-                y[0] = mfma32(kf[j], q[j], y[0]);
-            } else {
-                y[0] = mfma32(kr[j % AHEAD], q[j], y[0]);
-                if constexpr (j + AHEAD < NJ) kr[j % AHEAD] = key_operand(k_at, j + AHEAD, 0);
-                else vr[j + AHEAD - NJ] = value_operand(v_at, (j + AHEAD - NJ) % ND, (j + AHEAD - NJ) / ND);
-            }
+            y[0] = mfma32(kr[j % AHEAD], q[j], y[0]);
+            if constexpr (j + AHEAD < NJ) kr[j % AHEAD] = key_operand(k_at, j + AHEAD, 0);
+            else vr[j + AHEAD - NJ] = value_operand(v_at, (j + AHEAD - NJ) % ND, (j + AHEAD - NJ) / ND);
 #pragma unroll
             for (int c = 8 * j / NJ; c < 8 * (j + 1) / NJ; c++) {
                 weigh(c);
                 if (c) round(c - 1);
             }
-            if constexpr (PRE && j < ND) vg[j] = value_operand(v_at, j, 1);
 #pragma unroll
             for (int x = NI * j / NJ; x < NI * (j + 1) / NJ; x++) load_piece(run, to, x);
             if constexpr (j == NJ - 1) load_scales(i + D - 1, to);
@@ -527,39 +514,16 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         });
         round(7);
         float my = -INFINITY;
-        if constexpr (!PRE) {
-            unrolled<2 * ND>([&](auto index) {
-                constexpr int t = decltype(index)::value, d = t % ND;
-                o[d] = mfma32(vr[t % AHEAD], p[t / ND], o[d]);
-                if constexpr (t + AHEAD < 2 * ND) vr[t % AHEAD] = value_operand(v_at, (t + AHEAD) % ND, (t + AHEAD) / ND);
-                if constexpr (t + 1 == ND) scale_scores(y, i + 1);
-                if constexpr (t >= ND)
-#pragma unroll
-                    for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-        } else {
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                o[d] = mfma32(vf[d], p[0], o[d]);
-                if (PRE)
-#pragma unroll
-                    for (int j = NJ * d / (2 * ND); j < NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            scale_scores(y, i + 1);
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                o[d] = mfma32(vg[d], p[1], o[d]);
-                if (PRE)
-#pragma unroll
-                    for (int j = NJ / 2 + NJ * d / (2 * ND); j < NJ / 2 + NJ * (d + 1) / (2 * ND); j++) kf[j] = key_operand(k_pre, j, 0);
-                if (PREV) vf[d] = value_operand(v_pre, d, 0);
+        unrolled<2 * ND>([&](auto index) {
+            constexpr int t = decltype(index)::value, d = t % ND;
+            o[d] = mfma32(vr[t % AHEAD], p[t / ND], o[d]);
+            if constexpr (t + AHEAD < 2 * ND) vr[t % AHEAD] = value_operand(v_at, (t + AHEAD) % ND, (t + AHEAD) / ND);
+            if constexpr (t + 1 == ND) scale_scores(y, i + 1);
+            if constexpr (t >= ND)
 #pragma unroll
                 for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
+            __builtin_amdgcn_sched_barrier(0);
+        });
         mx = my;
     };
     if (tiles) {
@@ -567,16 +531,17 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             for (int x = threadIdx.x; x < D * 2 * RAW / 16; x += 64 * NW) *(u4v *)(lds + x * 16) = u4v{0, 0, 0, 0};
         fetch_pages(0);
         barrier();
-#pragma unroll
-        for (int i = 0; i < D - 1; i++) {
+        // the first tiles, then the queries (what waits for the pages must not wait for them), then the rest of the ring
+        auto load_tile = [&](int i) {
             const Run run = run_of(i);
 #pragma unroll
             for (int x = 0; x < NI; x++) load_piece(run, i, x);
             load_scales(i, i);
-        }
-        // (after the loads: what waits for the pages must not wait for the queries)
+        };
+#pragma unroll
+        for (int i = 0; i < LEAD; i++) load_tile(i);
         {
-            const int rr = std::min(r, it.R - 1), t = rr / rep, h = it.kvh * rep + rr - t * rep;
+            const int t = lim - 1 - it.base, h = it.kvh * g.rep + it.row0 + mine - t * g.rep;
             const _Float16 *p = (const _Float16 *)g.a.q + (size_t)(it.tok0 + t) * g.a.q_stride + (size_t)h * hd;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
@@ -584,41 +549,35 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
                 q[j] = d < hd ? *(const h8 *)(p + d) : h8{};
             }
         }
-        wait_tile(LEAD - 1, std::min(D - 1, tiles), std::integral_constant<int, D - 1 - LEAD>());
+        wait_dma<0>();
+#pragma unroll
+        for (int i = LEAD; i < D - 1; i++) load_tile(i);
         barrier();
         if constexpr (Q8) {
             decode(0, false), decode(1, false), decode(0, true);
         } else {
-#pragma unroll
-            for (int i = 0; i < LEAD; i++) look(i);
+            look(0);
         }
         barrier();
         if (g.a.scale < 0.f)
 #pragma unroll
             for (int j = 0; j < NJ; j++) q[j] = -q[j];
         zero_scores(sa);
-        read_keys(0);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) sa[0] = mfma32(kf[j], q[j], sa[0]);
+        for (int j = 0; j < NJ; j++) sa[0] = mfma32(key_operand(0, j, 0), q[j], sa[0]);
         scale_scores(sa, 0);
 #pragma unroll
         for (int e = 0; e < 16; e++) mx = fmaxf(mx, sa[0][e]);
-        if (PRE) read_keys(Q8 ? TILE : 2 * RAW);
-        if (PREV) read_values(0);
-        if constexpr (Q8 && PRE) {
-            barrier();  // the first tile's keys have been read
-            decode(2, false);
-        }
     }
     int slot = 0;  // i % D
     auto tile = [&](int i, f16v (&s)[KB], f16v (&y)[KB]) {
-        const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1, after2 = after == D - 1 ? 0 : after + 1;
+        const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1;
         // tile i + LEAD is there, the tiles behind it may still be on their way
         wait_tile(i + LEAD, std::min(i + D - 1, tiles), std::integral_constant<int, D - 2 - LEAD>());
         barrier();
         if (s0 < wn) {
-            if (Q8) step(i, (~i & 1) * TILE, (i & 1) * TILE, (i & 1) * TILE, 0, before, s, y);
-            else step(i, after * 2 * RAW, slot * 2 * RAW, after2 * 2 * RAW, after * 2 * RAW, before, s, y);
+            if (Q8) step(i, (~i & 1) * TILE, (i & 1) * TILE, before, s, y);
+            else step(i, after * 2 * RAW, slot * 2 * RAW, before, s, y);
         } else {
             const Run run = run_of(i + D - 1);
 #pragma unroll
@@ -669,11 +628,35 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     }
     const float lt = sum_halves(l);
     if (it.n_parts == 1) {
-        const OutRow out(g, it, r, lt);
+        const OutRow out(g, it, 32 * w + li, lt);
+        if (g.a.gate) {
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) out.put(32 * d + 8 * c + 4 * hf, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]});
+            return;
+        }
+        // through LDS (the ring is done with): 16 bytes a lane, whole rows an instruction
+        constexpr int PITCH_O = 2 * HDP + 16, LPO = HDP / 8;
+        static_assert(NW * 32 * PITCH_O <= sizeof lds, "the waves' outputs in the ring");
+        char *const mem = lds + w * 32 * PITCH_O;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) out.put(32 * d + 8 * c + 4 * hf, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]});
+            for (int c = 0; c < 4; c++) {
+                h4 y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = (_Float16)(o[d][4 * c + e] * out.inv);
+                *(h4 *)(mem + li * PITCH_O + 2 * (32 * d + 8 * c + 4 * hf)) = y;
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int x = lane; x < 32 * LPO; x += 64) {
+            const int row = x / LPO, d = 8 * (x % LPO);
+            if (r0 + row >= it.R || d >= hd) continue;
+            const int t = token_of(g, it, 32 * w + row), h = it.kvh * g.rep + r0 + row - t * g.rep;
+            *(u4v *)((_Float16 *)g.a.out + (size_t)(it.tok0 + t) * g.a.out_stride + (size_t)h * hd + d) = *(const u4v *)(mem + row * PITCH_O + 2 * d);
+        }
         return;
     }
     constexpr int ROWS = 32 * NW;
@@ -705,15 +688,15 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
-    const int hd = g.kv.head_dim, rep = g.rep;
-    const int n = it.base + (std::min(it.R, it.row0 + ROWS) - 1) / rep + 1, n_all = it.base + it.row0 / rep + 1;
+    const int hd = g.kv.head_dim;
+    const int n = it.n, n_all = it.base + it.t0 + 1;  // positions that some row, that every row sees
     const int end = std::min(it.k1, n);
 
     h8 q[QB][NJ];
     int lim[QB];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
-        const int r = std::min(it.row0 + 16 * b + li, it.R - 1), t = r / rep, h = it.kvh * rep + r - t * rep;
+        const int local = std::min(16 * b + li, it.R - 1 - it.row0), t = token_of(g, it, local), h = it.kvh * g.rep + it.row0 + local - t * g.rep;
         lim[b] = it.base + t + 1;
         const _Float16 *p = (const _Float16 *)g.a.q + (size_t)(it.tok0 + t) * g.a.q_stride + (size_t)h * hd;
 #pragma unroll
@@ -970,7 +953,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 #pragma unroll
         for (int u = 0; u < NW; u++) lt += ls[u][row] * part_scale(ms[u][row], mm);
         if (it.n_parts == 1) {
-            OutRow(g, it, it.row0 + row, lt).put(d, v);
+            OutRow(g, it, row, lt).put(d, v);
         } else {
             const uint32_t at = (uint32_t)((it.part * ROWS + row) * PARTF<HDP>) * 4u;
             buf_store16(rp, v, at + (uint32_t)d * 4u);
@@ -1036,7 +1019,8 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
     int cur = -1;
     SCK(hipGetDevice(&cur));
     if (cur != b->device) SCK(hipSetDevice(b->device));
-    Args g = {*kv, *a, nullptr, b->pages, b->parts, b->counters, b->n_heads, b->n_heads / kv->n_kv_heads, __builtin_ctz((unsigned)kv->page_size), 0.f, 0.f};
+    Args g = {*kv, *a, nullptr, b->pages, b->parts, b->counters, b->n_heads, b->n_heads / kv->n_kv_heads, __builtin_ctz((unsigned)kv->page_size), 0, 0.f, 0.f};
+    if (g.rep > 1) g.inverse = (uint32_t)((((uint64_t)1 << 32) + (uint64_t)g.rep - 1) / (uint64_t)g.rep);
     // (a smaller scale leaves every weight alike in fp32; 0 would make NaN of masked scores)
     g.sc = std::max(fabsf(a->scale) * 1.4426950408889634f, 1e-30f);
     g.slack = kv->type == HQ_KV_Q8 ? 8.0f : 8.0f / g.sc;  // weights up to 2^8 (2^9 with a value scale's mantissa) keep their 11 bits in fp16
