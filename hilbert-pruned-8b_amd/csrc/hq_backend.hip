@@ -31,11 +31,14 @@
 #include <string.h>
 #include <time.h>
 #include <algorithm>
+#include <new>
+#include <utility>
 #include <vector>
 
 #include "hq.h"
 #include "hq_attention.h"
 #include "hq_backend.h"
+#include "hq_serve.h"
 #include "hq_device.h"
 #include "hq_internal.h"
 #include "hq_kernels.h"
@@ -264,6 +267,18 @@ __global__ void __launch_bounds__(256) k_norm_readout(const float *__restrict__ 
     if (threadIdx.x == 0) logits[blockIdx.x] = acc;
 }
 
+// Row blockIdx.x of out: the final RMSNorm of row rows[blockIdx.x] of x, fp16 (the operand of the lm_head product).
+__global__ void __launch_bounds__(256) k_norm_rows(const float *__restrict__ x, const uint32_t *__restrict__ rows,
+                                                   const float *__restrict__ w, float off, float eps, _Float16 *__restrict__ out, int H) {
+    __shared__ float red[4];
+    const float *xr = x + (size_t)rows[blockIdx.x] * H;
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < H; i += 256) ss += xr[i] * xr[i];
+    ss = block_sum(ss, red);
+    const float inv = 1.0f / sqrtf(ss / (float)H + eps);
+    for (int i = threadIdx.x; i < H; i += 256) out[(size_t)blockIdx.x * H + i] = (_Float16)(xr[i] * inv * (off + w[i]));
+}
+
 unsigned blocks_for(size_t n, unsigned per) { return (unsigned)((n + per - 1) / per < 65535 ? (n + per - 1) / per : 65535); }
 
 // ------------------------------------------------------------------------------------ backend
@@ -365,58 +380,78 @@ int gemm(HipBackend *b, const hq_mat *W, const _Float16 *A, int T, float *C, boo
     return hq_gemm(W, (const uint16_t *)A, T, C, 1, accumulate ? 1 : 0, b->st);
 }
 
+// Where a layer's projections of T tokens stand: queries (with the gates) in rows of sq, keys and values in rows of skv.
+struct Qkv {
+    const float *q, *k, *v;
+    int sq, skv;
+};
+
+// A: what holds the activations, the backend itself or a hip_batch.
+template <class A>
+int norm_qkv(HipBackend *b, const A &a, const DevLayer &L, int T, Qkv *out) {
+    const hq_ref_config_t &c = b->m->cfg;
+    const int qw = (int)(c.n_heads * c.head_dim) * (c.attn_gate ? 2 : 1), kvw = (int)(c.n_kv_heads * c.head_dim);
+    // one token: the norm inside the GEMV where it has such a kernel
+    int fused = 0;
+    if (T == 1 && L.qkv) BCK(hq_launch_gemv_norm(hq_mat_dev(L.qkv), a.x, L.in_norm, c.norm_offset, c.eps, 0, a.qb, b->st, &fused));
+    if (!fused) {
+        k_rmsnorm<_Float16><<<T, 256, 0, b->st>>>(a.x, L.in_norm, c.norm_offset, c.eps, a.hb, (int)c.hidden);
+        BCK(hipGetLastError());
+    }
+    *out = {a.qb, a.kb, a.vb, qw, kvw};
+    if (L.qkv) {
+        if (!fused && gemm(b, L.qkv, a.hb, T, a.qb, false)) return -1;
+        *out = {a.qb, a.qb + qw, a.qb + qw + kvw, qw + 2 * kvw, qw + 2 * kvw};
+    } else if (gemm(b, L.q, a.hb, T, a.qb, false) || gemm(b, L.k, a.hb, T, a.kb, false) || gemm(b, L.v, a.hb, T, a.vb, false)) {
+        return -1;
+    }
+    return 0;
+}
+
+// x += o . ob, then the feed-forward block.
+template <class A>
+int out_ffn(HipBackend *b, const A &a, const DevLayer &L, int T) {
+    const hq_ref_config_t &c = b->m->cfg;
+    const int H = (int)c.hidden, I = (int)c.intermediate;
+    if (gemm(b, L.o, a.ob, T, a.x, true)) return -1;
+    int fused = 0;
+    if (T == 1 && L.pair) BCK(hq_launch_gemv_norm(hq_mat_dev(L.pair), a.x, L.post_norm, c.norm_offset, c.eps, 1, a.fb, b->st, &fused));
+    if (!fused) {
+        k_rmsnorm<_Float16><<<T, 256, 0, b->st>>>(a.x, L.post_norm, c.norm_offset, c.eps, a.hb, H);
+        BCK(hipGetLastError());
+    }
+    if (L.pair) {
+        if (!fused && hq_gemm_swiglu(L.pair, (const uint16_t *)a.hb, T, (uint16_t *)a.fb, b->st)) return -1;
+    } else if (T == 1) {
+        k_gateup_swiglu<<<(I + 3) / 4, 256, 0, b->st>>>(*hq_mat_dev(L.gate), *hq_mat_dev(L.up), a.hb, a.fb, I, H);
+        BCK(hipGetLastError());
+    } else {
+        if (gemm(b, L.gate, a.hb, T, a.gb, false) || gemm(b, L.up, a.hb, T, a.ub, false)) return -1;
+        k_swiglu<<<blocks_for((size_t)T * I, 256), 256, 0, b->st>>>(a.gb, a.ub, a.fb, (size_t)T * I);
+        BCK(hipGetLastError());
+    }
+    return gemm(b, L.down, a.fb, T, a.x, true);
+}
+
 // The layer loop over T tokens at position pos0; x holds their embedding rows.
 int run_layers(HipBackend *b, int T, int pos0) {
     const hq_ref_config_t &c = b->m->cfg;
-    const int H = (int)c.hidden, I = (int)c.intermediate, nh = (int)c.n_heads, nkv = (int)c.n_kv_heads;
-    const int hd = (int)c.head_dim, qw = nh * hd * (c.attn_gate ? 2 : 1);
-    const float off = c.norm_offset, eps = c.eps, scale = 1.0f / sqrtf((float)hd);
+    const int nh = (int)c.n_heads, nkv = (int)c.n_kv_heads, hd = (int)c.head_dim;
+    const float scale = 1.0f / sqrtf((float)hd);
     hipStream_t st = b->st;
     for (uint32_t li = 0; li < c.n_layers; li++) {
         const DevLayer &L = b->L[li];
-        // one token: the norm inside the GEMV where it has such a kernel
-        int fused = 0;
-        if (T == 1 && L.qkv) BCK(hq_launch_gemv_norm(hq_mat_dev(L.qkv), b->x, L.in_norm, off, eps, 0, b->qb, st, &fused));
-        if (!fused) {
-            k_rmsnorm<_Float16><<<T, 256, 0, st>>>(b->x, L.in_norm, off, eps, b->hb, H);
-            BCK(hipGetLastError());
-        }
-        const float *kb = b->kb, *vb = b->vb;
-        int sq = qw, skv = nkv * hd;
-        if (L.qkv) {
-            if (!fused && gemm(b, L.qkv, b->hb, T, b->qb, false)) return -1;
-            kb = b->qb + qw, vb = kb + skv;
-            sq = skv = qw + 2 * skv;
-        } else if (gemm(b, L.q, b->hb, T, b->qb, false) || gemm(b, L.k, b->hb, T, b->kb, false) ||
-                   gemm(b, L.v, b->hb, T, b->vb, false)) {
-            return -1;
-        }
+        Qkv p;
+        if (norm_qkv(b, *b, L, T, &p)) return -1;
         // few tokens: their heads over several workgroups, while there are fewer than 8 per CU
         const int rope_y = std::min((nh + nkv + ROPE_W - 1) / ROPE_W, std::max(8 * b->n_cu / T, 1));
-        k_qk_rope<<<dim3(T, rope_y), 64 * ROPE_W, 0, st>>>(b->qb, kb, vb, L.q_norm, L.k_norm, off, eps, b->inv_freq, b->qr,
-                                                           L.kc, L.vc, nh, nkv, hd, (int)c.rot_dim, sq, skv, skv,
+        k_qk_rope<<<dim3(T, rope_y), 64 * ROPE_W, 0, st>>>(p.q, p.k, p.v, L.q_norm, L.k_norm, c.norm_offset, c.eps, b->inv_freq,
+                                                           b->qr, L.kc, L.vc, nh, nkv, hd, (int)c.rot_dim, p.sq, p.skv, p.skv,
                                                            c.attn_gate, pos0, c.qk_norm);
         BCK(hipGetLastError());
-        const HqAttnArgs at = {b->qr, b->qb, L.kc, L.vc, b->ob, b->att_part, b->att_cnt, T, nh, nkv, hd, sq, c.attn_gate, pos0, scale};
+        const HqAttnArgs at = {b->qr, b->qb, L.kc, L.vc, b->ob, b->att_part, b->att_cnt, T, nh, nkv, hd, p.sq, c.attn_gate, pos0, scale};
         BCK(hq_launch_attention(at, b->n_cu, st));
-        if (gemm(b, L.o, b->ob, T, b->x, true)) return -1;
-        fused = 0;
-        if (T == 1 && L.pair) BCK(hq_launch_gemv_norm(hq_mat_dev(L.pair), b->x, L.post_norm, off, eps, 1, b->fb, st, &fused));
-        if (!fused) {
-            k_rmsnorm<_Float16><<<T, 256, 0, st>>>(b->x, L.post_norm, off, eps, b->hb, H);
-            BCK(hipGetLastError());
-        }
-        if (L.pair) {
-            if (!fused && hq_gemm_swiglu(L.pair, (const uint16_t *)b->hb, T, (uint16_t *)b->fb, st)) return -1;
-        } else if (T == 1) {
-            k_gateup_swiglu<<<(I + 3) / 4, 256, 0, st>>>(*hq_mat_dev(L.gate), *hq_mat_dev(L.up), b->hb, b->fb, I, H);
-            BCK(hipGetLastError());
-        } else {
-            if (gemm(b, L.gate, b->hb, T, b->gb, false) || gemm(b, L.up, b->hb, T, b->ub, false)) return -1;
-            k_swiglu<<<blocks_for((size_t)T * I, 256), 256, 0, st>>>(b->gb, b->ub, b->fb, (size_t)T * I);
-            BCK(hipGetLastError());
-        }
-        if (gemm(b, L.down, b->fb, T, b->x, true)) return -1;
+        if (out_ffn(b, *b, L, T)) return -1;
     }
     return 0;
 }
@@ -833,6 +868,219 @@ extern "C" hq_ref_backend_t *hip_backend_create(const hq_ref_model_t *m, size_t 
         return nullptr;
     }
     return &b->base;
+}
+
+// ------------------------------------------------------------------------------------ many sequences
+// The layer loop of run_layers with the paged operators in place of k_qk_rope and hq_launch_attention; the lm_head product
+// takes the last row of each sequence, and its logits stay on the device.
+struct hip_batch {
+    HipBackend *b = nullptr;
+    hq_batch *step = nullptr;
+    hq_kv_t kv = {};                  // of layer 0
+    std::vector<std::pair<void *, void *>> k, v;  // codes and scales of each layer
+    std::vector<void *> allocs;
+    int max_seqs = 0, max_tokens = 0, n_table = 0;
+    float *x = nullptr, *qb = nullptr, *kb = nullptr, *vb = nullptr, *gb = nullptr, *ub = nullptr, *table = nullptr, *logits = nullptr;
+    _Float16 *q = nullptr, *hb = nullptr, *ob = nullptr, *fb = nullptr;
+    uint32_t *d_in = nullptr, *h_in = nullptr;  // tokens, last rows, ids
+    size_t in_words = 0;
+    char *h_out = nullptr;  // pinned: logp, entropy, top_ids, top_logp; kernels write them
+    size_t out_bytes = 0;
+};
+
+namespace {
+
+int batch_init(hip_batch *s, HipBackend *b, int kv_type, int page_size, uint32_t n_pages, int max_seqs, int max_tokens, int max_pages) {
+    const hq_ref_config_t &c = b->m->cfg;
+    const char *const who = "hip_batch_create";
+    if (kv_type != HQ_KV_F16 && kv_type != HQ_KV_Q8) return hq_internal_fail("%s: cache type %d", who, kv_type);
+    if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1))) return hq_internal_fail("%s: page_size %d (a power of two, 16 .. 4096)", who, page_size);
+    if (c.head_dim % 16 || c.rot_dim % 8) return hq_internal_fail("%s: head_dim %u and rot_dim %u (multiples of 16 and of 8)", who, c.head_dim, c.rot_dim);
+    if (max_seqs < 1 || max_seqs > 65536 || max_tokens < 1 || max_tokens > 65536)
+        return hq_internal_fail("%s: %d sequences, %d tokens (1 .. 65536)", who, max_seqs, max_tokens);
+    if (n_pages < 1 || (uint64_t)n_pages * (uint64_t)page_size >= (1ull << 31) || max_pages < 1 || (int64_t)max_pages * page_size > (1 << 24))
+        return hq_internal_fail("%s: %u pages, %d a sequence (at least 1; below 2^31 positions, 2^24 a sequence)", who, n_pages, max_pages);
+    BCK(hipSetDevice(b->device));
+    s->b = b, s->max_seqs = max_seqs, s->max_tokens = max_tokens, s->n_table = max_pages * page_size;
+    if (hq_batch_create(b->device, max_seqs, max_tokens, max_pages, &s->step)) return -1;
+    const auto alloc = [&](auto **p, size_t bytes) {
+        *p = nullptr;
+        if (!bytes) return 0;
+        BCK(hipMalloc((void **)p, bytes));
+        s->allocs.push_back((void *)*p);
+        return 0;
+    };
+    const size_t H = c.hidden, hd = c.head_dim, I = c.intermediate, kvw = (size_t)c.n_kv_heads * hd, ow = (size_t)c.n_heads * hd;
+    const size_t qw = ow * (c.attn_gate ? 2 : 1), T = (size_t)max_tokens, positions = (size_t)n_pages * page_size;
+    // heads outermost in a page: a head's positions follow each other, whatever the number of heads
+    s->kv = {kv_type, page_size, (int)c.n_kv_heads, (int)hd, n_pages, nullptr, nullptr, nullptr, nullptr,
+             (int64_t)(page_size * kvw), (int64_t)hd, (int64_t)(page_size * hd)};
+    s->k.resize(c.n_layers), s->v.resize(c.n_layers);
+    for (uint32_t l = 0; l < c.n_layers; l++)
+        for (auto *m : {&s->k[l], &s->v[l]})
+            if (alloc(&m->first, positions * kvw * (kv_type == HQ_KV_Q8 ? 1 : 2)) || alloc(&m->second, kv_type == HQ_KV_Q8 ? positions * c.n_kv_heads * 2 : 0))
+                return -1;
+    bool qkv_one = false, kv_apart = false, gu_apart = false;
+    for (const DevLayer &d : b->L) qkv_one |= d.qkv != nullptr, kv_apart |= !d.qkv, gu_apart |= !d.pair;
+    const size_t Th = std::max(T, (size_t)max_seqs);  // rows of hb: the last ones of the sequences too
+    if (alloc(&s->x, T * H * 4) || alloc(&s->qb, T * (qw + (qkv_one ? 2 * kvw : 0)) * 4) || alloc(&s->kb, kv_apart ? T * kvw * 4 : 0) ||
+        alloc(&s->vb, kv_apart ? T * kvw * 4 : 0) || alloc(&s->gb, gu_apart ? T * I * 4 : 0) || alloc(&s->ub, gu_apart ? T * I * 4 : 0) ||
+        alloc(&s->q, T * ow * 2) || alloc(&s->hb, Th * H * 2) || alloc(&s->ob, T * ow * 2) || alloc(&s->fb, T * I * 2) ||
+        alloc(&s->table, (size_t)s->n_table * c.rot_dim * 4) || alloc(&s->logits, (size_t)max_seqs * c.vocab * 4))
+        return -1;
+    return c.rot_dim ? hq_rope_table(b->m->rope_inv_freq, (int)c.rot_dim, s->n_table, s->table, b->st) : 0;
+}
+
+// The step's host arrays, grown when a step needs more: what goes in, and what comes out.
+int batch_room(hip_batch *s, size_t in_words, size_t out_bytes) {
+    if (in_words > s->in_words) {
+        if (s->h_in) BCK(hipHostFree(s->h_in));
+        s->h_in = nullptr;
+        if (s->d_in) BCK(hipFree(s->d_in));
+        s->d_in = nullptr;
+        s->in_words = 0;
+        BCK(hipHostMalloc((void **)&s->h_in, in_words * 4, hipHostMallocDefault));
+        BCK(hipMalloc((void **)&s->d_in, in_words * 4));
+        s->in_words = in_words;
+    }
+    if (out_bytes > s->out_bytes) {
+        if (s->h_out) BCK(hipHostFree(s->h_out));
+        s->h_out = nullptr;
+        s->out_bytes = 0;
+        BCK(hipHostMalloc((void **)&s->h_out, out_bytes, hipHostMallocDefault));
+        s->out_bytes = out_bytes;
+    }
+    return 0;
+}
+
+int batch_layers(hip_batch *s, int T) {
+    HipBackend *b = s->b;
+    const hq_ref_config_t &c = b->m->cfg;
+    const int nh = (int)c.n_heads, hd = (int)c.head_dim, ow = nh * hd;
+    for (uint32_t li = 0; li < c.n_layers; li++) {
+        const DevLayer &L = b->L[li];
+        Qkv p;
+        if (norm_qkv(b, *s, L, T, &p)) return -1;
+        hq_kv_t kv = s->kv;
+        kv.k = s->k[li].first, kv.k_scale = (uint16_t *)s->k[li].second;
+        kv.v = s->v[li].first, kv.v_scale = (uint16_t *)s->v[li].second;
+        hq_rope_t r = {};
+        r.q = p.q, r.k = p.k, r.v = p.v, r.f32 = 1;
+        r.q_stride = p.sq, r.q_head_stride = c.attn_gate ? 2 * hd : hd, r.kv_stride = p.skv;
+        r.q_norm = L.q_norm, r.k_norm = L.k_norm, r.norm_offset = c.norm_offset, r.eps = c.eps;
+        r.table = s->table, r.n_table = s->n_table, r.rot_dim = (int)c.rot_dim, r.q_out = (uint16_t *)s->q;
+        if (hq_rope_append(s->step, &kv, &r, b->st)) return -1;
+        hq_attn_t a = {};
+        a.q = (const uint16_t *)s->q, a.q_stride = ow, a.scale = 1.0f / sqrtf((float)hd), a.out = (uint16_t *)s->ob, a.out_stride = ow;
+        if (c.attn_gate) a.gate = p.q + hd, a.gate_f32 = 1, a.gate_stride = p.sq, a.gate_head_stride = 2 * hd;
+        if (hq_attention(s->step, &kv, &a, b->st)) return -1;
+        if (out_ffn(b, *s, L, T)) return -1;
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int hip_batch_create(hq_ref_backend_t *backend, int kv_type, int page_size, uint32_t n_pages, int max_seqs, int max_tokens,
+                                int max_pages, hip_batch **out) {
+    if (!out) return hq_internal_fail("hip_batch_create: null argument");
+    *out = nullptr;
+    if (!backend || backend->destroy != be_destroy) return hq_internal_fail("hip_batch_create: not a backend of hip_backend_create");
+    hip_batch *s = new (std::nothrow) hip_batch();
+    if (!s) return hq_internal_fail("hip_batch_create: out of memory");
+    int rc;
+    try {
+        rc = batch_init(s, self(backend), kv_type, page_size, n_pages, max_seqs, max_tokens, max_pages);
+    } catch (const std::exception &) {
+        rc = hq_internal_fail("hip_batch_create: out of memory");
+    }
+    if (rc) {
+        char msg[512];
+        snprintf(msg, sizeof msg, "%s", hq_last_error());
+        hip_batch_free(s);
+        return hq_internal_fail("%s", msg);
+    }
+    *out = s;
+    return 0;
+}
+
+extern "C" void hip_batch_free(hip_batch *s) {
+    if (!s) return;
+    if (s->b) {
+        (void)hipSetDevice(s->b->device);
+        (void)hipStreamSynchronize(s->b->st);
+    }
+    hq_batch_free(s->step);
+    for (void *p : s->allocs) (void)hipFree(p);
+    if (s->d_in) (void)hipFree(s->d_in);
+    if (s->h_in) (void)hipHostFree(s->h_in);
+    if (s->h_out) (void)hipHostFree(s->h_out);
+    delete s;
+}
+
+extern "C" int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, const int32_t *n_new, const int32_t *n_pos,
+                              const uint32_t *pages, int pages_ld, const uint32_t *ids, int n_ids, int top_k, float *logp, float *entropy,
+                              uint32_t *top_ids, float *top_logp) {
+    const char *const who = "hip_batch_step";
+    if (!s) return hq_internal_fail("%s: null argument", who);
+    HipBackend *b = s->b;
+    const hq_ref_config_t &c = b->m->cfg;
+    if (n_seqs < 0 || n_seqs > s->max_seqs) return hq_internal_fail("%s: %d sequences (the batch takes %d)", who, n_seqs, s->max_seqs);
+    if (n_seqs && (!n_new || !n_pos)) return hq_internal_fail("%s: null argument", who);
+    if (n_ids < 0 || n_ids > MAX_IDS || (n_ids && logp && !ids)) return hq_internal_fail("%s: %d ids (0 .. %d)", who, n_ids, MAX_IDS);
+    if (top_k < 0 || top_k > HQ_LOGPROBS_MAX_TOP || (uint32_t)top_k > c.vocab)
+        return hq_internal_fail("%s: top_k %d (0 .. %d, at most the vocabulary's %u)", who, top_k, HQ_LOGPROBS_MAX_TOP, c.vocab);
+    if (!logp) n_ids = 0;
+    if (!top_ids && !top_logp) top_k = 0;
+    int64_t T = 0;
+    int rows = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        if (n_new[i] < 0 || n_new[i] > n_pos[i]) return hq_internal_fail("%s: sequence %d has %d new tokens of %d positions", who, i, n_new[i], n_pos[i]);
+        T += n_new[i], rows += n_new[i] > 0;
+    }
+    if (T > s->max_tokens) return hq_internal_fail("%s: %lld new tokens (the batch takes %d)", who, (long long)T, s->max_tokens);
+    if (T && !tokens) return hq_internal_fail("%s: null argument", who);
+    for (int64_t t = 0; t < T; t++)
+        if (tokens[t] >= c.vocab) return hq_internal_fail("%s: token %u out of range", who, tokens[t]);
+    for (size_t i = 0; i < (size_t)n_seqs * (size_t)n_ids; i++)
+        if (ids[i] >= c.vocab) return hq_internal_fail("%s: id %u out of range", who, ids[i]);
+    BCK(hipSetDevice(b->device));
+    const size_t n_lp = (size_t)rows * (size_t)n_ids, n_top = (size_t)rows * (size_t)top_k;
+    if (batch_room(s, (size_t)T + (size_t)rows + n_lp + 4, (n_lp + (size_t)rows + 2 * n_top + 4) * 4)) return -1;
+    if (hq_batch_set(s->step, &s->kv, (int)c.n_heads, n_seqs, n_new, n_pos, pages, pages_ld, b->st)) return -1;
+    if (!T) return 0;
+    uint32_t *const last = s->h_in + T, *const id = last + rows;
+    memcpy(s->h_in, tokens, (size_t)T * 4);
+    for (int i = 0, t = 0, r = 0; i < n_seqs; i++) {
+        t += n_new[i];
+        if (!n_new[i]) continue;
+        last[r] = (uint32_t)(t - 1);
+        if (n_ids) memcpy(id + (size_t)r * n_ids, ids + (size_t)i * n_ids, (size_t)n_ids * 4);
+        r++;
+    }
+    BCK(hipMemcpyAsync(s->d_in, s->h_in, ((size_t)T + rows + n_lp) * 4, hipMemcpyHostToDevice, b->st));
+    BCK(hq_launch_dequant(hq_mat_dev(b->embed), 0, s->d_in, (uint32_t)T, s->x, b->st));
+    if (batch_layers(s, (int)T)) return -1;
+    float *const o_lp = (float *)s->h_out, *const o_en = o_lp + n_lp, *const o_top = o_en + rows;
+    uint32_t *const o_ids = (uint32_t *)(o_top + n_top);
+    if (n_ids || top_k || entropy) {
+        k_norm_rows<<<rows, 256, 0, b->st>>>(s->x, s->d_in + T, b->final_norm, c.norm_offset, c.eps, s->hb, (int)c.hidden);
+        BCK(hipGetLastError());
+        if (gemm(b, b->lm_head, s->hb, rows, s->logits, false)) return -1;
+        if (hq_logprobs(s->logits, 1, rows, c.vocab, c.vocab, n_ids ? s->d_in + T + rows : nullptr, n_ids, top_k, n_ids ? o_lp : nullptr,
+                        entropy ? o_en : nullptr, top_ids ? o_ids : nullptr, top_logp ? o_top : nullptr, b->st))
+            return -1;
+    }
+    BCK(hipStreamSynchronize(b->st));
+    for (int i = 0, r = 0; i < n_seqs; i++) {
+        if (!n_new[i]) continue;
+        if (n_ids) memcpy(logp + (size_t)i * n_ids, o_lp + (size_t)r * n_ids, (size_t)n_ids * 4);
+        if (entropy) entropy[i] = o_en[r];
+        if (top_k && top_ids) memcpy(top_ids + (size_t)i * top_k, o_ids + (size_t)r * top_k, (size_t)top_k * 4);
+        if (top_k && top_logp) memcpy(top_logp + (size_t)i * top_k, o_top + (size_t)r * top_k, (size_t)top_k * 4);
+        r++;
+    }
+    return 0;
 }
 
 extern "C" int hip_selftest(const hq_ref_model_t *m, int device, size_t n_tokens, int verbose) {

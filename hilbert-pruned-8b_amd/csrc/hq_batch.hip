@@ -221,8 +221,8 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
                 return hq_internal_fail("%s: page %lld of sequence %d is %u (the cache has %u)", who, (long long)p, i, pages[(size_t)i * (size_t)pages_ld + (size_t)p], kv->n_pages);
         P += need;
     }
-    if (T * n_heads >= (1ll << 31)) return hq_internal_fail("%s: %lld tokens of %d heads", who, (long long)T, n_heads);
     if (T > b->max_tokens) return hq_internal_fail("%s: %lld new tokens (the batch takes %d)", who, (long long)T, b->max_tokens);
+    if (T * n_heads >= (1ll << 31)) return hq_internal_fail("%s: %lld tokens of %d heads", who, (long long)T, n_heads);
     if (P >= (1ll << 30)) return hq_internal_fail("%s: %lld pages in all", who, (long long)P);
     if (use_device(b->device)) return -1;
     b->set = false;

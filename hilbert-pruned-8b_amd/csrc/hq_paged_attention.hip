@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const uint32_t at0 = (uint32_t)(uintptr_t)lds;
     const size_t es = Q8 ? 1 : 2;
     const bool loads = w < 2 * WM, values = w >= WM;
-    const int row_w = RPI * NI * (w % WM), in_w = row_w & 15;
+    const int row_w = RPI * NI * (w % WM);
     const char *const kv0 = (const char *)(values ? g.kv.v : g.kv.k) + (size_t)it.kvh * g.kv.head_stride * es;
     const size_t page_b = (size_t)g.kv.page_stride * es;
     const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es), pmask = (uint32_t)g.kv.page_size - 1;
@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int x = lane; x < 32 * LPO; x += 64) {
-            const int row = x / LPO, d = 8 * (x % LPO);
+        for (int i = 0; i < LPO / 2; i++) {
+            const int x = lane + 64 * i, row = x / LPO, d = 8 * (x % LPO);
             if (r0 + row >= it.R || d >= hd) continue;
             const int t = token_of(g, it, 32 * w + row), h = it.kvh * g.rep + r0 + row - t * g.rep;
             *(u4v *)((_Float16 *)g.a.out + (size_t)(it.tok0 + t) * g.a.out_stride + (size_t)h * hd + d) = *(const u4v *)(mem + row * PITCH_O + 2 * d);

@@ -30,7 +30,7 @@ EXPORTS = (
     "hq_batch_create", "hq_batch_free", "hq_batch_set", "hq_rope_table", "hq_rope_append", "hq_attention", "hq_logprobs",
 )
 # include/hq_backend.h (no hq_ prefix: the names of the reference entry points they replace)
-BACKEND_EXPORTS = ("hip_backend_create", "hip_selftest")
+BACKEND_EXPORTS = ("hip_backend_create", "hip_selftest", "hip_batch_create", "hip_batch_free", "hip_batch_step")
 
 
 class WMat(C.Structure):
@@ -186,6 +186,9 @@ def load(path=LIB_PATH):
         "hq_gguf_find": (i, [vp, C.c_char_p, C.POINTER(sz)]),
         "hq_gguf_get_uint": (i, [vp, C.c_char_p, C.POINTER(C.c_uint64)]),
         "hq_gguf_wmat": (i, [vp, C.c_char_p, u32, C.POINTER(WMat)]),
+        "hip_batch_create": (i, [C.POINTER(RefBackend), i, i, C.c_uint32, i, i, i, C.POINTER(vp)]),
+        "hip_batch_free": (None, [vp]),
+        "hip_batch_step": (i, [vp, i, vp, vp, vp, vp, i, vp, i, i, vp, vp, vp, vp]),
         "hip_backend_create": (C.POINTER(RefBackend), [C.POINTER(RefModel), sz, i, C.c_bool]),
         "hip_selftest": (i, [C.POINTER(RefModel), i, sz, i]),
         "hq_gemm_workspace_bytes": (i, [i, i, u32, u32, i, C.POINTER(sz), C.POINTER(sz), C.POINTER(sz),
@@ -740,6 +743,39 @@ class HipBackend:
         if self.p:
             self.p.contents.destroy(self.p)
             self.p = None
+
+
+class HipBatch:
+    """hip_batch: steps of many sequences over a paged cache, with the weights of a HipBackend (which must outlive it)."""
+
+    def __init__(self, backend, n_pages, page_size, max_seqs, max_tokens, max_pages, kv_type=KV_F16):
+        self.h = None
+        self.backend = backend
+        h = C.c_void_p()
+        _check(load().hip_batch_create(backend.p, kv_type, page_size, n_pages, max_seqs, max_tokens, max_pages, C.byref(h)))
+        self.h = h.value
+
+    def step(self, tokens, n_new, n_pos, pages, ids=None, top_k=0):
+        """tokens: the new ones, sequence after sequence. Returns (logp [sequences, ids], entropy, top_ids, top_logp), rows of
+        sequences without new tokens NaN and 0."""
+        tokens, pages = np.ascontiguousarray(tokens, np.uint32), np.ascontiguousarray(pages, np.uint32)
+        n_new, n_pos = np.ascontiguousarray(n_new, np.int32), np.ascontiguousarray(n_pos, np.int32)
+        n = len(n_new)
+        if n_pos.shape != (n,) or pages.ndim != 2 or len(pages) != n or tokens.shape != (int(n_new.sum()),):
+            raise HQError(f"HipBatch.step: tokens {tokens.shape}, n_new {n_new.shape}, n_pos {n_pos.shape}, pages {pages.shape}")
+        ids = np.empty((n, 0), np.uint32) if ids is None else np.ascontiguousarray(ids, np.uint32)
+        if ids.ndim != 2 or len(ids) != n:
+            raise HQError(f"HipBatch.step: ids {ids.shape}")
+        logp, entropy = np.full(ids.shape, np.nan, np.float32), np.full(n, np.nan, np.float32)
+        top_ids, top_logp = np.zeros((n, top_k), np.uint32), np.full((n, top_k), np.nan, np.float32)
+        _check(_lib.hip_batch_step(self.h, n, _ptr(tokens), _ptr(n_new), _ptr(n_pos), _ptr(pages), pages.shape[1], _ptr(ids), ids.shape[1],
+                                   top_k, _ptr(logp), _ptr(entropy), _ptr(top_ids), _ptr(top_logp)))
+        return logp, entropy, top_ids, top_logp
+
+    def free(self):
+        if self.h:
+            _lib.hip_batch_free(self.h)
+            self.h = None
 
 
 def hip_selftest(view, device=0, n_tokens=64, verbose=1):

@@ -18,7 +18,7 @@
 #ifndef HQ_BACKEND_H
 #define HQ_BACKEND_H
 
-#include "hq.h"
+#include "hq_serve.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -107,6 +107,28 @@ hq_ref_backend_t *hip_backend_create(const hq_ref_model_t *m, size_t max_seq, in
  * state by cosine >= 0.999 as the reference checks it); last, a timed prefill of 2048 tokens
  * (tokens/s printed). Prints a report; returns 0 when every check passes, else -1. */
 int hip_selftest(const hq_ref_model_t *m, int device, size_t n_tokens, int verbose);
+
+/* ---- many sequences at a time, with a backend's weights (include/hq_serve.h)
+ *
+ * A hip_batch holds a paged cache of n_pages pages of page_size positions for every layer (kv_type: HQ_KV_F16 or HQ_KV_Q8)
+ * and the activations of up to max_tokens new tokens. Which pages a sequence has is the caller's to say, step by step; the
+ * backend's own cache and position are not touched. head_dim must be a multiple of 16 and rot_dim of 8; a sequence has at
+ * most max_pages pages. It works on the backend's stream: one call at a time on a backend and its batches; free a batch
+ * before its backend. */
+typedef struct hip_batch hip_batch;
+int hip_batch_create(hq_ref_backend_t *backend, int kv_type, int page_size, uint32_t n_pages, int max_seqs, int max_tokens,
+                     int max_pages, hip_batch **out);
+void hip_batch_free(hip_batch *s);
+
+/* One step: the new tokens of n_seqs sequences (tokens: sequence after sequence; n_new, n_pos, pages and pages_ld as in
+ * hq_batch_set, but n_new[i] <= n_pos[i]) through all layers, their keys and values into the pages. For the last new token
+ * of each sequence then, from its logits over the whole vocabulary: the log probabilities of n_ids tokens (ids and logp
+ * [n_seqs, n_ids]), the entropy [n_seqs], and the top_k likeliest tokens with their log probabilities [n_seqs, top_k], as
+ * hq_logprobs gives them; logp, entropy, top_ids and top_logp may be NULL. A sequence without new tokens leaves its rows
+ * as they are. All arrays are the host's. Synchronous. */
+int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, const int32_t *n_new, const int32_t *n_pos,
+                   const uint32_t *pages, int pages_ld, const uint32_t *ids, int n_ids, int top_k, float *logp, float *entropy,
+                   uint32_t *top_ids, float *top_logp);
 
 #ifdef __cplusplus
 }
