@@ -20,7 +20,7 @@ struct HqItem {
     int k0, k1;
     int page0;      // its pages
     int part, n_parts;
-    int block;        // the block's counter, where n_parts > 1
+    int block;        // HQ_STREAM*: the block's counter, where n_parts > 1
     uint32_t part_at; // its parts, in units of 16 bytes of hq_batch::parts
 };
 // Kernel bodies of hq_attention by the rows a workgroup takes.
@@ -42,7 +42,9 @@ struct hq_batch {
     const uint32_t *pages;
     const HqItem *items[HQ_BODIES];
     int n_items[HQ_BODIES];
-    int *counters;      // one per block cut into parts; zero between calls
+    const HqItem *joins[HQ_BODIES];  // HQ_ROWS*: the first part of each block that is cut into several
+    int n_joins[HQ_BODIES];
+    int *counters;      // one per block of HQ_STREAM* cut into parts; zero between calls
     float *parts;       // rows of such blocks
     size_t part_bytes;  // allocated
     // storage: one pinned copy of `dev`, which the next set waits for

@@ -75,7 +75,7 @@ int piece_length(const std::vector<Block> &bl, int unit, int slots, int over, in
 }
 
 struct Plan {
-    std::vector<HqItem> items[HQ_BODIES];
+    std::vector<HqItem> items[HQ_BODIES], joins[HQ_BODIES];
     int blocks = 0;          // counters
     uint64_t part_units = 0; // of 16 bytes
 };
@@ -109,7 +109,7 @@ void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const 
             HqItem it = b.it;
             it.n_parts = n;
             if (n > 1) {
-                it.block = out->blocks++;
+                if (stream) it.block = out->blocks++;
                 it.part_at = (uint32_t)out->part_units;
                 out->part_units += (uint64_t)n * rows_of[body] * (hq_attn_width(body, kv.head_dim) + HQ_PART_EXTRA) / 4;
             }
@@ -118,6 +118,7 @@ void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const 
                 it.k0 = (int)((int64_t)units * p / n) * unit;
                 it.k1 = p == n - 1 ? b.len : (int)((int64_t)units * (p + 1) / n) * unit;
                 all.push_back(it);
+                if (p == 0 && n > 1 && !stream) out->joins[body].push_back(it);
             }
         }
         const auto longer = [](const HqItem &a, const HqItem &b) { return a.k1 - a.k0 > b.k1 - b.k0; };
@@ -238,7 +239,7 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
     }
     if (plan.part_units >> 32) return hq_internal_fail("%s: %llu MiB of workspace", who, (unsigned long long)(plan.part_units >> 16));
     size_t n_items = 0;
-    for (auto &v : plan.items) n_items += v.size();
+    for (int i = 0; i < HQ_BODIES; i++) n_items += plan.items[i].size() + plan.joins[i].size();
     const size_t words = n_items * (sizeof(HqItem) / 4) + 2 * (size_t)T + (size_t)plan.blocks + (size_t)P + 16;
     if (words > b->words) {
         const size_t want = std::max(words, words + words / 2);
@@ -263,10 +264,14 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
     int *w = b->host;
     const auto dev = [&]() { return b->dev + (w - b->host); };
     for (int i = 0; i < HQ_BODIES; i++) {
-        b->items[i] = (const HqItem *)dev();
-        b->n_items[i] = (int)plan.items[i].size();
-        if (!plan.items[i].empty()) memcpy(w, plan.items[i].data(), plan.items[i].size() * sizeof(HqItem));
-        w += plan.items[i].size() * (sizeof(HqItem) / 4);
+        const auto send = [&](const std::vector<HqItem> &v, const HqItem **at, int *n) {
+            *at = (const HqItem *)dev();
+            *n = (int)v.size();
+            if (!v.empty()) memcpy(w, v.data(), v.size() * sizeof(HqItem));
+            w += v.size() * (sizeof(HqItem) / 4);
+        };
+        send(plan.items[i], &b->items[i], &b->n_items[i]);
+        send(plan.joins[i], &b->joins[i], &b->n_joins[i]);
     }
     b->counters = dev();
     if (plan.blocks) memset(w, 0, (size_t)plan.blocks * 4);
@@ -332,7 +337,7 @@ DEV void store4(_Float16 *p, f4 x) { *(h4 *)p = h4{(_Float16)x[0], (_Float16)x[1
 // rot_dim the dims 4u .. 4u + 3 and their partners rot_dim / 2 further, then eight dims in a row. Heads j < nh are
 // queries, the next n_kv_heads keys, the last n_kv_heads values. A workgroup takes heads of token blockIdx.x.
 template <bool F32, int G>
-__global__ void __launch_bounds__(256) k_rope_append(RopeArgs g) {
+__global__ void __launch_bounds__(256, 8) k_rope_append(RopeArgs g) {
     const int t = blockIdx.x, hd = g.kv.head_dim, nkv = g.kv.n_kv_heads, half = g.r.rot_dim / 2;
     const int u = threadIdx.x % G, first = threadIdx.x / G;
     const int d0 = 4 * u < half ? 4 * u : 2 * half + 8 * (u - half / 4), d1 = 4 * u < half ? half + 4 * u : d0 + 4;

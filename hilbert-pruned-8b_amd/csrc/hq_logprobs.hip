@@ -6,7 +6,7 @@
 // cancels. Few rows are split over workgroups; the last of a row's to arrive joins their sums in part order.
 //
 // The top k come from the same pass: the k-th largest of the threads' maxima, B, is no larger than the k-th largest logit, so
-// only the threads' shares whose maximum reaches B are read again (k of 512 or more, from cache), and the few logits found
+// only the threads' shares whose maximum reaches B are read again (k of 256 or more, from cache), and the few logits found
 // there are ranked by counting. No share is sorted and nothing is inserted anywhere in the stream.
 //
 // Bound: the bytes of the logits; for few rows the chain of launch, loads, the row's last workgroup and its second look.
@@ -21,7 +21,8 @@
 namespace {
 
 constexpr int NT = 512, WAVES = NT / 64;
-constexpr int MAX_BUCKETS = 256;   // shares of a row that the second look chooses from
+constexpr int MAX_PARTS = 32;      // of a row
+constexpr int MAX_BUCKETS = 512;   // shares of a row that the second look chooses from
 constexpr int FOUND = 1024, TIES = 256;
 
 struct LpArgs {
@@ -94,8 +95,9 @@ DEV void piece(const char *base, uint32_t v, uint32_t n_pieces, uint32_t mis, ui
 struct Shared {
     Sums sums[WAVES];
     uint32_t bucket[MAX_BUCKETS];
-    unsigned long long found[FOUND + TIES], out[64];
-    int n_found, n_ties, n_cand, last, count[WAVES];
+    int hit[MAX_BUCKETS];
+    alignas(16) unsigned long long found[FOUND + TIES], out[64];
+    int n_found, n_ties, n_hit, last, count[WAVES];
 };
 
 template <bool F32>
@@ -107,21 +109,39 @@ struct Row {
         const size_t a = (size_t)mis + i;
         return F32 ? ((const float *)base)[a] : (float)((const _Float16 *)base)[a];
     }
-    // f(order, token) of every logit that bucket b's threads read, by thread `tid` of `n`
+    // f(order, token) of the logits that the threads of the `n` buckets sh.hit[] read, but for pieces in which none reaches
+    // `least` (a logit; NaN: all pieces are wanted) (whole workgroup)
     template <class F>
-    __device__ __forceinline__ void bucket(int b, int tid, int n, F f) const {
-        const int per = NT / g.group, p = b / per, t0 = (b % per) * g.group;
-        const uint32_t v0 = (uint32_t)p * g.per, v1 = std::min(v0 + g.per, n_pieces);
-        for (uint32_t j = tid;; j += n) {
-            const uint32_t v = v0 + j / g.group * NT + t0 + j % g.group;
-            if (v0 + j / g.group * NT >= v1) break;
-            if (v >= v1) continue;
-            float x[VEC<F32>];
-            piece<F32>(base, v, n_pieces, mis, g.V, x);
+    __device__ __forceinline__ void buckets(const Shared &sh, int n, float least, F f) const {
+        constexpr int U = 4;  // pieces in flight per thread
+        const uint32_t rounds = (g.per + NT - 1) / NT, shift = __builtin_ctz(g.group), total = (uint32_t)n * rounds << shift;
+        for (uint32_t j0 = threadIdx.x; j0 < total; j0 += U * NT) {
+            float x[U][VEC<F32>];
+            uint32_t v[U];
 #pragma unroll
-            for (int e = 0; e < VEC<F32>; e++) {
-                const uint32_t i = v * VEC<F32> + e - mis;
-                if (i < g.V) f(order_of(x[e]), i);
+            for (int u = 0; u < U; u++) {
+                const uint32_t j = j0 + u * NT, y = j >> shift, h = y / rounds;
+                v[u] = n_pieces;
+                if (j >= total) continue;
+                const uint32_t t = (uint32_t)sh.hit[h] << shift, at = (y - h * rounds) * NT + t % NT + (j & (g.group - 1));  // t: the bucket's first thread
+                const uint32_t i = t / NT * g.per + at;
+                if (at < g.per && i < n_pieces) {
+                    v[u] = i;
+                    piece<F32>(base, i, n_pieces, mis, g.V, x[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (v[u] >= n_pieces) continue;
+                float mx = x[u][0];
+#pragma unroll
+                for (int e = 1; e < VEC<F32>; e++) mx = fmaxf(mx, x[u][e]);
+                if (mx < least) continue;
+#pragma unroll
+                for (int e = 0; e < VEC<F32>; e++) {
+                    const uint32_t i = v[u] * VEC<F32> + e - mis;
+                    if (i < g.V) f(order_of(x[u][e]), i);
+                }
             }
         }
     }
@@ -140,24 +160,41 @@ struct Row {
     }
 };
 
-// Largest B that at least k of the first n words of v reach (0 where there are fewer); every wave for itself.
-DEV uint32_t kth_largest(const uint32_t *v, int n, int k) {
-    uint32_t x[MAX_BUCKETS / 64];
+// A bound that at least k of the n words of sh.bucket reach (0 where there are fewer), every wave for itself: the k-th largest
+// of them, or for small k of the 64 maxima of words a lane, which is little less and takes one count per bit, not four. The
+// words that reach it to sh.hit (sh.n_hit, 0 before; any order).
+DEV uint32_t choose(Shared &sh, int n, int k) {
+    constexpr int W = MAX_BUCKETS / 64;
+    const int tid = threadIdx.x, lane = tid & 63;
+    uint32_t x[W], top = 0, b = 0;
 #pragma unroll
-    for (int i = 0; i < MAX_BUCKETS / 64; i++) {
-        const int at = 64 * i + (threadIdx.x & 63);
-        x[i] = at < n ? v[at] : 0u;
-    }
-    uint32_t b = 0;
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t mid = b | 1u << bit;
-        int c = 0;
+    for (int i = 0; i < W; i++) x[i] = 64 * i + lane < n ? sh.bucket[64 * i + lane] : 0u, top = std::max(top, x[i]);
+    if (k <= 32) {
+        for (int bit = 31; bit >= 0; bit--)
+            if (__popcll(__ballot(top >= (b | 1u << bit))) >= k) b |= 1u << bit;
+    } else {
+        for (int bit = 31; bit >= 0; bit--) {
+            int c = 0;
 #pragma unroll
-        for (int i = 0; i < MAX_BUCKETS / 64; i++)
-            if (64 * i < n) c += __popcll(__ballot(x[i] >= mid));
-        if (c >= k) b = mid;
+            for (int i = 0; i < W; i++) c += __popcll(__ballot(x[i] >= (b | 1u << bit)));
+            if (c >= k) b |= 1u << bit;
+        }
     }
+    if (tid < n && sh.bucket[tid] >= b) sh.hit[atomicAdd(&sh.n_hit, 1)] = tid;
     return b;
+}
+
+// how many of the first n keys of v (there is room for a multiple of eight) are larger
+DEV int larger_of(const unsigned long long *v, int n, unsigned long long key) {
+    int c = 0;
+    for (int i = 0; i < n; i += 8) {
+        unsigned long long y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = v[i + e];
+#pragma unroll
+        for (int e = 0; e < 8; e++) c += i + e < n && y[e] > key;
+    }
+    return c;
 }
 
 // The row's top k to sh.out as keys, likeliest first: buckets (n of them) hold the orders of their maxima; odd: the row has
@@ -167,7 +204,13 @@ DEV void top_k(const Row<F32> &row, int n, bool odd, Shared &sh) {
     const int k = row.g.k, tid = threadIdx.x;
     uint32_t B = 0;
     bool exact = odd;
-    if (!odd) B = kth_largest(sh.bucket, n, k);
+    if (tid == 0) sh.n_hit = odd ? n : 0;
+    if (odd) {
+        if (tid < n) sh.hit[tid] = tid;
+    } else {
+        __syncthreads();
+        B = choose(sh, n, k);
+    }
     for (;;) {
         if (exact) {  // B: the k-th largest logit itself
             B = 0;
@@ -188,9 +231,7 @@ DEV void top_k(const Row<F32> &row, int n, bool odd, Shared &sh) {
                 if (at < TIES) sh.found[FOUND + at] = key;
             }
         };
-        // a wave takes a bucket at a time
-        for (int b = tid >> 6; b < n; b += WAVES)
-            if (odd || sh.bucket[b] >= B) row.bucket(b, tid & 63, 64, take);
+        row.buckets(sh, sh.n_hit, odd ? NAN : from_order(B), take);  // (no bound, B = 0: NaN too)
         __syncthreads();
         if (sh.n_found <= FOUND) break;
         exact = true;  // more than FOUND logits pass the buckets' bound (a sorted row): fewer than k pass the exact one
@@ -221,9 +262,7 @@ DEV void top_k(const Row<F32> &row, int n, bool odd, Shared &sh) {
     const int nt = nf < k ? std::min(sh.n_ties, TIES) : 0, all = nf + nt;
     for (int x = tid; x < all; x += NT) {
         const unsigned long long key = sh.found[x < nf ? x : FOUND + x - nf];
-        int rank = 0;
-        for (int y = 0; y < nf; y++) rank += sh.found[y] > key;
-        for (int y = 0; y < nt; y++) rank += sh.found[FOUND + y] > key;
+        const int rank = larger_of(sh.found, nf, key) + larger_of(sh.found + FOUND, nt, key);
         if (rank < k) sh.out[rank] = key;
     }
     __syncthreads();
@@ -232,7 +271,7 @@ DEV void top_k(const Row<F32> &row, int n, bool odd, Shared &sh) {
 template <bool F32>
 __global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
     __shared__ Shared sh;
-    constexpr int U = F32 ? 4 : 2;  // pieces in flight per thread: 16 logits
+    constexpr int U = 2;  // pieces in flight per thread
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const size_t r = blockIdx.x / g.parts;
     const int part = blockIdx.x % g.parts;
@@ -240,6 +279,9 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
     const uint32_t mis = (uint32_t)((uintptr_t)start & 15u) / (F32 ? 4 : 2);
     const Row<F32> row = {g, start - ((uintptr_t)start & 15u), mis, (mis + g.V + VEC<F32> - 1) / VEC<F32>};
     const uint32_t v0 = (uint32_t)part * g.per, v1 = std::min(v0 + g.per, row.n_pieces);
+    // the first tokens asked for, before the pass: theirs is a chain of two loads
+    const uint32_t asked = g.logp && tid < g.n_ids ? g.ids[r * g.n_ids + tid] : 0u;
+    const float x_asked = g.logp && tid < g.n_ids && asked < g.V ? row.at(asked) : 0.f;
     Sums a = {-INFINITY, 0.f, 0.f};
     for (uint32_t v = v0 + tid; v < v1; v += U * NT) {
         float x[U][VEC<F32>];
@@ -295,14 +337,15 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
         }
         __syncthreads();
         if (!sh.last) return;
+        // a part a lane, in either half of every wave and in one order
+        const int mine = lane % MAX_PARTS;
+        const f4 o = buf_load16_sc1(rp, (uint32_t)std::min(mine, g.parts - 1) * each * 4u, 0);
+        if (want_top && tid < g.parts * per)
+            sh.bucket[tid] = __builtin_amdgcn_raw_buffer_load_b32(rp, ((uint32_t)(tid / per) * each + 4 + tid % per) * 4u, 0u, CPOL_SC1);
         a = {-INFINITY, 0.f, 0.f};
-        for (int p = 0; p < g.parts; p++) {
-            const f4 o = buf_load16_sc1(rp, (uint32_t)p * each * 4u, 0);
-            a.add({o.x, o.y, o.z});
-        }
-        if (want_top)
-            for (int b = tid; b < g.parts * per; b += NT)
-                sh.bucket[b] = __builtin_amdgcn_raw_buffer_load_b32(rp, ((uint32_t)(b / per) * each + 4 + b % per) * 4u, 0u, CPOL_SC1);
+        if (mine < g.parts) a = {o.x, o.y, o.z};
+#pragma unroll
+        for (int o = 1; o < MAX_PARTS; o <<= 1) a.add({__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)});
     } else if (want_top && tid % g.group == 0) {
         sh.bucket[tid / g.group] = big;
     }
@@ -310,11 +353,13 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
     const float logs = logf(a.s);
     const bool nothing = a.m == -INFINITY && a.s == 0.f;
     if (g.entropy && tid == 0) g.entropy[r] = nothing ? 0.f : logs - a.t / a.s;
-    if (g.logp)
-        for (int j = tid; j < g.n_ids; j += NT) {
+    if (g.logp) {
+        if (tid < g.n_ids) g.logp[r * g.n_ids + tid] = asked < g.V ? log_p(x_asked, a.m, logs) : NAN;
+        for (int j = tid + NT; j < g.n_ids; j += NT) {
             const uint32_t id = g.ids[r * g.n_ids + j];
             g.logp[r * g.n_ids + j] = id < g.V ? log_p(row.at(id), a.m, logs) : NAN;
         }
+    }
     if (!want_top) return;
     __syncthreads();
     top_k<F32>(row, g.parts * per, !(a.s >= 0.f), sh);
@@ -345,12 +390,12 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
     if (top_k == 0) top_ids = nullptr, top_logp = nullptr;
     if (!logp && !entropy && !top_ids && !top_logp) return 0;
     LpArgs g = {logits, ids, logp, entropy, top_logp, top_ids, stride, V, n_ids, top_k, 1, 1, 0, nullptr, nullptr};
-    // Few rows: parts of at least 512 threads x 4 pieces, while the chip has workgroups to spare (two per CU). Buckets stay
+    // Few rows: parts of three pieces a thread, while the chip has workgroups to spare (two per CU). Buckets stay
     // within MAX_BUCKETS: more parts, more threads to a bucket.
     int device, n_cu;
     if (hq_internal_device(&device, &n_cu)) return -1;
     const uint32_t pieces = (V + (f32 ? 3u : 7u)) / (f32 ? 4u : 8u) + 1;
-    g.parts = (int)std::max(1u, std::min({2u * (uint32_t)n_cu / (uint32_t)M, pieces / (NT * 4), (uint32_t)MAX_BUCKETS / 8}));
+    g.parts = (int)std::max(1u, std::min({2u * (uint32_t)n_cu / (uint32_t)M, (pieces + 3 * NT - 1) / (3 * NT), (uint32_t)MAX_PARTS}));
     while (g.parts * (NT / g.group) > MAX_BUCKETS) g.group *= 2;
     g.per = (pieces + (uint32_t)g.parts - 1) / (uint32_t)g.parts;
     if (g.parts > 1) {

@@ -118,46 +118,74 @@ DEV void decode16(u4v c, _Float16 d, h8 &lo, h8 &hi) {
     hi = h8{o[4].x, o[4].y, o[5].x, o[5].y, o[6].x, o[6].y, o[7].x, o[7].y};
 }
 
-// Where row `row0 + local` of an item goes: its outputs v / l, gated, four dims at a time.
+// Where row `row0 + local` of an item goes (`is`: there is such a row; else the last one's place, for reading), and its gate.
 struct OutRow {
-    _Float16 *out;  // null: not a row
+    _Float16 *out;
     const char *gate;
-    float inv;
     int hd, gate_f32;
-    __device__ __forceinline__ OutRow(const Args &g, const HqItem &it, int local, float l) : out(nullptr), gate(nullptr), inv(1.0f / l), hd(g.kv.head_dim), gate_f32(g.a.gate_f32) {
-        if (it.row0 + local >= it.R) return;
+    bool is, padding;
+    __device__ __forceinline__ OutRow(const Args &g, const HqItem &it, int local) : hd(g.kv.head_dim), gate_f32(g.a.gate_f32), is(it.row0 + local < it.R) {
+        local = std::min(local, it.R - 1 - it.row0);
         const int t = token_of(g, it, local), h = it.kvh * g.rep + it.row0 + local - t * g.rep;
         const size_t tok = (size_t)(it.tok0 + t);
         out = (_Float16 *)g.a.out + tok * g.a.out_stride + (size_t)h * hd;
-        if (g.a.gate) gate = (const char *)g.a.gate + (tok * g.a.gate_stride + (size_t)h * g.a.gate_head_stride) * (gate_f32 ? 4 : 2);
-        if (it.base + t < 0) inv = 0.f;  // padding: sees nothing, its sums are 0
+        gate = (const char *)g.a.gate + (tok * g.a.gate_stride + (size_t)h * g.a.gate_head_stride) * (gate_f32 ? 4 : 2);
+        padding = it.base + t < 0;  // before position 0: sees nothing, its sums are 0
+    }
+    // what the sums are multiplied with, l their weights' sum
+    __device__ __forceinline__ float scale(float l) const { return padding ? 0.f : 1.0f / l; }
+    // gates of dims d .. d + 3 (past head_dim: others)
+    __device__ __forceinline__ f4 gates(int d) const {
+        d = std::min(d, hd - 4);
+        if (gate_f32) return *(const f4 *)(gate + 4 * d);
+        const h4 y = *(const h4 *)(gate + 2 * d);
+        return f4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
     }
     __device__ __forceinline__ void put(int d, f4 v) const {
-        if (!out || d >= hd) return;
-        v *= inv;
-        if (gate) {
-            f4 x;
-            if (gate_f32) x = *(const f4 *)(gate + 4 * d);
-            else {
-                const h4 y = *(const h4 *)(gate + 2 * d);
-                x = f4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] *= 1.0f / (1.0f + expf(-x[e]));
-        }
-        *(h4 *)(out + d) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        if (is && d < hd) *(h4 *)(out + d) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
     }
 };
+DEV f4 gated(f4 v, f4 x) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] *= 1.0f / (1.0f + expf(-x[e]));
+    return v;
+}
 
-// A part's row: its sums [HDP], then (maximum in log2 units, sum). Parts are written and read at device scope; the last of
-// a block's items to arrive adds them in part order, so the result does not depend on the order of arrival.
+// A part's row: its sums [HDP], then (maximum in log2 units, sum). Parts are added in their order, so the result does not
+// depend on which came first.
 template <int HDP>
 constexpr int PARTF = HDP + HQ_PART_EXTRA;
 
-// scratch: LDS for 2 ROWS JOIN floats, which the workgroup is done with.
-constexpr int JOIN = 16;  // parts whose (maximum, sum) are in LDS at a time
+// Row `local` of an item from its parts, dims d .. d + 3 of it; load(p, at): 16 bytes at float `at` of part p's row.
+template <int HDP, class F>
+DEV void join_row(const Args &g, const HqItem &it, int local, int d, F load) {
+    constexpr int U = 4;  // parts on their way at a time
+    const OutRow out(g, it, local);
+    const f4 x = g.a.gate ? out.gates(d) : f4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < it.n_parts; p0 += U) {
+        f4 y[U], z[U];
+#pragma unroll
+        for (int e = 0; e < U; e++)
+            if (p0 + e < it.n_parts) y[e] = load(p0 + e, d), z[e] = load(p0 + e, HDP);
+#pragma unroll
+        for (int e = 0; e < U; e++) {
+            if (p0 + e >= it.n_parts) continue;
+            const float mn = fmaxf(m, z[e].x), a = part_scale(m, mn), b = part_scale(z[e].x, mn);
+            v = v * a + y[e] * b;
+            l = l * a + z[e].y * b;
+            m = mn;
+        }
+    }
+    v *= out.scale(l);
+    out.put(d, g.a.gate ? gated(v, x) : v);
+}
+
+// Few rows: parts are written and read at device scope, and the last of a block's items to arrive joins them, which is
+// quicker than another kernel.
 template <int HDP, int ROWS, int NT>
-DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float *scratch) {
+DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -167,60 +195,26 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float
     }
     __syncthreads();
     if (!*flag) return;
-    // a thread takes four dims of every (NT / C)-th row, RU rows and PU parts at a time
-    constexpr int C = HDP / 4, STEP = NT / C;
-    constexpr bool FEW = ROWS <= 32;  // a (maximum, sum) is then read by each thread, in the same round trip
-    constexpr int RU = FEW ? (ROWS + STEP - 1) / STEP : 8, PU = FEW || HDP > 128 ? 4 : 2;
-    static_assert(NT % C == 0 || HDP == 96 || HDP == 192, "whole rows per pass");
-    f2 *const ml = (f2 *)scratch;
-    const int d = 4 * (threadIdx.x % C), first = threadIdx.x / C;
-    const int rows = std::min(ROWS, it.R - it.row0);
-    for (int r0 = 0; r0 < rows; r0 += STEP * RU) {
-        float m[RU], l[RU];
-        f4 v[RU];
+    constexpr int C = HDP / 4;
+    static_assert(ROWS * C % NT == 0, "whole passes");
 #pragma unroll
-        for (int u = 0; u < RU; u++) m[u] = -INFINITY, l[u] = 0.f, v[u] = f4{0.f, 0.f, 0.f, 0.f};
-        for (int p0 = 0; p0 < it.n_parts; p0 += JOIN) {
-            if (!FEW && (r0 == 0 || it.n_parts > JOIN)) {
-                __syncthreads();
-                for (int x = threadIdx.x; x < ROWS * std::min(JOIN, it.n_parts - p0); x += NT) {
-                    const f4 y = buf_load16_sc1(rp, (uint32_t)((p0 * ROWS + x) * PARTF<HDP> + HDP) * 4u, 0);
-                    ml[x] = f2{y.x, y.y};
-                }
-                __syncthreads();
-            }
-            if (first >= STEP) continue;
-            for (int p1 = p0; p1 < std::min(p0 + JOIN, it.n_parts); p1 += PU) {
-                f4 y[RU][PU], zz[RU][PU];
-#pragma unroll
-                for (int u = 0; u < RU; u++)
-#pragma unroll
-                    for (int e = 0; e < PU; e++) {
-                        const int row = std::min(r0 + first + u * STEP, ROWS - 1), p = std::min(p1 + e, it.n_parts - 1);
-                        y[u][e] = buf_load16_sc1(rp, (uint32_t)((p * ROWS + row) * PARTF<HDP> + d) * 4u, 0);
-                        if (FEW) zz[u][e] = buf_load16_sc1(rp, (uint32_t)((p * ROWS + row) * PARTF<HDP> + HDP) * 4u, 0);
-                    }
-#pragma unroll
-                for (int u = 0; u < RU; u++)
-#pragma unroll
-                    for (int e = 0; e < PU; e++) {
-                        if (p1 + e >= it.n_parts) continue;
-                        f2 z;
-                        if (FEW) z = f2{zz[u][e].x, zz[u][e].y};
-                        else z = ml[(p1 + e - p0) * ROWS + std::min(r0 + first + u * STEP, ROWS - 1)];
-                        const float mn = fmaxf(m[u], z.x), a = part_scale(m[u], mn), b = part_scale(z.x, mn);
-                        v[u] = v[u] * a + y[u][e] * b;
-                        l[u] = l[u] * a + z.y * b;
-                        m[u] = mn;
-                    }
-            }
-        }
-        if (first < STEP)
-#pragma unroll
-            for (int u = 0; u < RU; u++) {
-                const int row = r0 + first + u * STEP;
-                if (row < rows) OutRow(g, it, row, l[u]).put(d, v[u]);
-            }
+    for (int i = 0; i < ROWS * C / NT; i++) {
+        const int local = (i * NT + (int)threadIdx.x) / C, d = 4 * ((int)threadIdx.x % C);
+        join_row<HDP>(g, it, local, d, [&](int p, int at) { return buf_load16_sc1(rp, (uint32_t)((p * ROWS + local) * PARTF<HDP> + at) * 4u, 0); });
+    }
+}
+
+// Many rows: a kernel behind k_rows. items: the first part of each block; a workgroup takes JOIN_ROWS rows.
+constexpr int JOIN_ROWS = 8;
+template <int HDP, int ROWS>
+__global__ void __launch_bounds__(256) k_join(Args g) {
+    constexpr int C = HDP / 4;
+    const HqItem it = g.items[blockIdx.x / (ROWS / JOIN_ROWS)];
+    const int first = blockIdx.x % (ROWS / JOIN_ROWS) * JOIN_ROWS;
+    const float *const parts = g.parts + (size_t)it.part_at * 4;
+    for (int x = threadIdx.x; x < JOIN_ROWS * C; x += 256) {
+        const int local = first + x / C, d = 4 * (x % C);
+        if (it.row0 + local < it.R) join_row<HDP>(g, it, local, d, [&](int p, int at) { return *(const f4 *)(parts + ((size_t)p * ROWS + local) * PARTF<HDP> + at); });
     }
 }
 
@@ -297,7 +291,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     constexpr int LEAD = Q8 ? 2 : 1;  // tile i + LEAD is in LDS when tile i's turn comes
     constexpr int RING = Q8 ? 4 * TILE : 0, SCALES = RING + D * 2 * RAW;  // Q8: K, K, V, V decoded; the ring; its scales
     __shared__ __align__(1024) char lds[SCALES + (Q8 ? D * 128 : 0)];
-    __shared__ int found_odd, last;
+    __shared__ int found_odd;
     __shared__ __align__(16) float fac[Q8 ? 4 * T : 4];  // Q8, two tiles: what a position's scores take (key scale, score scale); its weight
     const HqItem it = g.items[blockIdx.x];
     if (it.kvh < 0) return;
@@ -627,49 +621,47 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         }
     }
     const float lt = sum_halves(l);
-    if (it.n_parts == 1) {
-        const OutRow out(g, it, 32 * w + li, lt);
-        if (g.a.gate) {
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) out.put(32 * d + 8 * c + 4 * hf, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]});
-            return;
-        }
-        // through LDS (the ring is done with): 16 bytes a lane, whole rows an instruction
-        constexpr int PITCH_O = 2 * HDP + 16, LPO = HDP / 8;
-        static_assert(NW * 32 * PITCH_O <= sizeof lds, "the waves' outputs in the ring");
-        char *const mem = lds + w * 32 * PITCH_O;
+    if (it.n_parts > 1) {
+        float *const to = g.parts + (size_t)it.part_at * 4 + (size_t)(it.part * 32 * NW + 32 * w + li) * PARTF<HDP>;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                h4 y;
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (_Float16)(o[d][4 * c + e] * out.inv);
-                *(h4 *)(mem + li * PITCH_O + 2 * (32 * d + 8 * c + 4 * hf)) = y;
-            }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < LPO / 2; i++) {
-            const int x = lane + 64 * i, row = x / LPO, d = 8 * (x % LPO);
-            if (r0 + row >= it.R || d >= hd) continue;
-            const int t = token_of(g, it, 32 * w + row), h = it.kvh * g.rep + r0 + row - t * g.rep;
-            *(u4v *)((_Float16 *)g.a.out + (size_t)(it.tok0 + t) * g.a.out_stride + (size_t)h * hd + d) = *(const u4v *)(mem + row * PITCH_O + 2 * d);
-        }
+            for (int c = 0; c < 4; c++) *(f4 *)(to + 32 * d + 8 * c + 4 * hf) = f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+        if (hf == 0) *(f4 *)(to + HDP) = f4{m == -INFINITY ? -INFINITY : mref, lt, 0.f, 0.f};
         return;
     }
-    constexpr int ROWS = 32 * NW;
-    const rsrc_t rp = make_rsrc(g.parts + (size_t)it.part_at * 4, (uint32_t)it.n_parts * ROWS * PARTF<HDP> * 4u);
-    const uint32_t at = (uint32_t)((it.part * ROWS + 32 * w + li) * PARTF<HDP>) * 4u;
+    // outputs through LDS (the ring is done with): 16 bytes a lane, whole rows an instruction
+    constexpr int PITCH_O = 2 * HDP + 16, LPO = HDP / 8;
+    static_assert(NW * 32 * PITCH_O <= sizeof lds, "the waves' outputs in the ring");
+    char *const mem = lds + w * 32 * PITCH_O;
+    const OutRow out(g, it, 32 * w + li);
+    const float inv = out.scale(lt);
+    auto to_lds = [&](auto with) {
+        constexpr bool GATED = decltype(with)::value;
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++) {
+            f4 x[4];
+            if (GATED)
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-            buf_store16(rp, f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]}, at + (uint32_t)(32 * d + 8 * c + 4 * hf) * 4u);
-    if (hf == 0) buf_store16(rp, f4{m == -INFINITY ? -INFINITY : mref, lt, 0.f, 0.f}, at + HDP * 4u);
-    static_assert(2 * 4 * ROWS * JOIN <= sizeof lds, "the parts' maxima and sums in the ring");
-    join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last, (float *)lds);
+                for (int c = 0; c < 4; c++) x[c] = out.gates(32 * d + 8 * c + 4 * hf);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                f4 v = f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]} * inv;
+                if (GATED) v = gated(v, x[c]);
+                *(h4 *)(mem + li * PITCH_O + 2 * (32 * d + 8 * c + 4 * hf)) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+            }
+        }
+    };
+    if (g.a.gate) to_lds(std::true_type());
+    else to_lds(std::false_type());
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < LPO / 2; i++) {
+        const int x = lane + 64 * i, row = x / LPO, d = 8 * (x % LPO);
+        if (r0 + row >= it.R || d >= hd) continue;
+        const int t = token_of(g, it, 32 * w + row), h = it.kvh * g.rep + r0 + row - t * g.rep;
+        *(u4v *)((_Float16 *)g.a.out + (size_t)(it.tok0 + t) * g.a.out_stride + (size_t)h * hd + d) = *(const u4v *)(mem + row * PITCH_O + 2 * d);
+    }
 }
 
 // ------------------------------------------------------------------------------------ stream
@@ -953,20 +945,26 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
 #pragma unroll
         for (int u = 0; u < NW; u++) lt += ls[u][row] * part_scale(ms[u][row], mm);
         if (it.n_parts == 1) {
-            OutRow(g, it, row, lt).put(d, v);
+            const OutRow out(g, it, row);
+            v *= out.scale(lt);
+            out.put(d, g.a.gate ? gated(v, out.gates(d)) : v);
         } else {
             const uint32_t at = (uint32_t)((it.part * ROWS + row) * PARTF<HDP>) * 4u;
             buf_store16(rp, v, at + (uint32_t)d * 4u);
             if (d == 0) buf_store16(rp, f4{mm, lt, 0.f, 0.f}, at + HDP * 4u);
         }
     }
-    static_assert(2 * 4 * ROWS * JOIN <= sizeof os, "the parts' maxima and sums in the waves' arena");
-    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last, &os[0][0][0]);
+    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last);
 }
 
 template <bool Q8>
-hipError_t launch(int body, int width, const Args &g, unsigned grid, hipStream_t st) {
-#define HQ_ROWS(B, H, NW) case B + H: k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g); break
+hipError_t launch(int body, int width, Args g, unsigned grid, const HqItem *joins, unsigned n_joins, hipStream_t st) {
+#define HQ_ROWS(B, H, NW)                                                                        \
+    case B + H:                                                                                  \
+        k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g);                                          \
+        g.items = joins;                                                                         \
+        if (n_joins) k_join<H, 32 * NW><<<n_joins * (32 * NW / JOIN_ROWS), 256, 0, st>>>(g);     \
+        break
 #define HQ_STREAM(B, H, QB) case B + H: k_stream<H, Q8, QB, 4><<<grid, 256, 0, st>>>(g); break
     constexpr int B0 = 1000 * HQ_STREAM16, B1 = 1000 * HQ_STREAM32, B2 = 1000 * HQ_ROWS128, B3 = 1000 * HQ_ROWS256;
     switch (1000 * body + width) {
@@ -1028,7 +1026,7 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
         if (!b->n_items[body]) continue;
         g.items = b->items[body];
         const int width = hq_attn_width(body, kv->head_dim);
-        SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, g, (unsigned)b->n_items[body], (hipStream_t)stream));
+        SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, g, (unsigned)b->n_items[body], b->joins[body], (unsigned)b->n_joins[body], (hipStream_t)stream));
     }
     return 0;
 }
