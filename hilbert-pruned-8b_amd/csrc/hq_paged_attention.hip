@@ -317,13 +317,13 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const uint32_t pos_b = (uint32_t)(g.kv.pos_stride * es), pmask = (uint32_t)g.kv.page_size - 1;
     const uint32_t to_w = at0 + RING + (values ? RAW : 0) + row_w * RAWP;
     uint32_t piece_at[NI];  // byte of the lane's piece in its row
-    int row_at[NI];         // its row in the run
+    uint32_t row_at[NI];    // byte of that row in the run
     uint64_t on[NI];        // lanes whose piece is one
 #pragma unroll
     for (int x = 0; x < NI; x++) {
         const int row = row_w + RPI * x + lane / LPR, place = lane % LPR, piece = Q8 ? place : place ^ swizzle<HDP>(row);
         on[x] = loads ? __ballot(piece * (Q8 ? 16 : 8) < hd) : 0;
-        piece_at[x] = (uint32_t)piece * 16u, row_at[x] = row & 15;
+        piece_at[x] = (uint32_t)piece * 16u, row_at[x] = (uint32_t)(row & 15) * pos_b;
     }
     // Pages: lane t holds those of the wave's rows (Q8: of both runs of 16) of tile 64 c + t; read again every 64 tiles. (A scalar
     // load per tile would be waited for at every barrier.)
@@ -340,15 +340,15 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     // again, its weight is 0), and whether there is such a tile. The load of piece x to `slot`.
     struct Run {
         const char *at;
-        int last;
+        uint32_t last;  // (its first byte)
         bool is;
     };
     auto run_of = [&](int i) {
         const int first = std::min(it.k0 + i * T + (row_w & ~15), (n - 1) & ~15);
-        return Run{kv0 + (size_t)page_in(i, Q8 && row_w >= 16) * page_b + (size_t)((uint32_t)first & pmask) * pos_b, n - 1 - first, i < tiles};
+        return Run{kv0 + (size_t)page_in(i, Q8 && row_w >= 16) * page_b + (size_t)((uint32_t)first & pmask) * pos_b, (uint32_t)std::min(n - 1 - first, 15) * pos_b, i < tiles};
     };
     auto load_piece = [&](const Run &run, int slot, int x) {
-        const uint32_t at = (uint32_t)std::min(row_at[x], run.last) * pos_b + piece_at[x];
+        const uint32_t at = std::min(row_at[x], run.last) + piece_at[x];
         dma16_global(run.at, at, to_w + slot * 2 * RAW + RPI * x * RAWP, run.is ? on[x] : 0);
     };
     auto load_scales = [&](int i, int slot) {
