@@ -20,11 +20,12 @@ struct HqItem {
     int k0, k1;
     int page0;      // its pages
     int part, n_parts;
-    int block;        // HQ_STREAM*: the block's counter, where n_parts > 1
+    int block;        // HQ_STREAM: the block's counter, where n_parts > 1
     uint32_t part_at; // its parts, in units of 16 bytes of hq_batch::parts
 };
 // Kernel bodies of hq_attention by the rows a workgroup takes.
-enum { HQ_STREAM16, HQ_STREAM32, HQ_ROWS128, HQ_ROWS256, HQ_BODIES };
+enum { HQ_STREAM, HQ_ROWS128, HQ_ROWS256, HQ_BODIES };  // HQ_STREAM: 16, or 32 where the item has more rows
+constexpr int HQ_STREAM_PARTS = 128;  // most parts of a block of HQ_STREAM
 // The dims that a body's kernel for a head_dim holds; a part's row has HQ_PART_EXTRA floats more.
 int hq_attn_width(int body, int head_dim);
 constexpr int HQ_PART_EXTRA = 4;
@@ -42,9 +43,10 @@ struct hq_batch {
     const uint32_t *pages;
     const HqItem *items[HQ_BODIES];
     int n_items[HQ_BODIES];
+    int stream_rows;  // the most rows of an item of HQ_STREAM: 16 or 32
     const HqItem *joins[HQ_BODIES];  // HQ_ROWS*: the first part of each block that is cut into several
     int n_joins[HQ_BODIES];
-    int *counters;      // one per block of HQ_STREAM* cut into parts; zero between calls
+    int *counters;      // one per block of HQ_STREAM cut into parts; zero between calls
     float *parts;       // rows of such blocks
     size_t part_bytes;  // allocated
     // storage: one pinned copy of `dev`, which the next set waits for

@@ -39,7 +39,8 @@ int check_geometry(const char *who, const hq_kv_t *kv) {
 // ------------------------------------------------------------------------------------ hq_attention's work
 struct Block {
     HqItem it;
-    int len;  // positions, of its last row
+    int len;   // positions, of its last row
+    int rows;  // of its body
 };
 
 // Blocks of rows become items (see HqItem). Cutting a long block's positions fills the chip where blocks are few or uneven,
@@ -76,6 +77,7 @@ int piece_length(const std::vector<Block> &bl, int unit, int slots, int over, in
 
 struct Plan {
     std::vector<HqItem> items[HQ_BODIES], joins[HQ_BODIES];
+    int stream_rows = 16;
     int blocks = 0;          // counters
     uint64_t part_units = 0; // of 16 bytes
 };
@@ -83,35 +85,49 @@ struct Plan {
 constexpr int XCDS = 8;
 
 void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const int32_t *n_new, const int32_t *n_pos, Plan *out) {
-    const int rep = n_heads / kv.n_kv_heads, rows_of[HQ_BODIES] = {16, 32, 128, 256};
+    const int rep = n_heads / kv.n_kv_heads;
+    const auto body_of = [&](int R) { return R <= 16 || (R <= 32 && kv.head_dim <= 128) ? HQ_STREAM : R <= 128 || kv.head_dim > 128 ? HQ_ROWS128 : HQ_ROWS256; };
+    // A step with blocks of 256 rows does those of 128 in the same kernel, half its waves idle, while their positions are fewer
+    // than the time of a kernel of their own: about 256 positions on every workgroup that would run it.
+    int64_t small = 0;
+    bool large = false;
+    for (int i = 0; i < n_seqs; i++) {
+        const int body = body_of(n_new[i] * rep);
+        if (body == HQ_ROWS128 && n_new[i]) small += (int64_t)n_pos[i] * kv.n_kv_heads;
+        large |= body == HQ_ROWS256;
+    }
+    const bool together = large && small < 256 * 2 * n_cu;
     std::vector<Block> bl[HQ_BODIES];
     int tok0 = 0, page0 = 0;
     for (int i = 0; i < n_seqs; i++) {
         const int R = n_new[i] * rep, base = n_pos[i] - n_new[i];
-        const int body = R <= 16 ? HQ_STREAM16 : R <= 32 && kv.head_dim <= 128 ? HQ_STREAM32 : R <= 128 || kv.head_dim > 128 ? HQ_ROWS128 : HQ_ROWS256;
+        int body = body_of(R);
+        if (body == HQ_ROWS128 && together) body = HQ_ROWS256;
+        const int rows = body == HQ_ROWS256 ? 256 : body == HQ_ROWS128 ? 128 : R <= 16 ? 16 : 32;
+        if (body == HQ_STREAM) out->stream_rows = std::max(out->stream_rows, rows);
         for (int h = 0; h < kv.n_kv_heads && R; h++)
-            for (int row0 = (R - 1) / rows_of[body] * rows_of[body]; row0 >= 0; row0 -= rows_of[body]) {
-                const int see = base + (std::min(R, row0 + rows_of[body]) - 1) / rep + 1, n = std::max(0, see);
-                bl[body].push_back({{h, tok0, base, R, row0, row0 / rep, row0 % rep, see, 0, n, page0, 0, 1, 0, 0}, n});
+            for (int row0 = (R - 1) / rows * rows; row0 >= 0; row0 -= rows) {
+                const int see = base + (std::min(R, row0 + rows) - 1) / rep + 1, n = std::max(0, see);
+                bl[body].push_back({{h, tok0, base, R, row0, row0 / rep, row0 % rep, see, 0, n, page0, 0, 1, 0, 0}, n, rows});
             }
         tok0 += n_new[i];
         page0 += (n_pos[i] + kv.page_size - 1) / kv.page_size;
     }
     for (int body = 0; body < HQ_BODIES; body++) {
         if (bl[body].empty()) continue;
-        const bool stream = body <= HQ_STREAM32;
+        const bool stream = body == HQ_STREAM;
         const int unit = stream ? 128 : 64;
         const int slots = n_cu * (stream || (body == HQ_ROWS128 && kv.head_dim <= 128) ? 2 : 1);  // workgroups at a time
         const int L = piece_length(bl[body], unit, slots, stream ? 128 : 192, 256);
         std::vector<HqItem> all;
         for (const Block &b : bl[body]) {
-            const int units = (b.len + unit - 1) / unit, n = std::max(1, std::min((b.len + L / 2) / L, units));
+            const int units = (b.len + unit - 1) / unit, n = std::max(1, std::min({(b.len + L / 2) / L, units, stream ? HQ_STREAM_PARTS : units}));
             HqItem it = b.it;
             it.n_parts = n;
             if (n > 1) {
                 if (stream) it.block = out->blocks++;
                 it.part_at = (uint32_t)out->part_units;
-                out->part_units += (uint64_t)n * rows_of[body] * (hq_attn_width(body, kv.head_dim) + HQ_PART_EXTRA) / 4;
+                out->part_units += (uint64_t)n * b.rows * (hq_attn_width(body, kv.head_dim) + HQ_PART_EXTRA) / 4;
             }
             for (int p = 0; p < n; p++) {
                 it.part = p;
@@ -273,6 +289,7 @@ extern "C" int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_s
         send(plan.items[i], &b->items[i], &b->n_items[i]);
         send(plan.joins[i], &b->joins[i], &b->n_joins[i]);
     }
+    b->stream_rows = plan.stream_rows;
     b->counters = dev();
     if (plan.blocks) memset(w, 0, (size_t)plan.blocks * 4);
     w += plan.blocks;

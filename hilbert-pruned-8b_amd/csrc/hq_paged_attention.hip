@@ -156,10 +156,11 @@ DEV f4 gated(f4 v, f4 x) {
 template <int HDP>
 constexpr int PARTF = HDP + HQ_PART_EXTRA;
 
+constexpr int JOIN_AT_ONCE = 4;  // parts on their way at a time
 // Row `local` of an item from its parts, dims d .. d + 3 of it; load(p, at): 16 bytes at float `at` of part p's row.
 template <int HDP, class F>
 DEV void join_row(const Args &g, const HqItem &it, int local, int d, F load) {
-    constexpr int U = 4;  // parts on their way at a time
+    constexpr int U = JOIN_AT_ONCE;
     const OutRow out(g, it, local);
     const f4 x = g.a.gate ? out.gates(d) : f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
@@ -183,9 +184,14 @@ DEV void join_row(const Args &g, const HqItem &it, int local, int d, F load) {
 }
 
 // Few rows: parts are written and read at device scope, and the last of a block's items to arrive joins them, which is
-// quicker than another kernel.
+// quicker than another kernel. The parts' weights first, a part a lane; then the sums, the parts of a row over as many groups
+// of threads as there are, so that the chain of reads is short. One token of 2 heads behind 10485 positions, 41 parts a head:
+// 28.5 us reading four parts at a time, 10 us
+// so; of 8 heads behind 1000, 4 parts: 7.1 and 7.8 us, so few parts go the first way. arena: LDS that the workgroup is done with.
 template <int HDP, int ROWS, int NT>
-DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
+constexpr int JOIN_ARENA = (HQ_STREAM_PARTS + 1) * ROWS + 4 * NT;  // floats
+template <int HDP, int ROWS, int NT>
+DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float *arena) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -196,11 +202,74 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag) {
     __syncthreads();
     if (!*flag) return;
     constexpr int C = HDP / 4;
-    static_assert(ROWS * C % NT == 0, "whole passes");
+    const int rows = std::min(ROWS, it.R - it.row0);
+    if (it.n_parts <= JOIN_AT_ONCE) {  // one round trip, and nothing to share
+        for (int x = threadIdx.x; x < rows * C; x += NT) {
+            const int row = x / C;
+            join_row<HDP>(g, it, row, 4 * (x % C), [&](int p, int f) { return buf_load16_sc1(rp, (uint32_t)((p * ROWS + row) * PARTF<HDP> + f) * 4u, 0); });
+        }
+        return;
+    }
+    constexpr int NW = NT / 64, RW = ROWS / NW, PL = HQ_STREAM_PARTS / 64, U = 8;
+    float *const weight = arena, *const sum = arena + HQ_STREAM_PARTS * ROWS, *const share = sum + ROWS;  // [part][row], [row], [thread][4]
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    auto at = [&](int part, int row, int f) { return (uint32_t)((part * ROWS + row) * PARTF<HDP> + f) * 4u; };
+    f4 z[RW][PL];
 #pragma unroll
-    for (int i = 0; i < ROWS * C / NT; i++) {
-        const int local = (i * NT + (int)threadIdx.x) / C, d = 4 * ((int)threadIdx.x % C);
-        join_row<HDP>(g, it, local, d, [&](int p, int at) { return buf_load16_sc1(rp, (uint32_t)((p * ROWS + local) * PARTF<HDP> + at) * 4u, 0); });
+    for (int u = 0; u < RW; u++)
+#pragma unroll
+        for (int e = 0; e < PL; e++) {
+            const int row = w + NW * u, part = lane + 64 * e;
+            z[u][e] = f4{-INFINITY, 0.f, 0.f, 0.f};
+            if (row < rows && part < it.n_parts) z[u][e] = buf_load16_sc1(rp, at(part, row, HDP), 0);
+        }
+#pragma unroll
+    for (int u = 0; u < RW; u++) {
+        const int row = w + NW * u;
+        if (row >= rows) continue;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int e = 0; e < PL; e++) m = fmaxf(m, z[u][e].x);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+#pragma unroll
+        for (int e = 0; e < PL; e++) {
+            const float x = part_scale(z[u][e].x, m);
+            weight[(lane + 64 * e) * ROWS + row] = x;
+            l += z[u][e].y * x;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+        if (lane == 0) sum[row] = l;
+    }
+    __syncthreads();
+    int groups = 1;
+    while (2 * groups * rows * C <= NT) groups *= 2;
+    const int width = NT / groups, group = tid / width;
+    for (int s0 = 0; s0 < rows * C; s0 += width) {
+        const int slot = s0 + tid % width, row = slot / C, d = 4 * (slot % C);
+        const bool on = slot < rows * C;
+        const OutRow out(g, it, row);
+        const f4 x = g.a.gate ? out.gates(d) : f4{0.f, 0.f, 0.f, 0.f};
+        f4 v = {0.f, 0.f, 0.f, 0.f};
+        if (on)
+            for (int p0 = group; p0 < it.n_parts; p0 += groups * U) {
+                f4 y[U];
+#pragma unroll
+                for (int e = 0; e < U; e++) y[e] = p0 + e * groups < it.n_parts ? buf_load16_sc1(rp, at(p0 + e * groups, row, d), 0) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < U; e++)
+                    if (p0 + e * groups < it.n_parts) v += y[e] * weight[(p0 + e * groups) * ROWS + row];
+            }
+        if (groups > 1) {
+            *(f4 *)(share + 4 * tid) = v;
+            __syncthreads();
+            if (group) return;  // (one pass: the rows' threads fit)
+            for (int k = 1; k < groups; k++) v += *(const f4 *)(share + 4 * (tid + k * width));
+        }
+        if (!on) continue;
+        v *= out.scale(sum[row]);
+        out.put(d, g.a.gate ? gated(v, x) : v);
     }
 }
 
@@ -670,15 +739,17 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 // straight into the operand (key li, 16 bytes of dims), and of V the DPL dims DPL li .. of the eight positions 4 lg + r and
 // 16 + 4 lg + r, which are the positions of its score registers; pairs of positions are put together by v_perm into the
 // operand of block b, whose row li is dim DPL li + b.
+template <int HDP, int QB, int NW>
+struct StreamLds {
+    float os[NW][16 * QB][HDP + 4], ms[NW][16 * QB], ls[NW][16 * QB];
+    int last;
+};
 template <int HDP, bool Q8, int QB, int NW>
-__global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
-    constexpr int DPL = HDP / 16, NJ = HDP / 32, ROWS = 16 * QB, VW = Q8 ? DPL / 4 : DPL / 2, LDO = HDP + 4;
+DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &lds) {
+    constexpr int DPL = HDP / 16, NJ = HDP / 32, ROWS = 16 * QB, VW = Q8 ? DPL / 4 : DPL / 2;
     constexpr int KL = Q8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a key
-    __shared__ __align__(16) float os[NW > 4 ? 4 : NW][ROWS][LDO];
-    __shared__ float ms[NW][ROWS], ls[NW][ROWS];
-    __shared__ int last;
-    const HqItem it = g.items[blockIdx.x];
-    if (it.kvh < 0) return;
+    auto &os = lds.os;
+    auto &ms = lds.ms, &ls = lds.ls;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
     const int hd = g.kv.head_dim;
     const int n = it.n, n_all = it.base + it.t0 + 1;  // positions that some row, that every row sees
@@ -954,37 +1025,47 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
             if (d == 0) buf_store16(rp, f4{mm, lt, 0.f, 0.f}, at + HDP * 4u);
         }
     }
-    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &last);
+    static_assert(JOIN_ARENA<HDP, ROWS, 64 * NW> * 4 <= sizeof os, "the parts' weights in the waves' arena");
+    if (it.n_parts > 1) join_parts<HDP, ROWS, 64 * NW>(g, it, rp, &lds.last, &os[0][0][0]);
+}
+
+// QB: the most rows of an item, by 16. Steps that have items of 32 rows do those of 16 in the same kernel: they need no more
+// of it, and one behind the other they would each wait for their longest item.
+template <int HDP, bool Q8, int QB, int NW>
+__global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_stream(Args g) {
+    __shared__ __align__(16) char lds[sizeof(StreamLds<HDP, QB, NW>)];
+    const HqItem it = g.items[blockIdx.x];
+    if (QB == 1 || it.R <= 16) stream_item<HDP, Q8, 1, NW>(g, it, *(StreamLds<HDP, 1, NW> *)lds);
+    else stream_item<HDP, Q8, QB, NW>(g, it, *(StreamLds<HDP, QB, NW> *)lds);
 }
 
 template <bool Q8>
-hipError_t launch(int body, int width, Args g, unsigned grid, const HqItem *joins, unsigned n_joins, hipStream_t st) {
-#define HQ_ROWS(B, H, NW)                                                                        \
-    case B + H:                                                                                  \
-        k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g);                                          \
-        g.items = joins;                                                                         \
-        if (n_joins) k_join<H, 32 * NW><<<n_joins * (32 * NW / JOIN_ROWS), 256, 0, st>>>(g);     \
-        break
-#define HQ_STREAM(B, H, QB) case B + H: k_stream<H, Q8, QB, 4><<<grid, 256, 0, st>>>(g); break
-    constexpr int B0 = 1000 * HQ_STREAM16, B1 = 1000 * HQ_STREAM32, B2 = 1000 * HQ_ROWS128, B3 = 1000 * HQ_ROWS256;
-    switch (1000 * body + width) {
-        HQ_STREAM(B0, 64, 1);
-        HQ_STREAM(B0, 128, 1);
-        HQ_STREAM(B0, 256, 1);
-        HQ_STREAM(B1, 64, 2);
-        HQ_STREAM(B1, 128, 2);
-        HQ_ROWS(B2, 64, 4);
-        HQ_ROWS(B2, 96, 4);
-        HQ_ROWS(B2, 128, 4);
-        HQ_ROWS(B2, 192, 4);
-        HQ_ROWS(B2, 256, 4);
-        HQ_ROWS(B3, 64, 8);
-        HQ_ROWS(B3, 96, 8);
-        HQ_ROWS(B3, 128, 8);
-    default: return hipErrorInvalidValue;
+hipError_t launch(int body, int width, int stream_rows, Args g, unsigned grid, const HqItem *joins, unsigned n_joins, hipStream_t st) {
+#define HQ_STREAMS(H, QB) k_stream<H, Q8, QB, 4><<<grid, 256, 0, st>>>(g)
+#define HQ_ROWS(H, NW)                                                                                    \
+    do {                                                                                                  \
+        k_rows<H, Q8, NW><<<grid, 64 * NW, 0, st>>>(g);                                                   \
+        g.items = joins;                                                                                  \
+        if (n_joins) k_join<H, 32 * NW><<<n_joins * (32 * NW / JOIN_ROWS), 256, 0, st>>>(g);              \
+    } while (0)
+    const bool two = stream_rows > 16;
+    if (body == HQ_STREAM) {
+        if (width == 256) HQ_STREAMS(256, 1);
+        else if (width == 128) two ? HQ_STREAMS(128, 2) : HQ_STREAMS(128, 1);
+        else two ? HQ_STREAMS(64, 2) : HQ_STREAMS(64, 1);
+    } else if (body == HQ_ROWS256) {
+        if (width == 128) HQ_ROWS(128, 8);
+        else if (width == 96) HQ_ROWS(96, 8);
+        else HQ_ROWS(64, 8);
+    } else {
+        if (width == 256) HQ_ROWS(256, 4);
+        else if (width == 192) HQ_ROWS(192, 4);
+        else if (width == 128) HQ_ROWS(128, 4);
+        else if (width == 96) HQ_ROWS(96, 4);
+        else HQ_ROWS(64, 4);
     }
 #undef HQ_ROWS
-#undef HQ_STREAM
+#undef HQ_STREAMS
     return hipGetLastError();
 }
 
@@ -992,7 +1073,7 @@ hipError_t launch(int body, int width, Args g, unsigned grid, const HqItem *join
 
 // (a part's row is PARTF<width> floats: its size in the plan and in the kernels comes from this one rule)
 int hq_attn_width(int body, int hd) {
-    if (body == HQ_STREAM16 || body == HQ_STREAM32) return hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    if (body == HQ_STREAM) return hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     return hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : hd <= 192 ? 192 : 256;
 }
 
@@ -1026,7 +1107,7 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
         if (!b->n_items[body]) continue;
         g.items = b->items[body];
         const int width = hq_attn_width(body, kv->head_dim);
-        SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, g, (unsigned)b->n_items[body], b->joins[body], (unsigned)b->n_joins[body], (hipStream_t)stream));
+        SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, b->stream_rows, g, (unsigned)b->n_items[body], b->joins[body], (unsigned)b->n_joins[body], (hipStream_t)stream));
     }
     return 0;
 }

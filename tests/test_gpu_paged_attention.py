@@ -89,6 +89,22 @@ def test_blocks_cut_into_parts(hqlib, hd, q8):
         check(got, *attention(pool, q, [a for a, _ in lens], [t for _, t in lens], hd ** -0.5))
 
 
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("nh,hd,lens", [(1, 64, [(1, 40000)]), (16, 128, [(1, 20000), (1, 3)]), (24, 64, [(1, 20000), (16, 16), (0, 5)]), (9, 256, [(1, 30000)]),
+                                        (20, 128, [(1, 300), (2, 9000)]), (4, 64, [(100, 500), (20, 3000), (1, 700)])])
+def test_many_parts_and_shared_kernels(hqlib, nh, hd, lens, gate):
+    """One kv head behind up to 128 parts a block, more than a wave's lanes; 16 and 32 rows, and 128 and 256, in one step."""
+    rng = np.random.default_rng(nh + hd)
+    pool = Pool(rng, [t for _, t in lens], 64, 1, hd, False)
+    fill(pool, rng, [t for _, t in lens])
+    T = sum(a for a, _ in lens)
+    q = rng.normal(0, 1.5, (T, nh, hd)).astype(np.float16)
+    g = rng.normal(0, 2, (T, nh, hd)).astype(np.float16) if gate else None
+    print(f"[gpu] many parts: {nh} heads x {hd} {lens} gate={gate}", flush=True)
+    got = run(hqlib, pool, nh, lens, q, hd ** -0.5, gate=g)
+    check(got, *attention(pool, q, [a for a, _ in lens], [t for _, t in lens], hd ** -0.5, gate=g))
+
+
 @pytest.mark.parametrize("gate_f32", [False, True])
 @pytest.mark.parametrize("q8", [False, True])
 def test_gate_strides_and_stream(hqlib, q8, gate_f32):
