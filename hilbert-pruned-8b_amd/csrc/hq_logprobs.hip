@@ -9,7 +9,9 @@
 // only the threads' shares whose maximum reaches B are read again (k of 256 or more, from cache), and the few logits found
 // there are ranked by counting. No share is sorted and nothing is inserted anywhere in the stream.
 //
-// Bound: the bytes of the logits; for few rows the chain of launch, loads, the row's last workgroup and its second look.
+// Bound: the bytes of the logits. 512 rows of 151936, fp32: 311 MB in 55 us, 5.6 TB/s (59 where none of them is in cache).
+// Few rows: the chain of launch, loads, the row's last workgroup (5.5 us for one row of 32000, 8 for 16 of 151936, fp16) and the
+// second look (3 us more with the top 5 of the one, 7 with the top 20 of the other).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -390,8 +392,8 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
     if (top_k == 0) top_ids = nullptr, top_logp = nullptr;
     if (!logp && !entropy && !top_ids && !top_logp) return 0;
     LpArgs g = {logits, ids, logp, entropy, top_logp, top_ids, stride, V, n_ids, top_k, 1, 1, 0, nullptr, nullptr};
-    // Few rows: parts of three pieces a thread, while the chip has workgroups to spare (two per CU). Buckets stay
-    // within MAX_BUCKETS: more parts, more threads to a bucket.
+    // Few rows: parts of three pieces a thread, while the chip has workgroups to spare (two per CU); 16 rows of 151936 with two: 1.9
+    // us more, with four 0.3 more. Buckets stay within MAX_BUCKETS: more parts, more threads to a bucket.
     int device, n_cu;
     if (hq_internal_device(&device, &n_cu)) return -1;
     const uint32_t pieces = (V + (f32 ? 3u : 7u)) / (f32 ? 4u : 8u) + 1;

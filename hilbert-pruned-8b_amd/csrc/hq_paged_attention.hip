@@ -186,8 +186,8 @@ DEV void join_row(const Args &g, const HqItem &it, int local, int d, F load) {
 // Few rows: parts are written and read at device scope, and the last of a block's items to arrive joins them, which is
 // quicker than another kernel. The parts' weights first, a part a lane; then the sums, the parts of a row over as many groups
 // of threads as there are, so that the chain of reads is short. One token of 2 heads behind 10485 positions, 41 parts a head:
-// 28.5 us reading four parts at a time, 10 us
-// so; of 8 heads behind 1000, 4 parts: 7.1 and 7.8 us, so few parts go the first way. arena: LDS that the workgroup is done with.
+// 28 us reading four parts at a time, 10 us so; of 8 heads behind 1000, 4 parts a head: 6.8 and 7.9 us, so few parts go the
+// first way. arena: LDS that the workgroup is done with.
 template <int HDP, int ROWS, int NT>
 constexpr int JOIN_ARENA = (HQ_STREAM_PARTS + 1) * ROWS + 4 * NT;  // floats
 template <int HDP, int ROWS, int NT>
@@ -273,7 +273,9 @@ DEV void join_parts(const Args &g, const HqItem &it, rsrc_t rp, int *flag, float
     }
 }
 
-// Many rows: a kernel behind k_rows. items: the first part of each block; a workgroup takes JOIN_ROWS rows.
+// Many rows: a kernel behind k_rows, so that the whole chip reads the parts; one workgroup per block did it at a tenth of its
+// rate (heads of 256, 2 parts of 128 rows a block: 35 us behind the loop, now 11; 64 blocks of 4 parts of 256 rows, 35 MB: 8 us).
+// items: the first part of each block; a workgroup takes JOIN_ROWS rows. Bound: the parts' bytes.
 constexpr int JOIN_ROWS = 8;
 template <int HDP, int ROWS>
 __global__ void __launch_bounds__(256) k_join(Args g) {
@@ -352,9 +354,17 @@ constexpr int DEPTH = HDP <= 128 && NW == 8 ? 6 : Q8 ? 5 : 4;
 // weights (vector instructions), the matrix cores form the scores of the next one. It holds its queries, two S^T [KT x 32] and
 // O^T [HDP x 32] in registers; V's operand is read transposed from LDS, its key order that of S^T's registers. Q8 tiles are
 // decoded a tile ahead from the ring into two more buffers of each matrix, once for all waves.
+// Eight waves of 32 rows, two per SIMD, for heads up to 128: a key is read from LDS once per 32 rows and from the cache once
+// per 256. 64 rows per wave spill, and four waves in each of two workgroups read every tile twice (10 % slower). Heads above
+// 128 leave room for one wave per SIMD.
+// Bound: the matrix products. 4 rows positions head_dim products, of which 2 % are masked ones. Heads of 128: 2300 cycles a tile
+// and SIMD, 1088 of them the matrix cores' (39 % busy with what is around the loop), at the 1.8 GHz that the power allows; no
+// one part is behind the rest (2180 without the rescaling, 1970 without the exponentials, 1930 without the DMA). 16384 tokens
+// of ten prompts, 32 / 8 heads: 655 us, 795 TFLOP/s; 512 tokens behind 32256: 312 us, 875 TFLOP/s. Heads of 256: 2750 cycles,
+// 900 of them the DMA's issue, which no second wave hides; 1000 tokens behind 2001, 16 / 4 heads: 77 us, 530 TFLOP/s.
 template <int HDP, bool Q8, int NW>
 __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
-    constexpr int P = PITCH<HDP>, T = KT, KB = T / 32, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
+    constexpr int P = PITCH<HDP>, T = KT, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
     constexpr int RAWP = Q8 ? P / 2 : P, RAW = T * RAWP;  // a ring tile's pitch and bytes
     constexpr int LPR = RAWP / 16, RPI = 64 / LPR, UNITS = T / RPI, NI = 2 * UNITS > NW ? 2 * UNITS / NW : 1;
     constexpr int LEAD = Q8 ? 2 : 1;  // tile i + LEAD is in LDS when tile i's turn comes
@@ -471,7 +481,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     float mx = -INFINITY;                      // of the lane's scores of the tile whose turn it is
     h8 q[NJ];
     float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores; Q8: in log2 units), what the exponents are taken against, the sum
-    f16v o[ND], sa[KB], sb[KB];  // outputs; scores of a tile and of the next
+    f16v o[ND], sa, sb;  // outputs; scores of a tile and of the next
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -482,8 +492,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     const uint32_t vx = at0 + (uint32_t)((Q8 ? 2 * TILE : RAW) + vrow * P + ((vc ^ swizzle<HDP>(vrow)) << 4) + 8 * (i16 & 1));
     typedef __attribute__((address_space(3))) s4 lds_s4;
     typedef const __attribute__((address_space(3))) h8 lds_h8;
-    // operands of the tile at `buf` (bytes): keys 32 b .. by dims 16 j ..; dims 32 d .. by positions 16 k ..
-    auto key_operand = [&](uint32_t buf, int j, int b) { return *(lds_h8 *)(uintptr_t)(((kx + buf) ^ (32u * j)) + 32 * P * b); };
+    // operands of the tile at `buf` (bytes): its keys by dims 16 j ..; dims 32 d .. by positions 16 k ..
+    auto key_operand = [&](uint32_t buf, int j) { return *(lds_h8 *)(uintptr_t)((kx + buf) ^ (32u * j)); };
     auto value_operand = [&](uint32_t buf, int d, int k) {
         const uint32_t x = (vx + buf) ^ (64u * d);
         const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)(x + 16 * P * k)));
@@ -491,40 +501,36 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         return h8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
     };
     // y times the key scales of tile i
-    auto scale_scores = [&](f16v (&y)[KB], int i) {
+    auto scale_scores = [&](f16v &y, int i) {
         if (!Q8) return;
 #pragma unroll
-        for (int b = 0; b < KB; b++)
+        for (int c = 0; c < 4; c++) {
+            const f4 f = *(const f4 *)&fac[(i & 1) * T + 8 * c + 4 * hf];
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const f4 f = *(const f4 *)&fac[(i & 1) * T + 32 * b + 8 * c + 4 * hf];
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[b][4 * c + e] *= f[e];
-            }
+            for (int e = 0; e < 4; e++) y[4 * c + e] *= f[e];
+        }
     };
-    auto zero_scores = [&](f16v (&y)[KB]) {
+    auto zero_scores = [&](f16v &y) {
 #pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) y[b][e] = 0.f;
+        for (int e = 0; e < 16; e++) y[e] = 0.f;
     };
-    static_assert(KB == 1, "one block of scores a tile");
+    static_assert(T == 32, "one block of scores a tile");
     // Scores s of tile i to weights, and its values' product; y: the scores of the tile after it (of whatever the buffer holds,
     // behind the last). k_at, v_at: the next tile's keys and this one's values in LDS. Written out in the
     // order of issue: a score product, its share of the exponentials and a load; then a product of values beside the maxima of
     // the new scores; operands are read AHEAD products before theirs.
-    auto step = [&](int i, uint32_t k_at, uint32_t v_at, int to, f16v (&s)[KB], f16v (&y)[KB]) {
+    auto step = [&](int i, uint32_t k_at, uint32_t v_at, int to, f16v &s, f16v &y) {
         const int s0 = it.k0 + i * T;
         constexpr int AHEAD = 4;
         h8 kr[AHEAD], vr[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++) kr[j] = key_operand(k_at, j, 0);
+        for (int j = 0; j < AHEAD; j++) kr[j] = key_operand(k_at, j);
         if (s0 + T > wn_all) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[0][e] = s0 + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[0][e] : -INFINITY;
-            mx = s[0][0];
+            for (int e = 0; e < 16; e++) s[e] = s0 + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[e] : -INFINITY;
+            mx = s[0];
 #pragma unroll
-            for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[0][e]);
+            for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[e]);
         }
         if (__any(mx > m + g.slack)) {
             const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
@@ -547,7 +553,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         // weights 2 c and 2 c + 1: their exponentials; later, as fp16 (and summed)
         auto weigh = [&](int c) {
 #pragma unroll
-            for (int e = 2 * c; e < 2 * c + 2; e++) x[e] = ex2(Q8 ? s[0][e] - mref : fmaf(s[0][e], g.sc, -mref));
+            for (int e = 2 * c; e < 2 * c + 2; e++) x[e] = ex2(Q8 ? s[e] - mref : fmaf(s[e], g.sc, -mref));
         };
         auto round = [&](int c) {
             const int e = 2 * c;
@@ -562,8 +568,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         __builtin_amdgcn_sched_barrier(0);
         unrolled<NJ>([&](auto index) {
             constexpr int j = decltype(index)::value;
-            y[0] = mfma32(kr[j % AHEAD], q[j], y[0]);
-            if constexpr (j + AHEAD < NJ) kr[j % AHEAD] = key_operand(k_at, j + AHEAD, 0);
+            y = mfma32(kr[j % AHEAD], q[j], y);
+            if constexpr (j + AHEAD < NJ) kr[j % AHEAD] = key_operand(k_at, j + AHEAD);
             else vr[j + AHEAD - NJ] = value_operand(v_at, (j + AHEAD - NJ) % ND, (j + AHEAD - NJ) / ND);
 #pragma unroll
             for (int c = 8 * j / NJ; c < 8 * (j + 1) / NJ; c++) {
@@ -584,7 +590,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             if constexpr (t + 1 == ND) scale_scores(y, i + 1);
             if constexpr (t >= ND)
 #pragma unroll
-                for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[0][e]);
+                for (int e = 16 * d / ND; e < 16 * (d + 1) / ND; e++) my = fmaxf(my, y[e]);
             __builtin_amdgcn_sched_barrier(0);
         });
         mx = my;
@@ -627,13 +633,13 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             for (int j = 0; j < NJ; j++) q[j] = -q[j];
         zero_scores(sa);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) sa[0] = mfma32(key_operand(0, j, 0), q[j], sa[0]);
+        for (int j = 0; j < NJ; j++) sa = mfma32(key_operand(0, j), q[j], sa);
         scale_scores(sa, 0);
 #pragma unroll
-        for (int e = 0; e < 16; e++) mx = fmaxf(mx, sa[0][e]);
+        for (int e = 0; e < 16; e++) mx = fmaxf(mx, sa[e]);
     }
     int slot = 0;  // i % D
-    auto tile = [&](int i, f16v (&s)[KB], f16v (&y)[KB]) {
+    auto tile = [&](int i, f16v &s, f16v &y) {
         const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1;
         // tile i + LEAD is there, the tiles behind it may still be on their way
         wait_tile(i + LEAD, std::min(i + D - 1, tiles), std::integral_constant<int, D - 2 - LEAD>());
@@ -738,7 +744,10 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 // the waves' (maximum, sum, output) are added in wave order at the end. A lane (li = lane % 16, lg = lane / 16) loads keys
 // straight into the operand (key li, 16 bytes of dims), and of V the DPL dims DPL li .. of the eight positions 4 lg + r and
 // 16 + 4 lg + r, which are the positions of its score registers; pairs of positions are put together by v_perm into the
-// operand of block b, whose row li is dim DPL li + b.
+// operand of block b, whose row li is dim DPL li + b. Nothing goes through LDS before the end: few rows use an operand once.
+// Bound: the cache's bytes. 64 tokens behind 200 .. 8192 positions, 32 / 8 heads of 128: 113 us, 5.1 TB/s; 8 behind 20000 ..
+// 40000 of a Q8 cache: 97 us, 5.0 TB/s. A single sequence: the chain of page, keys, softmax and join, 6.8 us behind 1000
+// positions (8 heads of 64).
 template <int HDP, int QB, int NW>
 struct StreamLds {
     float os[NW][16 * QB][HDP + 4], ms[NW][16 * QB], ls[NW][16 * QB];
