@@ -900,6 +900,11 @@ int batch_init(hip_batch *s, HipBackend *b, int kv_type, int page_size, uint32_t
         return hq_internal_fail("%s: %d sequences, %d tokens (1 .. 65536)", who, max_seqs, max_tokens);
     if (n_pages < 1 || (uint64_t)n_pages * (uint64_t)page_size >= (1ull << 31) || max_pages < 1 || (int64_t)max_pages * page_size > (1 << 24))
         return hq_internal_fail("%s: %u pages, %d a sequence (at least 1; below 2^31 positions, 2^24 a sequence)", who, n_pages, max_pages);
+    // a projection's rows, and the logits, are one matrix of hq_gemm, which its kernels address in 32 bits
+    const uint64_t heads = (uint64_t)c.n_heads * (c.attn_gate ? 2 : 1) + 2 * (uint64_t)c.n_kv_heads;
+    const uint64_t widest = std::max({heads * c.head_dim, (uint64_t)c.intermediate, (uint64_t)c.hidden});
+    if (widest * (uint64_t)max_tokens * 4 >> 32 || (uint64_t)c.vocab * (uint64_t)max_seqs * 4 >> 32)
+        return hq_internal_fail("%s: %d tokens of %llu values or %d sequences of %u logits (below 4 GiB each)", who, max_tokens, (unsigned long long)widest, max_seqs, c.vocab);
     BCK(hipSetDevice(b->device));
     s->b = b, s->max_seqs = max_seqs, s->max_tokens = max_tokens, s->n_table = max_pages * page_size;
     if (hq_batch_create(b->device, max_seqs, max_tokens, max_pages, &s->step)) return -1;
@@ -922,10 +927,9 @@ int batch_init(hip_batch *s, HipBackend *b, int kv_type, int page_size, uint32_t
                 return -1;
     bool qkv_one = false, kv_apart = false, gu_apart = false;
     for (const DevLayer &d : b->L) qkv_one |= d.qkv != nullptr, kv_apart |= !d.qkv, gu_apart |= !d.pair;
-    const size_t Th = std::max(T, (size_t)max_seqs);  // rows of hb: the last ones of the sequences too
     if (alloc(&s->x, T * H * 4) || alloc(&s->qb, T * (qw + (qkv_one ? 2 * kvw : 0)) * 4) || alloc(&s->kb, kv_apart ? T * kvw * 4 : 0) ||
         alloc(&s->vb, kv_apart ? T * kvw * 4 : 0) || alloc(&s->gb, gu_apart ? T * I * 4 : 0) || alloc(&s->ub, gu_apart ? T * I * 4 : 0) ||
-        alloc(&s->q, T * ow * 2) || alloc(&s->hb, Th * H * 2) || alloc(&s->ob, T * ow * 2) || alloc(&s->fb, T * I * 2) ||
+        alloc(&s->q, T * ow * 2) || alloc(&s->hb, T * H * 2) || alloc(&s->ob, T * ow * 2) || alloc(&s->fb, T * I * 2) ||
         alloc(&s->table, (size_t)s->n_table * c.rot_dim * 4) || alloc(&s->logits, (size_t)max_seqs * c.vocab * 4))
         return -1;
     return c.rot_dim ? hq_rope_table(b->m->rope_inv_freq, (int)c.rot_dim, s->n_table, s->table, b->st) : 0;

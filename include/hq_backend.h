@@ -111,10 +111,10 @@ int hip_selftest(const hq_ref_model_t *m, int device, size_t n_tokens, int verbo
 /* ---- many sequences at a time, with a backend's weights (include/hq_serve.h)
  *
  * A hip_batch holds a paged cache of n_pages pages of page_size positions for every layer (kv_type: HQ_KV_F16 or HQ_KV_Q8)
- * and the activations of up to max_tokens new tokens. Which pages a sequence has is the caller's to say, step by step; the
- * backend's own cache and position are not touched. head_dim must be a multiple of 16 and rot_dim of 8; a sequence has at
- * most max_pages pages. It works on the backend's stream: one call at a time on a backend and its batches; free a batch
- * before its backend. */
+ * and the activations of up to max_tokens new tokens. Which pages a sequence has (at most max_pages) is the caller's to say,
+ * step by step; the backend's own cache and position are not touched. head_dim must be a multiple of 16 and rot_dim of 8;
+ * max_tokens rows of the widest projection, and max_seqs rows of logits, in fp32, stay below 4 GiB each. It works on the
+ * backend's stream: one call at a time on a backend and its batches; free a batch before its backend. */
 typedef struct hip_batch hip_batch;
 int hip_batch_create(hq_ref_backend_t *backend, int kv_type, int page_size, uint32_t n_pages, int max_seqs, int max_tokens,
                      int max_pages, hip_batch **out);
