@@ -320,22 +320,20 @@ DEV const void *uniform(const void *p) {
 }
 // LDS DMA: lane i's 16 (4) bytes at base + off land at lds + 16 i (4 i). Untracked by the compiler, which would otherwise wait
 // for all of them before every LDS read: callers wait with wait_dma.
-// `lanes`: which take part; as data, so that a conditional load is no branch. m0 and exec are restored.
+// `lanes`: which take part; as data, so that a conditional load is no branch. Called with all lanes on; m0 is restored.
 DEV void dma16_global(const void *base, uint32_t off, uint32_t lds, uint64_t lanes) {
     uint32_t save;
-    uint64_t all;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b64 %1, exec\n\ts_mov_b32 m0, %2\n\ts_mov_b64 exec, %5\n\ts_nop 1\n\t"
-                 "global_load_lds_dwordx4 %3, %4\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(save), "=&s"(all)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_mov_b64 exec, %4\n\ts_nop 1\n\t"
+                 "global_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save)
                  : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(uniform(base)), "s"(lanes)
                  : "memory");
 }
 DEV void dma4_global(const void *at, uint32_t lds, uint64_t lanes) {
     uint32_t save;
-    uint64_t all;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b64 %1, exec\n\ts_mov_b32 m0, %2\n\ts_mov_b64 exec, %4\n\ts_nop 1\n\t"
-                 "global_load_lds_dword %3, off\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(save), "=&s"(all)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_mov_b64 exec, %3\n\ts_nop 1\n\t"
+                 "global_load_lds_dword %2, off\n\ts_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save)
                  : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at), "s"(lanes)
                  : "memory");
 }
@@ -404,28 +402,35 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         on[x] = loads ? __ballot(piece * (Q8 ? 16 : 8) < hd) : 0;
         piece_at[x] = (uint32_t)piece * 16u, row_at[x] = (uint32_t)(row & 15) * pos_b;
     }
-    // Pages: lane t holds those of the wave's rows (Q8: of both runs of 16) of tile 64 c + t; read again every 64 tiles. (A scalar
-    // load per tile would be waited for at every barrier.)
-    uint32_t pages[Q8 ? 2 : 1];
+    // The wave's rows of a tile in memory: their run of 16, the first byte of its last row that is to be read (behind the last
+    // position: that one again, its weight is 0). Lane t holds those of tile 64 c + t (Q8: and the pages of the tile's scales),
+    // formed again every 64 tiles. (A scalar load of a page per tile would be waited for at every barrier.)
+    uint32_t run_lo = 0, run_hi = 0, run_last = 0, pages[2];
     auto fetch_pages = [&](int i) {
+        const int p = it.k0 + (i + lane) * T;
+        const int first = std::min(p + (row_w & ~15), (n - 1) & ~15);
+        const uint32_t page = g.pages[it.page0 + (first >> g.shift)];
+        const uint64_t at = (uint64_t)kv0 + (uint64_t)page * page_b + (uint64_t)((uint32_t)first & pmask) * pos_b;
+        run_lo = (uint32_t)at, run_hi = (uint32_t)(at >> 32), run_last = (uint32_t)std::min(n - 1 - first, 15) * pos_b;
+        if (Q8)
 #pragma unroll
-        for (int x = 0; x < (Q8 ? 2 : 1); x++) {
-            pages[x] = g.pages[it.page0 + (std::min(it.k0 + (i + lane) * T + (Q8 ? 16 * x : row_w & ~15), n - 1) >> g.shift)];
-            asm volatile("" : "+v"(pages[x]));  // here, not where they are used
-        }
+            for (int x = 0; x < 2; x++) pages[x] = g.pages[it.page0 + (std::min(p + 16 * x, n - 1) >> g.shift)];
+        asm volatile("" : "+v"(run_lo), "+v"(run_hi), "+v"(run_last));  // here, not where they are used
+        if (Q8) asm volatile("" : "+v"(pages[0]), "+v"(pages[1]));
     };
-    auto page_in = [&](int i, bool second) { return (uint32_t)__builtin_amdgcn_readlane((int)(second ? pages[Q8 ? 1 : 0] : pages[0]), i & 63); };
-    // The wave's rows of tile i in memory: their run of 16, its last row that is to be read (behind the last position: that one
-    // again, its weight is 0), and whether there is such a tile. The load of piece x to `slot`.
+    auto of_tile = [&](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i & 63); };
     struct Run {
         const char *at;
-        uint32_t last;  // (its first byte)
-        bool is;
+        uint32_t last;
+        bool is;  // there is such a tile
     };
     auto run_of = [&](int i) {
-        const int first = std::min(it.k0 + i * T + (row_w & ~15), (n - 1) & ~15);
-        return Run{kv0 + (size_t)page_in(i, Q8 && row_w >= 16) * page_b + (size_t)((uint32_t)first & pmask) * pos_b, (uint32_t)std::min(n - 1 - first, 15) * pos_b, i < tiles};
+        return Run{(const char *)((uint64_t)of_tile(run_hi, i) << 32 | of_tile(run_lo, i)), of_tile(run_last, i), i < tiles};
     };
+    // a tile within `inside` (below): all of its rows are there
+    const uint32_t all_rows = 15 * pos_b;
+    auto run_inside = [&](int i) { return Run{(const char *)((uint64_t)of_tile(run_hi, i) << 32 | of_tile(run_lo, i)), all_rows, true}; };
+    // the load of piece x to `slot`
     auto load_piece = [&](const Run &run, int slot, int x) {
         const uint32_t at = std::min(row_at[x], run.last) + piece_at[x];
         dma16_global(run.at, at, to_w + slot * 2 * RAW + RPI * x * RAWP, run.is ? on[x] : 0);
@@ -435,7 +440,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         // two positions a lane: lanes 0 .. 15 keys', 16 .. 31 values'; whole runs of 16 (what lies behind the last position is
         // not used)
         const uint32_t p = (uint32_t)(it.k0 + i * T + 2 * (lane & 15));
-        const uint32_t page = lane & 8 ? page_in(i, true) : page_in(i, false);
+        const uint32_t page = lane & 8 ? of_tile(pages[1], i) : of_tile(pages[0], i);
         const uint16_t *const sc = lane & 16 ? g.kv.v_scale : g.kv.k_scale;
         dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + (p & pmask), at0 + SCALES + slot * 128, w == 0 && i < tiles ? 0xffffffffull : 0);
     };
@@ -519,13 +524,14 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     // behind the last). k_at, v_at: the next tile's keys and this one's values in LDS. Written out in the
     // order of issue: a score product, its share of the exponentials and a load; then a product of values beside the maxima of
     // the new scores; operands are read AHEAD products before theirs.
-    auto step = [&](int i, uint32_t k_at, uint32_t v_at, int to, f16v &s, f16v &y) {
+    auto step = [&](int i, uint32_t k_at, uint32_t v_at, int to, f16v &s, f16v &y, auto within) {
+        constexpr bool INSIDE = decltype(within)::value;
         const int s0 = it.k0 + i * T;
         constexpr int AHEAD = 4;
         h8 kr[AHEAD], vr[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) kr[j] = key_operand(k_at, j);
-        if (s0 + T > wn_all) {
+        if (!INSIDE && s0 + T > wn_all) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = s0 + 8 * (e >> 2) + 4 * hf + (e & 3) < lim ? s[e] : -INFINITY;
             mx = s[0];
@@ -542,7 +548,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= a;
         }
-        const Run run = run_of(i + D - 1);
+        const Run run = INSIDE ? run_inside(i + D - 1) : run_of(i + D - 1);
         zero_scores(y);
         float x[16];
         h8 p[2];
@@ -638,29 +644,39 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
         for (int e = 0; e < 16; e++) mx = fmaxf(mx, sa[e]);
     }
-    int slot = 0;  // i % D
-    auto tile = [&](int i, f16v &s, f16v &y) {
-        const int s0 = it.k0 + i * T, before = slot == 0 ? D - 1 : slot - 1, after = slot == D - 1 ? 0 : slot + 1;
+    int before = D - 1, slot = 0, after = 1;  // of tiles i - 1, i and i + 1
+    auto tile = [&](int i, f16v &s, f16v &y, auto within) {
+        constexpr bool INSIDE = decltype(within)::value;
         // tile i + LEAD is there, the tiles behind it may still be on their way
-        wait_tile(i + LEAD, std::min(i + D - 1, tiles), std::integral_constant<int, D - 2 - LEAD>());
+        if (INSIDE) wait_dma<(D - 2 - LEAD) * NI>();
+        else wait_tile(i + LEAD, std::min(i + D - 1, tiles), std::integral_constant<int, D - 2 - LEAD>());
         barrier();
-        if (s0 < wn) {
-            if (Q8) step(i, (~i & 1) * TILE, (i & 1) * TILE, before, s, y);
-            else step(i, after * 2 * RAW, slot * 2 * RAW, before, s, y);
+        if (INSIDE || it.k0 + i * T < wn) {
+            if (Q8) step(i, (~i & 1) * TILE, (i & 1) * TILE, before, s, y, within);
+            else step(i, after * 2 * RAW, slot * 2 * RAW, before, s, y, within);
         } else {
             const Run run = run_of(i + D - 1);
 #pragma unroll
             for (int x = 0; x < NI; x++) load_piece(run, before, x);
             load_scales(i + D - 1, before);
         }
-        if (((i + D) & 63) == 0) fetch_pages(i + D);
+        if (!INSIDE && ((i + D) & 63) == 0) fetch_pages(i + D);
         if constexpr (Q8) decode(i + LEAD, false), decode(i + 1, true);
-        else look(i + LEAD);
-        slot = after;
+        else if (!INSIDE) look(i + LEAD);
+        before = slot, slot = after, after = __builtin_amdgcn_readfirstlane(after == D - 1 ? 0 : after + 1);
     };
+    // Two tiles at a time (their score registers change places). Below `inside` every row sees all of both tiles and of the one
+    // that is looked at next, and all that is loaded is there: no test but the maximum's is left. (A wave without rows stays out.
+    // Q8: a second copy of its longer loop spills, and scratch would count among the loads that wait_dma counts.)
+    const int inside = !Q8 && r0 < it.R ? std::min(tiles - D, (n_blk - it.k0) / T - 1 - LEAD) : 0;
     for (int i = 0; i < tiles; i += 2) {
-        tile(i, sa, sb);
-        if (i + 1 < tiles) tile(i + 1, sb, sa);
+        if constexpr (!Q8)
+            for (; i < inside && ((i + D) & 63) && ((i + 1 + D) & 63); i += 2) {
+                tile(i, sa, sb, std::true_type());
+                tile(i + 1, sb, sa, std::true_type());
+            }
+        tile(i, sa, sb, std::false_type());
+        if (i + 1 < tiles) tile(i + 1, sb, sa, std::false_type());
     }
     wait_dma<0>();
     __syncthreads();
