@@ -146,7 +146,7 @@ void plan_attention(const hq_kv_t &kv, int n_heads, int n_cu, int n_seqs, const 
         }
         // blocks of one sequence and kv head read the same keys and values: items go to the XCDs (workgroup i runs on XCD
         // i % 8) in eight runs, each longest first: of equal work, or, where every item has a workgroup's place of its own, of
-        // equal numbers (30 decoded sequences and a chunk of 1000, 256 items of unlike lengths: 103 -> 77 us)
+        // equal numbers (30 decoded sequences and a chunk of 1000, 256 items of unlike lengths: 103 -> 77 us then)
         int64_t total = 0, run = 0;
         for (const HqItem &it : all) total += it.k1 - it.k0 + unit;
         std::vector<HqItem> q[XCDS];

@@ -355,11 +355,13 @@ constexpr int DEPTH = HDP <= 128 && NW == 8 ? 6 : Q8 ? 5 : 4;
 // Eight waves of 32 rows, two per SIMD, for heads up to 128: a key is read from LDS once per 32 rows and from the cache once
 // per 256. 64 rows per wave spill, and four waves in each of two workgroups read every tile twice (10 % slower). Heads above
 // 128 leave room for one wave per SIMD.
-// Bound: the matrix products. 4 rows positions head_dim products, of which 2 % are masked ones. Heads of 128: 2300 cycles a tile
-// and SIMD, 1088 of them the matrix cores' (39 % busy with what is around the loop), at the 1.8 GHz that the power allows; no
-// one part is behind the rest (2180 without the rescaling, 1970 without the exponentials, 1930 without the DMA). 16384 tokens
-// of ten prompts, 32 / 8 heads: 655 us, 795 TFLOP/s; 512 tokens behind 32256: 312 us, 875 TFLOP/s. Heads of 256: 2750 cycles,
-// 900 of them the DMA's issue, which no second wave hides; 1000 tokens behind 2001, 16 / 4 heads: 77 us, 530 TFLOP/s.
+// Bound: the matrix products, 4 head_dim per row and position (2 % more for the masked ones), and the power they take. Heads of
+// 128: 1800 cycles a tile and SIMD, 1024 of them the matrix cores' (54 % busy with what is around the loop), at 1.7 GHz; without
+// the loop's DMA 1730 cycles at 1.6 GHz. What made it 1800 from 2300 is fewer scalar instructions and branches: a SIMD has two
+// waves to hide them. Two groups of waves half a tile apart (products of values beside exponentials) or priorities changed
+// nothing. 16384 tokens of ten prompts, 32 / 8 heads: 615 us, 850 TFLOP/s; 512 tokens behind 32256: 280 us, 970 TFLOP/s. Heads of
+// 256: 2150 cycles, 470 of them the DMA's issue, which no second wave hides; 1000 tokens behind 2001, 16 / 4 heads: 64 us, 640
+// TFLOP/s.
 template <int HDP, bool Q8, int NW>
 __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     constexpr int P = PITCH<HDP>, T = KT, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
