@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         mx = my;
     };
     if (tiles) {
-        if (!Q8 && hd < HDP)  // (decode() writes zeros itself)
+        if (!Q8 && 2 * hd < P)  // what no load writes: 0, for the products and for look() (decode() writes zeros itself)
             for (int x = threadIdx.x; x < D * 2 * RAW / 16; x += 64 * NW) *(u4v *)(lds + x * 16) = u4v{0, 0, 0, 0};
         fetch_pages(0);
         barrier();
