@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         asm volatile("" : "+v"(run_lo), "+v"(run_hi), "+v"(run_last));  // here, not where they are used
         if (Q8) asm volatile("" : "+v"(pages[0]), "+v"(pages[1]));
     };
+    // (with all lanes on: under a mask the register may be a copy made for the lanes that are on, and lane i's of it anything)
     auto of_tile = [&](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i & 63); };
     struct Run {
         const char *at;
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         // two positions a lane: lanes 0 .. 15 keys', 16 .. 31 values'; whole runs of 16 (what lies behind the last position is
         // not used)
         const uint32_t p = (uint32_t)(it.k0 + i * T + 2 * (lane & 15));
-        const uint32_t page = lane & 8 ? of_tile(pages[1], i) : of_tile(pages[0], i);
+        const uint32_t low = of_tile(pages[0], i), high = of_tile(pages[1], i), page = lane & 8 ? high : low;
         const uint16_t *const sc = lane & 16 ? g.kv.v_scale : g.kv.k_scale;
         dma4_global(sc + ((size_t)page * g.kv.n_kv_heads + it.kvh) * g.kv.page_size + (p & pmask), at0 + SCALES + slot * 128, w == 0 && i < tiles ? 0xffffffffull : 0);
     };
