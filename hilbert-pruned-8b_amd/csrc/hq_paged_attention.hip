@@ -11,8 +11,10 @@
 //
 // Precision: fp16 operands, fp32 products, sums, maxima and outputs. Rounded to 16 bits are the weights p alone (2^-11 of each;
 // the sum takes them unrounded). Of a Q8 cache the operands are exact: keys enter as their codes and the scores take the
-// scale in fp32; values enter as code * 2^e, the scale's power of two (exact down to fp16's last bit), and its mantissa
-// joins the weight before that is rounded. Decoding to fp16 instead doubled the error of the outputs (2.1e-4 -> 4.8e-4).
+// scale in fp32; values enter as code * 2^(e-7), e the exponent of their scale: a normal or subnormal fp16 number, finite and
+// exact for every finite scale (2^e itself made infinities of codes from 64 on under scales from 1024 on). The scale's mantissa
+// joins the weight before that is rounded, the 2^7 the weights' sum. Decoding to fp16 instead doubled the error of the outputs
+// (2.1e-4 -> 4.8e-4).
 //
 // Places that a row does not see weigh 0, and 0 times an infinity or NaN would be NaN: in a tile that some row sees only part
 // of, values that are not finite (`odd` below) enter the product as 0, and are added to the outputs of the rows that do see
@@ -97,11 +99,17 @@ DEV h2 codes2(uint32_t w) {
     const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
     return as_h2(w) - bias;
 }
-// A value scale as a power of two (the scale itself where it is not finite) and what remains, fp32 in [1, 2), below 1 for
-// scales under fp16's normal range; 1 where it is not finite.
-DEV uint32_t pow2_of(uint32_t d) { return (d & 0x7c00u) == 0x7c00u ? d : (d & 0x7c00u) < 0x400u ? 0x400u : d & 0x7c00u; }
+// A value scale as the power of two of its exponent (of fp16's lowest normal one below that) and what remains, fp32 in [1, 2),
+// below 1 for subnormal scales; the scale itself and 1 where it is not finite. The power comes 2^-7 smaller: 127 2^8 is the
+// largest product with a code, 2^-21 the smallest. Q8_SUM makes up for it in the weights' sum.
+constexpr float Q8_SUM = 1.0f / 128.0f;
+DEV uint16_t exponent_of(uint32_t d) { return (uint16_t)std::max(d & 0x7c00u, 0x400u); }
+DEV uint32_t pow2_of(uint32_t d) {
+    const uint16_t small = __builtin_bit_cast(uint16_t, (_Float16)(__builtin_bit_cast(_Float16, exponent_of(d)) * (_Float16)Q8_SUM));
+    return (d & 0x7c00u) == 0x7c00u ? d : small;
+}
 DEV float rest_of(uint32_t d) {
-    const uint32_t inverse = 0x7f000000u - __builtin_bit_cast(uint32_t, h2f((uint16_t)pow2_of(d)));  // of 2^k: 2^-k
+    const uint32_t inverse = 0x7f000000u - __builtin_bit_cast(uint32_t, h2f(exponent_of(d)));  // of 2^k: 2^-k
     return (d & 0x7c00u) == 0x7c00u ? 1.f : h2f((uint16_t)d) * __builtin_bit_cast(float, inverse);
 }
 // 16 codes times d: a power of two, or 1
@@ -714,7 +722,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
                 }
         }
     }
-    const float lt = sum_halves(l);
+    const float lt = sum_halves(l) * (Q8 ? Q8_SUM : 1.f);
     if (it.n_parts > 1) {
         float *const to = g.parts + (size_t)it.part_at * 4 + (size_t)(it.part * 32 * NW + 32 * w + li) * PARTF<HDP>;
 #pragma unroll
@@ -966,8 +974,8 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
         if (cut) {
 #pragma unroll
             for (int p = 0; p < 2; p++) {
-                // Q8: scales from 512 on (their products may pass fp16), infinities and NaN
-                if (Q8) bad |= ((vsc[p].x | vsc[p].x >> 16 | vsc[p].y | vsc[p].y >> 16) & 0x6000u) == 0x6000u;
+                // (Q8: values are not finite where their scale is not)
+                if (Q8) bad |= odd2(vsc[p].x) || odd2(vsc[p].y);
                 else
 #pragma unroll
                     for (int r = 0; r < 4; r++)
@@ -1008,7 +1016,7 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
     // the waves' parts, in wave order
 #pragma unroll
     for (int b = 0; b < QB; b++) {
-        const float lt = sum_lg(l[b]);
+        const float lt = sum_lg(l[b]) * (Q8 ? Q8_SUM : 1.f);
         if (lg == 0) ms[w][16 * b + li] = m[b] == -INFINITY ? -INFINITY : mref[b], ls[w][16 * b + li] = lt;
     }
     __syncthreads();
