@@ -9,8 +9,9 @@
 // every lane and positions in its registers, which is the B operand of O^T = V^T P^T. Both run the online softmax: a running
 // maximum and sum per row, outputs scaled when the maximum grows.
 //
-// Precision: fp16 operands, fp32 products, sums, maxima and outputs. Rounded to 16 bits are the weights p alone (2^-11 of each;
-// the sum takes them unrounded). Of a Q8 cache the operands are exact: keys enter as their codes and the scores take the
+// Precision: fp16 operands, fp32 products, sums, maxima and outputs. Rounded to 16 bits are the weights p alone: off by 2^-11 of
+// each or 2^-31 of the row's largest, whichever is more (LIFT below). Their sum takes them as they are multiplied in k_rows over
+// an fp16 cache, before the rounding elsewhere. Of a Q8 cache the operands are exact: keys enter as their codes and the scores take the
 // scale in fp32; values enter as code * 2^(e-7), e the exponent of their scale: a normal or subnormal fp16 number, finite and
 // exact for every finite scale (2^e itself made infinities of codes from 64 on under scales from 1024 on). The scale's mantissa
 // joins the weight before that is rounded, the 2^7 the weights' sum. Decoding to fp16 instead doubled the error of the outputs
@@ -68,6 +69,12 @@ DEV float max_lg(float v) { return max_halves(fmaxf(v, __shfl_xor(v, 16, 64))); 
 DEV float sum_lg(float v) { return sum_halves(v + __shfl_xor(v, 16, 64)); }
 
 DEV float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+// Weights are 2^(score - m + LIFT), m a row's maximum when its outputs were last rescaled, at most SLACK below the present one
+// (log2 units): up to 2^14, 2^15 with a value scale's mantissa, in fp16. LIFT keeps light weights out of fp16's subnormal range:
+// without it those below 2^-25 of the largest are 0, and with many of them so is a part of the answer. A smaller SLACK leaves
+// more room for LIFT and rescales more often: packed prompts 626 us with 8 and 6, 634 with 6 and 8, 647 with 4 and 10 (624 with 8
+// and 0).
+constexpr float SLACK = 8.0f, LIFT = 6.0f;
 // 2^(x - m) of a part's maximum x (log2 units) against the row's m; a part that saw nothing has x = -inf
 DEV float part_scale(float x, float m) { return x == -INFINITY ? 0.f : ex2(x - m); }
 
@@ -550,7 +557,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
             for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[e]);
         }
         if (__any(mx > m + g.slack)) {
-            const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
+            const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : (Q8 ? mn : mn * g.sc) - LIFT;
             const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
             m = mn, mref = nref;
             l *= a;
@@ -937,7 +944,7 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
 #pragma unroll
                 for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[b][p][r]);
             if (__any(mx > m[b] + g.slack)) {
-                const float mn = fmaxf(m[b], max_lg(mx)), nref = mn == -INFINITY ? 0.f : Q8 ? mn : mn * g.sc;
+                const float mn = fmaxf(m[b], max_lg(mx)), nref = mn == -INFINITY ? 0.f : (Q8 ? mn : mn * g.sc) - LIFT;
                 const float a = m[b] == -INFINITY ? 0.f : ex2(mref[b] - nref);
                 m[b] = mn, mref[b] = nref;
                 l[b] *= a;
@@ -1138,7 +1145,7 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
     if (g.rep > 1) g.inverse = (uint32_t)((((uint64_t)1 << 32) + (uint64_t)g.rep - 1) / (uint64_t)g.rep);
     // (a smaller scale leaves every weight alike in fp32; 0 would make NaN of masked scores)
     g.sc = std::max(fabsf(a->scale) * 1.4426950408889634f, 1e-30f);
-    g.slack = kv->type == HQ_KV_Q8 ? 8.0f : 8.0f / g.sc;  // weights up to 2^8 (2^9 with a value scale's mantissa) keep their 11 bits in fp16
+    g.slack = kv->type == HQ_KV_Q8 ? SLACK : SLACK / g.sc;
     for (int body = 0; body < HQ_BODIES; body++) {
         if (!b->n_items[body]) continue;
         g.items = b->items[body];

@@ -108,9 +108,10 @@ typedef struct {
 } hq_attn_t;
 
 /* out = softmax(scale * q . K) V for every new token and head over positions 0 .. the token's own of its sequence, which
- * the cache holds (the step's own among them: hq_rope_append first). fp16 products, everything else fp32. Positions after
- * a token, and what else a page holds, do not affect it whatever their bits. The result does not depend on how the work
- * was split over time: the same batch gives the same bits. */
+ * the cache holds (the step's own among them: hq_rope_append first). fp16 products (a weight is off by 2^-11 of itself or
+ * 2^-31 of its row's largest, whichever is more), everything else fp32. Positions after a token, and what else a page holds,
+ * do not affect it whatever their bits. The result does not depend on how the work was split over time: the same batch gives
+ * the same bits. */
 int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_t *a, void *stream);
 
 /* ---- log probabilities */

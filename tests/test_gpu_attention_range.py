@@ -44,3 +44,29 @@ def test_q8_value_scales_over_their_range(hqlib, scale, nh, hd, lens, cancel):
     assert np.abs(want).max() < 6e4
     print(f"[gpu] Q8 value scale {scale}: {nh} heads x {hd} {lens} cancel={cancel}", flush=True)
     check(run(hqlib, pool, nh, [lens], q, 1.0), want, bound)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("nh,hd,lens", [(1, 64, (1, 9000)), (8, 128, (2, 3000)), (3, 256, (1, 5000)), (2, 96, (40, 3000)), (4, 128, (70, 2000)), (1, 256, (60, 3000))])
+@pytest.mark.parametrize("bits", [13, 17, 21, 25.1])
+def test_light_tails(hqlib, bits, nh, hd, lens, q8):
+    """One position in 97 has nearly all of the weight, the others 2^-bits of it each, and some dims' values are 0 at the heavy
+    ones: those outputs are the tail's alone. Beside serve_ref's bound a weight may be off by half of fp16's subnormal step in
+    units of the row's largest, which is 2^6 when it is rounded: 2^-31, in the outputs' sums and in the sum of weights."""
+    rng = np.random.default_rng(hd + int(bits))
+    new, n = lens
+    heavy = np.arange(n) % 97 == 5
+    base = np.zeros(hd)
+    base[::4] = 1
+    q = np.broadcast_to(2 * base, (new, nh, hd)).astype(np.float16)
+    top = bits * np.log(2) / (2 * base.sum())  # of a heavy key's dims: its score is bits * ln 2, the others' are near 0
+    k = np.where(heavy[:, None, None], top * base, 0) + rng.normal(0, 0.2 / np.sqrt(hd), (n, 1, hd)) * base
+    v = rng.uniform(0.5, 1, (n, 1, hd))
+    v[heavy, :, :hd // 2] = 0
+    pool = Pool(rng, [n], 16, 1, hd, q8)
+    pool.put(0, np.arange(n), k.astype(np.float16), v.astype(np.float16))
+    want, bound = attention(pool, q, [new], [n], 1.0)
+    seen = n - new + 1 + np.arange(new)[:, None, None]
+    bound += 2.0 ** -31 * seen / (seen // 97) * (np.abs(v).max() + np.abs(want))
+    print(f"[gpu] light tails: 2^-{bits}, {nh} heads x {hd} {lens} q8={q8}", flush=True)
+    check(run(hqlib, pool, nh, [lens], q, 1.0), want, bound)
