@@ -75,6 +75,26 @@ DEV float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 // more room for LIFT and rescales more often: packed prompts 626 us with 8 and 6, 634 with 6 and 8, 647 with 4 and 10 (624 with 8
 // and 0).
 constexpr float SLACK = 8.0f, LIFT = 6.0f;
+// m of a row (raw scores; Q8: in log2 units) and what its exponents are taken against. Against a reference past FAR, whose rounding is no small part of a weight's exponent, weights would be infinite or all 0: such
+// rows take their scores against m first, and are rescaled at every tile, so that the common case has no test of it.
+constexpr float FAR = 4194304.0f;
+template <bool Q8>
+struct Top {
+    float m = -INFINITY, ref = 0.f;
+    // the score from which on the row is rescaled
+    __device__ __forceinline__ float limit(const Args &g) const { return ref == -LIFT ? -INFINITY : m + g.slack; }
+    __device__ __forceinline__ float log2_of(const Args &g, float x) const { return fmaf(x, Q8 ? 1.f : g.sc, -LIFT); }
+    // m rises to mn: what the outputs are scaled with; far: scores lose m
+    __device__ __forceinline__ float raise(const Args &g, float mn, bool &far) {
+        const float from = log2_of(g, m), to = log2_of(g, mn);
+        far = fabsf(to) > FAR && mn != -INFINITY;
+        const float a = m == -INFINITY ? 0.f : ex2(far ? (m - mn) * (Q8 ? 1.f : g.sc) : from - to);
+        m = mn, ref = far ? -LIFT : mn == -INFINITY ? 0.f : to;
+        return a;
+    }
+    // of a part, for part_scale
+    __device__ __forceinline__ float part(const Args &g) const { return m == -INFINITY ? -INFINITY : log2_of(g, m); }
+};
 // 2^(x - m) of a part's maximum x (log2 units) against the row's m; a part that saw nothing has x = -inf
 DEV float part_scale(float x, float m) { return x == -INFINITY ? 0.f : ex2(x - m); }
 
@@ -503,7 +523,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 
     float mx = -INFINITY;                      // of the lane's scores of the tile whose turn it is
     h8 q[NJ];
-    float m = -INFINITY, mref = 0.f, l = 0.f;  // the running maximum (raw scores; Q8: in log2 units), what the exponents are taken against, the sum
+    Top<Q8> top;
+    float limit = -INFINITY, l = 0.f;  // top's limit; the weights' sum
     f16v o[ND], sa, sb;  // outputs; scores of a tile and of the next
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -556,10 +577,13 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 #pragma unroll
             for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[e]);
         }
-        if (__any(mx > m + g.slack)) {
-            const float mn = fmaxf(m, max_halves(mx)), nref = mn == -INFINITY ? 0.f : (Q8 ? mn : mn * g.sc) - LIFT;
-            const float a = m == -INFINITY ? 0.f : ex2(mref - nref);
-            m = mn, mref = nref;
+        if (__any(mx > limit)) {
+            bool far;
+            const float a = top.raise(g, fmaxf(top.m, max_halves(mx)), far);
+            limit = top.limit(g);
+            if (__any(far))
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] -= far ? top.m : 0.f;
             l *= a;
 #pragma unroll
             for (int d = 0; d < ND; d++)
@@ -577,7 +601,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         // weights 2 c and 2 c + 1: their exponentials; later, as fp16 (and summed)
         auto weigh = [&](int c) {
 #pragma unroll
-            for (int e = 2 * c; e < 2 * c + 2; e++) x[e] = ex2(Q8 ? s[e] - mref : fmaf(s[e], g.sc, -mref));
+            for (int e = 2 * c; e < 2 * c + 2; e++) x[e] = ex2(Q8 ? s[e] - top.ref : fmaf(s[e], g.sc, -top.ref));
         };
         auto round = [&](int c) {
             const int e = 2 * c;
@@ -736,7 +760,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int c = 0; c < 4; c++) *(f4 *)(to + 32 * d + 8 * c + 4 * hf) = f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
-        if (hf == 0) *(f4 *)(to + HDP) = f4{m == -INFINITY ? -INFINITY : mref, lt, 0.f, 0.f};
+        if (hf == 0) *(f4 *)(to + HDP) = f4{top.part(g), lt, 0.f, 0.f};
         return;
     }
     // outputs through LDS (the ring is done with): 16 bytes a lane, whole rows an instruction
@@ -865,11 +889,12 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
         }
     };
 
-    float m[QB], mref[QB], l[QB];
+    Top<Q8> top[QB];
+    float l[QB];
     f4 o[QB][DPL];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
-        m[b] = -INFINITY, mref[b] = 0.f, l[b] = 0.f;
+        l[b] = 0.f;
 #pragma unroll
         for (int c = 0; c < DPL; c++) o[b][c] = f4{0.f, 0.f, 0.f, 0.f};
     }
@@ -943,10 +968,14 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
             for (int p = 0; p < 2; p++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[b][p][r]);
-            if (__any(mx > m[b] + g.slack)) {
-                const float mn = fmaxf(m[b], max_lg(mx)), nref = mn == -INFINITY ? 0.f : (Q8 ? mn : mn * g.sc) - LIFT;
-                const float a = m[b] == -INFINITY ? 0.f : ex2(mref[b] - nref);
-                m[b] = mn, mref[b] = nref;
+            if (__any(mx > top[b].limit(g))) {
+                bool far;
+                const float a = top[b].raise(g, fmaxf(top[b].m, max_lg(mx)), far);
+                if (__any(far))
+#pragma unroll
+                    for (int p = 0; p < 2; p++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) s[b][p][r] -= far ? top[b].m : 0.f;
                 l[b] *= a;
 #pragma unroll
                 for (int c = 0; c < DPL; c++) o[b][c] *= a;
@@ -955,7 +984,7 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
             for (int p = 0; p < 2; p++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float x = ex2(Q8 ? s[b][p][r] - mref[b] : fmaf(s[b][p][r], g.sc, -mref[b]));
+                    const float x = ex2(Q8 ? s[b][p][r] - top[b].ref : fmaf(s[b][p][r], g.sc, -top[b].ref));
                     l[b] += x;
                     pr[b][4 * p + r] = (_Float16)(Q8 ? x * rest[p][r] : x);
                 }
@@ -1024,7 +1053,7 @@ DEV void stream_item(const Args &g, const HqItem &it, StreamLds<HDP, QB, NW> &ld
 #pragma unroll
     for (int b = 0; b < QB; b++) {
         const float lt = sum_lg(l[b]) * (Q8 ? Q8_SUM : 1.f);
-        if (lg == 0) ms[w][16 * b + li] = m[b] == -INFINITY ? -INFINITY : mref[b], ls[w][16 * b + li] = lt;
+        if (lg == 0) ms[w][16 * b + li] = top[b].part(g), ls[w][16 * b + li] = lt;
     }
     __syncthreads();
 #pragma unroll

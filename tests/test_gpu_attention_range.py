@@ -70,3 +70,29 @@ def test_light_tails(hqlib, bits, nh, hd, lens, q8):
     bound += 2.0 ** -31 * seen / (seen // 97) * (np.abs(v).max() + np.abs(want))
     print(f"[gpu] light tails: 2^-{bits}, {nh} heads x {hd} {lens} q8={q8}", flush=True)
     check(run(hqlib, pool, nh, [lens], q, 1.0), want, bound)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("nh,hd,lens", [(1, 64, (1, 900)), (8, 128, (2, 3000)), (3, 256, (1, 500)), (2, 96, (40, 300)), (4, 128, (70, 2000)), (1, 256, (60, 700))])
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+@pytest.mark.parametrize("scale", [3e5, -1e9, 1e20])
+def test_large_scores(hqlib, scale, order, nh, hd, lens, q8):
+    """Scores whose fp32 steps are many powers of two of a weight: the row's largest ones share all of it, whatever their size.
+    Scores here are exact in fp32 and 10^5 apart at least, so the weights are equal or 0: outputs are off by the weights' and
+    their own rounding, and the sums'."""
+    rng = np.random.default_rng(hd)
+    new, n = lens
+    c = rng.integers(-2000, 2001, n)
+    c = np.sort(c) if order == "up" else np.sort(c)[::-1] if order == "down" else c
+    c[rng.integers(0, n, 4)] = c.max()
+    c[rng.integers(0, n, 4)] = c.min()
+    k = np.zeros((n, 1, hd), np.float16)
+    k[:, 0, 3] = c
+    q = np.zeros((new, nh, hd), np.float16)
+    q[:, :, 3] = 1
+    pool = Pool(rng, [n], 16, 1, hd, q8)
+    pool.put(0, np.arange(n), k, rng.normal(0, 1, (n, 1, hd)).astype(np.float16))
+    want, _ = attention(pool, q, [new], [n], scale)
+    v = np.abs(pool.get("v", 0, n)).max()
+    print(f"[gpu] large scores: {scale} {order}, {nh} heads x {hd} {lens} q8={q8}", flush=True)
+    check(run(hqlib, pool, nh, [lens], q, scale), want, np.full(want.shape, 3 * 2.0 ** -11 * v))
