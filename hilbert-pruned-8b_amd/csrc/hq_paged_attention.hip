@@ -710,7 +710,9 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     // Two tiles at a time (their score registers change places). Below `inside` every row sees all of both tiles and of the one
     // that is looked at next, and all that is loaded is there: no test but the maximum's is left. (A wave without rows stays out.
     // Q8: a second copy of its longer loop spills, and scratch would count among the loads that wait_dma counts.)
-    const int inside = !Q8 && r0 < it.R ? std::min(tiles - D, (n_blk - it.k0) / T - 1 - LEAD) : 0;
+    // (Tile i + D, which the second of them loads, is a whole one: behind the last position may stand infinities or NaN, which
+    // would send the block through the loop over odd values for nothing.)
+    const int inside = !Q8 && r0 < it.R ? std::min((end - it.k0) / T - D, (n_blk - it.k0) / T - 1 - LEAD) : 0;
     for (int i = 0; i < tiles; i += 2) {
         if constexpr (!Q8)
             for (; i < inside && ((i + D) & 63) && ((i + 1 + D) & 63); i += 2) {

@@ -2,6 +2,8 @@
 formed again every 64 tiles, and most tiles go through the loop without tests. The step's plan leaves a block of rows whole where
 there are as many blocks as the chip has places for workgroups (256 CUs, one or two each), so there are that many kv heads here;
 they share one head's memory (head_stride 0), which lets the reference be one float64 product."""
+import time
+
 import numpy as np
 import pytest
 
@@ -57,4 +59,35 @@ def test_long_items(hqlib, nkv, rep, hd, lens, q8):
         check(got[t:t + new][:, heads], *reference(pool, s, q[t:t + new][:, heads], n, hd ** -0.5))
         t += new
     assert np.isfinite(got).all()
+    b.free()
+
+
+@pytest.mark.parametrize("nkv,rep,hd,n", [(256, 8, 128, 660), (256, 8, 96, 660), (256, 4, 256, 660), (512, 4, 64, 660)])
+def test_places_behind_the_end_cost_nothing(hqlib, nkv, rep, hd, n):
+    """What stands behind a sequence's last position, in the same tile of 32, costs no time: NaN there take as long as zeros. (An
+    odd number of tiles, the last one partial; the loop over values that are not finite would take more than twice as long.)"""
+    rng = np.random.default_rng(hd)
+    new = 32 if hd != 64 else 20
+    page, nh = 64, nkv * rep
+    pool = Pool(rng, [n], page, 1, hd)
+    fill(pool, rng, [n])
+    dq, out = hqlib.DevBuf.from_array(rng.normal(0, 1, (new, nh, hd)).astype(np.float16)), hqlib.DevBuf(new * nh * hd * 2)
+    kvs = []
+    for empty in (np.nan, 0):
+        dev = [hqlib.DevBuf.from_array(np.where(np.isnan(pool.c[m]), np.float16(empty), pool.c[m])) for m in "kv"]
+        kvs.append(hqlib.KvCache(hqlib.KV_F16, pool.n_pages, page, nkv, hd, *dev, (page * hd, hd, 0)))
+    b = hqlib.Batch(1, new, pool.table.shape[1])
+    b.set(kvs[0], nh, [new], [n], pool.table)
+    print(f"[gpu] places behind the end: {nkv} x {rep} heads of {hd}", flush=True)
+    best = [1e9, 1e9]
+    for _ in range(12):
+        for i, kv in enumerate(kvs):
+            hqlib.synchronize()
+            t = time.perf_counter()
+            for _ in range(20):
+                hqlib.attention(b, kv, dq, out, hd ** -0.5)
+            hqlib.synchronize()
+            best[i] = min(best[i], time.perf_counter() - t)
+    print(f"[gpu]   {best[0] / 20 * 1e6:.1f} us, with zeros {best[1] / 20 * 1e6:.1f}", flush=True)
+    assert best[0] <= 1.3 * best[1]
     b.free()
