@@ -983,6 +983,23 @@ int batch_layers(hip_batch *s, int T) {
     return 0;
 }
 
+// The queued part of a step, from the copy of its host array (words of it) to the last output.
+int batch_run(hip_batch *s, size_t words, int T, int rows, int n_ids, int top_k, float *logp, float *entropy, uint32_t *top_ids, float *top_logp) {
+    HipBackend *b = s->b;
+    const hq_ref_config_t &c = b->m->cfg;
+    BCK(hipMemcpyAsync(s->d_in, s->h_in, words * 4, hipMemcpyHostToDevice, b->st));
+    BCK(hq_launch_dequant(hq_mat_dev(b->embed), 0, s->d_in, (uint32_t)T, s->x, b->st));
+    if (batch_layers(s, T)) return -1;
+    if (n_ids || top_k || entropy) {
+        k_norm_rows<<<rows, 256, 0, b->st>>>(s->x, s->d_in + T, b->final_norm, c.norm_offset, c.eps, s->hb, (int)c.hidden);
+        BCK(hipGetLastError());
+        if (gemm(b, b->lm_head, s->hb, rows, s->logits, false)) return -1;
+        if (hq_logprobs(s->logits, 1, rows, c.vocab, c.vocab, n_ids ? s->d_in + T + rows : nullptr, n_ids, top_k, logp, entropy, top_ids, top_logp, b->st))
+            return -1;
+    }
+    return 0;
+}
+
 }  // namespace
 
 extern "C" int hip_batch_create(hq_ref_backend_t *backend, int kv_type, int page_size, uint32_t n_pages, int max_seqs, int max_tokens,
@@ -1062,18 +1079,12 @@ extern "C" int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, 
         if (n_ids) memcpy(id + (size_t)r * n_ids, ids + (size_t)i * n_ids, (size_t)n_ids * 4);
         r++;
     }
-    BCK(hipMemcpyAsync(s->d_in, s->h_in, ((size_t)T + rows + n_lp) * 4, hipMemcpyHostToDevice, b->st));
-    BCK(hq_launch_dequant(hq_mat_dev(b->embed), 0, s->d_in, (uint32_t)T, s->x, b->st));
-    if (batch_layers(s, (int)T)) return -1;
     float *const o_lp = (float *)s->h_out, *const o_en = o_lp + n_lp, *const o_top = o_en + rows;
     uint32_t *const o_ids = (uint32_t *)(o_top + n_top);
-    if (n_ids || top_k || entropy) {
-        k_norm_rows<<<rows, 256, 0, b->st>>>(s->x, s->d_in + T, b->final_norm, c.norm_offset, c.eps, s->hb, (int)c.hidden);
-        BCK(hipGetLastError());
-        if (gemm(b, b->lm_head, s->hb, rows, s->logits, false)) return -1;
-        if (hq_logprobs(s->logits, 1, rows, c.vocab, c.vocab, n_ids ? s->d_in + T + rows : nullptr, n_ids, top_k, n_ids ? o_lp : nullptr,
-                        entropy ? o_en : nullptr, top_ids ? o_ids : nullptr, top_logp ? o_top : nullptr, b->st))
-            return -1;
+    if (batch_run(s, (size_t)T + rows + n_lp, (int)T, rows, n_ids, top_k, n_ids ? o_lp : nullptr, entropy ? o_en : nullptr, top_ids ? o_ids : nullptr, top_logp ? o_top : nullptr)) {
+        // what was queued before the failure still reads h_in, which the next step rewrites
+        (void)hipStreamSynchronize(b->st);
+        return -1;
     }
     BCK(hipStreamSynchronize(b->st));
     for (int i = 0, r = 0; i < n_seqs; i++) {
