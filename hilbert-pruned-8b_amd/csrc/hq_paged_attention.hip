@@ -169,12 +169,19 @@ struct OutRow {
     }
     // what the sums are multiplied with, l their weights' sum
     __device__ __forceinline__ float scale(float l) const { return padding ? 0.f : 1.0f / l; }
-    // gates of dims d .. d + 3 (past head_dim: others)
+    // gates of dims d .. d + 3 (past head_dim: others; of padding, whose row may hold anything: 0)
     __device__ __forceinline__ f4 gates(int d) const {
         d = std::min(d, hd - 4);
-        if (gate_f32) return *(const f4 *)(gate + 4 * d);
-        const h4 y = *(const h4 *)(gate + 2 * d);
-        return f4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+        f4 x;
+        if (gate_f32) {
+            x = *(const f4 *)(gate + 4 * d);
+        } else {
+            const h4 y = *(const h4 *)(gate + 2 * d);
+            x = f4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = padding ? 0.f : x[e];
+        return x;
     }
     __device__ __forceinline__ void put(int d, f4 v) const {
         if (is && d < hd) *(h4 *)(out + d) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
