@@ -359,8 +359,9 @@ DEV void store4(_Float16 *p, f4 x) { *(h4 *)p = h4{(_Float16)x[0], (_Float16)x[1
 // row. Heads j < nh are queries, the next n_kv_heads keys, the last n_kv_heads values. A workgroup takes heads of token
 // blockIdx.x: its cosines and sines are read once.
 // Bound: bytes. 2048 tokens of 32 + 8 + 8 heads of 128, fp32 in: 75 MB in 15.7 us, 4.8 TB/s; 8191 of 16 + 4 + 4 of 256, fp16: 201
-// MB in 46 us, 62 where the inputs come from HBM; 16 tokens: 3.9 us, a launch. Slower at 8191: a workgroup per 8 heads (67 us),
-// workgroups over several tokens (52 .. 58), the next head's values read ahead (50).
+// MB in 46 us, 62 where the inputs come from HBM; 16 tokens: 3.7 us, a launch. To a Q8 cache: 2048 tokens 18 us, 8191 51. Slower
+// at 8191, with the inputs in cache (not compared from HBM): a workgroup per 8 heads (67 us), workgroups over several tokens (52
+// .. 58), the next head's values read ahead (50).
 template <bool F32, int G>
 __global__ void __launch_bounds__(256, 8) k_rope_append(RopeArgs g) {
     const int t = blockIdx.x, hd = g.kv.head_dim, nkv = g.kv.n_kv_heads, half = g.r.rot_dim / 2;

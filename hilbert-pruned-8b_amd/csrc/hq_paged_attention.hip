@@ -403,7 +403,8 @@ constexpr int DEPTH = HDP <= 128 && NW == 8 ? 6 : Q8 ? 5 : 4;
 // waves to hide them. Two groups of waves half a tile apart (products of values beside exponentials) or priorities changed
 // nothing. 16384 tokens of ten prompts, 32 / 8 heads: 615 us, 850 TFLOP/s; 512 tokens behind 32256: 280 us, 970 TFLOP/s. Heads of
 // 256: 2150 cycles, 470 of them the DMA's issue, which no second wave hides; 1000 tokens behind 2001, 16 / 4 heads: 64 us, 640
-// TFLOP/s.
+// TFLOP/s. Over a Q8 cache, which is decoded between barriers and has no loop without tests, the prompts take 764 us, the 512
+// tokens 345.
 template <int HDP, bool Q8, int NW>
 __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     constexpr int P = PITCH<HDP>, T = KT, NJ = HDP / 16, ND = HDP / 32, TILE = T * P, D = DEPTH<HDP, Q8, NW>;
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
     };
     // Two tiles at a time (their score registers change places). Below `inside` every row sees all of both tiles and of the one
     // that is looked at next, and all that is loaded is there: no test but the maximum's is left. (A wave without rows stays out.
-    // Q8: a second copy of its longer loop spills, and scratch would count among the loads that wait_dma counts.)
+    // Q8: a second copy of its longer loop spills, and waits that count loads would wait for the scratch accesses behind them too.)
     // (Tile i + D, which the second of them loads, is a whole one: behind the last position may stand infinities or NaN, which
     // would send the block through the loop over odd values for nothing.)
     const int inside = !Q8 && r0 < it.R ? std::min((end - it.k0) / T - D, (n_blk - it.k0) / T - 1 - LEAD) : 0;
@@ -813,7 +814,8 @@ __global__ void __launch_bounds__(64 * NW, HDP > 128 ? 1 : 2) k_rows(Args g) {
 // 16 + 4 lg + r, which are the positions of its score registers; pairs of positions are put together by v_perm into the
 // operand of block b, whose row li is dim DPL li + b. Nothing goes through LDS before the end: few rows use an operand once.
 // Bound: the cache's bytes. 64 tokens behind 200 .. 8192 positions, 32 / 8 heads of 128: 113 us, 5.1 TB/s; 8 behind 20000 ..
-// 40000 of a Q8 cache: 97 us, 5.0 TB/s. A single sequence: the chain of page, keys, softmax and join, 6.8 us behind 1000
+// 40000 of a Q8 cache: 97 us, 5.0 TB/s. 32 rows of heads of 128 do not fit the registers of two workgroups per CU and spill (412
+// bytes a lane, Q8 324): 16 sequences with 5 new tokens each behind 500 .. 8000, 32 / 8 heads: 54 us, Q8 46. A single sequence: the chain of page, keys, softmax and join, 6.8 us behind 1000
 // positions (8 heads of 64).
 template <int HDP, int QB, int NW>
 struct StreamLds {

@@ -54,8 +54,9 @@ void hq_batch_free(hq_batch *b);
  * not stored, and give zeros. kv: the cache's geometry (its pointers may differ in each call that follows); n_heads: query
  * heads, a multiple of the kv heads (head h reads kv head h / (n_heads / n_kv_heads)). Page numbers are checked here.
  * Also plans hq_attention's work and grows its workspace: the only call of this header, with hq_batch_create and the
- * growing of hq_logprobs' workspace, that allocates. Calls that use the batch must be ordered after it on the device,
- * and the next set after them; calls that overlap in time need batches of their own. */
+ * growing of hq_logprobs' workspace, that allocates. It waits until the last set's transfer is done, and with growing for
+ * the device. Calls that use the batch must be ordered after it on the device, and the next set after them; calls that
+ * overlap in time need batches of their own. */
 int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_seqs, const int32_t *n_new, const int32_t *n_pos,
                  const uint32_t *pages, int pages_ld, void *stream);
 
