@@ -450,9 +450,10 @@ namespace {
 struct Staging {  // slots: 0 x fp32, 1 x fp16, 2 y fp32 (hq_matmul_host), 3 embedding ids, 4 readout ids,
                   // 5 GEMM partial tiles, 6 GEMM tile counters (kept zero), 7 activation sub-block sums,
                   // 8 fp32 gate/up product of the unfused hq_gemm_swiglu path,
-                  // 9 sums of split rows and 10 row counters (kept zero) of hq_logprobs
-    void *buf[11] = {};
-    size_t cap[11] = {};
+                  // 9 sums of split rows and 10 row counters (kept zero) of hq_logprobs,
+                  // 11 rows and 12 counters (kept zero) of hq_beam
+    void *buf[13] = {};
+    size_t cap[13] = {};
 };
 std::mutex g_staging_mu;
 std::map<std::pair<int, void *>, Staging> g_staging;

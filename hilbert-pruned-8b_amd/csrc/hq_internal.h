@@ -28,7 +28,7 @@ int hq_internal_pass_tokens(size_t max_seq, size_t bytes_per_token, size_t free_
 
 /* The current device and its CUs; and a library buffer of at least `bytes` for (device, stream), grown on first need
  * (*grew = 1 then; contents are not kept), freed by hq_stream_destroy. */
-enum { HQ_STAGE_LOGPROBS = 9, HQ_STAGE_LOGPROBS_COUNT = 10 };
+enum { HQ_STAGE_LOGPROBS = 9, HQ_STAGE_LOGPROBS_COUNT = 10, HQ_STAGE_BEAM = 11, HQ_STAGE_BEAM_COUNT = 12 };
 int hq_internal_device(int *device, int *n_cu);
 int hq_internal_staging(int device, void *stream, int slot, size_t bytes, void **p, int *grew);
 

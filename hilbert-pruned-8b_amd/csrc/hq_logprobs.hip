@@ -1,5 +1,5 @@
 // hq_logprobs.hip - log probabilities of given tokens, entropy and likeliest tokens of rows of logits (hq_logprobs,
-// include/hq_serve.h).
+// include/hq_serve.h), and the best continuations of groups of beams (hq_beam).
 //
 // One pass over the logits: each thread keeps m = max x, s = sum e^(x - m) and t = sum (x - m) e^(x - m) of what it reads,
 // rescaled when m grows, so that log p = x - m - log s and the entropy is log s - t / s; both sums have one sign, nothing
@@ -372,8 +372,249 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
     }
 }
 
+// ------------------------------------------------------------------------------------ beams
+// The k best of a group's candidates are among the k likeliest tokens of each of its rows, so each row is read once as above, its
+// top k and the logarithm of its sum go to the workspace, and the last workgroup of the group merges the rows: a candidate's place
+// is the number of candidates before it, found in every other row by bisection (a row's values fall along its list).
+//
+// Values of unlike rows are compared, and a beam's tokens are a choice that cannot be taken back, so the sum of a row is kept to
+// about 2^-23 of itself: the exponentials' arguments as a product and its remainder, eight of them to a 32-bit sum, those to a
+// 64-bit one; a value is formed in 64 bits. Equal logits of one row compare equal whatever the sum.
+struct BeamArgs {
+    LpArgs lp;  // its k: places of a row, k or V
+    int k;
+    const float *score;
+    const uint8_t *done;
+    uint32_t done_token;
+    int n_beams;
+    char *rows;        // [rows][row_bytes]: m and the sum (as 64 bits), what the row is; then its k keys
+    uint32_t row_bytes;
+    int *group_counters;
+    float *out_score;
+    uint32_t *out_token;
+    int32_t *out_beam;
+};
+enum { BEAM_ROW, BEAM_NONE, BEAM_DONE, BEAM_ODD };  // a row with candidates; none; the one of a done beam; NaN or +inf somewhere
+
+// e^d for d <= 0 to about 2^-23 of itself, NaN for NaN
+DEV float ex_sharp(float d) {
+    constexpr float LOG2E_LO = 1.925963033500e-8f, LN2 = 0.69314718055994531f;  // log2 e = LOG2E + LOG2E_LO
+    const float c = fmaxf(d, -1e4f), t = c * LOG2E, lo = fmaf(c, LOG2E_LO, fmaf(c, LOG2E, -t));
+    const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+    return fmaf(e, lo * LN2, e);
+}
+
+struct BeamSum {
+    float m;
+    double s;
+    __device__ __forceinline__ void add(float om, double os) {
+        const float mn = fmaxf(m, om);
+        s = (m == -INFINITY ? s : s * (double)ex_sharp(m - mn)) + (om == -INFINITY ? os : os * (double)ex_sharp(om - mn));
+        m = mn;
+    }
+};
+
+struct BeamMerge {
+    unsigned long long key[HQ_BEAM_MAX * HQ_BEAM_MAX];
+    int rank[HQ_BEAM_MAX * HQ_BEAM_MAX];
+    double m[HQ_BEAM_MAX], logs[HQ_BEAM_MAX], score[HQ_BEAM_MAX];
+    int what[HQ_BEAM_MAX];
+    int odd, n;
+    // the value of place j of row b (k places each)
+    __device__ __forceinline__ double value(int b, int j, int k) const {
+        if (what[b] == BEAM_NONE || (what[b] == BEAM_DONE && j)) return -INFINITY;
+        if (what[b] == BEAM_DONE) return score[b];
+        const float x = from_order((uint32_t)(key[b * k + j] >> 32));
+        return x == -INFINITY ? -INFINITY : score[b] + (((double)x - m[b]) - logs[b]);
+    }
+};
+
+template <bool F32>
+__global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
+    __shared__ union Both {
+        Shared sh;
+        BeamMerge merge;
+    } both;
+    __shared__ struct {
+        float m[WAVES];
+        double s[WAVES];
+        int last;
+    } top;
+    constexpr int U = 2;  // pieces in flight per thread
+    const LpArgs &g = a.lp;
+    Shared &sh = both.sh;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, k = g.k;
+    const size_t r = blockIdx.x / g.parts;
+    const int part = blockIdx.x % g.parts;
+    const float score = a.score[r];
+    int what = a.done && a.done[r] ? BEAM_DONE : BEAM_ROW;
+    if (!(score < INFINITY)) what = BEAM_ODD;
+    else if (score == -INFINITY) what = BEAM_NONE;
+    BeamSum z = {-INFINITY, 0.0};
+    if (what != BEAM_ROW) {
+        if (part) return;
+    } else {
+        const char *const start = (const char *)g.x + r * (size_t)g.stride * (F32 ? 4 : 2);
+        const uint32_t mis = (uint32_t)((uintptr_t)start & 15u) / (F32 ? 4 : 2);
+        const Row<F32> row = {g, start - ((uintptr_t)start & 15u), mis, (mis + g.V + VEC<F32> - 1) / VEC<F32>};
+        const uint32_t v0 = (uint32_t)part * g.per, v1 = std::min(v0 + g.per, row.n_pieces);
+        for (uint32_t v = v0 + tid; v < v1; v += U * NT) {
+            float x[U][VEC<F32>];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (v + u * NT < v1) piece<F32>(row.base, v + u * NT, row.n_pieces, mis, g.V, x[u]);
+                else
+#pragma unroll
+                    for (int e = 0; e < VEC<F32>; e++) x[u][e] = -INFINITY;
+            }
+            float mn = z.m;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < VEC<F32>; e++) mn = fmaxf(mn, x[u][e]);
+            if (mn > z.m) {
+                if (z.m != -INFINITY) z.s *= (double)ex_sharp(z.m - mn);
+                z.m = mn;
+            }
+            const float m0 = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float p = 0.f;
+#pragma unroll
+                for (int e = 0; e < VEC<F32>; e++) p += ex_sharp(x[u][e] - m0);
+                z.s += (double)p;
+            }
+        }
+        const int per = NT / g.group;
+        float mx = z.m;
+        for (int o = 1; o < g.group; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+        const uint32_t big = order_of(mx);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) z.add(__shfl_xor(z.m, o, 64), __shfl_xor(z.s, o, 64));
+        if (lane == 0) top.m[w] = z.m, top.s[w] = z.s;
+        __syncthreads();
+        z = {top.m[0], top.s[0]};
+#pragma unroll
+        for (int i = 1; i < WAVES; i++) z.add(top.m[i], top.s[i]);
+        if (g.parts > 1) {
+            const uint32_t each = 4 + per;
+            const rsrc_t rp = make_rsrc(g.work + r * (size_t)g.parts * each, (uint32_t)g.parts * each * 4u);
+            const unsigned long long bits = __builtin_bit_cast(unsigned long long, z.s);
+            if (tid == 0) buf_store16(rp, f4{z.m, __builtin_bit_cast(float, (uint32_t)bits), __builtin_bit_cast(float, (uint32_t)(bits >> 32)), 0.f}, (uint32_t)part * each * 4u);
+            if (tid % g.group == 0) __builtin_amdgcn_raw_buffer_store_b32(big, rp, ((uint32_t)part * each + 4 + tid / g.group) * 4u, 0u, CPOL_SC1);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) {
+                top.last = atomicAdd(&g.counters[r], 1) == g.parts - 1;
+                if (top.last) atomicExch(&g.counters[r], 0);
+            }
+            __syncthreads();
+            if (!top.last) return;
+            const int mine = lane % MAX_PARTS;  // a part a lane, in one order
+            const u4v o = __builtin_bit_cast(u4v, buf_load16_sc1(rp, (uint32_t)std::min(mine, g.parts - 1) * each * 4u, 0));
+            if (tid < g.parts * per) sh.bucket[tid] = __builtin_amdgcn_raw_buffer_load_b32(rp, ((uint32_t)(tid / per) * each + 4 + tid % per) * 4u, 0u, CPOL_SC1);
+            z = {-INFINITY, 0.0};
+            const uint32_t om = o.x;
+            if (mine < g.parts) z = {__builtin_bit_cast(float, om), __builtin_bit_cast(double, (unsigned long long)o.z << 32 | o.y)};
+#pragma unroll
+            for (int i = 1; i < MAX_PARTS; i <<= 1) z.add(__shfl_xor(z.m, i, 64), __shfl_xor(z.s, i, 64));
+        } else if (tid % g.group == 0) {
+            sh.bucket[tid / g.group] = big;
+        }
+        __syncthreads();
+        if (!(z.s >= 0.0)) what = BEAM_ODD;
+        else if (z.s == 0.0) what = BEAM_NONE;
+        else top_k<F32>(row, g.parts * per, false, sh);
+    }
+    // the row to the workspace; the last one of the group goes on
+    const size_t group = r / a.n_beams;
+    const rsrc_t rr = make_rsrc(a.rows + group * (size_t)a.n_beams * a.row_bytes, (uint32_t)a.n_beams * a.row_bytes);
+    const uint32_t mine = (uint32_t)(r - group * a.n_beams) * a.row_bytes;
+    if (tid == 0) {
+        const unsigned long long bits = __builtin_bit_cast(unsigned long long, z.s);
+        buf_store16(rr, f4{z.m, __builtin_bit_cast(float, (uint32_t)bits), __builtin_bit_cast(float, (uint32_t)(bits >> 32)), __builtin_bit_cast(float, what)}, mine);
+    }
+    if (what == BEAM_ROW)
+        for (int j = tid; j < 2 * k; j += NT) {
+            const unsigned long long key = sh.out[j / 2];
+            __builtin_amdgcn_raw_buffer_store_b32((uint32_t)(j & 1 ? key >> 32 : key), rr, mine + 16u + 4u * (uint32_t)j, 0u, CPOL_SC1);
+        }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        top.last = atomicAdd(&a.group_counters[group], 1) == a.n_beams - 1;
+        if (top.last) atomicExch(&a.group_counters[group], 0);
+    }
+    __syncthreads();
+    if (!top.last) return;
+    BeamMerge &m = both.merge;
+    const int B = a.n_beams;
+    if (tid < B) {
+        const u4v o = __builtin_bit_cast(u4v, buf_load16_sc1(rr, (uint32_t)tid * a.row_bytes, 0));
+        const uint32_t om = o.x, kind = o.w;
+        m.m[tid] = (double)__builtin_bit_cast(float, om);
+        m.logs[tid] = log(__builtin_bit_cast(double, (unsigned long long)o.z << 32 | o.y));
+        m.score[tid] = (double)a.score[group * B + tid];
+        m.what[tid] = (int)kind;
+    }
+    if (tid == 0) m.odd = m.n = 0;
+    for (int i = tid; i < B * k; i += NT) {
+        const uint32_t at = (uint32_t)(i / k) * a.row_bytes + 16u + 8u * (uint32_t)(i % k);
+        const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b32(rr, at, 0u, CPOL_SC1), hi = __builtin_amdgcn_raw_buffer_load_b32(rr, at + 4u, 0u, CPOL_SC1);
+        m.key[i] = (unsigned long long)hi << 32 | lo;
+        m.rank[i] = 0;
+    }
+    __syncthreads();
+    if (tid < B && m.what[tid] == BEAM_ODD) m.odd = 1;
+    __syncthreads();
+    const size_t to = group * (size_t)a.k;
+    if (m.odd) {
+        for (int j = tid; j < a.k; j += NT) a.out_score[to + j] = NAN, a.out_token[to + j] = 0xffffffffu, a.out_beam[to + j] = -1;
+        return;
+    }
+    // places before candidate (b, j): its own row's j, and of each other row those of a larger value, or of an equal one in a lower row
+    for (int i = tid; i < B * B * k; i += NT) {
+        const int c = i / B, b = c / k, j = c - b * k, other = i - c * B;
+        const double v = m.value(b, j, k);
+        if (v == -INFINITY) continue;
+        int n = j;
+        if (other != b) {
+            int lo = 0, hi = k;  // the first place of the other row that does not come before
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                const double y = m.value(other, mid, k);
+                if (y > v || (y == v && other < b)) lo = mid + 1;
+                else hi = mid;
+            }
+            n = lo;
+        }
+        atomicAdd(&m.rank[c], n);
+        if (other == b) atomicAdd(&m.n, 1);
+    }
+    __syncthreads();
+    for (int c = tid; c < B * k; c += NT) {
+        const int b = c / k, j = c - b * k, at = m.rank[c];
+        const double v = m.value(b, j, k);
+        if (v == -INFINITY || at >= a.k) continue;
+        a.out_score[to + at] = (float)v;
+        a.out_token[to + at] = m.what[b] == BEAM_DONE ? a.done_token : ~(uint32_t)m.key[c];
+        a.out_beam[to + at] = b;
+    }
+    for (int j = tid; j < a.k; j += NT)
+        if (j >= m.n) a.out_score[to + j] = -INFINITY, a.out_token[to + j] = 0xffffffffu, a.out_beam[to + j] = -1;
+}
+
 __global__ void k_zero(int *p, int n) {
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0;
+}
+
+// Few rows: parts of three pieces a thread, while the chip has workgroups to spare (two per CU); 16 rows of 151936 with two: 1.9
+// us more, with four 0.3 more. Buckets stay within MAX_BUCKETS: more parts, more threads to a bucket.
+void split_rows(LpArgs *g, int M, bool f32, int n_cu) {
+    const uint32_t pieces = (g->V + (f32 ? 3u : 7u)) / (f32 ? 4u : 8u) + 1;
+    g->parts = (int)std::max(1u, std::min({2u * (uint32_t)n_cu / (uint32_t)M, (pieces + 3 * NT - 1) / (3 * NT), (uint32_t)MAX_PARTS}));
+    while (g->parts * (NT / g->group) > MAX_BUCKETS) g->group *= 2;
+    g->per = (pieces + (uint32_t)g->parts - 1) / (uint32_t)g->parts;
 }
 
 }  // namespace
@@ -392,14 +633,9 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
     if (top_k == 0) top_ids = nullptr, top_logp = nullptr;
     if (!logp && !entropy && !top_ids && !top_logp) return 0;
     LpArgs g = {logits, ids, logp, entropy, top_logp, top_ids, stride, V, n_ids, top_k, 1, 1, 0, nullptr, nullptr};
-    // Few rows: parts of three pieces a thread, while the chip has workgroups to spare (two per CU); 16 rows of 151936 with two: 1.9
-    // us more, with four 0.3 more. Buckets stay within MAX_BUCKETS: more parts, more threads to a bucket.
     int device, n_cu;
     if (hq_internal_device(&device, &n_cu)) return -1;
-    const uint32_t pieces = (V + (f32 ? 3u : 7u)) / (f32 ? 4u : 8u) + 1;
-    g.parts = (int)std::max(1u, std::min({2u * (uint32_t)n_cu / (uint32_t)M, (pieces + 3 * NT - 1) / (3 * NT), (uint32_t)MAX_PARTS}));
-    while (g.parts * (NT / g.group) > MAX_BUCKETS) g.group *= 2;
-    g.per = (pieces + (uint32_t)g.parts - 1) / (uint32_t)g.parts;
+    split_rows(&g, M, f32, n_cu);
     if (g.parts > 1) {
         const size_t each = 4 + NT / (size_t)g.group, sums = (size_t)M * g.parts * each * 4;
         void *work, *cnt;
@@ -416,6 +652,49 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
     const unsigned grid = (unsigned)M * (unsigned)g.parts;
     if (f32) k_logprobs<true><<<grid, NT, 0, (hipStream_t)stream>>>(g);
     else k_logprobs<false><<<grid, NT, 0, (hipStream_t)stream>>>(g);
+    SCK(hipGetLastError());
+    return 0;
+}
+
+extern "C" int hq_beam(const void *logits, int f32, int n_groups, int n_beams, uint32_t V, int64_t stride, const float *score, const uint8_t *done,
+                       uint32_t done_token, int k, float *out_score, uint32_t *out_token, int32_t *out_beam, void *stream) {
+    const char *const who = "hq_beam";
+    if (n_beams < 1 || n_beams > HQ_BEAM_MAX || n_groups < 0 || n_groups > (1 << 24) / n_beams)
+        return hq_internal_fail("%s: %d groups of %d beams (1 .. %d beams, at most 2^24 rows)", who, n_groups, n_beams, HQ_BEAM_MAX);
+    if (V < 1 || V > (1u << 30) || stride < (int64_t)V || stride > ((int64_t)1 << 40)) return hq_internal_fail("%s: rows of %u (at most 2^30), stride %lld", who, V, (long long)stride);
+    if (k < 1 || k > HQ_BEAM_MAX) return hq_internal_fail("%s: k %d (1 .. %d)", who, k, HQ_BEAM_MAX);
+    if (n_groups == 0) return 0;
+    if (!logits || !score || !out_score || !out_token || !out_beam) return hq_internal_fail("%s: null argument", who);
+    if ((uintptr_t)logits % (f32 ? 4 : 2)) return hq_internal_fail("%s: the logits are misaligned", who);
+    for (const void *p : {(const void *)score, (const void *)out_score, (const void *)out_token, (const void *)out_beam})
+        if ((uintptr_t)p % 4) return hq_internal_fail("%s: scores and outputs must be 4-byte aligned", who);
+    const int M = n_groups * n_beams;
+    BeamArgs a = {};
+    LpArgs &g = a.lp;
+    g.x = logits, g.stride = stride, g.V = V, g.k = (int)std::min((uint32_t)k, V), g.parts = g.group = 1;
+    int device, n_cu;
+    if (hq_internal_device(&device, &n_cu)) return -1;
+    split_rows(&g, M, f32, n_cu);
+    a.score = score, a.done = done, a.done_token = done_token, a.n_beams = n_beams, a.k = k;
+    a.out_score = out_score, a.out_token = out_token, a.out_beam = out_beam;
+    // the rows' results, and behind them the sums of split rows; counters of rows and groups
+    a.row_bytes = 16u + 8u * (uint32_t)((g.k + 1) & ~1);
+    const size_t each = 4 + NT / (size_t)g.group, rows = (size_t)M * a.row_bytes, sums = g.parts > 1 ? (size_t)M * g.parts * each * 4 : 0;
+    const int n_count = M + n_groups;
+    void *work, *cnt;
+    int grew;
+    if (hq_internal_staging(device, stream, HQ_STAGE_BEAM, rows + sums, &work, &grew) ||
+        hq_internal_staging(device, stream, HQ_STAGE_BEAM_COUNT, (size_t)n_count * 4, &cnt, &grew))
+        return -1;
+    if (grew) {
+        k_zero<<<1, 256, 0, (hipStream_t)stream>>>((int *)cnt, n_count);
+        SCK(hipGetLastError());
+    }
+    a.rows = (char *)work, g.work = (float *)((char *)work + rows);
+    a.group_counters = (int *)cnt, g.counters = (int *)cnt + n_groups;
+    const unsigned grid = (unsigned)M * (unsigned)g.parts;
+    if (f32) k_beam<true><<<grid, NT, 0, (hipStream_t)stream>>>(a);
+    else k_beam<false><<<grid, NT, 0, (hipStream_t)stream>>>(a);
     SCK(hipGetLastError());
     return 0;
 }

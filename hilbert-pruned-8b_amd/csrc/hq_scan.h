@@ -1,0 +1,51 @@
+// hq_scan.h - a step's sequences and states on the device (hq_scan.hip), as the kernels of recurrent layers read them.
+#ifndef HQ_SCAN_H
+#define HQ_SCAN_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "hq_internal.h"
+#include "hq_serve.h"
+
+struct HqSeq {
+    int tok0, n;   // its first new token and how many there are
+    int from, to;  // slots, or -1
+};
+// Tokens t0 .. t0 + n - 1 of sequence seq, for one workgroup.
+struct HqTile {
+    int seq, t0, n;
+};
+constexpr int HQ_CONV_TILE = 8;  // most tokens of a tile of hq_delta_append
+
+struct hq_scan {
+    int device, n_cu;
+    int max_seqs, max_tokens;
+    // the step
+    int n_seqs, n_tokens;
+    hq_state_t geom;
+    bool set;
+    // device arrays, parts of `dev`
+    const HqSeq *seqs;
+    const HqTile *tiles;  // of hq_delta_append: every sequence's first tile, which has its convolution's state, is there
+    int n_tiles;
+    const int *steps;  // the sequences that hq_delta takes token by token, longest first
+    int n_steps;
+    // storage: one pinned copy of `dev`, which the next set waits for
+    int *host, *dev;
+    size_t words;
+    hipEvent_t sent;
+    bool sending;
+};
+
+// A state argument against the step's geometry: 0, or -1 with a message naming `who`.
+int hq_state_check(const char *who, const hq_state_t *st, const hq_scan *c);
+
+#define SCK(call)                                                                                         \
+    do {                                                                                                  \
+        hipError_t e_ = (call);                                                                           \
+        if (e_ != hipSuccess)                                                                             \
+            return hq_internal_fail("HIP %s failed: %s (%s:%d)", #call, hipGetErrorString(e_), __FILE__, __LINE__); \
+    } while (0)
+
+#endif

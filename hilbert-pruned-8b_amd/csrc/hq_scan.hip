@@ -1,0 +1,319 @@
+// hq_scan.hip - the sequences and states of a step through recurrent layers (hq_scan_*, include/hq_serve.h), and what stands in
+// front of their recurrence: causal convolution, norms and gates (hq_delta_append).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <math.h>
+#include <new>
+#include <string.h>
+#include <vector>
+
+#include "hq_device.h"
+#include "hq_scan.h"
+
+namespace {
+
+bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
+
+int use_device(int device) {
+    int cur = -1;
+    SCK(hipGetDevice(&cur));
+    if (cur != device) SCK(hipSetDevice(device));
+    return 0;
+}
+
+int check_geometry(const char *who, const hq_state_t *st) {
+    if (st->n_k_heads < 1 || st->n_k_heads > 1024 || st->n_v_heads < 1 || st->n_v_heads > 1024 || st->n_v_heads % st->n_k_heads)
+        return hq_internal_fail("%s: %d value heads over %d key heads (1 .. 1024, a multiple)", who, st->n_v_heads, st->n_k_heads);
+    for (int d : {st->k_dim, st->v_dim})
+        if (d < 16 || d > 256 || d % 16) return hq_internal_fail("%s: heads of %d and %d (multiples of 16, 16 .. 256)", who, st->k_dim, st->v_dim);
+    if (st->conv_taps < 1 || st->conv_taps > 8) return hq_internal_fail("%s: a convolution of %d taps (1 .. 8)", who, st->conv_taps);
+    if (st->n_slots < 1 || st->n_slots > 0x7fffffffu) return hq_internal_fail("%s: %u slots", who, st->n_slots);
+    return 0;
+}
+
+}  // namespace
+
+int hq_state_check(const char *who, const hq_state_t *st, const hq_scan *c) {
+    if (check_geometry(who, st)) return -1;
+    const hq_state_t &g = c->geom;
+    if (st->n_k_heads != g.n_k_heads || st->n_v_heads != g.n_v_heads || st->k_dim != g.k_dim || st->v_dim != g.v_dim ||
+        st->conv_taps != g.conv_taps || st->n_slots != g.n_slots)
+        return hq_internal_fail("%s: the states (%u slots, %d / %d heads of %d and %d, %d taps) are not those hq_scan_set was given (%u "
+                                "slots, %d / %d heads of %d and %d, %d taps)", who, st->n_slots, st->n_k_heads, st->n_v_heads, st->k_dim, st->v_dim,
+                                st->conv_taps, g.n_slots, g.n_k_heads, g.n_v_heads, g.k_dim, g.v_dim, g.conv_taps);
+    return 0;
+}
+
+extern "C" int hq_scan_create(int device, int max_seqs, int max_tokens, hq_scan **out) {
+    if (!out) return hq_internal_fail("hq_scan_create: null argument");
+    *out = nullptr;
+    if (max_seqs < 1 || max_seqs > (1 << 20) || max_tokens < 0 || max_tokens > (1 << 24))
+        return hq_internal_fail("hq_scan_create: %d sequences, %d tokens (at least 1, 0; at most 2^20, 2^24)", max_seqs, max_tokens);
+    if (use_device(device)) return -1;
+    hq_scan *c = new (std::nothrow) hq_scan();
+    if (!c) return hq_internal_fail("hq_scan_create: out of memory");
+    c->device = device;
+    c->max_seqs = max_seqs, c->max_tokens = max_tokens;
+    hipError_t e = hipDeviceGetAttribute(&c->n_cu, hipDeviceAttributeMultiprocessorCount, device);
+    if (e == hipSuccess) e = hipEventCreateWithFlags(&c->sent, hipEventDisableTiming);
+    if (e != hipSuccess) {
+        hq_scan_free(c);
+        return hq_internal_fail("hq_scan_create: %s", hipGetErrorString(e));
+    }
+    *out = c;
+    return 0;
+}
+
+extern "C" void hq_scan_free(hq_scan *c) {
+    if (!c) return;
+    (void)use_device(c->device);
+    (void)hipDeviceSynchronize();
+    if (c->dev) (void)hipFree(c->dev);
+    if (c->host) (void)hipHostFree(c->host);
+    if (c->sent) (void)hipEventDestroy(c->sent);
+    delete c;
+}
+
+extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const int32_t *n_new, const int32_t *from, const int32_t *to, void *stream) {
+    const char *const who = "hq_scan_set";
+    if (!c || !st) return hq_internal_fail("%s: null argument", who);
+    if (check_geometry(who, st)) return -1;
+    if (n_seqs < 0 || n_seqs > c->max_seqs) return hq_internal_fail("%s: %d sequences (the step takes %d)", who, n_seqs, c->max_seqs);
+    if (n_seqs && (!n_new || !from || !to)) return hq_internal_fail("%s: null argument", who);
+    int64_t T = 0;
+    const auto slot = [&](int s) { return s >= -1 && (s < 0 || (uint32_t)s < st->n_slots); };
+    for (int i = 0; i < n_seqs; i++) {
+        if (n_new[i] < 0) return hq_internal_fail("%s: sequence %d has %d new tokens", who, i, n_new[i]);
+        if (!slot(from[i]) || !slot(to[i])) return hq_internal_fail("%s: sequence %d goes from slot %d to slot %d (there are %u)", who, i, from[i], to[i], st->n_slots);
+        T += n_new[i];
+    }
+    if (T > c->max_tokens) return hq_internal_fail("%s: %lld new tokens (the step takes %d)", who, (long long)T, c->max_tokens);
+    std::vector<HqTile> tiles;
+    std::vector<int> steps;
+    try {
+        // slots that are written: each by one sequence, and read by no other
+        std::vector<std::pair<int, int>> w, r;
+        for (int i = 0; i < n_seqs; i++) {
+            if (to[i] >= 0) w.push_back({to[i], i});
+            if (from[i] >= 0) r.push_back({from[i], i});
+        }
+        std::sort(w.begin(), w.end());
+        std::sort(r.begin(), r.end());
+        size_t j = 0;
+        for (size_t i = 0; i < w.size(); i++) {
+            if (i && w[i].first == w[i - 1].first) return hq_internal_fail("%s: sequences %d and %d leave their states in slot %d", who, w[i - 1].second, w[i].second, w[i].first);
+            while (j < r.size() && r[j].first < w[i].first) j++;
+            for (size_t k = j; k < r.size() && r[k].first == w[i].first; k++)
+                if (r[k].second != w[i].second) return hq_internal_fail("%s: sequence %d goes on from slot %d, where sequence %d leaves its state", who, r[k].second, w[i].first, w[i].second);
+        }
+        for (int i = 0; i < n_seqs; i++) {
+            if (n_new[i] == 0 && (to[i] < 0 || to[i] == from[i])) continue;
+            for (int t = 0; t == 0 || t < n_new[i]; t += HQ_CONV_TILE) tiles.push_back({i, t, std::min(HQ_CONV_TILE, n_new[i] - t)});
+            steps.push_back(i);
+        }
+        std::stable_sort(steps.begin(), steps.end(), [&](int a, int b) { return n_new[a] > n_new[b]; });
+    } catch (const std::exception &) {
+        return hq_internal_fail("%s: out of memory", who);
+    }
+    if (use_device(c->device)) return -1;
+    c->set = false;
+    if (c->sending) {  // the pinned copy is free again when the last transfer has read it
+        SCK(hipEventSynchronize(c->sent));
+        c->sending = false;
+    }
+    const size_t words = (size_t)n_seqs * (sizeof(HqSeq) / 4) + tiles.size() * (sizeof(HqTile) / 4) + steps.size() + 16;
+    if (words > c->words) {
+        const size_t want = words + words / 2;
+        SCK(hipDeviceSynchronize());
+        if (c->dev) SCK(hipFree(c->dev));
+        c->dev = nullptr;
+        if (c->host) SCK(hipHostFree(c->host));
+        c->host = nullptr;
+        c->words = 0;
+        SCK(hipMalloc((void **)&c->dev, want * 4));
+        SCK(hipHostMalloc((void **)&c->host, want * 4, hipHostMallocDefault));
+        c->words = want;
+    }
+    int *w = c->host;
+    const auto dev = [&]() { return c->dev + (w - c->host); };
+    c->seqs = (const HqSeq *)dev();
+    for (int i = 0, t = 0; i < n_seqs; t += n_new[i], i++, w += sizeof(HqSeq) / 4) {
+        const HqSeq s = {t, n_new[i], from[i], to[i]};
+        memcpy(w, &s, sizeof s);
+    }
+    c->tiles = (const HqTile *)dev(), c->n_tiles = (int)tiles.size();
+    if (!tiles.empty()) memcpy(w, tiles.data(), tiles.size() * sizeof(HqTile));
+    w += tiles.size() * (sizeof(HqTile) / 4);
+    c->steps = dev(), c->n_steps = (int)steps.size();
+    if (!steps.empty()) memcpy(w, steps.data(), steps.size() * 4);
+    w += steps.size();
+    const size_t used = (size_t)(w - c->host);
+    if (used) {
+        SCK(hipMemcpyAsync(c->dev, c->host, used * 4, hipMemcpyHostToDevice, (hipStream_t)stream));
+        SCK(hipEventRecord(c->sent, (hipStream_t)stream));
+        c->sending = true;
+    }
+    c->n_seqs = n_seqs, c->n_tokens = (int)T;
+    c->geom = *st;
+    c->set = true;
+    return 0;
+}
+
+// ------------------------------------------------------------------------------------ convolution, norms and gates
+namespace {
+
+struct AppendArgs {
+    hq_state_t st;
+    hq_delta_in_t r;
+    const HqSeq *seqs;
+    const HqTile *tiles;
+};
+
+typedef float f8 __attribute__((ext_vector_type(8)));
+
+template <bool F32>
+DEV f8 load8(const void *p, size_t at) {
+    if (F32) {
+        const f4 a = *(const f4 *)((const float *)p + at), b = *(const f4 *)((const float *)p + at + 4);
+        return f8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+    const h8 x = *(const h8 *)((const _Float16 *)p + at);
+    return f8{(float)x[0], (float)x[1], (float)x[2], (float)x[3], (float)x[4], (float)x[5], (float)x[6], (float)x[7]};
+}
+
+template <bool F32>
+DEV float load1(const void *p, size_t at) { return F32 ? ((const float *)p)[at] : (float)((const _Float16 *)p)[at]; }
+
+// A workgroup takes the heads (of queries, keys, values: one sequence of them) 256 / G blockIdx.y .. of a tile's tokens, G lanes a
+// head, eight channels a lane. A lane holds a window of its channels' last inputs, so that each input is read once for a tile and
+// taps - 1 times more at its border. The tile with a sequence's first token reads the slot's inputs and afterwards writes those
+// that the sequence leaves: the same lane the same channels, so one slot may be both.
+// TAPS: conv_taps or more; taps beyond it have no input and no weight.
+template <bool F32, int G, int TAPS>
+__global__ void __launch_bounds__(256) k_delta_append(AppendArgs g) {
+    const HqTile tile = g.tiles[blockIdx.x];
+    const HqSeq seq = g.seqs[tile.seq];
+    const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim, taps = g.st.conv_taps;
+    const size_t channels = 2 * (size_t)nk * dk + (size_t)nv * dv;
+    const int tok0 = seq.tok0 + tile.t0;
+    if (blockIdx.y == 0)
+        for (int i = threadIdx.x; i < tile.n * nv; i += 256) {
+            const int t = i / nv, h = i - t * nv;
+            const size_t at = (size_t)(tok0 + t) * g.r.ab_stride + h, o = (size_t)(tok0 + t) * nv + h;
+            const float y = load1<F32>(g.r.a, at) + g.r.dt_bias[h];
+            g.r.decay[o] = -expf(g.r.a_log[h]) * (fmaxf(y, 0.f) + log1pf(expf(-fabsf(y))));
+            g.r.beta[o] = 1.0f / (1.0f + expf(-load1<F32>(g.r.b, at)));
+        }
+    const int u = threadIdx.x % G;
+    for (int j = blockIdx.y * (256 / G) + threadIdx.x / G; j < 2 * nk + nv; j += gridDim.y * (256 / G)) {
+        const bool is_v = j >= 2 * nk;
+        const bool on = 8 * u < (is_v ? dv : dk);
+        const size_t ch = (is_v ? 2 * (size_t)nk * dk + (size_t)(j - 2 * nk) * dv : (size_t)j * dk) + (on ? 8 * u : 0);
+        f8 w[TAPS], x[TAPS];  // of the inputs TAPS - 1 .. 0 tokens back
+#pragma unroll
+        for (int i = 0; i < TAPS; i++) {
+            const int tap = i - (TAPS - taps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[i][e] = tap >= 0 ? g.r.conv_w[(ch + e) * taps + tap] : 0.f;
+            // the input at token t0 - (TAPS - 1) + i of the sequence
+            const int t = tile.t0 - (TAPS - 1) + i;
+            x[i] = f8{};
+            if (i < TAPS - 1 && tap >= 0) {
+                if (t >= 0) x[i] = load8<F32>(g.r.x, (size_t)(seq.tok0 + t) * g.r.x_stride + ch);
+                else if (seq.from >= 0) x[i] = load8<true>(g.st.conv, ((size_t)seq.from * (taps - 1) + (taps - 1 + t)) * channels + ch);
+            }
+        }
+        if (tile.t0 == 0 && seq.to >= 0 && on) {
+            // the last taps - 1 of the old inputs and the new ones
+            f8 keep[TAPS];
+#pragma unroll
+            for (int i = 0; i < TAPS - 1; i++) {
+                const int r = i - (TAPS - taps), t = seq.n - (taps - 1) + r;  // row r is token t
+                if (r < 0) continue;
+                keep[i] = f8{};
+                if (t >= 0) keep[i] = load8<F32>(g.r.x, (size_t)(seq.tok0 + t) * g.r.x_stride + ch);
+                else if (seq.from >= 0) keep[i] = load8<true>(g.st.conv, ((size_t)seq.from * (taps - 1) + (taps - 1 + t)) * channels + ch);
+            }
+#pragma unroll
+            for (int i = 0; i < TAPS - 1; i++) {
+                const int r = i - (TAPS - taps);
+                if (r < 0) continue;
+                f4 *o = (f4 *)(g.st.conv + ((size_t)seq.to * (taps - 1) + r) * channels + ch);
+                o[0] = f4{keep[i][0], keep[i][1], keep[i][2], keep[i][3]};
+                o[1] = f4{keep[i][4], keep[i][5], keep[i][6], keep[i][7]};
+            }
+        }
+        for (int t = 0; t < tile.n; t++) {
+            x[TAPS - 1] = load8<F32>(g.r.x, (size_t)(tok0 + t) * g.r.x_stride + ch);
+            f8 y;
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < TAPS; i++) s = fmaf(w[i][e], x[i][e], s);
+                y[e] = s / (1.0f + expf(-s));
+                ss = fmaf(y[e], y[e], ss);
+            }
+            if (!on) ss = 0.f;
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            const float inv = is_v ? 1.0f : 1.0f / sqrtf(ss + g.r.eps);
+            h8 o;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = (_Float16)(y[e] * inv);
+            if (on) *(h8 *)((_Float16 *)g.r.qkv + (size_t)(tok0 + t) * channels + ch) = o;
+#pragma unroll
+            for (int i = 0; i < TAPS - 1; i++) x[i] = x[i + 1];
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_delta_in_t *r, void *stream) {
+    const char *const who = "hq_delta_append";
+    if (!c || !st || !r) return hq_internal_fail("%s: null argument", who);
+    if (!c->set) return hq_internal_fail("%s: no step is described (hq_scan_set)", who);
+    if (hq_state_check(who, st, c)) return -1;
+    if (c->n_tiles == 0) return 0;
+    if (st->conv_taps > 1 && (!st->conv || !aligned(st->conv, 16))) return hq_internal_fail("%s: 16-byte aligned memory of the convolution's inputs is needed", who);
+    if (!r->conv_w || !aligned(r->conv_w, 16)) return hq_internal_fail("%s: 16-byte aligned weights are needed", who);
+    if (c->n_tokens) {
+        if (!r->x || !r->a || !r->b || !r->a_log || !r->dt_bias || !r->qkv || !r->decay || !r->beta) return hq_internal_fail("%s: null argument", who);
+        if (!aligned(r->x, 16) || !aligned(r->qkv, 16)) return hq_internal_fail("%s: x and qkv must be 16-byte aligned", who);
+        const size_t size = r->f32 ? 4 : 2;
+        if (!aligned(r->a, size) || !aligned(r->b, size) || !aligned(r->a_log, 4) || !aligned(r->dt_bias, 4) || !aligned(r->decay, 4) || !aligned(r->beta, 4))
+            return hq_internal_fail("%s: a, b, their parameters or outputs are misaligned", who);
+        const int64_t most = (int64_t)1 << 40;
+        if (r->x_stride < 0 || r->x_stride > most || r->x_stride % 8 || r->ab_stride < 0 || r->ab_stride > most)
+            return hq_internal_fail("%s: strides %lld (a multiple of 8), %lld", who, (long long)r->x_stride, (long long)r->ab_stride);
+    }
+    if (!(r->eps >= 0.f)) return hq_internal_fail("%s: eps %g", who, (double)r->eps);
+    if (use_device(c->device)) return -1;
+    const AppendArgs g = {*st, *r, c->seqs, c->tiles};
+    const int widest = std::max(st->k_dim, st->v_dim), lanes = widest <= 64 ? 8 : widest <= 128 ? 16 : 32, per = 256 / lanes;
+    const int heads = 2 * st->n_k_heads + st->n_v_heads;
+    const dim3 grid((unsigned)c->n_tiles, (unsigned)((heads + per - 1) / per));
+    hipStream_t s = (hipStream_t)stream;
+#define HQ_APPEND_T(F, G, N) k_delta_append<F, G, N><<<grid, 256, 0, s>>>(g)
+#define HQ_APPEND_G(F, G)                      \
+    do {                                       \
+        if (st->conv_taps <= 4) HQ_APPEND_T(F, G, 4); \
+        else HQ_APPEND_T(F, G, 8);             \
+    } while (0)
+#define HQ_APPEND(F)                       \
+    do {                                   \
+        if (lanes == 8) HQ_APPEND_G(F, 8); \
+        else if (lanes == 16) HQ_APPEND_G(F, 16); \
+        else HQ_APPEND_G(F, 32);           \
+    } while (0)
+    if (r->f32) HQ_APPEND(true);
+    else HQ_APPEND(false);
+#undef HQ_APPEND
+#undef HQ_APPEND_G
+#undef HQ_APPEND_T
+    SCK(hipGetLastError());
+    return 0;
+}

@@ -28,6 +28,8 @@ EXPORTS = (
     "hq_gguf_wmat", "hq_mat_upload_pair", "hq_gemm_swiglu", "hq_time_gemm_swiglu", "hq_time_read",
     # include/hq_serve.h
     "hq_batch_create", "hq_batch_free", "hq_batch_set", "hq_rope_table", "hq_rope_append", "hq_attention", "hq_logprobs",
+    "hq_scan_create", "hq_scan_free", "hq_scan_set", "hq_delta_append", "hq_delta", "hq_pages_create", "hq_pages_free", "hq_pages_resize",
+    "hq_pages_fork", "hq_pages_compact", "hq_pages_copies", "hq_pages_table", "hq_pages_count", "hq_kv_copy", "hq_beam",
 )
 # include/hq_backend.h (no hq_ prefix: the names of the reference entry points they replace)
 BACKEND_EXPORTS = ("hip_backend_create", "hip_selftest", "hip_batch_create", "hip_batch_free", "hip_batch_step")
@@ -116,6 +118,26 @@ class Attn(C.Structure):
                 ("gate_stride", C.c_int64), ("gate_head_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)]
 
 
+class State(C.Structure):
+    """hq_state_t: one layer's recurrent states."""
+    _fields_ = [("n_k_heads", C.c_int), ("n_v_heads", C.c_int), ("k_dim", C.c_int), ("v_dim", C.c_int), ("conv_taps", C.c_int),
+                ("n_slots", C.c_uint32), ("s", C.c_void_p), ("conv", C.c_void_p)]
+
+
+class DeltaIn(C.Structure):
+    """hq_delta_in_t."""
+    _fields_ = [("x", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p), ("f32", C.c_int), ("x_stride", C.c_int64), ("ab_stride", C.c_int64),
+                ("conv_w", C.c_void_p), ("a_log", C.c_void_p), ("dt_bias", C.c_void_p), ("eps", C.c_float), ("qkv", C.c_void_p),
+                ("decay", C.c_void_p), ("beta", C.c_void_p)]
+
+
+class Delta(C.Structure):
+    """hq_delta_t."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("qk_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("decay", C.c_void_p), ("beta", C.c_void_p), ("scale", C.c_float), ("norm", C.c_void_p), ("gate", C.c_void_p),
+                ("gate_f32", C.c_int), ("gate_stride", C.c_int64), ("eps", C.c_float), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
 class HQError(RuntimeError):
     pass
 
@@ -178,6 +200,21 @@ def load(path=LIB_PATH):
         "hq_rope_append": (i, [vp, C.POINTER(Kv), C.POINTER(Rope), vp]),
         "hq_attention": (i, [vp, C.POINTER(Kv), C.POINTER(Attn), vp]),
         "hq_logprobs": (i, [vp, i, i, u32, C.c_int64, vp, i, i, vp, vp, vp, vp, vp]),
+        "hq_scan_create": (i, [i, i, i, C.POINTER(vp)]),
+        "hq_scan_free": (None, [vp]),
+        "hq_scan_set": (i, [vp, C.POINTER(State), i, vp, vp, vp, vp]),
+        "hq_delta_append": (i, [vp, C.POINTER(State), C.POINTER(DeltaIn), vp]),
+        "hq_delta": (i, [vp, C.POINTER(State), C.POINTER(Delta), vp]),
+        "hq_pages_create": (i, [u32, i, i, C.POINTER(vp)]),
+        "hq_pages_free": (None, [vp]),
+        "hq_pages_resize": (i, [vp, i, i, i]),
+        "hq_pages_fork": (i, [vp, i, i, i]),
+        "hq_pages_compact": (i, [vp]),
+        "hq_pages_copies": (i, [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(i)]),
+        "hq_pages_table": (i, [vp, vp, i, vp, i]),
+        "hq_pages_count": (i, [vp, i, C.POINTER(i), C.POINTER(u32)]),
+        "hq_kv_copy": (i, [C.POINTER(Kv), i, vp, vp, vp, i, vp]),
+        "hq_beam": (i, [vp, i, i, i, u32, C.c_int64, vp, vp, u32, i, vp, vp, vp, vp]),
         "hq_gguf_open": (i, [C.c_char_p, C.POINTER(vp)]),
         "hq_gguf_close": (None, [vp]),
         "hq_gguf_n_tensors": (sz, [vp]),
@@ -577,6 +614,125 @@ def logprobs(logits, M, V, *, f32, stride=None, ids=None, n_ids=0, top_k=0, logp
     """hq_logprobs on device memory (DevBuf or raw pointers)."""
     _check(load().hq_logprobs(_dev(logits), int(f32), M, V, V if stride is None else stride, _dev(ids), n_ids, top_k, _dev(logp),
                               _dev(entropy), _dev(top_ids), _dev(top_logp), stream))
+
+
+class States:
+    """A layer's recurrent states (hq_state_t) over device memory: s [slots, value heads, k_dim, v_dim] and conv [slots, taps - 1,
+    channels], fp32, DevBuf or raw pointers."""
+
+    def __init__(self, n_k_heads, n_v_heads, k_dim, v_dim, conv_taps, n_slots, s, conv):
+        self.keep = (s, conv)
+        self.channels = 2 * n_k_heads * k_dim + n_v_heads * v_dim
+        self.s = State(n_k_heads, n_v_heads, k_dim, v_dim, conv_taps, n_slots, _dev(s), _dev(conv))
+
+
+class Scan:
+    """hq_scan: the sequences and states of one step through recurrent layers (hq_scan_create, hq_scan_set)."""
+
+    def __init__(self, max_seqs, max_tokens, device=0):
+        self.h = None
+        h = C.c_void_p()
+        _check(load().hq_scan_create(device, max_seqs, max_tokens, C.byref(h)))
+        self.h = h.value
+
+    def set(self, states, n_new, src, dst, stream=None):
+        """The step: sequence i's n_new[i] new tokens go on from slot src[i] (-1: it begins), the state behind them to dst[i]."""
+        n_new, src, dst = (np.ascontiguousarray(a, np.int32) for a in (n_new, src, dst))
+        if n_new.ndim != 1 or src.shape != n_new.shape or dst.shape != n_new.shape:
+            raise HQError(f"Scan.set: n_new {n_new.shape}, src {src.shape}, dst {dst.shape}")
+        _check(_lib.hq_scan_set(self.h, C.byref(states.s), len(n_new), _ptr(n_new), _ptr(src), _ptr(dst), stream))
+
+    def free(self):
+        if self.h:
+            _lib.hq_scan_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def delta_append(scan, states, x, conv_w, a, b, a_log, dt_bias, qkv, decay, beta, *, f32, x_stride=None, ab_stride=None, eps=1e-6, stream=None):
+    """hq_delta_append on device memory (DevBuf or raw pointers); rows of x, a and b are contiguous unless strides are given."""
+    r = DeltaIn(_dev(x), _dev(a), _dev(b), int(f32), states.channels if x_stride is None else x_stride,
+                states.s.n_v_heads if ab_stride is None else ab_stride, _dev(conv_w), _dev(a_log), _dev(dt_bias), eps, _dev(qkv), _dev(decay), _dev(beta))
+    _check(_lib.hq_delta_append(scan.h, C.byref(states.s), C.byref(r), stream))
+
+
+def delta(scan, states, q, k, v, decay, beta, out, scale, *, qk_stride, v_stride, norm=None, gate=None, gate_f32=False, gate_stride=None,
+          eps=1e-6, out_stride=None, stream=None):
+    """hq_delta on device memory (DevBuf or raw pointers); rows of gate and out are contiguous unless strides are given."""
+    row = states.s.n_v_heads * states.s.v_dim
+    d = Delta(_dev(q), _dev(k), _dev(v), qk_stride, v_stride, _dev(decay), _dev(beta), scale, _dev(norm), _dev(gate), int(gate_f32),
+              row if gate_stride is None else gate_stride, eps, _dev(out), row if out_stride is None else out_stride)
+    _check(_lib.hq_delta(scan.h, C.byref(states.s), C.byref(d), stream))
+
+
+class Pages:
+    """hq_pages: which pages of a cache each sequence holds."""
+
+    def __init__(self, n_pages, page_size, max_seqs):
+        self.h = None
+        h = C.c_void_p()
+        _check(load().hq_pages_create(n_pages, page_size, max_seqs, C.byref(h)))
+        self.h = h.value
+
+    def resize(self, seq, n_keep, n_pos):
+        _check(_lib.hq_pages_resize(self.h, seq, n_keep, n_pos))
+
+    def fork(self, parent, child, n_pos):
+        _check(_lib.hq_pages_fork(self.h, parent, child, n_pos))
+
+    def compact(self):
+        _check(_lib.hq_pages_compact(self.h))
+
+    def copies(self):
+        """(src, dst, n_pos) of the copies that wait, for kv_copy; they wait no longer."""
+        s, d, m, n = C.c_void_p(), C.c_void_p(), C.c_void_p(), C.c_int()
+        _check(_lib.hq_pages_copies(self.h, C.byref(s), C.byref(d), C.byref(m), C.byref(n)))
+        return tuple(np.ctypeslib.as_array((t * n.value).from_address(p.value)).copy() if n.value else np.empty(0, t)
+                     for p, t in ((s, C.c_uint32), (d, C.c_uint32), (m, C.c_int32)))
+
+    def table(self, seqs, pages_ld):
+        seqs = np.ascontiguousarray(seqs, np.int32)
+        out = np.empty((len(seqs), pages_ld), np.uint32)
+        _check(_lib.hq_pages_table(self.h, _ptr(seqs), len(seqs), _ptr(out), pages_ld))
+        return out
+
+    def count(self, seq=0):
+        """(positions of seq, free pages)."""
+        n, f = C.c_int(), C.c_uint32()
+        _check(_lib.hq_pages_count(self.h, seq, C.byref(n), C.byref(f)))
+        return n.value, f.value
+
+    def free(self):
+        if self.h:
+            _lib.hq_pages_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def kv_copy(kvs, src, dst, n_pos=None, stream=None):
+    """hq_kv_copy: pages src to pages dst (their first n_pos positions) in every cache of the list kvs."""
+    src, dst = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
+    n_pos = None if n_pos is None else np.ascontiguousarray(n_pos, np.int32)
+    if src.ndim != 1 or dst.shape != src.shape or (n_pos is not None and n_pos.shape != src.shape):
+        raise HQError(f"kv_copy: src {src.shape}, dst {dst.shape}, n_pos {None if n_pos is None else n_pos.shape}")
+    kv = (Kv * len(kvs))(*[k.s for k in kvs])
+    _check(load().hq_kv_copy(kv, len(kvs), _ptr(src), _ptr(dst), None if n_pos is None else _ptr(n_pos), len(src), stream))
+
+
+def beam(logits, n_groups, n_beams, V, score, k, out_score, out_token, out_beam, *, f32, stride=None, done=None, done_token=0, stream=None):
+    """hq_beam on device memory (DevBuf or raw pointers)."""
+    _check(load().hq_beam(_dev(logits), int(f32), n_groups, n_beams, V, V if stride is None else stride, _dev(score), _dev(done), done_token, k,
+                          _dev(out_score), _dev(out_token), _dev(out_beam), stream))
 
 
 class LlamaModel:

@@ -127,6 +127,119 @@ int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_t *a, void 
 int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64_t stride, const uint32_t *ids, int n_ids, int top_k,
                 float *logp, float *entropy, uint32_t *top_ids, float *top_logp, void *stream);
 
+/* ---- layers with a recurrent state: gated delta attention
+ *
+ * Such a layer keeps, in place of keys and values, one matrix S (k_dim x v_dim) for each value head and sequence, and the last
+ * inputs of a causal convolution. Both lie in slots of the caller's memory; a step reads each sequence's slot and writes the same
+ * or another one, so that a sequence that branches (a beam, a second sample) costs no copy. hq_scan_set describes a step once;
+ * every such layer then calls hq_delta_append (convolution, norms and gates of the projections) and hq_delta (the recurrence). */
+typedef struct {
+    int n_k_heads, n_v_heads; /* queries and keys; values: a multiple, value head h takes key head h / (n_v_heads / n_k_heads) */
+    int k_dim, v_dim;         /* multiples of 16, 16 .. 256 */
+    int conv_taps;            /* 1 .. 8 */
+    uint32_t n_slots;         /* below 2^31 */
+    /* fp32, 16-byte aligned: S of slot i and head h at s + (i * n_v_heads + h) * k_dim * v_dim, v_dim contiguous; the inputs of
+     * slot i at conv + i * (conv_taps - 1) * channels, rows of channels = 2 n_k_heads k_dim + n_v_heads v_dim, the oldest first */
+    float *s, *conv;
+} hq_state_t;
+
+/* A step's sequences, for up to max_seqs of them and max_tokens new tokens in all. hq_scan_free waits for the device. */
+typedef struct hq_scan hq_scan;
+int hq_scan_create(int device, int max_seqs, int max_tokens, hq_scan **out);
+void hq_scan_free(hq_scan *c);
+/* Describes a step (host arrays, copied): sequence i has n_new[i] new tokens (0 or more; the step's tokens are numbered sequence
+ * after sequence), goes on from the state in slot from[i] (-1: begins, all zeros) and leaves the state behind them in slot to[i]
+ * (-1: nowhere). Without new tokens the state is copied. Several sequences may go on from one slot. No two leave theirs in one
+ * slot, nor in a slot that another goes on from. st: the geometry (its pointers may differ in each call that follows). Plans the
+ * work and grows the workspace: allocation, waiting and order as with hq_batch_set. */
+int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const int32_t *n_new, const int32_t *from, const int32_t *to, void *stream);
+
+typedef struct {
+    /* the new tokens' projections, fp16 (f32 = 0) or fp32: channels of token t at x + t * x_stride in the order query heads, key
+     * heads, value heads; n_v_heads values each at a and b + t * ab_stride. x 16-byte aligned, x_stride a multiple of 8. */
+    const void *x, *a, *b;
+    int f32;
+    int64_t x_stride, ab_stride;
+    const float *conv_w;         /* [channels, conv_taps] on the device, the newest input's tap last; 16-byte aligned */
+    const float *a_log, *dt_bias; /* [n_v_heads] on the device */
+    float eps;
+    uint16_t *qkv;               /* [tokens, channels] fp16, 16-byte aligned */
+    float *decay, *beta;         /* [tokens, n_v_heads] */
+} hq_delta_in_t;
+
+/* For every new token: y = silu(sum_j conv_w[j] x[t - (conv_taps - 1) + j]) over the sequence's inputs (the slot's before its
+ * first new one), heads of queries and keys divided by sqrt(sum y^2 + eps), to qkv; decay = -e^a_log softplus(a + dt_bias), the
+ * logarithm of the state's decay; beta = 1 / (1 + e^-b). Each sequence's last conv_taps - 1 inputs to its slot. fp32 arithmetic,
+ * results rounded once. One kernel. */
+int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_delta_in_t *r, void *stream);
+
+typedef struct {
+    /* fp16: head h of token t at q and k + t * qk_stride + h * k_dim, v + t * v_stride + h * v_dim; 16-byte aligned, strides
+     * multiples of 8 */
+    const uint16_t *q, *k, *v;
+    int64_t qk_stride, v_stride;
+    const float *decay, *beta; /* [tokens, n_v_heads]; decay: a logarithm, 0 or less, -inf allowed */
+    float scale;               /* of the outputs, 1 / sqrt(k_dim) as a rule */
+    /* optional norm and output gate: out = o / sqrt(mean(o^2) + eps) * norm * gate / (1 + e^-gate), over each head's v_dim; norm
+     * fp32 [v_dim] on the device, gate fp16 or fp32 (gate_f32), head h of token t at gate + t * gate_stride + h * v_dim; both or
+     * neither, 16-byte aligned, gate_stride a multiple of 8 */
+    const float *norm;
+    const void *gate;
+    int gate_f32;
+    int64_t gate_stride;
+    float eps;
+    uint16_t *out; /* fp16, head h of token t at out + t * out_stride + h * v_dim; 16-byte aligned, out_stride a multiple of 8 */
+    int64_t out_stride;
+} hq_delta_t;
+
+/* For every new token, value head and its key head, from the sequence's state: S' = e^decay S; S = S' + k (beta (v - S'^T k))^T;
+ * o = scale S^T q. States to their slots. Keys are to have a norm of at most 1 and beta to lie in 0 .. 1 (as hq_delta_append gives
+ * them): the recurrence itself grows without bound otherwise. States and sums are fp32; the same step gives the same bits. */
+int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t *d, void *stream);
+
+/* ---- pages of sequences that branch and end */
+/* Which pages of a cache each of max_seqs sequences holds (host memory only; one thread at a time). Pages that several sequences
+ * share are counted; a page goes back to the pool with its last holder. */
+typedef struct hq_pages hq_pages;
+int hq_pages_create(uint32_t n_pages, int page_size, int max_seqs, hq_pages **out);
+void hq_pages_free(hq_pages *p);
+/* Sequence seq has n_pos positions from now on, of which it keeps the first n_keep (at most n_pos and those it has): pages are
+ * taken from the pool, the lowest first, or go back to it (0, 0: all of them). Where positions behind n_keep lie in a page that
+ * others hold too, the sequence gets one of its own in its place, with a copy of what it keeps there (hq_pages_copies). Too few
+ * pages in the pool: -1, and nothing is changed. */
+int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos);
+/* child, which must have no positions, gets the first n_pos of parent's and shares their pages. */
+int hq_pages_fork(hq_pages *p, int parent, int child, int n_pos);
+/* Pages are moved so that those held are the lowest ones. No copies may wait (hq_pages_copies). */
+int hq_pages_compact(hq_pages *p);
+/* The copies that resize and compact have asked for since the last call of this function, as hq_kv_copy takes them; they must run
+ * before a step reads or writes the pages. The arrays belong to p, until its next call. A page that a waiting copy reads is in
+ * nobody's hands again only after this call. */
+int hq_pages_copies(hq_pages *p, const uint32_t **src, const uint32_t **dst, const int32_t **n_pos, int *n);
+/* The pages of n sequences as rows of hq_batch_set's table: row i, pages_ld wide, those of seqs[i] (places behind them: 0). */
+int hq_pages_table(const hq_pages *p, const int32_t *seqs, int n, uint32_t *pages, int pages_ld);
+/* A sequence's positions, and the pages that resize could take now. Either may be NULL. */
+int hq_pages_count(const hq_pages *p, int seq, int *n_pos, uint32_t *n_free);
+
+/* Positions 0 .. n_pos[i] - 1 (n_pos NULL: all) of page src[i] to page dst[i], i < n, in the n_kv caches of kv (layers of one
+ * geometry): keys, values and scales. src, dst, n_pos are the host's; all n copies are as if at once: no dst may be another's dst
+ * or any src. Asynchronous; the arrays may change when the call returns. */
+int hq_kv_copy(const hq_kv_t *kv, int n_kv, const uint32_t *src, const uint32_t *dst, const int32_t *n_pos, int n, void *stream);
+
+/* ---- beam search */
+#define HQ_BEAM_MAX 64 /* beams of a group, and candidates chosen */
+/* The k best continuations of each of n_groups groups of n_beams beams. Row i * n_beams + j of the logits (fp16, or fp32 with f32;
+ * V each, row m at logits + m * stride) and score[i * n_beams + j] belong to beam j of group i; its candidates are the tokens v
+ * with the value score + log softmax(row)[v]. A beam with done != 0 (done may be NULL) has the one candidate done_token, with its
+ * score as the value. To out_score, out_token and out_beam [n_groups, k], best first, equal values by the lower beam, then the
+ * lower token; candidates of -inf (barred tokens, beams with a score of -inf) are none, and places beyond the last candidate get
+ * -inf, UINT32_MAX and -1. Rows of done beams and of those with a score of -inf are not read. A NaN or +inf in a group's scores or
+ * in a row that is read: NaN, UINT32_MAX and -1 in all of the group's places. Values are formed and compared in 64 bits from 32-bit
+ * exponentials. Its workspace belongs to (device, stream) as hq_logprobs' does. score and
+ * the outputs must not overlap. */
+int hq_beam(const void *logits, int f32, int n_groups, int n_beams, uint32_t V, int64_t stride, const float *score, const uint8_t *done,
+            uint32_t done_token, int k, float *out_score, uint32_t *out_token, int32_t *out_beam, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
