@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <vector>
+
 #include "hq_internal.h"
 #include "hq_serve.h"
 
@@ -17,6 +19,25 @@ struct HqTile {
     int seq, t0, n;
 };
 constexpr int HQ_CONV_TILE = 8;  // most tokens of a tile of hq_delta_append
+
+// hq_delta by chunks of 64 tokens. A chunk's operands that depend on its value head but not on the state are formed first, for many
+// chunks at a time (a pass), into HQ_CHUNK_BYTES of workspace each: 18 fragments and a vector of 1 KB (hq_delta.hip).
+constexpr int HQ_STEP_TOKENS = 16;  // most new tokens of a sequence that it takes token by token
+constexpr int HQ_CHUNK = 64;
+constexpr size_t HQ_CHUNK_BYTES = 19 * 1024;
+struct HqChunk {
+    int tok0, n;
+};
+// A sequence, or the part of one that a pass has: its tokens, its first chunk in the pass, slots as in HqSeq; a state on its way from
+// one pass to the next lies in one of two places of the workspace, -2 and -3.
+struct HqRun {
+    int tok0, n, chunk0;
+    int from, to;
+};
+struct HqPass {
+    int chunk0, n_chunks;  // of hq_scan::chunks
+    int run0, n_runs;      // of hq_scan::runs
+};
 
 struct hq_scan {
     int device, n_cu;
@@ -31,6 +52,11 @@ struct hq_scan {
     int n_tiles;
     const int *steps;  // the sequences that hq_delta takes token by token, longest first
     int n_steps;
+    const HqChunk *chunks;  // and those that it takes by chunks
+    const HqRun *runs;      // (a pass's longest first)
+    std::vector<HqPass> passes;
+    char *work;             // chunks of a pass, then two states
+    size_t work_bytes, carry_at;
     // storage: one pinned copy of `dev`, which the next set waits for
     int *host, *dev;
     size_t words;

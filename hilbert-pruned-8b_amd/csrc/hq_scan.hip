@@ -13,6 +13,8 @@
 
 namespace {
 
+constexpr size_t MOST_WORK = (size_t)640 << 20;  // of the chunks of a pass
+
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 int use_device(int device) {
@@ -70,6 +72,7 @@ extern "C" void hq_scan_free(hq_scan *c) {
     (void)use_device(c->device);
     (void)hipDeviceSynchronize();
     if (c->dev) (void)hipFree(c->dev);
+    if (c->work) (void)hipFree(c->work);
     if (c->host) (void)hipHostFree(c->host);
     if (c->sent) (void)hipEventDestroy(c->sent);
     delete c;
@@ -91,6 +94,13 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     if (T > c->max_tokens) return hq_internal_fail("%s: %lld new tokens (the step takes %d)", who, (long long)T, c->max_tokens);
     std::vector<HqTile> tiles;
     std::vector<int> steps;
+    std::vector<HqChunk> chunks;
+    std::vector<HqRun> runs;
+    std::vector<HqPass> passes;
+    // chunks of a pass: what fits MOST_WORK, and 64 at least
+    const size_t per_chunk = (size_t)st->n_v_heads * HQ_CHUNK_BYTES;
+    const int most_chunks = (int)std::max<size_t>(64, MOST_WORK / per_chunk);
+    bool carries = false;
     try {
         // slots that are written: each by one sequence, and read by no other
         std::vector<std::pair<int, int>> w, r;
@@ -107,11 +117,33 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
             for (size_t k = j; k < r.size() && r[k].first == w[i].first; k++)
                 if (r[k].second != w[i].second) return hq_internal_fail("%s: sequence %d goes on from slot %d, where sequence %d leaves its state", who, r[k].second, w[i].first, w[i].second);
         }
-        for (int i = 0; i < n_seqs; i++) {
+        std::vector<std::pair<int, int>> long_seqs;
+        for (int i = 0, tok = 0; i < n_seqs; tok += n_new[i], i++) {
             if (n_new[i] == 0 && (to[i] < 0 || to[i] == from[i])) continue;
             for (int t = 0; t == 0 || t < n_new[i]; t += HQ_CONV_TILE) tiles.push_back({i, t, std::min(HQ_CONV_TILE, n_new[i] - t)});
-            steps.push_back(i);
+            if (n_new[i] <= HQ_STEP_TOKENS) {
+                steps.push_back(i);
+                continue;
+            }
+            long_seqs.push_back({i, tok});
         }
+        for (const auto &l : long_seqs) {
+            int from_now = from[l.first];
+            for (int t = 0; t < n_new[l.first];) {
+                if (passes.empty() || passes.back().n_chunks == most_chunks) passes.push_back({(int)chunks.size(), 0, (int)runs.size(), 0});
+                HqPass &p = passes.back();
+                const int n = std::min<int64_t>((int64_t)n_new[l.first] - t, (int64_t)(most_chunks - p.n_chunks) * HQ_CHUNK);
+                const bool cut = t + n < n_new[l.first];
+                const int carry = -2 - (int)(passes.size() & 1);
+                runs.push_back({l.second + t, n, p.n_chunks, from_now, cut ? carry : to[l.first]});
+                for (int j = 0; j < n; j += HQ_CHUNK) chunks.push_back({l.second + t + j, std::min(HQ_CHUNK, n - j)}), p.n_chunks++;
+                p.n_runs++;
+                from_now = carry, carries |= cut;
+                t += n;
+            }
+        }
+        for (const HqPass &p : passes)
+            std::stable_sort(runs.begin() + p.run0, runs.begin() + p.run0 + p.n_runs, [](const HqRun &a, const HqRun &b) { return a.n > b.n; });
         std::stable_sort(steps.begin(), steps.end(), [&](int a, int b) { return n_new[a] > n_new[b]; });
     } catch (const std::exception &) {
         return hq_internal_fail("%s: out of memory", who);
@@ -122,7 +154,8 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
         SCK(hipEventSynchronize(c->sent));
         c->sending = false;
     }
-    const size_t words = (size_t)n_seqs * (sizeof(HqSeq) / 4) + tiles.size() * (sizeof(HqTile) / 4) + steps.size() + 16;
+    const size_t words = (size_t)n_seqs * (sizeof(HqSeq) / 4) + tiles.size() * (sizeof(HqTile) / 4) + steps.size() + chunks.size() * (sizeof(HqChunk) / 4) +
+                         runs.size() * (sizeof(HqRun) / 4) + 16;
     if (words > c->words) {
         const size_t want = words + words / 2;
         SCK(hipDeviceSynchronize());
@@ -134,6 +167,18 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
         SCK(hipMalloc((void **)&c->dev, want * 4));
         SCK(hipHostMalloc((void **)&c->host, want * 4, hipHostMallocDefault));
         c->words = want;
+    }
+    size_t work = 0;
+    for (const HqPass &p : passes) work = std::max(work, (size_t)p.n_chunks * per_chunk);
+    c->carry_at = work;
+    if (carries) work += 2 * (size_t)st->n_v_heads * st->k_dim * st->v_dim * 4;
+    if (work > c->work_bytes) {
+        SCK(hipDeviceSynchronize());
+        if (c->work) SCK(hipFree(c->work));
+        c->work = nullptr;
+        c->work_bytes = 0;
+        SCK(hipMalloc((void **)&c->work, work));
+        c->work_bytes = work;
     }
     int *w = c->host;
     const auto dev = [&]() { return c->dev + (w - c->host); };
@@ -148,6 +193,13 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     c->steps = dev(), c->n_steps = (int)steps.size();
     if (!steps.empty()) memcpy(w, steps.data(), steps.size() * 4);
     w += steps.size();
+    c->chunks = (const HqChunk *)dev();
+    if (!chunks.empty()) memcpy(w, chunks.data(), chunks.size() * sizeof(HqChunk));
+    w += chunks.size() * (sizeof(HqChunk) / 4);
+    c->runs = (const HqRun *)dev();
+    if (!runs.empty()) memcpy(w, runs.data(), runs.size() * sizeof(HqRun));
+    w += runs.size() * (sizeof(HqRun) / 4);
+    c->passes.swap(passes);
     const size_t used = (size_t)(w - c->host);
     if (used) {
         SCK(hipMemcpyAsync(c->dev, c->host, used * 4, hipMemcpyHostToDevice, (hipStream_t)stream));

@@ -175,7 +175,7 @@ int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_delta_in_t 
 
 typedef struct {
     /* fp16: head h of token t at q and k + t * qk_stride + h * k_dim, v + t * v_stride + h * v_dim; 16-byte aligned, strides
-     * multiples of 8 */
+     * multiples of 8 (these and out_stride at most 2^22 where a sequence has more than 16 new tokens) */
     const uint16_t *q, *k, *v;
     int64_t qk_stride, v_stride;
     const float *decay, *beta; /* [tokens, n_v_heads]; decay: a logarithm, 0 or less, -inf allowed */
@@ -194,7 +194,10 @@ typedef struct {
 
 /* For every new token, value head and its key head, from the sequence's state: S' = e^decay S; S = S' + k (beta (v - S'^T k))^T;
  * o = scale S^T q. States to their slots. Keys are to have a norm of at most 1 and beta to lie in 0 .. 1 (as hq_delta_append gives
- * them): the recurrence itself grows without bound otherwise. States and sums are fp32; the same step gives the same bits. */
+ * them): the recurrence itself grows without bound otherwise. States and sums are fp32; sequences of more than 16 new tokens are
+ * taken in chunks, as products on the matrix cores whose operands are two fp16 terms each (2^-22 of a column's largest; for the
+ * outputs, which end in fp16, one term, 2^-11). A value that is not a number stays in its value column (and head, with the norm).
+ * The same step gives the same bits. Kernels in a row, no allocation. */
 int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t *d, void *stream);
 
 /* ---- pages of sequences that branch and end */

@@ -3,7 +3,11 @@
 Errors of the recurrence, by the 2-norm of a column of S, e: a step S' = (I - beta k k^T) a S + beta k v^T with |k| <= 1, 0 <= beta <= 1
 and a <= 1 is a contraction, so errors add up and never grow: e <- a e + c. A token's own error c: the product k^T S is a 32-bit sum
 over k_dim products, (k_dim + 8) 2^-24 of |k| |S| at most; operands that are held as two fp16 terms are off by 2^-22 of their
-column's largest; a chunked form has sums over up to 64 tokens beside them. c = 4 (k_dim + 80) 2^-24 (|a S| + |v|) covers both."""
+column's largest; a chunked form has sums over up to 64 tokens beside them. c = 4 (k_dim + 80) 2^-24 (|a S| + |v|) covers both.
+
+Outputs end in fp16, and the chunked form rounds the operands of their products to it: of o = scale (e^G q S0 + sum_j M_j u_j) with S0
+the state before the chunk (of 64 tokens from the sequence's first), S0 once and M and u once each, so 2^-11 of sum |e^G q S0| and 2
+2^-11 of sum |M_j u_j| are added to the state's error and the rounding of the result."""
 import numpy as np
 
 U16, U32 = 2.0 ** -11, 2.0 ** -24
@@ -55,7 +59,11 @@ def delta(q, k, v, decay, beta, states, n_new, scale, norm=None, gate=None, eps=
     out, bound, after, e_after, t = np.zeros((T, hv, dv)), np.zeros((T, hv, dv)), [], [], 0
     for s0, n in zip(states, n_new):
         S, e = s0.astype(np.float64), np.zeros((hv, 1, dv))
-        for _ in range(n):
+        for i in range(n):
+            if i % 64 == 0:  # a chunk: the state before it, what its tokens have written, the logarithm of the decay since
+                S0, first, G, us = np.abs(S), t, np.zeros((hv, 0)), np.zeros((0, hv, dv))
+            g_t = np.maximum(decay[t].astype(np.float64), -1e4)
+            G = np.concatenate([G + g_t[:, None], np.zeros((hv, 1))], 1)  # [hv, tokens of the chunk]: to now from each of them
             keep = np.exp(decay[t].astype(np.float64))[:, None, None]
             # (a decay's exponential is off by 2^-22 of itself: its argument's sums and the function)
             S = S * keep
@@ -64,12 +72,16 @@ def delta(q, k, v, decay, beta, states, n_new, scale, norm=None, gate=None, eps=
             u = (v[t] - (k[t][:, :, None] * S).sum(1)) * beta[t].astype(np.float64)[:, None]
             S = S + k[t][:, :, None] * u[:, None]
             o = scale * (S * q[t][:, :, None]).sum(1)
-            # operands of the outputs' products may be rounded to fp16, beside the state's own error
-            b = abs(scale) * ((np.abs(S) * np.abs(q[t])[:, :, None]).sum(1) * 2 * U16 + (np.abs(u) + np.sqrt((S * S).sum(1))) * 2 * U16 * np.linalg.norm(q[t], axis=-1)[:, None]
-                              + e[:, 0] * np.linalg.norm(q[t], axis=-1)[:, None])
+            us = np.concatenate([us, np.abs(u)[None]])
+            with np.errstate(under="ignore"):
+                M = np.exp(G) * np.abs((k[first:t + 1] * q[t]).sum(-1)).T
+                old = np.exp(G[:, :1] + (np.maximum(decay[first].astype(np.float64), -1e4)[:, None])) * (S0 * np.abs(q[t])[:, :, None]).sum(1)
+            b = abs(scale) * (U16 * old + 2 * U16 * (M.T[:, :, None] * us).sum(0) + e[:, 0] * np.linalg.norm(q[t], axis=-1)[:, None])
             if norm is not None:
                 z = silu(gate[t].astype(np.float64)) * norm.astype(np.float64)
                 ms = (o * o).mean(-1, keepdims=True) + eps
+                # (with the norm, chunks round o to fp16 before it)
+                b = b + U16 * np.abs(o) + 2.0 ** -25
                 rel = (np.abs(o) * b).mean(-1, keepdims=True) / ms + (dv + 16) * U32
                 # (second order: the norm itself moves by at most rel)
                 b = (b + np.abs(o) * rel) / np.sqrt(ms) * np.abs(z) * (1 + 2 * rel)
