@@ -13,6 +13,9 @@ bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 constexpr int64_t MOST_CHUNK_STRIDE = 1 << 22;  // 64 rows of it stay below 2^29 bytes
 
+// z / (1 + e^-z) with the hardware's exponential and reciprocal (2^-22 of the result together; -inf gives NaN, as the formula)
+DEV float silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
+
 struct DeltaArgs {
     hq_state_t st;
     hq_delta_t d;
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(16 * CG) k_delta_step(DeltaArgs g) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float z = g.d.gate_f32 ? ((const float *)g.d.gate)[at + e] : (float)((const _Float16 *)g.d.gate)[at + e];
-                            o[e] = o[e] * inv * g.d.norm[4 * cg + e] * (z / (1.0f + expf(-z)));
+                            o[e] = o[e] * inv * g.d.norm[4 * cg + e] * silu(z);
                         }
                     }
                 }
@@ -154,110 +157,114 @@ __global__ void __launch_bounds__(16 * CG) k_delta_step(DeltaArgs g) {
 // Precision: K, Q and V are exact. S, U and T enter products as two fp16 terms each, scaled by a power of two of their column's largest
 // (T: of the matrix), good to 2^-22 of it; only for the outputs, which end in fp16, one term of S, M and U does.
 constexpr int FRAG_T = 0, FRAG_T_LO = 6, FRAG_M = 12, FRAG_VEC = 18;  // of a chunk's workspace, in KB; fragments (block, half) in the order below
-constexpr float T_SCALE = 4096.f;
+constexpr int T_BITS = 12;  // T is held 2^12 times as large
+constexpr float T_SCALE = 1 << T_BITS;
 DEV int frag_of(int b, int s) { return b < 2 ? b : 2 * b - 2 + s; }
 DEV int token_of(int b, int row) { return 32 * (b >> 1) + 8 * (row >> 2) + (row & 3) + 4 * (b & 1); }
-// A row's 16-byte pieces lie in LDS in an order of the row's own, so that 16 rows' pieces of one column fall into different banks.
+// A row's 16-byte pieces lie in LDS in an order of the row's own, so that what is read together falls into different banks: a piece of
+// each of a block's 16 rows (by lanes 0 - 3, 12 - 15 of one lane group with 4 - 11 of the next), or, transposed, four pieces in a row of
+// each of four rows. (With the row's number alone as the key, the transposed reads go at half the rate: 94 against 81 us.)
 template <int CPR>
 DEV int piece_at(int row, int c) {
-    const int key = CPR >= 16 ? (row & 3) | ((row >> 1) & 12) : ((row >> 1) & 1) | ((row >> 2) & 6);
-    return row * CPR + (c ^ key);
+    const int mid = (row >> 3 & 1 ? 2 : 0) ^ (row >> 4 & 1 ? 3 : 0);
+    return row * CPR + (c ^ ((CPR >= 16 ? (row & 3) << 2 : (row & 2) << 1) | mid));
 }
 
-DEV float pow2(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
-// The exponent that takes a largest magnitude to 2^14 .. 2^15 by pow2(268 - e), and back by pow2(e - 14)
-DEV uint32_t exponent(float largest) {
-    const uint32_t e = __builtin_bit_cast(uint32_t, largest) >> 23;
-    return e < 15u ? 15u : e > 253u ? 253u : e;
+DEV float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)e << 23); }
+// A largest magnitude's exponent: its 2^14 .. 2^15 is reached by pow2(268 - e), and left by pow2(e - 14).
+DEV int exponent(float largest) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);
+    return min(max(e, 15), 253);
 }
+DEV int in_range(int e) { return min(max(e, 1), 253); }
 
 struct ChunkArgs {
     hq_state_t st;
     hq_delta_t d;
     const HqChunk *chunks;
     const HqRun *runs;
-    int n_runs;
+    int n_runs, n_chunks;
     char *work;
     float *carry;
+    float one;  // 1: a factor that the compiler does not know, so that a difference is one fused instruction
 };
 
-// T and M of a chunk's value heads; a workgroup takes those of one key head. Wave w forms rows 16 w .. of K K^T and Q K^T, then inverts
-// the 16 x 16 block (w, w) of I + A by substitution, a column a lane, and last computes block column w of the inverse from the top
-// down, T_ij = -T_ii sum_l A_il T_lj, on the fp32 matrix cores: each block of the column is the next one's operand.
+// T and M of a chunk and value head. Wave w forms rows 16 w .. of K K^T and Q K^T, then inverts the 16 x 16 block (w, w) of I + A by
+// substitution, a column a lane, and last computes block column w of the inverse from the top down, T_ij = -T_ii sum_l A_il T_lj, on
+// the fp32 matrix cores: each block of the column is the next one's operand.
 template <int KS>
-__global__ void __launch_bounds__(256) k_delta_prep(ChunkArgs g) {
+__global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g) {
     constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS, LD = 72, LA = 68, LT = 20;
     __shared__ union {
         u4v kq[2][64 * CPR];
-        _Float16 f[3][64 * LD];  // T, its second term, M
+        struct {
+            _Float16 f[3][64 * LD];  // T, its second term, M
+            float At[64 * LA];       // A transposed
+        };
     } sh;
-    __shared__ alignas(16) float At[64 * LA];  // A transposed
     __shared__ alignas(16) float Td[4][16 * LT];
-    __shared__ double gam[4][64];
-    __shared__ float bet[4][64], ms[64];
-    const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim;
-    const int at = blockIdx.x / nk, hk = blockIdx.x % nk, rep = nv / nk;
+    __shared__ double gam[4][64];  // (a copy a wave)
+    __shared__ float bet[4][64], ms[4];
+    // workgroup i runs on XCD i % 8: the value heads of a key head on one
+    const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, rep = nv / nk;
+    const int unit = blockIdx.x / (8 * rep) * 8 + blockIdx.x % 8;
+    if (unit >= g.n_chunks * nk) return;
+    const int at = unit / nk, hk = unit % nk, h = hk * rep + blockIdx.x / 8 % rep;
     const HqChunk ch = g.chunks[at];
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = lane & 15, q = lane >> 4;
-    for (int i = tid; i < 2 * 64 * CPR; i += 256) {
-        const int which = i / (64 * CPR), row = (i / CPR) % 64, c = i % CPR;
-        u4v x = {0, 0, 0, 0};
-        if (row < ch.n && 8 * c < dk) x = *(const u4v *)((which ? g.d.q : g.d.k) + (size_t)(ch.tok0 + row) * g.d.qk_stride + hk * dk + 8 * c);
-        sh.kq[which][piece_at<CPR>(row, c)] = x;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
+    const float gl = lane < ch.n ? g.d.decay[(size_t)(ch.tok0 + lane) * nv + h] : 0.f, bl = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
+#pragma unroll
+    for (int i0 = 0; i0 < 64 * CPR; i0 += 256) {
+        const int i = i0 + tid, row = i / CPR, c = i % CPR;
+        const size_t from = (size_t)(ch.tok0 + row) * g.d.qk_stride + hk * dk + 8 * c;
+        u4v k = {0, 0, 0, 0}, x = k;
+        if (row < ch.n && 8 * c < dk) k = *(const u4v *)(g.d.k + from), x = *(const u4v *)(g.d.q + from);
+        sh.kq[0][piece_at<CPR>(row, c)] = k, sh.kq[1][piece_at<CPR>(row, c)] = x;
     }
+    // sums of the decays' logarithms, to base 2
+    double sum = (double)(gl < -1e4f ? -1e4f : gl) * 1.4426950408889634074;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += y;
+    }
+    gam[w][lane] = sum;
+    bet[w][lane] = bl;
     __syncthreads();
-    f4 G[4], H[4];
+    f4 A[4], M[4];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-        G[b] = H[b] = f4{0.f, 0.f, 0.f, 0.f};
+        A[b] = M[b] = f4{0.f, 0.f, 0.f, 0.f};
         if (b > w) continue;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const h8 x = __builtin_bit_cast(h8, sh.kq[0][piece_at<CPR>(16 * b + n, 4 * s + q)]);
-            G[b] = mfma(__builtin_bit_cast(h8, sh.kq[0][piece_at<CPR>(16 * w + n, 4 * s + q)]), x, G[b]);
-            H[b] = mfma(__builtin_bit_cast(h8, sh.kq[1][piece_at<CPR>(16 * w + n, 4 * s + q)]), x, H[b]);
+            A[b] = mfma(__builtin_bit_cast(h8, sh.kq[0][piece_at<CPR>(16 * w + n, 4 * s + q)]), x, A[b]);
+            M[b] = mfma(__builtin_bit_cast(h8, sh.kq[1][piece_at<CPR>(16 * w + n, 4 * s + q)]), x, M[b]);
         }
     }
-    for (int e = 0; e < rep; e++) {
-        const int h = hk * rep + e;
-        const float gl = lane < ch.n ? g.d.decay[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
-        double sum = (double)(gl < -1e4f ? -1e4f : gl);
+    const int i0 = 16 * w + 4 * q;
+    float mx = 0.f;
+    __syncthreads();
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += y;
-        }
-        gam[w][lane] = sum;
-        bet[w][lane] = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
-        __syncthreads();  // (the last head's reads of At are done as well)
-        f4 M[4];
-        float mx[4] = {0.f, 0.f, 0.f, 0.f};
-        const int i0 = 16 * w + 4 * q;
-#pragma unroll
-        for (int b = 0; b < 4; b++) {
-            M[b] = f4{0.f, 0.f, 0.f, 0.f};
-            if (b > w) continue;
-            const int j = 16 * b + n;
-            f4 a;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float x = j <= i0 + r ? expf((float)(gam[w][i0 + r] - gam[w][j])) : 0.f;
-                a[r] = j < i0 + r ? bet[w][i0 + r] * x * G[b][r] : 0.f;
-                M[b][r] = j <= i0 + r ? x * H[b][r] : 0.f;
-                mx[r] = fmaxf(mx[r], fabsf(M[b][r]));
-            }
-            *(f4 *)(At + j * LA + i0) = a;
-        }
+    for (int b = 0; b < 4; b++) {
+        if (b > w) continue;
+        const int j = 16 * b + n;
+        const double gj = gam[w][j];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor(mx[r], o, 64));
-            const uint32_t ex = exponent(mx[r]);
-            if (n == 0) ms[i0 + r] = pow2(ex - 14u);
-#pragma unroll
-            for (int b = 0; b < 4; b++) M[b][r] *= pow2(268u - ex);
+            const float x = j <= i0 + r ? __builtin_amdgcn_exp2f((float)(gam[w][i0 + r] - gj)) : 0.f;
+            A[b][r] = j < i0 + r ? bet[w][i0 + r] * x * A[b][r] : 0.f;
+            M[b][r] = j <= i0 + r ? x * M[b][r] : 0.f;
+            mx = fmaxf(mx, fabsf(M[b][r]));
         }
-        __syncthreads();
+        *(f4 *)(sh.At + j * LA + i0) = A[b];
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    if (lane == 0) ms[w] = mx;
+    __syncthreads();
+    {
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = i == n ? 1.f : 0.f;
@@ -265,7 +272,7 @@ __global__ void __launch_bounds__(256) k_delta_prep(ChunkArgs g) {
         for (int j = 0; j < 15; j++)
 #pragma unroll
             for (int i4 = (j + 1) / 4; i4 < 4; i4++) {
-                const f4 a = *(const f4 *)(At + (16 * w + j) * LA + 16 * w + 4 * i4);
+                const f4 a = *(const f4 *)(sh.At + (16 * w + j) * LA + 16 * w + 4 * i4);
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (4 * i4 + r > j) x[4 * i4 + r] = fmaf(-a[r], x[j], x[4 * i4 + r]);
@@ -273,93 +280,136 @@ __global__ void __launch_bounds__(256) k_delta_prep(ChunkArgs g) {
 #pragma unroll
         for (int i = 0; i < 16; i++)
             if (i / 4 == q) Td[w][i * LT + n] = x[i];
-        __syncthreads();
-        f4 T[4];
+    }
+    __syncthreads();
+    f4 T[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            T[i] = f4{0.f, 0.f, 0.f, 0.f};
-            if (i < w) continue;
-            if (i == w) {
+    for (int i = 0; i < 4; i++) {
+        T[i] = f4{0.f, 0.f, 0.f, 0.f};
+        if (i < w) continue;
+        if (i == w) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) T[i][r] = Td[w][(4 * q + r) * LT + n];
-                continue;
+            for (int r = 0; r < 4; r++) T[i][r] = Td[w][(4 * q + r) * LT + n];
+            continue;
+        }
+        f4 y = {0.f, 0.f, 0.f, 0.f}, z = y;
+#pragma unroll
+        for (int l = 0; l < i; l++)
+            if (l >= w) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(sh.At[(16 * l + 4 * q + r) * LA + 16 * i + n], T[l][r], y, 0, 0, 0);
             }
-            f4 y = {0.f, 0.f, 0.f, 0.f}, z = y;
+        const f4 t = *(const f4 *)(Td[i] + n * LT + 4 * q);
 #pragma unroll
-            for (int l = 0; l < i; l++)
-                if (l >= w) {
+        for (int r = 0; r < 4; r++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(t[r], y[r], z, 0, 0, 0);
+        T[i] = -z;
+    }
+    const float scale = T_SCALE * bet[w][16 * w + n];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(At[(16 * l + 4 * q + r) * LA + 16 * i + n], T[l][r], y, 0, 0, 0);
-                }
-            const f4 t = *(const f4 *)(Td[i] + n * LT + 4 * q);
+    for (int i = 0; i < 4; i++) {
+        if (i < (w & ~1)) continue;  // (above the diagonal: the half of a fragment that is zero)
 #pragma unroll
-            for (int r = 0; r < 4; r++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(t[r], y[r], z, 0, 0, 0);
-            T[i] = -z;
+        for (int r = 0; r < 4; r++) {
+            const float v = T[i][r] * scale;
+            const _Float16 hi = (_Float16)v;
+            const int o = (16 * i + 4 * q + r) * LD + 16 * w + n;
+            sh.f[0][o] = hi;
+            sh.f[1][o] = (_Float16)(v - (float)hi);
         }
-        const float scale = T_SCALE * bet[w][16 * w + n];
+    }
+    const int em = exponent(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i < (w & ~1)) continue;  // (above the diagonal: the half of a fragment that is zero)
+    for (int b = 0; b < 4; b++) {
+        if (b > (w | 1)) continue;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float v = T[i][r] * scale;
-                const _Float16 hi = (_Float16)v;
-                const int o = (16 * i + 4 * q + r) * LD + 16 * w + n;
-                sh.f[0][o] = hi;
-                sh.f[1][o] = (_Float16)(v - (float)hi);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < 4; b++) {
-            if (b > (w | 1)) continue;
-#pragma unroll
-            for (int r = 0; r < 4; r++) sh.f[2][(i0 + r) * LD + 16 * b + n] = (_Float16)M[b][r];
-        }
-        __syncthreads();
-        char *const to = g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES;
-        for (int p = w; p < 18; p += 4) {
-            const int k = p % 6, b = k < 2 ? k : k / 2 + 1, s = k < 2 ? 0 : k & 1;
-            *(u4v *)(to + p * 1024 + lane * 16) = *(const u4v *)(sh.f[p / 6] + token_of(b, n) * LD + 32 * s + 8 * q);
-        }
-        if (w == 3) {
-            float *const v = (float *)(to + FRAG_VEC * 1024);
-            v[lane] = expf((float)gam[3][lane]);
-            v[64 + lane] = expf((float)(gam[3][63] - gam[3][lane]));
-            v[128 + lane] = ms[lane];
-            v[192 + lane] = expf((float)gam[3][63]);
-        }
+        for (int r = 0; r < 4; r++) sh.f[2][(i0 + r) * LD + 16 * b + n] = (_Float16)(M[b][r] * pow2(268 - em));
+    }
+    __syncthreads();
+    char *const to = g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES;
+    for (int p = w; p < 18; p += 4) {
+        const int k = p % 6, b = k < 2 ? k : k / 2 + 1, s = k < 2 ? 0 : k & 1;
+        *(u4v *)(to + p * 1024 + lane * 16) = *(const u4v *)(sh.f[p / 6] + token_of(b, n) * LD + 32 * s + 8 * q);
+    }
+    if (w == 3) {
+        float *const v = (float *)(to + FRAG_VEC * 1024);
+        v[lane] = __builtin_amdgcn_exp2f((float)gam[3][lane]);
+        v[64 + lane] = __builtin_amdgcn_exp2f((float)(gam[3][63] - gam[3][lane]));
+        if (lane == 0) v[128] = g.d.scale * pow2(em - 14);
     }
 }
 
 typedef short s4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4v lds_s4v;
+typedef const __attribute__((address_space(3))) u4v lds_u4;
+typedef const __attribute__((address_space(3))) float lds_f;
+typedef const __attribute__((address_space(3))) _Float16 lds_h;
 
-// Two fp16 terms of 8 values scaled by sc: accumulator blocks a and b as an operand
-DEV void two_terms(const f4 &a, const f4 &b, float sc, h8 &hi, h8 &lo) {
+// Two fp16 terms of 8 values scaled by sc: accumulator blocks a and b as an operand. Scaling and conversion stay two instructions:
+// fused into one that writes half a register they go at half the rate (9.4 clocks an instruction against 5.4).
+DEV h8 halves(const f4 &a, const f4 &b) {
+    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float x = (j < 4 ? a[j & 3] : b[j & 3]) * sc;
-        hi[j] = (_Float16)x;
-        lo[j] = (_Float16)(x - (float)hi[j]);
+    for (int j = 0; j < 4; j++) {
+        const f4 &x = j < 2 ? a : b;
+        w[j] = __builtin_bit_cast(uint32_t, h2{(_Float16)x[2 * j & 3], (_Float16)x[(2 * j & 3) + 1]});
+        asm("" : "+v"(w[j]));  // (a pair from one conversion is not to be converted again, value by value, where it is subtracted)
     }
+    return __builtin_bit_cast(h8, u4v{w[0], w[1], w[2], w[3]});
 }
+DEV h8 first_term(const f4 &a, const f4 &b, float sc) { return halves(a * sc, b * sc); }
+DEV h8 second_term(const f4 &a, const f4 &b, float sc, h8 hi) {
+    f4 x, y;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        x[j] = fmaf(a[j], sc, -(float)hi[j]), y[j] = fmaf(b[j], sc, -(float)hi[4 + j]);
+        float u = x[j], v = y[j];
+        asm("" : "+v"(u), "+v"(v));
+        x[j] = u, y[j] = v;
+    }
+    return halves(x, y);
+}
+// The largest magnitude of a column: 4 N values of each of the four lanes that have it
 template <int N>
 DEV float column_max(const f4 (&x)[N]) {
-    float m = 0.f;
+    float m[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; i++) m = fmaxf(fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3]))), m);
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    return fmaxf(m, __shfl_xor(m, 32, 64));
+    for (int i = 0; i < N; i++) {
+        m[0] = fmaxf(fmaxf(m[0], fabsf(x[i][0])), fabsf(x[i][1]));
+        m[1] = fmaxf(fmaxf(m[1], fabsf(x[i][2])), fabsf(x[i][3]));
+    }
+    uint32_t v = __builtin_bit_cast(uint32_t, fmaxf(m[0], m[1]));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);  // (magnitudes: their order as integers)
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_bit_cast(float, max(b[0], b[1]));
 }
 
-// The chunks of a run in order; a wave holds S for 16 of a head's value columns and needs no other wave's results. All waves of a
-// workgroup (W of them with columns, four at least) bring the next chunk's keys, queries, T and M to LDS by DMA meanwhile.
+// The chunks of a run in order. A workgroup has 16 W value columns of a head; wave w < W holds S for 16 of them, takes it from chunk to
+// chunk and needs no other wave's results. The four waves behind them bring the next chunk's operands to LDS by DMA: an instruction of
+// it holds its wave for some 70 clocks, which the way from one state to the next, what bounds a long run, has no room for.
+//
+// A column of S is held in units of a power of two, taken from a bound of its magnitudes (the bound before, decayed, and what a chunk can
+// add, 64 times its largest U as no key's element exceeds 1; every 16 chunks the largest itself): so S can enter products without a
+// look over it, and fp16's range leaves what the bound is too large by.
+// (wider keys' operands do not all fit the registers: they are read where they are used)
+#define STAGE if (KS <= 4) __builtin_amdgcn_sched_barrier(0)
+// N times a product and M other instructions (what: 2 arithmetic, 0x100 reads of LDS), in the order of issue
+#define MIX(N, what, M)                                          \
+    if (KS <= 4) {                                               \
+        _Pragma("unroll") for (int i_ = 0; i_ < (N); i_++) {     \
+            __builtin_amdgcn_sched_group_barrier(8, 1, 0);       \
+            __builtin_amdgcn_sched_group_barrier(what, M, 0);    \
+        }                                                        \
+    }
 template <int KS, int W>
-__global__ void __launch_bounds__(64 * (W < 4 ? 4 : W)) k_delta_scan(ChunkArgs g) {
-    constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS, NW = W < 4 ? 4 : W;
-    constexpr int KB = CPR;  // of a chunk's keys: 64 rows of CPR pieces of 16 bytes
-    constexpr int BUFS = KS <= 6 ? 2 : 1;  // (two chunks of wider keys do not fit: the next one's wait until this one is done)
-    __shared__ alignas(1024) char buf[BUFS][(2 * KB + 19) * 1024];
+__global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
+    constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS;
+    constexpr int KB = CPR, VB = 2 * W;    // KB of a chunk's keys or queries (64 rows of CPR pieces of 16 bytes) and of its values
+    constexpr int BUFS = KS <= 4 ? 2 : 1;  // (two chunks of wider keys do not fit: the next one's wait until this one is done)
+    constexpr int AHEAD = 2;               // steps of K or Q that are read before their use
+    constexpr int AT_F = 2 * KB, AT_VEC = AT_F + FRAG_VEC, AT_V = AT_VEC + 1, SIZE = AT_V + VB;
+    static_assert(KB % 4 == 0, "whole rounds of loads");
+    __shared__ alignas(1024) char lds[BUFS * SIZE * 1024];
     const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim;
     const int groups = (dv + 16 * W - 1) / (16 * W);
     // workgroup i runs on XCD i % 8: the groups of one head on one, where they share its keys
@@ -367,10 +417,58 @@ __global__ void __launch_bounds__(64 * (W < 4 ? 4 : W)) k_delta_scan(ChunkArgs g
     if (head >= g.n_runs * nv) return;
     const HqRun run = g.runs[head / nv];
     const int h = head % nv, hk = h / (nv / nk);
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+    const int chunks = (run.n + HQ_CHUNK - 1) / HQ_CHUNK;
+    const auto buffer = [&](int c) { return (uint32_t)(uintptr_t)lds + 1024u * (uint32_t)(SIZE * (c % BUFS)); };
+    const auto rows_of = [&](int c) { return (uint32_t)min(HQ_CHUNK, run.n - c * HQ_CHUNK); };
+    // Rows behind the run's last lie past the buffers' ranges, as a row of heads is no longer than the stride: loads give zeros, stores
+    // nothing. A row's values lie in LDS so that the four rows which a wave reads together fall into different banks.
+    const auto v_piece = [](int row, int x) { return VB >= 8 ? x ^ (2 * (row >> 3 & 3)) : x; };
+    if (w >= W) {
+        const int lw = w - W;
+        const uint32_t row_bytes = (uint32_t)g.d.qk_stride * 2u, v_bytes = (uint32_t)g.d.v_stride * 2u;
+        uint32_t k_off[KB / 4], v_off[(VB + 3) / 4];
+#pragma unroll
+        for (int i = 0; i < KB / 4; i++) {
+            const int slot = 64 * (4 * i + lw) + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
+            k_off[i] = 8 * x < dk ? (uint32_t)row * row_bytes + 16u * (uint32_t)x : 0x80000000u;
+        }
+#pragma unroll
+        for (int i = 0; i < (VB + 3) / 4; i++) {
+            const int slot = 64 * (4 * i + lw) + lane, row = slot / VB, x = 8 * (2 * W * group + v_piece(row, slot % VB));
+            v_off[i] = x < dv ? (uint32_t)row * v_bytes + 2u * (uint32_t)x : 0x80000000u;
+        }
+        const auto load = [&](int c) {
+            const size_t tok = (size_t)(run.tok0 + c * HQ_CHUNK);
+            const uint32_t range = (rows_of(c) - 1u) * row_bytes + (uint32_t)dk * 2u, to = buffer(c) + 1024u * (uint32_t)lw;
+            const rsrc_t rk = make_rsrc(g.d.k + tok * g.d.qk_stride + hk * dk, range), rq = make_rsrc(g.d.q + tok * g.d.qk_stride + hk * dk, range);
+            const rsrc_t rv = make_rsrc(g.d.v + tok * g.d.v_stride + (size_t)h * dv, (rows_of(c) - 1u) * v_bytes + (uint32_t)dv * 2u);
+            const rsrc_t rw = make_rsrc(g.work + ((size_t)(run.chunk0 + c) * nv + h) * HQ_CHUNK_BYTES, (uint32_t)HQ_CHUNK_BYTES);
+#pragma unroll
+            for (int i = 0; i < KB; i += 4) dma16_untracked(rk, to + 1024u * (uint32_t)i, k_off[i / 4]);
+#pragma unroll
+            for (int i = 0; i < VB; i += 4)
+                if (VB % 4 == 0 || i + lw < VB) dma16_untracked(rv, to + 1024u * (uint32_t)(AT_V + i), v_off[i / 4]);
+#pragma unroll
+            for (int i = 0; i < 20; i += 4)
+                if (i < 16 || lw < 3) dma16_untracked(rw, to + 1024u * (uint32_t)(AT_F + i), 1024u * (uint32_t)(i + lw) + 16u * (uint32_t)lane);
+#pragma unroll
+            for (int i = 0; i < KB; i += 4) dma16_untracked(rq, to + 1024u * (uint32_t)(KB + i), k_off[i / 4]);
+        };
+        if (BUFS == 2) load(0);
+        for (int c = 0; c < chunks; c++) {
+            if (BUFS == 1) {
+                __syncthreads();
+                load(c);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (BUFS == 2 && c + 1 < chunks) load(c + 1);
+        }
+        return;
+    }
     const int col = 16 * (group * W + w) + n;
-    const bool on = w < W && 16 * (group * W + w) < dv;  // (of a wave as a whole)
-    const uint32_t NOWHERE = 0x80000000u;  // past every range: loads give zeros, stores nothing
+    const bool on = 16 * (group * W + w) < dv;  // (of a wave as a whole)
     const size_t size = (size_t)dk * dv;
     f4 S[2 * KS];
 #pragma unroll
@@ -385,136 +483,167 @@ __global__ void __launch_bounds__(64 * (W < 4 ? 4 : W)) k_delta_scan(ChunkArgs g
                 if (d < dk) S[t][r] = s[(size_t)d * dv];
             }
     }
-    const int chunks = (run.n + HQ_CHUNK - 1) / HQ_CHUNK;
-    const uint32_t row_bytes = (uint32_t)g.d.qk_stride * 2u;
-    const auto load = [&](int c) {
-        const int rows = min(HQ_CHUNK, run.n - c * HQ_CHUNK);
-        const size_t tok = (size_t)(run.tok0 + c * HQ_CHUNK);
-        const uint32_t range = (uint32_t)(rows - 1) * row_bytes + (uint32_t)dk * 2u;
-        const rsrc_t rk = make_rsrc(g.d.k + tok * g.d.qk_stride + hk * dk, range), rq = make_rsrc(g.d.q + tok * g.d.qk_stride + hk * dk, range);
-        const rsrc_t rw = make_rsrc(g.work + ((size_t)(run.chunk0 + c) * nv + h) * HQ_CHUNK_BYTES, (uint32_t)HQ_CHUNK_BYTES);
-        const uint32_t to = (uint32_t)(uintptr_t)buf[c % BUFS];
+    float bound = column_max(S);
+    int unit = exponent(bound) - 14;
+    {
+        const float to_unit = pow2(in_range(254 - unit));
 #pragma unroll
-        for (int i0 = 0; i0 < KB; i0 += NW) {
-            const int i = i0 + w, slot = 64 * i + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
-            if (KB % NW && i >= KB) break;
-            const uint32_t off = row < rows && 8 * x < dk ? (uint32_t)row * row_bytes + 16u * (uint32_t)x : NOWHERE;
-            dma16_untracked(rk, to + 1024u * (uint32_t)i, off);
-            dma16_untracked(rq, to + 1024u * (uint32_t)(KB + i), off);
-        }
-        for (int i = w; i < 19; i += NW) dma16_untracked(rw, to + 1024u * (uint32_t)(2 * KB + i), 1024u * (uint32_t)i + 16u * (uint32_t)lane);
-    };
-    const uint32_t v_bytes = (uint32_t)g.d.v_stride * 2u, o_bytes = (uint32_t)g.d.out_stride * 2u;
-    _Float16 V[16];
-    const auto load_v = [&](int c) {
-        const int rows = min(HQ_CHUNK, run.n - c * HQ_CHUNK);
-        const rsrc_t rv = make_rsrc(g.d.v + (size_t)(run.tok0 + c * HQ_CHUNK) * g.d.v_stride + (size_t)h * dv, (uint32_t)(rows - 1) * v_bytes + (uint32_t)dv * 2u);
+        for (int t = 0; t < 2 * KS; t++) S[t] = S[t] * to_unit;
+    }
+    const uint32_t o_bytes = (uint32_t)g.d.out_stride * 2u;
+    uint32_t o_off[16], k_in[KS], t_in[KS];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int row = token_of(i >> 2, 4 * q + (i & 3));
-            V[i] = __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(rv, row < rows ? (uint32_t)row * v_bytes + 2u * (uint32_t)col : NOWHERE, 0u, 0));
-        }
-    };
-    if (BUFS == 2) load(0);
-    if (on) load_v(0);
+    for (int i = 0; i < 16; i++) o_off[i] = (uint32_t)token_of(i >> 2, 4 * q + (i & 3)) * o_bytes + 2u * (uint32_t)col;
+    // what a lane reads of K and Q, of K transposed and of V, as offsets into a chunk's buffer
+#pragma unroll
+    for (int s = 0; s < KS; s++) k_in[s] = 16u * (uint32_t)piece_at<CPR>(token_of(0, n), 4 * s + q), t_in[s] = 16u * (uint32_t)piece_at<CPR>(8 * q + (n >> 2), 4 * s + (n & 3));
+    const uint32_t v_in = 1024u * AT_V + 16u * (uint32_t)(8 * q * VB + v_piece(8 * q, 2 * w + (n >> 3))) + 2u * (uint32_t)(n & 7);
+    const auto read16 = [](uint32_t at) { return __builtin_bit_cast(h8, *(lds_u4 *)(uintptr_t)at); };
     for (int c = 0; c < chunks; c++) {
-        if (BUFS == 1) {
-            __syncthreads();
-            load(c);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (BUFS == 1) __syncthreads();
         __syncthreads();
-        if (BUFS == 2 && c + 1 < chunks) load(c + 1);
         if (!on) continue;
-        const char *const b0 = buf[c % BUFS];
-        const u4v *const K = (const u4v *)b0, *const Q = K + 64 * KB, *const F = K + 128 * KB;
-        const float *const vec = (const float *)(F + 64 * FRAG_VEC);
-        const auto frag = [&](int i) { return __builtin_bit_cast(h8, F[64 * i + lane]); };
-        const int rows = min(HQ_CHUNK, run.n - c * HQ_CHUNK);
-        const uint32_t es = exponent(column_max(S));
+        const uint32_t base = buffer(c), f_at = base + 1024u * AT_F + 16u * (uint32_t)lane, vec_at = base + 1024u * AT_VEC + 32u * (uint32_t)q;
+        uint32_t k_at[KS], t_at[KS];
+#pragma unroll
+        for (int s = 0; s < KS; s++) k_at[s] = base + k_in[s], t_at[s] = base + t_in[s];
+        const auto rows4 = [&](int which, int b) { return __builtin_bit_cast(f4, read16(vec_at + 256u * (uint32_t)which + 4u * (uint32_t)token_of(b, 0))); };
+        const float keep = *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 63u), m_unit = *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 128u);
+        // Reads of LDS are issued a stage ahead of their use (STAGE: nothing moves past it), and what the outputs need is put between the
+        // steps of the state.
+        const auto read_rows = [&](int what, int s, h8(&x)[4]) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) x[b] = read16(k_at[s] + 1024u * KB * (uint32_t)what + 16u * CPR * (uint32_t)token_of(b, 0));
+        };
+        h8 K[KS][4], Q[KS][4];
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) read_rows(0, s, K[s]);
         h8 Sh[KS], Sl[KS];
 #pragma unroll
-        for (int s = 0; s < KS; s++) two_terms(S[2 * s], S[2 * s + 1], pow2(268u - es), Sh[s], Sl[s]);
-        const float back = pow2(es - 14u);
-        f4 X[4], O[4];
+        for (int s = 0; s < KS; s++) Sh[s] = halves(S[2 * s], S[2 * s + 1]), Sl[s] = second_term(S[2 * s], S[2 * s + 1], g.one, Sh[s]);
+        const float back = pow2(unit);
+        f4 X[4], O[4], eg[4];
+        _Float16 V[16];
+#pragma unroll
+        for (int b = 0; b < 4; b++) X[b] = O[b] = f4{0.f, 0.f, 0.f, 0.f};
+        STAGE;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            if (s + AHEAD < KS) read_rows(0, s + AHEAD, K[s + AHEAD]);
+            else read_rows(1, s + AHEAD - KS, Q[s + AHEAD - KS]);
+            if (s == KS - 1) {
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    eg[b] = rows4(0, b);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) V[4 * b + r] = *(lds_h *)(uintptr_t)(base + v_in + 16u * VB * (uint32_t)token_of(b, r));
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 4; b++) X[b] = mfma(K[s][b], Sl[s], X[b]);
+#pragma unroll
+            for (int b = 0; b < 4; b++) X[b] = mfma(K[s][b], Sh[s], X[b]);
+            MIX(8, 0x100, 3);
+            STAGE;
+        }
+#pragma unroll
+        for (int s = AHEAD; s < KS; s++) read_rows(1, s, Q[s]);
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            const int row = token_of(b, n);
-            f4 p = {0.f, 0.f, 0.f, 0.f}, o = p;
+            eg[b] = eg[b] * back;
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const h8 k = __builtin_bit_cast(h8, K[piece_at<CPR>(row, 4 * s + q)]);
-                p = mfma(k, Sh[s], p);
-                p = mfma(k, Sl[s], p);
-                o = mfma(__builtin_bit_cast(h8, Q[piece_at<CPR>(row, 4 * s + q)]), Sh[s], o);
-            }
-            const f4 eg = *(const f4 *)(vec + token_of(b, 4 * q)) * back;
-#pragma unroll
-            for (int r = 0; r < 4; r++) X[b][r] = (float)V[4 * b + r] - eg[r] * p[r];
-            O[b] = eg * o;
+            for (int r = 0; r < 4; r++) X[b][r] = fmaf(-eg[b][r], X[b][r], (float)V[4 * b + r]);
         }
-        if (c + 1 < chunks) load_v(c + 1);
-        const uint32_t ex = exponent(column_max(X));
+        MIX(4 * AHEAD, 2, 4);
+        STAGE;
+        h8 T[6], Tl[6];
+#pragma unroll
+        for (int i = 0; i < 6; i++) T[i] = read16(f_at + 1024u * (uint32_t)(FRAG_T + i)), Tl[i] = read16(f_at + 1024u * (uint32_t)(FRAG_T_LO + i));
+#pragma unroll
+        for (int s = AHEAD; s < KS; s++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+        const int ex = exponent(column_max(X));
         h8 Xh[2], Xl[2];
-        two_terms(X[0], X[1], pow2(268u - ex), Xh[0], Xl[0]);
-        two_terms(X[2], X[3], pow2(268u - ex), Xh[1], Xl[1]);
-        f4 U[4];
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            f4 u = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < 2; s++) Xh[s] = first_term(X[2 * s], X[2 * s + 1], pow2(268 - ex)), Xl[s] = second_term(X[2 * s], X[2 * s + 1], pow2(268 - ex), Xh[s]);
+        f4 U[4];  // in units of 2^(uu - 127)
+        const int uu = ex - 14 - T_BITS;
 #pragma unroll
-            for (int s = 0; s <= b / 2; s++) {
-                const h8 t = frag(FRAG_T + frag_of(b, s)), tl = frag(FRAG_T_LO + frag_of(b, s));
-                u = mfma(tl, Xh[s], u);
-                u = mfma(t, Xl[s], u);
-                u = mfma(t, Xh[s], u);
-            }
-            U[b] = u * (pow2(ex - 14u) / T_SCALE);
-        }
-        const uint32_t eu = exponent(column_max(U));
-        const float su = pow2(268u - eu), bu = pow2(eu - 14u);
+        for (int b = 0; b < 4; b++) U[b] = f4{0.f, 0.f, 0.f, 0.f};
+        MIX(4 * (KS - AHEAD), 2, 6);
+        STAGE;
+        // lane i of a group of 16 hands over 4 values of k_dim of row i / 4, and gets one of k_dim of 4 rows
+        s4v Kt[2][2 * KS][2];
+        const auto read_columns = [&](int s) {
+#pragma unroll
+            for (int t = 0; t < 2 * KS; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    Kt[s][t][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(uintptr_t)(t_at[t >> 1] + 8u * (uint32_t)(t & 1) + 16u * CPR * (uint32_t)(32 * s + 4 * e)));
+        };
+        const auto column = [&](int s, int t) { return __builtin_bit_cast(h8, __builtin_shufflevector(Kt[s][t][0], Kt[s][t][1], 0, 1, 2, 3, 4, 5, 6, 7)); };
+        f4 dec[4];
+#pragma unroll
+        for (int b = 0; b < 4; b++) dec[b] = rows4(1, b);
+        read_columns(0);
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+#pragma unroll
+                for (int b = 2 * s; b < 4; b++) U[b] = mfma(i == 0 ? Tl[frag_of(b, s)] : T[frag_of(b, s)], i == 1 ? Xl[s] : Xh[s], U[b]);
+        MIX(18, 0x100, 1);
+        STAGE;
+        h8 M[6];
+#pragma unroll
+        for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i));
+        read_columns(1);
+        const float mu = column_max(U);
+        bound = fmaf(bound, keep, 64.f * mu * pow2(in_range(uu)));
+        const int next = exponent(bound) - 14;
+        const float sd = pow2(in_range(uu - next + 127)), ratio = keep * pow2(in_range(unit - next + 127));
+        unit = next;
         h8 Uh[2], Dh[2], Dl[2];
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            h8 unused;
-            two_terms(U[2 * s], U[2 * s + 1], su, Uh[s], unused);
-            two_terms(U[2 * s] * *(const f4 *)(vec + 64 + token_of(2 * s, 4 * q)), U[2 * s + 1] * *(const f4 *)(vec + 64 + token_of(2 * s + 1, 4 * q)), su, Dh[s], Dl[s]);
+            const f4 x = U[2 * s] * sd, y = U[2 * s + 1] * sd, xd = x * dec[2 * s], yd = y * dec[2 * s + 1];
+            Uh[s] = halves(x, y);
+            Dh[s] = halves(xd, yd), Dl[s] = second_term(xd, yd, g.one, Dh[s]);
         }
-        const rsrc_t ro = make_rsrc(g.d.out + (size_t)(run.tok0 + c * HQ_CHUNK) * g.d.out_stride + (size_t)h * dv, (uint32_t)(rows - 1) * o_bytes + (uint32_t)dv * 2u);
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            f4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 2 * KS; t++) S[t] = S[t] * ratio;
+        STAGE;
+        f4 y[4];
 #pragma unroll
-            for (int s = 0; s <= b / 2; s++) o = mfma(frag(FRAG_M + frag_of(b, s)), Uh[s], o);
-            const f4 m = *(const f4 *)(vec + 128 + token_of(b, 4 * q)) * bu;
+        for (int b = 0; b < 4; b++) y[b] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int row = token_of(b, 4 * q + r);
-                const _Float16 y = (_Float16)(g.d.scale * fmaf(m[r], o[r], O[b][r]));
-                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, y), ro, row < rows ? (uint32_t)row * o_bytes + 2u * (uint32_t)col : NOWHERE, 0u, 0);
-            }
-        }
-        const float keep = vec[192];
-        const uint32_t k0 = (uint32_t)(uintptr_t)b0;
+        for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(0, t), Dl[0], S[t]);
 #pragma unroll
-        for (int t = 0; t < 2 * KS; t++) {
-            f4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(0, t), Dh[0], S[t]);
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                // lane i of a group of 16 hands over 4 values of k_dim of row i / 4, and gets one of k_dim of 4 rows
-                s4v x[2];
+        for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int row = 32 * s + 8 * q + (n >> 2) + 4 * e;
-                    x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(uintptr_t)(k0 + 16u * (uint32_t)piece_at<CPR>(row, 4 * (t >> 1) + (n & 3)) + 8u * (uint32_t)(t & 1)));
-                }
-                const h8 k = __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                a = mfma(k, Dl[s], a);
-                a = mfma(k, Dh[s], a);
-            }
+            for (int b = 2 * s; b < 4; b++) y[b] = mfma(M[frag_of(b, s)], Uh[s], y[b]);
+        MIX(4 * KS, 2, 2);
+        STAGE;
+        const float bu = pow2(next) * m_unit;
+        const rsrc_t ro = make_rsrc(g.d.out + (size_t)(run.tok0 + c * HQ_CHUNK) * g.d.out_stride + (size_t)h * dv, (rows_of(c) - 1u) * o_bytes + (uint32_t)dv * 2u);
 #pragma unroll
-            for (int r = 0; r < 4; r++) S[t][r] = fmaf(bu, a[r], keep * S[t][r]);
-        }
+        for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dl[1], S[t]);
+#pragma unroll
+        for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dh[1], S[t]);
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)fmaf(bu, y[b][r], eg[b][r] * g.d.scale * O[b][r])), ro, o_off[4 * b + r], 0u, 0);
+        MIX(4 * KS, 2, 3);
+        if ((c & 15) == 15) bound = column_max(S) * pow2(unit);
     }
     if (on && run.to != -1) {
         float *s = (run.to >= 0 ? g.st.s + ((size_t)run.to * nv + h) * size : g.carry + ((size_t)(-2 - run.to) * nv + h) * size) + col;
@@ -523,47 +652,59 @@ __global__ void __launch_bounds__(64 * (W < 4 ? 4 : W)) k_delta_scan(ChunkArgs g
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int d = 32 * (t >> 1) + 8 * q + r + 4 * (t & 1);
-                if (d < dk) s[(size_t)d * dv] = S[t][r];
+                if (d < dk) s[(size_t)d * dv] = S[t][r] * pow2(unit);
             }
     }
 }
 
 // The outputs' norm and gate of chunks, in place: G lanes a head, eight columns a lane. (The outputs have been rounded to fp16 by
 // then, 2^-11 of each beside the rounding of the result.)
-template <int G>
+// Bound: bytes.
+template <int G, bool F32>
 __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
     const int nv = g.st.n_v_heads, dv = g.st.v_dim, u = threadIdx.x % G;
+    const bool on = 8 * u < dv;
     const HqChunk ch = g.chunks[blockIdx.x];
-    for (int i = blockIdx.y * (256 / G) + threadIdx.x / G; i < ch.n * nv; i += gridDim.y * (256 / G)) {
-        const int t = i / nv, h = i - t * nv;
-        const bool on = 8 * u < dv;
-        const size_t tok = (size_t)(ch.tok0 + t), in = (size_t)h * dv + (on ? 8 * u : 0);
-        _Float16 *const at = (_Float16 *)g.d.out + tok * g.d.out_stride + in;
-        const h8 x = *(const h8 *)at;
-        float ss = 0.f;
+    f4 wa = {0.f, 0.f, 0.f, 0.f}, wb = wa;
+    if (on) wa = *(const f4 *)(g.d.norm + 8 * u), wb = *(const f4 *)(g.d.norm + 8 * u + 4);
+    for (int h = threadIdx.x / G; h < nv; h += 256 / G) {
+        const size_t in = (size_t)h * dv + (on ? 8 * u : 0);
+        for (int t = blockIdx.y; t < ch.n; t += gridDim.y) {
+            const size_t tok = (size_t)(ch.tok0 + t), zat = tok * g.d.gate_stride + in;
+            _Float16 *const at = (_Float16 *)g.d.out + tok * g.d.out_stride + in;
+            const h8 x = *(const h8 *)at;
+            float z[8];
+            if (F32) {
+                const f4 a = *(const f4 *)((const float *)g.d.gate + zat), b = *(const f4 *)((const float *)g.d.gate + zat + 4);
 #pragma unroll
-        for (int e = 0; e < 8; e++) ss = fmaf((float)x[e], (float)x[e], ss);
-        if (!on) ss = 0.f;
+                for (int e = 0; e < 4; e++) z[e] = a[e], z[4 + e] = b[e];
+            } else {
+                const h8 a = *(const h8 *)((const _Float16 *)g.d.gate + zat);
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
-        const size_t zat = tok * g.d.gate_stride + in;
-        h8 y;
+                for (int e = 0; e < 8; e++) z[e] = (float)a[e];
+            }
+            float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float z = g.d.gate_f32 ? ((const float *)g.d.gate)[zat + e] : (float)((const _Float16 *)g.d.gate)[zat + e];
-            y[e] = (_Float16)((float)x[e] * inv * g.d.norm[(on ? 8 * u : 0) + e] * (z / (1.0f + expf(-z))));
+            for (int e = 0; e < 8; e++) ss = fmaf((float)x[e], (float)x[e], ss);
+            if (!on) ss = 0.f;
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
+            h8 y;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = (_Float16)((float)x[e] * inv * (e < 4 ? wa[e & 3] : wb[e & 3]) * silu(z[e]));
+            if (on) *(h8 *)at = y;
         }
-        if (on) *(h8 *)at = y;
     }
 }
 
 template <int KS>
-void launch_chunks(const ChunkArgs &g, int n_chunks, hipStream_t s) {
-    k_delta_prep<KS><<<(unsigned)n_chunks * (unsigned)g.st.n_k_heads, 256, 0, s>>>(g);
+void launch_chunks(const ChunkArgs &g, hipStream_t s) {
+    k_delta_prep<KS><<<((unsigned)g.n_chunks * (unsigned)g.st.n_k_heads + 7) / 8 * 8 * (unsigned)(g.st.n_v_heads / g.st.n_k_heads), 256, 0, s>>>(g);
     const unsigned heads = ((unsigned)g.n_runs * (unsigned)g.st.n_v_heads + 7) / 8 * 8;
     const auto grid = [&](int W) { return heads * (unsigned)((g.st.v_dim + 16 * W - 1) / (16 * W)); };
-    k_delta_scan<KS, 4><<<grid(4), 256, 0, s>>>(g);
+    constexpr int W = KS == 8 ? 2 : 4;
+    k_delta_scan<KS, W><<<grid(W), 64 * (W + 4), 0, s>>>(g);
 }
 
 }  // namespace
@@ -585,6 +726,10 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
         const int64_t most = (int64_t)1 << 40;
         for (int64_t s : {d->qk_stride, d->v_stride, d->out_stride, d->norm ? d->gate_stride : 0})
             if (s < 0 || s > most || s % 8) return hq_internal_fail("%s: stride %lld (a multiple of 8)", who, (long long)s);
+        const int64_t k_row = (int64_t)st->n_k_heads * st->k_dim, v_row = (int64_t)st->n_v_heads * st->v_dim;
+        if (d->qk_stride < k_row || d->v_stride < v_row || d->out_stride < v_row)
+            return hq_internal_fail("%s: strides %lld, %lld and %lld of tokens whose heads take %lld, %lld and %lld", who, (long long)d->qk_stride, (long long)d->v_stride,
+                                    (long long)d->out_stride, (long long)k_row, (long long)v_row, (long long)v_row);
         // a chunk's rows are addressed by 32 bits
         if (!c->passes.empty())
             for (int64_t s : {d->qk_stride, d->v_stride, d->out_stride})
@@ -596,16 +741,22 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     if (cur != c->device) SCK(hipSetDevice(c->device));
     hipStream_t s = (hipStream_t)stream;
     for (const HqPass &p : c->passes) {
-        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, c->runs + p.run0, p.n_runs, c->work, (float *)(c->work + c->carry_at)};
-        if (st->k_dim <= 64) launch_chunks<2>(g, p.n_chunks, s);
-        else if (st->k_dim <= 128) launch_chunks<4>(g, p.n_chunks, s);
-        else launch_chunks<8>(g, p.n_chunks, s);
+        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, c->runs + p.run0, p.n_runs, p.n_chunks, c->work, (float *)(c->work + c->carry_at), 1.0f};
+        if (st->k_dim <= 64) launch_chunks<2>(g, s);
+        else if (st->k_dim <= 128) launch_chunks<4>(g, s);
+        else launch_chunks<8>(g, s);
         if (d->norm) {
             const int lanes = st->v_dim <= 64 ? 8 : st->v_dim <= 128 ? 16 : 32;
-            const dim3 grid((unsigned)p.n_chunks, (unsigned)std::max(1, std::min(32, HQ_CHUNK * st->n_v_heads * lanes / 1024)));
-            if (lanes == 8) k_delta_norm<8><<<grid, 256, 0, s>>>(g);
-            else if (lanes == 16) k_delta_norm<16><<<grid, 256, 0, s>>>(g);
-            else k_delta_norm<32><<<grid, 256, 0, s>>>(g);
+            const dim3 grid((unsigned)p.n_chunks, 16);
+#define HQ_NORM(G)                                                          \
+    do {                                                                    \
+        if (d->gate_f32) k_delta_norm<G, true><<<grid, 256, 0, s>>>(g);     \
+        else k_delta_norm<G, false><<<grid, 256, 0, s>>>(g);                \
+    } while (0)
+            if (lanes == 8) HQ_NORM(8);
+            else if (lanes == 16) HQ_NORM(16);
+            else HQ_NORM(32);
+#undef HQ_NORM
         }
         SCK(hipGetLastError());
     }

@@ -175,7 +175,8 @@ int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_delta_in_t 
 
 typedef struct {
     /* fp16: head h of token t at q and k + t * qk_stride + h * k_dim, v + t * v_stride + h * v_dim; 16-byte aligned, strides
-     * multiples of 8 (these and out_stride at most 2^22 where a sequence has more than 16 new tokens) */
+     * multiples of 8, those and out_stride no less than the heads of a token (and at most 2^22 where a sequence has more than 16
+     * new tokens) */
     const uint16_t *q, *k, *v;
     int64_t qk_stride, v_stride;
     const float *decay, *beta; /* [tokens, n_v_heads]; decay: a logarithm, 0 or less, -inf allowed */
