@@ -23,120 +23,146 @@ struct DeltaArgs {
     const int *steps;
 };
 
-DEV f4 sum_over(f4 x, int lanes) {
-    return f4{x[0] + __shfl_xor(x[0], lanes, 64), x[1] + __shfl_xor(x[1], lanes, 64), x[2] + __shfl_xor(x[2], lanes, 64), x[3] + __shfl_xor(x[3], lanes, 64)};
+// The sum of x over the lane groups of eight: all lanes have it. (Elements are bit-cast from plain scalars.)
+DEV float sum_groups(float x) {
+    const uint32_t v = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    const float y = __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
+    const uint32_t w = __builtin_bit_cast(uint32_t, y);
+    const auto b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    const float z = __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
+    return z + __shfl_xor(z, 8, 64);
 }
 
-// Token by token. A workgroup holds one head's S in registers, 16 rows x 4 columns a lane: column group tid % CG, row group tid / CG.
-// With p = S^T k and r = S^T q of the state before the token, formed together, a token costs one meeting of the waves:
+// Token by token. A wave holds 32 columns of a head's S in registers, a lane four of them and an eighth of the rows: no wave waits for
+// another within a token. With p = S^T k and r = S^T q of the state before the token, formed together:
 //   u = beta (v - e^g p),  o = scale (e^g r + (k q) u),  S' = e^g S + k u.
-template <int CG>
-__global__ void __launch_bounds__(16 * CG) k_delta_step(DeltaArgs g) {
-    constexpr int TB = 8, WAVES = 16 * CG / 64, RED = 8 * CG + 4;
-    __shared__ alignas(16) float in[TB][2 * 256 + 4 * CG];  // k, q, v of tokens
-    __shared__ alignas(16) float red[2][WAVES][RED];
-    const int nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim;
+// What tokens bring besides lies in LDS for eight of them; the outputs' norm, for which a head's waves meet, follows for eight together.
+// Bound: the bytes of the states. 64 sequences of one token, 32 heads of 128: 268 MB in 53 us; more tokens: some 330 instructions each.
+// FULL: dk = 8 ROWS (less otherwise).
+template <int ROWS, bool FULL>
+__global__ void __launch_bounds__(512, ROWS <= 16 ? 4 : 2) k_delta_step(DeltaArgs g) {
+    constexpr int TB = 8;
+    __shared__ alignas(16) _Float16 in[TB][2][8 * ROWS];  // k and q, each lane group's rows in ROWS places
+    __shared__ alignas(16) _Float16 in_v[TB][256];
+    __shared__ alignas(16) float z[TB][256], o[TB][256];  // gates and outputs
+    __shared__ float keep[TB], beta[TB];
+    const int nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim, rows = FULL ? ROWS : dk / 8;
     const HqSeq seq = g.seqs[g.steps[blockIdx.x / nv]];
     const int h = blockIdx.x % nv, hk = h / (nv / g.st.n_k_heads);
-    const int tid = threadIdx.x, nt = blockDim.x, w = tid >> 6, lane = tid & 63, waves = nt >> 6;
-    const int cg = tid % CG, rg = tid / CG;
-    const bool col = 4 * cg < dv, on = col && 16 * rg < dk;
-    f4 S[16];
-    const size_t size = (size_t)dk * dv;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, cl = lane & 7, rg = lane >> 3;
+    const int col = 32 * (int)(blockIdx.y * (nt >> 6) + (tid >> 6)) + 4 * cl;
+    const bool on = col < dv;
+    const size_t size = (size_t)dk * dv, at = (size_t)(rg * rows) * dv + col;
+    f4 S[ROWS];
 #pragma unroll
-    for (int i = 0; i < 16; i++) S[i] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < ROWS; i++) S[i] = f4{0.f, 0.f, 0.f, 0.f};
     if (seq.from >= 0 && on) {
-        const float *s = g.st.s + ((size_t)seq.from * nv + h) * size + (size_t)(16 * rg) * dv + 4 * cg;
+        const float *s = g.st.s + ((size_t)seq.from * nv + h) * size + at;
 #pragma unroll
-        for (int i = 0; i < 16; i++) S[i] = *(const f4 *)(s + (size_t)i * dv);
+        for (int i = 0; i < ROWS; i++)
+            if (i < rows) S[i] = *(const f4 *)(s + (size_t)i * dv);
     }
-    int buf = 0;
     for (int t0 = 0; t0 < seq.n; t0 += TB) {
-        const int m = min(TB, seq.n - t0), pieces = (2 * dk + dv) / 8;
+        const int m = min(TB, seq.n - t0), pk = dk / 8, pv = dv / 8;
+        const size_t tok0 = (size_t)(seq.tok0 + t0);
         __syncthreads();
-        for (int i = tid; i < m * pieces; i += nt) {
-            const int t = i / pieces, e = 8 * (i - t * pieces);
-            const size_t tok = (size_t)(seq.tok0 + t0 + t);
-            const uint16_t *src = e < dk ? g.d.k + tok * g.d.qk_stride + hk * dk + e
-                                  : e < 2 * dk ? g.d.q + tok * g.d.qk_stride + hk * dk + (e - dk)
-                                               : g.d.v + tok * g.d.v_stride + h * dv + (e - 2 * dk);
-            float *to = in[t] + (e < dk ? e : e < 2 * dk ? 256 + e - dk : 512 + e - 2 * dk);
-            const h8 x = *(const h8 *)src;
+        // pieces of eight values: k and q, v, gates
+        for (int i = tid; i < m * (2 * pk + 2 * pv); i += nt) {
+            const int t = i / (2 * pk + 2 * pv), e = i - t * (2 * pk + 2 * pv);
+            const size_t tok = tok0 + t;
+            if (e < 2 * pk) {
+                const int which = e >= pk, d = 8 * (e - which * pk);
+                const h8 x = *(const h8 *)((which ? g.d.q : g.d.k) + tok * g.d.qk_stride + hk * dk + d);
+                if (FULL) *(h8 *)(in[t][which] + d) = x;
+                else
 #pragma unroll
-            for (int j = 0; j < 8; j++) to[j] = (float)x[j];
+                    for (int j = 0; j < 8; j++) in[t][which][(d + j) / rows * ROWS + (d + j) % rows] = x[j];
+            } else if (e < 2 * pk + pv) {
+                const int d = 8 * (e - 2 * pk);
+                *(h8 *)(in_v[t] + d) = *(const h8 *)(g.d.v + tok * g.d.v_stride + h * dv + d);
+            } else if (g.d.norm) {
+                const int d = 8 * (e - 2 * pk - pv);
+                const size_t from = tok * g.d.gate_stride + (size_t)h * dv + d;
+                if (g.d.gate_f32) *(f4 *)(z[t] + d) = *(const f4 *)((const float *)g.d.gate + from), *(f4 *)(z[t] + d + 4) = *(const f4 *)((const float *)g.d.gate + from + 4);
+                else {
+                    const h8 x = *(const h8 *)((const _Float16 *)g.d.gate + from);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) z[t][d + j] = (float)x[j];
+                }
+            }
         }
+        if (tid < m) keep[tid] = expf(g.d.decay[(tok0 + tid) * nv + h]), beta[tid] = g.d.beta[(tok0 + tid) * nv + h];
         __syncthreads();
         for (int t = 0; t < m; t++) {
-            const size_t tok = (size_t)(seq.tok0 + t0 + t);
-            const float keep = expf(g.d.decay[tok * nv + h]), beta = g.d.beta[tok * nv + h];
-            f4 k[4], p = {0.f, 0.f, 0.f, 0.f}, r = p;
+            const float kp = keep[t], bt = beta[t];
+            h8 k[ROWS / 8];
+            f4 p = {0.f, 0.f, 0.f, 0.f}, r = p;
             float kq = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                k[i] = f4{0.f, 0.f, 0.f, 0.f};
-                f4 q = k[i];
-                if (16 * rg < dk) k[i] = *(const f4 *)(in[t] + 16 * rg + 4 * i), q = *(const f4 *)(in[t] + 256 + 16 * rg + 4 * i);
+            for (int i = 0; i < ROWS / 8; i++) {
+                k[i] = *(const h8 *)(in[t][0] + rg * ROWS + 8 * i);
+                const h8 q = *(const h8 *)(in[t][1] + rg * ROWS + 8 * i);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const f4 s = S[4 * i + j];
+                for (int j = 0; j < 8; j++) {
+                    const int row = 8 * i + j;
+                    if (row >= rows) continue;  // (places behind the rows hold anything)
+                    const float a = (float)k[i][j], b = (float)q[j];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = fmaf(s[e], k[i][j], p[e]), r[e] = fmaf(s[e], q[j], r[e]);
-                    kq = fmaf(k[i][j], q[j], kq);
+                    for (int e = 0; e < 4; e++) p[e] = fmaf(S[row][e], a, p[e]), r[e] = fmaf(S[row][e], b, r[e]);
+                    kq = fmaf(a, b, kq);
                 }
             }
 #pragma unroll
-            for (int o = CG; o < 64; o *= 2) p = sum_over(p, o), r = sum_over(r, o), kq += __shfl_xor(kq, o, 64);
-            if (lane < CG) {
-                *(f4 *)(red[buf][w] + 4 * cg) = p;
-                *(f4 *)(red[buf][w] + 4 * CG + 4 * cg) = r;
-                if (cg == 0) red[buf][w][8 * CG] = kq;
-            }
-            __syncthreads();
-            p = r = f4{0.f, 0.f, 0.f, 0.f}, kq = 0.f;
-            for (int i = 0; i < waves; i++) {
-                p += *(const f4 *)(red[buf][i] + 4 * cg);
-                r += *(const f4 *)(red[buf][i] + 4 * CG + 4 * cg);
-                kq += red[buf][i][8 * CG];
-            }
-            buf ^= 1;
-            f4 u = {0.f, 0.f, 0.f, 0.f}, o = u;
-            if (col) {
-                const f4 v = *(const f4 *)(in[t] + 512 + 4 * cg);
+            for (int e = 0; e < 4; e++) p[e] = sum_groups(p[e]), r[e] = sum_groups(r[e]);
+            kq = sum_groups(kq);
+            f4 u = {0.f, 0.f, 0.f, 0.f}, y = u;
+            if (on) {
+                const h4 v = *(const h4 *)(in_v[t] + col);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    u[e] = beta * (v[e] - keep * p[e]);
-                    o[e] = g.d.scale * (keep * r[e] + kq * u[e]);
+                    u[e] = bt * ((float)v[e] - kp * p[e]);
+                    y[e] = g.d.scale * (kp * r[e] + kq * u[e]);
                 }
             }
-            if (on) {
 #pragma unroll
-                for (int i = 0; i < 16; i++)
+            for (int i = 0; i < ROWS; i++)
+                if (i < rows) {
+                    const float a = (float)k[i / 8][i % 8];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) S[i][e] = fmaf(k[i / 4][i % 4], u[e], keep * S[i][e]);
-            }
-            if (rg == 0) {
-                if (g.d.norm) {
-                    float ss = col ? o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3] : 0.f;
-#pragma unroll
-                    for (int i = CG / 2; i > 0; i >>= 1) ss += __shfl_xor(ss, i, 64);
-                    const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
-                    if (col) {
-                        const size_t at = tok * g.d.gate_stride + (size_t)h * dv + 4 * cg;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float z = g.d.gate_f32 ? ((const float *)g.d.gate)[at + e] : (float)((const _Float16 *)g.d.gate)[at + e];
-                            o[e] = o[e] * inv * g.d.norm[4 * cg + e] * silu(z);
-                        }
-                    }
+                    for (int e = 0; e < 4; e++) S[i][e] = fmaf(a, u[e], kp * S[i][e]);
                 }
-                if (col) *(h4 *)((_Float16 *)g.d.out + tok * g.d.out_stride + (size_t)h * dv + 4 * cg) = h4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+            if (rg == 0 && on) {
+                if (g.d.norm) *(f4 *)(o[t] + col) = y;
+                else *(h4 *)((_Float16 *)g.d.out + (tok0 + t) * g.d.out_stride + (size_t)h * dv + col) = h4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
             }
+        }
+        if (!g.d.norm) continue;
+        // a wave a token
+        __syncthreads();
+        for (int t = tid >> 6; t < m; t += nt >> 6) {
+            const int d = 4 * lane;
+            f4 y = {0.f, 0.f, 0.f, 0.f};
+            if (d < dv) y = *(const f4 *)(o[t] + d);
+            float ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
+#pragma unroll
+            for (int i = 32; i > 0; i >>= 1) ss += __shfl_xor(ss, i, 64);
+            const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
+            if (d >= dv) continue;
+            const f4 zz = *(const f4 *)(z[t] + d), nw = *(const f4 *)(g.d.norm + d);
+            h4 w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = (_Float16)(y[e] * inv * nw[e] * silu(zz[e]));
+            *(h4 *)((_Float16 *)g.d.out + (tok0 + t) * g.d.out_stride + (size_t)h * dv + d) = w;
         }
     }
     if (seq.to >= 0 && on) {
-        float *s = g.st.s + ((size_t)seq.to * nv + h) * size + (size_t)(16 * rg) * dv + 4 * cg;
+        float *s = g.st.s + ((size_t)seq.to * nv + h) * size + at;
 #pragma unroll
-        for (int i = 0; i < 16; i++) *(f4 *)(s + (size_t)i * dv) = S[i];
+        for (int i = 0; i < ROWS; i++)
+            if (i < rows) *(f4 *)(s + (size_t)i * dv) = S[i];
     }
 }
 
@@ -170,6 +196,7 @@ DEV int piece_at(int row, int c) {
     return row * CPR + (c ^ ((CPR >= 16 ? (row & 3) << 2 : (row & 2) << 1) | mid));
 }
 
+typedef float f2 __attribute__((ext_vector_type(2)));
 DEV float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)e << 23); }
 // A largest magnitude's exponent: its 2^14 .. 2^15 is reached by pow2(268 - e), and left by pow2(e - 14).
 DEV int exponent(float largest) {
@@ -192,44 +219,56 @@ struct ChunkArgs {
 // T and M of a chunk and value head. Wave w forms rows 16 w .. of K K^T and Q K^T, then inverts the 16 x 16 block (w, w) of I + A by
 // substitution, a column a lane, and last computes block column w of the inverse from the top down, T_ij = -T_ii sum_l A_il T_lj, on
 // the fp32 matrix cores: each block of the column is the next one's operand.
+// e^(G_i - G_j) of a block left of the diagonal is a factor of the row, from the block's first row, times one of the column, to it:
+// neither exceeds 1. Sums of logarithms are formed in 64 bits and held as a multiple of 2^-9 and a rest, so that their differences
+// lose nothing; below -150 a decay is 0 in 32 bits.
 template <int KS>
 __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g) {
     constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS, LD = 72, LA = 68, LT = 20;
     __shared__ union {
         u4v kq[2][64 * CPR];
         struct {
-            _Float16 f[3][64 * LD];  // T, its second term, M
-            float At[64 * LA];       // A transposed
+            uint32_t t[64 * LD];  // T: its two terms
+            _Float16 m[64 * LD];  // M
+            float At[64 * LA];    // A transposed
         };
     } sh;
     __shared__ alignas(16) float Td[4][16 * LT];
-    __shared__ double gam[4][64];  // (a copy a wave)
-    __shared__ float bet[4][64], ms[4];
+    __shared__ alignas(16) f2 gam[64];
+    __shared__ alignas(16) float bet[64], ms[4];
     // workgroup i runs on XCD i % 8: the value heads of a key head on one
     const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, rep = nv / nk;
     const int unit = blockIdx.x / (8 * rep) * 8 + blockIdx.x % 8;
     if (unit >= g.n_chunks * nk) return;
     const int at = unit / nk, hk = unit % nk, h = hk * rep + blockIdx.x / 8 % rep;
     const HqChunk ch = g.chunks[at];
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
-    const float gl = lane < ch.n ? g.d.decay[(size_t)(ch.tok0 + lane) * nv + h] : 0.f, bl = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
+    // (the waves' shares are unlike: turned from workgroup to workgroup, so that no SIMD has all the long ones)
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = (wave + (int)(blockIdx.x / 8)) & 3;
+    const int lane = tid & 63, n = lane & 15, q = lane >> 4;
+    {
+        const uint32_t row_bytes = (uint32_t)g.d.qk_stride * 2u, range = (uint32_t)(ch.n - 1) * row_bytes + (uint32_t)dk * 2u;
+        const rsrc_t rk = make_rsrc(g.d.k + (size_t)ch.tok0 * g.d.qk_stride + hk * dk, range), rq = make_rsrc(g.d.q + (size_t)ch.tok0 * g.d.qk_stride + hk * dk, range);
 #pragma unroll
-    for (int i0 = 0; i0 < 64 * CPR; i0 += 256) {
-        const int i = i0 + tid, row = i / CPR, c = i % CPR;
-        const size_t from = (size_t)(ch.tok0 + row) * g.d.qk_stride + hk * dk + 8 * c;
-        u4v k = {0, 0, 0, 0}, x = k;
-        if (row < ch.n && 8 * c < dk) k = *(const u4v *)(g.d.k + from), x = *(const u4v *)(g.d.q + from);
-        sh.kq[0][piece_at<CPR>(row, c)] = k, sh.kq[1][piece_at<CPR>(row, c)] = x;
+        for (int i = 0; i < CPR; i += 4) {
+            const int slot = 64 * (i + wave) + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
+            const uint32_t off = 8 * x < dk ? (uint32_t)row * row_bytes + 16u * (uint32_t)x : 0x80000000u, to = (uint32_t)(uintptr_t)sh.kq + 1024u * (uint32_t)(i + wave);
+            dma16_untracked(rk, to, off);
+            dma16_untracked(rq, to + 1024u * CPR, off);
+        }
     }
-    // sums of the decays' logarithms, to base 2
-    double sum = (double)(gl < -1e4f ? -1e4f : gl) * 1.4426950408889634074;
+    if (w == 0) {
+        const float gl = lane < ch.n ? g.d.decay[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
+        bet[lane] = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
+        double sum = (double)(gl < -150.f ? -150.f : gl) * 1.4426950408889634074;  // to base 2
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += y;
+        for (int o = 1; o < 64; o <<= 1) {
+            const double y = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += y;
+        }
+        const double top = rint(sum * 512.0) * (1.0 / 512.0);
+        gam[lane] = f2{(float)top, (float)(sum - top)};
     }
-    gam[w][lane] = sum;
-    bet[w][lane] = bl;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     f4 A[4], M[4];
 #pragma unroll
@@ -244,21 +283,35 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
         }
     }
     const int i0 = 16 * w + 4 * q;
-    float mx = 0.f;
+    const auto decay = [](f2 i, f2 j) { return __builtin_amdgcn_exp2f((i[0] - j[0]) + (i[1] - j[1])); };
+    f2 gi[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) gi[r] = gam[i0 + r];
+    const f2 first = gam[16 * w];
+    const f4 beta = *(const f4 *)(bet + i0);
+    float mx = 0.f, row[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) row[r] = decay(gi[r], first);
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < 4; b++) {
         if (b > w) continue;
-        const int j = 16 * b + n;
-        const double gj = gam[w][j];
+        const f2 gj = gam[16 * b + n];
+        if (b < w) {
+            const float col = decay(first, gj);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const float x = j <= i0 + r ? __builtin_amdgcn_exp2f((float)(gam[w][i0 + r] - gj)) : 0.f;
-            A[b][r] = j < i0 + r ? bet[w][i0 + r] * x * A[b][r] : 0.f;
-            M[b][r] = j <= i0 + r ? x * M[b][r] : 0.f;
-            mx = fmaxf(mx, fabsf(M[b][r]));
+            for (int r = 0; r < 4; r++) A[b][r] = beta[r] * row[r] * (col * A[b][r]), M[b][r] = row[r] * (col * M[b][r]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float x = decay(gi[r], gj);  // (above the diagonal anything)
+                A[b][r] = n < 4 * q + r ? beta[r] * x * A[b][r] : 0.f;
+                M[b][r] = n <= 4 * q + r ? x * M[b][r] : 0.f;
+            }
         }
-        *(f4 *)(sh.At + j * LA + i0) = A[b];
+        mx = fmaxf(fmaxf(mx, fabsf(M[b][0])), fabsf(M[b][1]));
+        mx = fmaxf(fmaxf(mx, fabsf(M[b][2])), fabsf(M[b][3]));
+        *(f4 *)(sh.At + (16 * b + n) * LA + i0) = A[b];
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
@@ -304,36 +357,44 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
         for (int r = 0; r < 4; r++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(t[r], y[r], z, 0, 0, 0);
         T[i] = -z;
     }
-    const float scale = T_SCALE * bet[w][16 * w + n];
+    const float scale = T_SCALE * bet[16 * w + n];
+    const int em = exponent(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
+    const float to_m = pow2(268 - em);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if (i < (w & ~1)) continue;  // (above the diagonal: the half of a fragment that is zero)
+        if (i >= (w & ~1)) {  // (above the diagonal: the half of a fragment that is zero)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const float v = T[i][r] * scale;
-            const _Float16 hi = (_Float16)v;
-            const int o = (16 * i + 4 * q + r) * LD + 16 * w + n;
-            sh.f[0][o] = hi;
-            sh.f[1][o] = (_Float16)(v - (float)hi);
+            for (int r = 0; r < 4; r++) {
+                const float v = T[i][r] * scale;
+                sh.t[(16 * i + 4 * q + r) * LD + 16 * w + n] = __builtin_bit_cast(uint32_t, h2{(_Float16)v, (_Float16)(v - (float)(_Float16)v)});
+            }
+        }
+        if (i <= (w | 1)) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) sh.m[(i0 + r) * LD + 16 * i + n] = (_Float16)(M[i][r] * to_m);
         }
     }
-    const int em = exponent(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
-#pragma unroll
-    for (int b = 0; b < 4; b++) {
-        if (b > (w | 1)) continue;
-#pragma unroll
-        for (int r = 0; r < 4; r++) sh.f[2][(i0 + r) * LD + 16 * b + n] = (_Float16)(M[b][r] * pow2(268 - em));
-    }
     __syncthreads();
-    char *const to = g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES;
-    for (int p = w; p < 18; p += 4) {
-        const int k = p % 6, b = k < 2 ? k : k / 2 + 1, s = k < 2 ? 0 : k & 1;
-        *(u4v *)(to + p * 1024 + lane * 16) = *(const u4v *)(sh.f[p / 6] + token_of(b, n) * LD + 32 * s + 8 * q);
+    char *const to = g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES + lane * 16;
+#pragma unroll
+    for (int p0 = 0; p0 < 12; p0 += 4) {
+        const int p = p0 + wave, k = p % 6, b = k < 2 ? k : k / 2 + 1, s = k < 2 ? 0 : k & 1;
+        if (p < 6) {
+            const u4v *const x = (const u4v *)(sh.t + token_of(b, n) * LD + 32 * s + 8 * q);
+            const u4v u = x[0], v = x[1];
+            // (the terms of neighbouring values lie side by side)
+            *(u4v *)(to + (FRAG_T + k) * 1024) = u4v{__builtin_amdgcn_perm(u.y, u.x, 0x05040100u), __builtin_amdgcn_perm(u.w, u.z, 0x05040100u),
+                                                     __builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x05040100u)};
+            *(u4v *)(to + (FRAG_T_LO + k) * 1024) = u4v{__builtin_amdgcn_perm(u.y, u.x, 0x07060302u), __builtin_amdgcn_perm(u.w, u.z, 0x07060302u),
+                                                        __builtin_amdgcn_perm(v.y, v.x, 0x07060302u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u)};
+        } else {
+            *(u4v *)(to + (FRAG_M + k) * 1024) = *(const u4v *)(sh.m + token_of(b, n) * LD + 32 * s + 8 * q);
+        }
     }
-    if (w == 3) {
-        float *const v = (float *)(to + FRAG_VEC * 1024);
-        v[lane] = __builtin_amdgcn_exp2f((float)gam[3][lane]);
-        v[64 + lane] = __builtin_amdgcn_exp2f((float)(gam[3][63] - gam[3][lane]));
+    if (wave == 3) {
+        float *const v = (float *)(g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES + FRAG_VEC * 1024);
+        v[lane] = decay(gam[lane], f2{0.f, 0.f});
+        v[64 + lane] = decay(gam[63], gam[lane]);
         if (lane == 0) v[128] = g.d.scale * pow2(em - 14);
     }
 }
@@ -762,12 +823,17 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     }
     if (c->n_steps == 0) return 0;
     const DeltaArgs g = {*st, *d, c->seqs, c->steps};
-    const int rows = st->k_dim / 16;
-    const unsigned grid = (unsigned)c->n_steps * (unsigned)st->n_v_heads;
-    const auto threads = [&](int cg) { return (unsigned)std::max(64, (cg * rows + 63) / 64 * 64); };
-    if (st->v_dim <= 64) k_delta_step<16><<<grid, threads(16), 0, s>>>(g);
-    else if (st->v_dim <= 128) k_delta_step<32><<<grid, threads(32), 0, s>>>(g);
-    else k_delta_step<64><<<grid, threads(64), 0, s>>>(g);
+    // a head's waves in one workgroup; few heads without a norm, for which they would have to meet, a wave each
+    const int waves = (st->v_dim + 31) / 32, heads = c->n_steps * st->n_v_heads;
+    const bool apart = !d->norm && heads * waves <= 2 * c->n_cu;
+    const dim3 grid((unsigned)heads, apart ? (unsigned)waves : 1u);
+    const unsigned threads = apart ? 64u : 64u * (unsigned)waves;
+    if (st->k_dim == 64) k_delta_step<8, true><<<grid, threads, 0, s>>>(g);
+    else if (st->k_dim < 64) k_delta_step<8, false><<<grid, threads, 0, s>>>(g);
+    else if (st->k_dim == 128) k_delta_step<16, true><<<grid, threads, 0, s>>>(g);
+    else if (st->k_dim < 128) k_delta_step<16, false><<<grid, threads, 0, s>>>(g);
+    else if (st->k_dim == 256) k_delta_step<32, true><<<grid, threads, 0, s>>>(g);
+    else k_delta_step<32, false><<<grid, threads, 0, s>>>(g);
     SCK(hipGetLastError());
     return 0;
 }
