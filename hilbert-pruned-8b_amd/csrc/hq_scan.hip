@@ -237,19 +237,21 @@ DEV f8 load8(const void *p, size_t at) {
 template <bool F32>
 DEV float load1(const void *p, size_t at) { return F32 ? ((const float *)p)[at] : (float)((const _Float16 *)p)[at]; }
 
+DEV float silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }  // 2^-22 of itself
+
 // A workgroup takes the heads (of queries, keys, values: one sequence of them) 256 / G blockIdx.y .. of a tile's tokens, G lanes a
-// head, eight channels a lane. A lane holds a window of its channels' last inputs, so that each input is read once for a tile and
-// taps - 1 times more at its border. The tile with a sequence's first token reads the slot's inputs and afterwards writes those
-// that the sequence leaves: the same lane the same channels, so one slot may be both.
-// TAPS: conv_taps or more; taps beyond it have no input and no weight.
-template <bool F32, int G, int TAPS>
+// head, eight channels a lane; the last blockIdx.y the tile's gates. A lane holds a window of its channels' last inputs, so that each
+// input is read once for a tile and taps - 1 times more at its border, four tokens ahead of its use. The tile with a sequence's first
+// token reads the slot's inputs and writes those that the sequence leaves: the same lane the same channels, so one slot may be both.
+// TAPS: conv_taps, or with EXACT false more: taps beyond it have no input and no weight.
+template <bool F32, int G, int TAPS, bool EXACT>
 __global__ void __launch_bounds__(256) k_delta_append(AppendArgs g) {
     const HqTile tile = g.tiles[blockIdx.x];
     const HqSeq seq = g.seqs[tile.seq];
-    const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim, taps = g.st.conv_taps;
+    const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim, taps = EXACT ? TAPS : g.st.conv_taps;
     const size_t channels = 2 * (size_t)nk * dk + (size_t)nv * dv;
     const int tok0 = seq.tok0 + tile.t0;
-    if (blockIdx.y == 0)
+    if (blockIdx.y == gridDim.y - 1) {
         for (int i = threadIdx.x; i < tile.n * nv; i += 256) {
             const int t = i / nv, h = i - t * nv;
             const size_t at = (size_t)(tok0 + t) * g.r.ab_stride + h, o = (size_t)(tok0 + t) * nv + h;
@@ -257,67 +259,93 @@ __global__ void __launch_bounds__(256) k_delta_append(AppendArgs g) {
             g.r.decay[o] = -expf(g.r.a_log[h]) * (fmaxf(y, 0.f) + log1pf(expf(-fabsf(y))));
             g.r.beta[o] = 1.0f / (1.0f + expf(-load1<F32>(g.r.b, at)));
         }
-    const int u = threadIdx.x % G;
-    for (int j = blockIdx.y * (256 / G) + threadIdx.x / G; j < 2 * nk + nv; j += gridDim.y * (256 / G)) {
-        const bool is_v = j >= 2 * nk;
-        const bool on = 8 * u < (is_v ? dv : dk);
-        const size_t ch = (is_v ? 2 * (size_t)nk * dk + (size_t)(j - 2 * nk) * dv : (size_t)j * dk) + (on ? 8 * u : 0);
-        f8 w[TAPS], x[TAPS];  // of the inputs TAPS - 1 .. 0 tokens back
+        return;
+    }
+    const int u = threadIdx.x % G, j = blockIdx.y * (256 / G) + threadIdx.x / G;
+    if (j >= 2 * nk + nv) return;  // (of whole lane groups)
+    const bool is_v = j >= 2 * nk;
+    const bool on = 8 * u < (is_v ? dv : dk);
+    const size_t ch = (is_v ? 2 * (size_t)nk * dk + (size_t)(j - 2 * nk) * dv : (size_t)j * dk) + (on ? 8 * u : 0);
+    // the input of token t of the sequence
+    const auto input = [&](int t) {
+        if (t >= 0) return load8<F32>(g.r.x, (size_t)(seq.tok0 + t) * g.r.x_stride + ch);
+        if (seq.from >= 0) return load8<true>(g.st.conv, ((size_t)seq.from * (taps - 1) + (taps - 1 + t)) * channels + ch);
+        return f8{};
+    };
+    f8 x[TAPS - 1 + HQ_CONV_TILE];  // from TAPS - 1 tokens before the tile on
+    f8 w[TAPS];                     // of the inputs TAPS - 1 .. 0 tokens back
 #pragma unroll
-        for (int i = 0; i < TAPS; i++) {
-            const int tap = i - (TAPS - taps);
+    for (int i = 0; i < TAPS - 1; i++) {
+        x[i] = f8{};
+        if (i >= TAPS - taps) x[i] = input(tile.t0 - (TAPS - 1) + i);
+    }
+    constexpr int AHEAD = 4;
+    const auto fetch = [&](int t) {
+        if (t < tile.n) x[TAPS - 1 + t] = load8<F32>(g.r.x, (size_t)(tok0 + t) * g.r.x_stride + ch);
+    };
 #pragma unroll
-            for (int e = 0; e < 8; e++) w[i][e] = tap >= 0 ? g.r.conv_w[(ch + e) * taps + tap] : 0.f;
-            // the input at token t0 - (TAPS - 1) + i of the sequence
-            const int t = tile.t0 - (TAPS - 1) + i;
-            x[i] = f8{};
-            if (i < TAPS - 1 && tap >= 0) {
-                if (t >= 0) x[i] = load8<F32>(g.r.x, (size_t)(seq.tok0 + t) * g.r.x_stride + ch);
-                else if (seq.from >= 0) x[i] = load8<true>(g.st.conv, ((size_t)seq.from * (taps - 1) + (taps - 1 + t)) * channels + ch);
+    for (int t = 0; t < AHEAD; t++) fetch(t);
+    if (EXACT && TAPS % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int i = 0; i < TAPS; i += 4) {
+                const f4 v = *(const f4 *)(g.r.conv_w + (ch + e) * TAPS + i);
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (i + r < TAPS) w[i + r][e] = v[r];
             }
+    } else {
+#pragma unroll
+        for (int i = 0; i < TAPS; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[i][e] = i >= TAPS - taps ? g.r.conv_w[(ch + e) * taps + i - (TAPS - taps)] : 0.f;
+    }
+    const auto keep = [&](int r, f8 v) {
+        f4 *o = (f4 *)(g.st.conv + ((size_t)seq.to * (taps - 1) + r) * channels + ch);
+        o[0] = f4{v[0], v[1], v[2], v[3]};
+        o[1] = f4{v[4], v[5], v[6], v[7]};
+    };
+    const bool leaves = tile.t0 == 0 && seq.to >= 0 && on;
+    if (leaves && tile.n < seq.n) {
+        // the sequence goes on behind the tile: its last taps - 1 inputs are its last tokens' (a tile holds as many)
+#pragma unroll
+        for (int r = 0; r < TAPS - 1; r++)
+            if (r < taps - 1) keep(r, input(seq.n - (taps - 1) + r));
+    }
+#pragma unroll
+    for (int t = 0; t < HQ_CONV_TILE; t++) {
+        if (t >= tile.n) break;
+        fetch(t + AHEAD < HQ_CONV_TILE ? t + AHEAD : HQ_CONV_TILE);
+        f8 y;
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < TAPS; i++) s = fmaf(w[i][e], x[t + i][e], s);
+            y[e] = silu(s);
+            ss = fmaf(y[e], y[e], ss);
         }
-        if (tile.t0 == 0 && seq.to >= 0 && on) {
-            // the last taps - 1 of the old inputs and the new ones
-            f8 keep[TAPS];
-#pragma unroll
-            for (int i = 0; i < TAPS - 1; i++) {
-                const int r = i - (TAPS - taps), t = seq.n - (taps - 1) + r;  // row r is token t
-                if (r < 0) continue;
-                keep[i] = f8{};
-                if (t >= 0) keep[i] = load8<F32>(g.r.x, (size_t)(seq.tok0 + t) * g.r.x_stride + ch);
-                else if (seq.from >= 0) keep[i] = load8<true>(g.st.conv, ((size_t)seq.from * (taps - 1) + (taps - 1 + t)) * channels + ch);
-            }
-#pragma unroll
-            for (int i = 0; i < TAPS - 1; i++) {
-                const int r = i - (TAPS - taps);
-                if (r < 0) continue;
-                f4 *o = (f4 *)(g.st.conv + ((size_t)seq.to * (taps - 1) + r) * channels + ch);
-                o[0] = f4{keep[i][0], keep[i][1], keep[i][2], keep[i][3]};
-                o[1] = f4{keep[i][4], keep[i][5], keep[i][6], keep[i][7]};
-            }
-        }
-        for (int t = 0; t < tile.n; t++) {
-            x[TAPS - 1] = load8<F32>(g.r.x, (size_t)(tok0 + t) * g.r.x_stride + ch);
-            f8 y;
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float s = 0.f;
-#pragma unroll
-                for (int i = 0; i < TAPS; i++) s = fmaf(w[i][e], x[i][e], s);
-                y[e] = s / (1.0f + expf(-s));
-                ss = fmaf(y[e], y[e], ss);
-            }
-            if (!on) ss = 0.f;
+        if (!on) ss = 0.f;
+        if (!is_v) {  // (not the same for all lanes of a wave, but for those that exchange)
 #pragma unroll
             for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const float inv = is_v ? 1.0f : 1.0f / sqrtf(ss + g.r.eps);
-            h8 o;
+        }
+        const float inv = is_v ? 1.0f : 1.0f / sqrtf(ss + g.r.eps);
+        h8 o;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = (_Float16)(y[e] * inv);
-            if (on) *(h8 *)((_Float16 *)g.r.qkv + (size_t)(tok0 + t) * channels + ch) = o;
+        for (int e = 0; e < 8; e++) o[e] = (_Float16)(y[e] * inv);
+        if (on) *(h8 *)((_Float16 *)g.r.qkv + (size_t)(tok0 + t) * channels + ch) = o;
+    }
+    if (leaves && tile.n == seq.n) {
+        // the last taps - 1 of the old inputs and the new ones
 #pragma unroll
-            for (int i = 0; i < TAPS - 1; i++) x[i] = x[i + 1];
+        for (int n = 0; n <= HQ_CONV_TILE; n++) {
+            if (n != tile.n) continue;
+#pragma unroll
+            for (int r = 0; r < TAPS - 1; r++)
+                if (r >= TAPS - taps) keep(r - (TAPS - taps), x[n + r]);
         }
     }
 }
@@ -347,13 +375,13 @@ extern "C" int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_
     const AppendArgs g = {*st, *r, c->seqs, c->tiles};
     const int widest = std::max(st->k_dim, st->v_dim), lanes = widest <= 64 ? 8 : widest <= 128 ? 16 : 32, per = 256 / lanes;
     const int heads = 2 * st->n_k_heads + st->n_v_heads;
-    const dim3 grid((unsigned)c->n_tiles, (unsigned)((heads + per - 1) / per));
+    const dim3 grid((unsigned)c->n_tiles, (unsigned)((heads + per - 1) / per) + 1u);
     hipStream_t s = (hipStream_t)stream;
-#define HQ_APPEND_T(F, G, N) k_delta_append<F, G, N><<<grid, 256, 0, s>>>(g)
-#define HQ_APPEND_G(F, G)                      \
-    do {                                       \
-        if (st->conv_taps <= 4) HQ_APPEND_T(F, G, 4); \
-        else HQ_APPEND_T(F, G, 8);             \
+#define HQ_APPEND_G(F, G)                                                            \
+    do {                                                                             \
+        if (st->conv_taps == 4) k_delta_append<F, G, 4, true><<<grid, 256, 0, s>>>(g); \
+        else if (st->conv_taps < 4) k_delta_append<F, G, 4, false><<<grid, 256, 0, s>>>(g); \
+        else k_delta_append<F, G, 8, false><<<grid, 256, 0, s>>>(g);                 \
     } while (0)
 #define HQ_APPEND(F)                       \
     do {                                   \
@@ -365,7 +393,6 @@ extern "C" int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_
     else HQ_APPEND(false);
 #undef HQ_APPEND
 #undef HQ_APPEND_G
-#undef HQ_APPEND_T
     SCK(hipGetLastError());
     return 0;
 }
