@@ -378,8 +378,14 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs g) {
 // is the number of candidates before it, found in every other row by bisection (a row's values fall along its list).
 //
 // Values of unlike rows are compared, and a beam's tokens are a choice that cannot be taken back, so the sum of a row is kept to
-// about 2^-23 of itself: the exponentials' arguments as a product and its remainder, eight of them to a 32-bit sum, those to a
-// 64-bit one; a value is formed in 64 bits. Equal logits of one row compare equal whatever the sum.
+// about 2^-22 of itself: eight exponentials to a 32-bit sum, those to a 64-bit one, an exponent within 2^-22; a value is formed in
+// 64 bits. Equal logits of one row compare equal whatever the sum. Threads, waves and parts join by their common maximum first, one
+// exponential each, then by sums of what is left: pair by pair, with two exponentials a step, it was 2.5 us more of a chain of 19 steps.
+//
+// Bound: the bytes of the logits where rows are many: 64 groups of 8 of 151936, fp32 (311 MB), k 16: 69 us, of which the pass over
+// them is 55. 16 groups of 8, fp16 (39 MB): 21.6 us; the pass 14 with its launch, the second look 6, the merge 1.4 (as 64-bit values
+// in lists; as keys whose values are formed at each comparison 2.4, and with k 64 20 more). One group of 4 of 32000: 12.8 us, a chain of
+// launch, loads, two meetings of workgroups and the second look.
 struct BeamArgs {
     LpArgs lp;  // its k: places of a row, k or V
     int k;
@@ -396,7 +402,7 @@ struct BeamArgs {
 };
 enum { BEAM_ROW, BEAM_NONE, BEAM_DONE, BEAM_ODD };  // a row with candidates; none; the one of a done beam; NaN or +inf somewhere
 
-// e^d for d <= 0 to about 2^-23 of itself, NaN for NaN
+// e^d for d <= 0 to about 2^-23 of itself, NaN for NaN: the exponent as a product and its remainder
 DEV float ex_sharp(float d) {
     constexpr float LOG2E_LO = 1.925963033500e-8f, LN2 = 0.69314718055994531f;  // log2 e = LOG2E + LOG2E_LO
     const float c = fmaxf(d, -1e4f), t = c * LOG2E, lo = fmaf(c, LOG2E_LO, fmaf(c, LOG2E, -t));
@@ -404,45 +410,93 @@ DEV float ex_sharp(float d) {
     return fmaf(e, lo * LN2, e);
 }
 
+// s e^m: the sum of the exponentials of some logits, m the largest
 struct BeamSum {
     float m;
     double s;
-    __device__ __forceinline__ void add(float om, double os) {
-        const float mn = fmaxf(m, om);
-        s = (m == -INFINITY ? s : s * (double)ex_sharp(m - mn)) + (om == -INFINITY ? os : os * (double)ex_sharp(om - mn));
-        m = mn;
+    // of N neighbouring lanes, in an order of its own that is the same in each
+    template <int N>
+    __device__ __forceinline__ void join() {
+        float n = m;
+#pragma unroll
+        for (int o = 1; o < N; o <<= 1) n = fmaxf(n, __shfl_xor(n, o, 64));
+        s = m == -INFINITY ? s : s * (double)ex_sharp(m - n);
+#pragma unroll
+        for (int o = 1; o < N; o <<= 1) s += __shfl_xor(s, o, 64);
+        m = n;
     }
 };
 
-struct BeamMerge {
-    unsigned long long key[HQ_BEAM_MAX * HQ_BEAM_MAX];
-    int rank[HQ_BEAM_MAX * HQ_BEAM_MAX];
-    double m[HQ_BEAM_MAX], logs[HQ_BEAM_MAX], score[HQ_BEAM_MAX];
-    int what[HQ_BEAM_MAX];
-    int odd, n;
-    // the value of place j of row b (k places each)
-    __device__ __forceinline__ double value(int b, int j, int k) const {
-        if (what[b] == BEAM_NONE || (what[b] == BEAM_DONE && j)) return -INFINITY;
-        if (what[b] == BEAM_DONE) return score[b];
-        const float x = from_order((uint32_t)(key[b * k + j] >> 32));
-        return x == -INFINITY ? -INFINITY : score[b] + (((double)x - m[b]) - logs[b]);
+// A thread's sum in the pass over a row: 2^(x log2 e - M) with one fused operation an exponent, M = m log2 e - 8 rounded (the same M in
+// every exponent, so that its rounding costs nothing; 8 less than the largest exponent, which puts the terms that count on both
+// sides of 0, where a rounding of the exponent is 2^-22 at most): with e^(x - m) itself, seven operations, 128 rows of 151936, fp16,
+// take 4 us more. Where M's rounding is no longer small or leaves fp32's range
+// (|m| of 2^17 or more: no finite fp16 logit, fp32 ones barred with the type's lowest value), e^(x - m).
+template <bool F32>
+struct BeamPass {
+    float m = -INFINITY, M = 0.f;
+    double s = 0.0;
+    static __device__ __forceinline__ bool far(float m) { return !(fabsf(m) < 0x1p17f); }
+    template <int U>
+    __device__ __forceinline__ void add(const float (&x)[U][VEC<F32>]) {
+        float n = m;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < VEC<F32>; e++) n = fmaxf(n, x[u][e]);
+        const bool wide = far(n);
+        if (n > m) {
+            const float N = fmaf(n, LOG2E, -8.f);
+            if (!wide && !far(m)) {
+                s *= (double)__builtin_amdgcn_exp2f(M - N);
+            } else if (m != -INFINITY) {
+                s = sum().s * (double)ex_sharp(m - n);
+                if (!wide) s *= (double)__builtin_amdgcn_exp2f(fmaf(n, LOG2E, -N));
+            }
+            m = n, M = N;
+        }
+        const float n0 = n == -INFINITY ? 0.f : n;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float p = 0.f;
+            if (!wide) {
+#pragma unroll
+                for (int e = 0; e < VEC<F32>; e++) p += __builtin_amdgcn_exp2f(fmaf(x[u][e], LOG2E, -M));
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC<F32>; e++) p += ex_sharp(x[u][e] - n0);
+            }
+            s += (double)p;
+        }
     }
+    __device__ __forceinline__ BeamSum sum() const { return {m, far(m) ? s : s * (double)__builtin_amdgcn_exp2f(fmaf(-m, LOG2E, M))}; }
 };
+
+// Lists of a group's k best candidates, best first: values as integers in their order (0: no candidate) and which of the group's
+// n_beams * k they are. Two at a time become one, whose places are found by bisection, half the lists from buffer to buffer.
+constexpr size_t beam_lists(int n_beams, int k) { return (size_t)(n_beams + (n_beams + 1) / 2) * k * 10; }
+DEV unsigned long long order_of(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v + 0.0);
+    return v == -INFINITY ? 0ull : b >> 63 ? ~b : b | 1ull << 63;
+}
+DEV float value_of(unsigned long long o) {
+    const unsigned long long b = o >> 63 ? o & ~(1ull << 63) : ~o;
+    return (float)__builtin_bit_cast(double, b);
+}
 
 template <bool F32>
 __global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
-    __shared__ union Both {
-        Shared sh;
-        BeamMerge merge;
-    } both;
+    extern __shared__ unsigned long long lds[];  // the row's Shared, then the group's lists
     __shared__ struct {
         float m[WAVES];
         double s[WAVES];
-        int last;
+        double logs[HQ_BEAM_MAX];  // of each row of the group: the logarithm of its sum
+        float big[HQ_BEAM_MAX], score[HQ_BEAM_MAX];
+        int what[HQ_BEAM_MAX], last, odd;
     } top;
     constexpr int U = 2;  // pieces in flight per thread
     const LpArgs &g = a.lp;
-    Shared &sh = both.sh;
+    Shared &sh = *(Shared *)lds;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, k = g.k;
     const size_t r = blockIdx.x / g.parts;
     const int part = blockIdx.x % g.parts;
@@ -458,6 +512,7 @@ __global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
         const uint32_t mis = (uint32_t)((uintptr_t)start & 15u) / (F32 ? 4 : 2);
         const Row<F32> row = {g, start - ((uintptr_t)start & 15u), mis, (mis + g.V + VEC<F32> - 1) / VEC<F32>};
         const uint32_t v0 = (uint32_t)part * g.per, v1 = std::min(v0 + g.per, row.n_pieces);
+        BeamPass<F32> pass;
         for (uint32_t v = v0 + tid; v < v1; v += U * NT) {
             float x[U][VEC<F32>];
 #pragma unroll
@@ -467,35 +522,18 @@ __global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
 #pragma unroll
                     for (int e = 0; e < VEC<F32>; e++) x[u][e] = -INFINITY;
             }
-            float mn = z.m;
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int e = 0; e < VEC<F32>; e++) mn = fmaxf(mn, x[u][e]);
-            if (mn > z.m) {
-                if (z.m != -INFINITY) z.s *= (double)ex_sharp(z.m - mn);
-                z.m = mn;
-            }
-            const float m0 = mn == -INFINITY ? 0.f : mn;
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float p = 0.f;
-#pragma unroll
-                for (int e = 0; e < VEC<F32>; e++) p += ex_sharp(x[u][e] - m0);
-                z.s += (double)p;
-            }
+            pass.add(x);
         }
+        z = pass.sum();
         const int per = NT / g.group;
         float mx = z.m;
         for (int o = 1; o < g.group; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
         const uint32_t big = order_of(mx);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) z.add(__shfl_xor(z.m, o, 64), __shfl_xor(z.s, o, 64));
+        z.join<64>();
         if (lane == 0) top.m[w] = z.m, top.s[w] = z.s;
         __syncthreads();
-        z = {top.m[0], top.s[0]};
-#pragma unroll
-        for (int i = 1; i < WAVES; i++) z.add(top.m[i], top.s[i]);
+        z = {top.m[lane % WAVES], top.s[lane % WAVES]};
+        z.join<WAVES>();
         if (g.parts > 1) {
             const uint32_t each = 4 + per;
             const rsrc_t rp = make_rsrc(g.work + r * (size_t)g.parts * each, (uint32_t)g.parts * each * 4u);
@@ -516,8 +554,7 @@ __global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
             z = {-INFINITY, 0.0};
             const uint32_t om = o.x;
             if (mine < g.parts) z = {__builtin_bit_cast(float, om), __builtin_bit_cast(double, (unsigned long long)o.z << 32 | o.y)};
-#pragma unroll
-            for (int i = 1; i < MAX_PARTS; i <<= 1) z.add(__shfl_xor(z.m, i, 64), __shfl_xor(z.s, i, 64));
+            z.join<MAX_PARTS>();
         } else if (tid % g.group == 0) {
             sh.bucket[tid / g.group] = big;
         }
@@ -547,61 +584,67 @@ __global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
     }
     __syncthreads();
     if (!top.last) return;
-    BeamMerge &m = both.merge;
-    const int B = a.n_beams;
+    const int B = a.n_beams, L = a.k;
+    unsigned long long *val = lds, *val2 = lds + B * L;
+    uint16_t *which = (uint16_t *)(val2 + (B + 1) / 2 * L), *which2 = which + B * L;
+    if (tid == 0) top.odd = 0;
+    __syncthreads();
     if (tid < B) {
         const u4v o = __builtin_bit_cast(u4v, buf_load16_sc1(rr, (uint32_t)tid * a.row_bytes, 0));
         const uint32_t om = o.x, kind = o.w;
-        m.m[tid] = (double)__builtin_bit_cast(float, om);
-        m.logs[tid] = log(__builtin_bit_cast(double, (unsigned long long)o.z << 32 | o.y));
-        m.score[tid] = (double)a.score[group * B + tid];
-        m.what[tid] = (int)kind;
-    }
-    if (tid == 0) m.odd = m.n = 0;
-    for (int i = tid; i < B * k; i += NT) {
-        const uint32_t at = (uint32_t)(i / k) * a.row_bytes + 16u + 8u * (uint32_t)(i % k);
-        const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b32(rr, at, 0u, CPOL_SC1), hi = __builtin_amdgcn_raw_buffer_load_b32(rr, at + 4u, 0u, CPOL_SC1);
-        m.key[i] = (unsigned long long)hi << 32 | lo;
-        m.rank[i] = 0;
+        top.big[tid] = __builtin_bit_cast(float, om);
+        top.logs[tid] = log(__builtin_bit_cast(double, (unsigned long long)o.z << 32 | o.y));
+        top.score[tid] = a.score[group * B + tid];
+        top.what[tid] = (int)kind;
+        if ((int)kind == BEAM_ODD) top.odd = 1;
     }
     __syncthreads();
-    if (tid < B && m.what[tid] == BEAM_ODD) m.odd = 1;
-    __syncthreads();
-    const size_t to = group * (size_t)a.k;
-    if (m.odd) {
-        for (int j = tid; j < a.k; j += NT) a.out_score[to + j] = NAN, a.out_token[to + j] = 0xffffffffu, a.out_beam[to + j] = -1;
+    const size_t to = group * (size_t)L;
+    if (top.odd) {
+        for (int j = tid; j < L; j += NT) a.out_score[to + j] = NAN, a.out_token[to + j] = 0xffffffffu, a.out_beam[to + j] = -1;
         return;
     }
-    // places before candidate (b, j): its own row's j, and of each other row those of a larger value, or of an equal one in a lower row
-    for (int i = tid; i < B * B * k; i += NT) {
-        const int c = i / B, b = c / k, j = c - b * k, other = i - c * B;
-        const double v = m.value(b, j, k);
-        if (v == -INFINITY) continue;
-        int n = j;
-        if (other != b) {
-            int lo = 0, hi = k;  // the first place of the other row that does not come before
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                const double y = m.value(other, mid, k);
-                if (y > v || (y == v && other < b)) lo = mid + 1;
-                else hi = mid;
-            }
-            n = lo;
+    for (int i = tid; i < B * L; i += NT) {
+        const int b = i / L, j = i - b * L, kind = top.what[b];
+        double v = -INFINITY;
+        if (kind == BEAM_DONE) {
+            if (j == 0) v = (double)top.score[b];
+        } else if (kind == BEAM_ROW && j < k) {
+            const float x = from_order(__builtin_amdgcn_raw_buffer_load_b32(rr, (uint32_t)b * a.row_bytes + 20u + 8u * (uint32_t)j, 0u, CPOL_SC1));
+            if (x != -INFINITY) v = (double)top.score[b] + (((double)x - (double)top.big[b]) - top.logs[b]);
         }
-        atomicAdd(&m.rank[c], n);
-        if (other == b) atomicAdd(&m.n, 1);
+        val[i] = order_of(v), which[i] = (uint16_t)i;
     }
     __syncthreads();
-    for (int c = tid; c < B * k; c += NT) {
-        const int b = c / k, j = c - b * k, at = m.rank[c];
-        const double v = m.value(b, j, k);
-        if (v == -INFINITY || at >= a.k) continue;
-        a.out_score[to + at] = (float)v;
-        a.out_token[to + at] = m.what[b] == BEAM_DONE ? a.done_token : ~(uint32_t)m.key[c];
-        a.out_beam[to + at] = b;
+    for (int n = B; n > 1; n = (n + 1) / 2) {
+        for (int i = tid; i < n * L; i += NT) {
+            const int l = i / L, j = i - l * L, other = l ^ 1;
+            const unsigned long long v = val[i];
+            int at = j;
+            if (other < n) {
+                const unsigned long long *const y = val + other * L, least = v + (l & 1 ? 0 : 1);  // those that come before: of a lower beam equal ones too
+                int lo = 0, hi = L;
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (y[mid] >= least) lo = mid + 1;
+                    else hi = mid;
+                }
+                at += lo;
+            }
+            if (at < L) val2[l / 2 * L + at] = v, which2[l / 2 * L + at] = which[i];
+        }
+        __syncthreads();
+        unsigned long long *const v = val;
+        uint16_t *const w = which;
+        val = val2, val2 = v, which = which2, which2 = w;
     }
-    for (int j = tid; j < a.k; j += NT)
-        if (j >= m.n) a.out_score[to + j] = -INFINITY, a.out_token[to + j] = 0xffffffffu, a.out_beam[to + j] = -1;
+    for (int j = tid; j < L; j += NT) {
+        const unsigned long long v = val[j];
+        const int b = v ? which[j] / L : -1;
+        uint32_t token = 0xffffffffu;
+        if (v) token = top.what[b] == BEAM_DONE ? a.done_token : ~__builtin_amdgcn_raw_buffer_load_b32(rr, (uint32_t)b * a.row_bytes + 16u + 8u * (uint32_t)(which[j] - b * L), 0u, CPOL_SC1);
+        a.out_score[to + j] = v ? value_of(v) : -INFINITY, a.out_token[to + j] = token, a.out_beam[to + j] = b;
+    }
 }
 
 __global__ void k_zero(int *p, int n) {
@@ -693,8 +736,9 @@ extern "C" int hq_beam(const void *logits, int f32, int n_groups, int n_beams, u
     a.rows = (char *)work, g.work = (float *)((char *)work + rows);
     a.group_counters = (int *)cnt, g.counters = (int *)cnt + n_groups;
     const unsigned grid = (unsigned)M * (unsigned)g.parts;
-    if (f32) k_beam<true><<<grid, NT, 0, (hipStream_t)stream>>>(a);
-    else k_beam<false><<<grid, NT, 0, (hipStream_t)stream>>>(a);
+    const size_t lds = std::max(sizeof(Shared), beam_lists(n_beams, k));
+    if (f32) k_beam<true><<<grid, NT, lds, (hipStream_t)stream>>>(a);
+    else k_beam<false><<<grid, NT, lds, (hipStream_t)stream>>>(a);
     SCK(hipGetLastError());
     return 0;
 }

@@ -140,3 +140,46 @@ def test_two_streams(hqlib):
             go(hqlib, *draw(rng, G, 4, V, True), 8, stream=st.ptr)
     for st in s:
         st.destroy()
+
+
+@pytest.mark.parametrize("G,B,V,k", [(1, 4, 3000, 8), (20, 3, 17000, 6)])
+def test_lowest_values(hqlib, G, B, V, k):
+    """fp32 rows barred with the type's lowest value, rows of nothing else (all tokens alike), and logits near either end of the type."""
+    print(f"[gpu] beam lowest values {G} x {B} of {V}", flush=True)
+    lowest = np.finfo(np.float32).min
+    x, score = draw(np.random.default_rng(V), G, B, V, True)
+    x[np.random.default_rng(V + 1).random(x.shape) < 0.7] = lowest
+    x[0, 1] = lowest                      # every token 1 / V
+    x[0, 2] = -np.inf
+    x[0, 2, ::3], score[0, 2] = lowest, -25  # every third token, and worth less than row 1's
+    score[0, 1] = -0.25
+    if G > 1:
+        x[1, 0, 5], x[1, 0, 6] = 3e38, 2.9e38  # one token has it all
+        x[2, 1, :] = np.where(np.arange(V) < V // 2, np.float32(-2.0 ** 100), np.float32(-2.0 ** 100 * (1 - 2.0 ** -24)))
+        score[2] = -30, -1, -40
+    go(hqlib, x, score, k)
+    y = np.full((1, 2, V), lowest, np.float32)
+    y[0, 1] = -np.inf
+    got = go(hqlib, y, np.array([[-0.5, -0.1]]), k)
+    assert got[1].tolist() == [list(range(k))] and (got[2] == 0).all() and np.allclose(got[0], -0.5 - np.log(V), rtol=0, atol=2.0 ** -20)
+
+
+def test_more_places_than_a_row_has(hqlib):
+    """Rows shorter than k: places come from several beams, and their number need not be a power of two."""
+    for B, V, k in ((3, 4, 11), (5, 2, 10), (64, 1, 64), (7, 9, 64)):
+        x, score = draw(np.random.default_rng(B), 2, B, V, True)
+        x += np.linspace(0, 2.0 ** -8, x.size, dtype=np.float32).reshape(x.shape)  # (no two alike)
+        go(hqlib, x, score, k)
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("at", [0.0, 60000.0, -60000.0, 131071.0, 131073.0, -131073.0, 1.5e6, -2.0e30])
+def test_where_logits_lie(hqlib, f32, at):
+    """Rows whose largest logits lie anywhere: near 0, at fp16's ends, and on both sides of 2^17, thread by thread."""
+    if not f32 and abs(at) > 65504:
+        at = np.sign(at) * 65000.0
+    rng = np.random.default_rng(int(abs(at) % 1000))
+    G, B, V, k = 2, 3, 40000, 4
+    x = (at + rng.integers(-64, 1, (G, B, V)) / 8.0).astype(np.float32 if f32 else np.float16)
+    x[:, 1, rng.random(V) < 0.5] = -6e4
+    go(hqlib, x, rng.uniform(-20, 0, (G, B)).astype(np.float32), k)
