@@ -929,7 +929,7 @@ int batch_init(hip_batch *s, HipBackend *b, int kv_type, int page_size, uint32_t
     for (const DevLayer &d : b->L) qkv_one |= d.qkv != nullptr, kv_apart |= !d.qkv, gu_apart |= !d.pair;
     if (alloc(&s->x, T * H * 4) || alloc(&s->qb, T * (qw + (qkv_one ? 2 * kvw : 0)) * 4) || alloc(&s->kb, kv_apart ? T * kvw * 4 : 0) ||
         alloc(&s->vb, kv_apart ? T * kvw * 4 : 0) || alloc(&s->gb, gu_apart ? T * I * 4 : 0) || alloc(&s->ub, gu_apart ? T * I * 4 : 0) ||
-        alloc(&s->q, T * ow * 2) || alloc(&s->hb, T * H * 2) || alloc(&s->ob, T * ow * 2) || alloc(&s->fb, T * I * 2) ||
+        alloc(&s->q, T * ow * 2) || alloc(&s->hb, std::max(T, (size_t)max_seqs) * H * 2) || alloc(&s->ob, T * ow * 2) || alloc(&s->fb, T * I * 2) ||
         alloc(&s->table, (size_t)s->n_table * c.rot_dim * 4) || alloc(&s->logits, (size_t)max_seqs * c.vocab * 4))
         return -1;
     return c.rot_dim ? hq_rope_table(b->m->rope_inv_freq, (int)c.rot_dim, s->n_table, s->table, b->st) : 0;
@@ -983,20 +983,38 @@ int batch_layers(hip_batch *s, int T) {
     return 0;
 }
 
-// The queued part of a step, from the copy of its host array (words of it) to the last output.
-int batch_run(hip_batch *s, size_t words, int T, int rows, int n_ids, int top_k, float *logp, float *entropy, uint32_t *top_ids, float *top_logp) {
+// The queued part of a step up to the last layer: words of the step's host array to the device, T tokens from there.
+int batch_run(hip_batch *s, size_t words, int T) {
     HipBackend *b = s->b;
-    const hq_ref_config_t &c = b->m->cfg;
     BCK(hipMemcpyAsync(s->d_in, s->h_in, words * 4, hipMemcpyHostToDevice, b->st));
+    if (!T) return 0;
     BCK(hq_launch_dequant(hq_mat_dev(b->embed), 0, s->d_in, (uint32_t)T, s->x, b->st));
-    if (batch_layers(s, T)) return -1;
-    if (n_ids || top_k || entropy) {
-        k_norm_rows<<<rows, 256, 0, b->st>>>(s->x, s->d_in + T, b->final_norm, c.norm_offset, c.eps, s->hb, (int)c.hidden);
-        BCK(hipGetLastError());
-        if (gemm(b, b->lm_head, s->hb, rows, s->logits, false)) return -1;
-        if (hq_logprobs(s->logits, 1, rows, c.vocab, c.vocab, n_ids ? s->d_in + T + rows : nullptr, n_ids, top_k, logp, entropy, top_ids, top_logp, b->st))
-            return -1;
+    return batch_layers(s, T);
+}
+
+// The logits behind `rows` of the step's tokens, which the array says behind the tokens.
+int batch_logits(hip_batch *s, int T, int rows) {
+    HipBackend *b = s->b;
+    k_norm_rows<<<rows, 256, 0, b->st>>>(s->x, s->d_in + T, b->final_norm, b->m->cfg.norm_offset, b->m->cfg.eps, s->hb, (int)b->m->cfg.hidden);
+    BCK(hipGetLastError());
+    return gemm(b, b->lm_head, s->hb, rows, s->logits, false);
+}
+
+// The new tokens of a step's sequences: how many, and how many sequences have some.
+int batch_tokens(const char *who, const hip_batch *s, int n_seqs, const uint32_t *tokens, const int32_t *n_new, const int32_t *n_pos, int64_t *n_tokens, int *rows) {
+    if (n_seqs < 0 || n_seqs > s->max_seqs) return hq_internal_fail("%s: %d sequences (the batch takes %d)", who, n_seqs, s->max_seqs);
+    if (n_seqs && (!n_new || !n_pos)) return hq_internal_fail("%s: null argument", who);
+    int64_t T = 0;
+    *rows = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        if (n_new[i] < 0 || n_new[i] > n_pos[i]) return hq_internal_fail("%s: sequence %d has %d new tokens of %d positions", who, i, n_new[i], n_pos[i]);
+        T += n_new[i], *rows += n_new[i] > 0;
     }
+    if (T > s->max_tokens) return hq_internal_fail("%s: %lld new tokens (the batch takes %d)", who, (long long)T, s->max_tokens);
+    if (T && !tokens) return hq_internal_fail("%s: null argument", who);
+    for (int64_t t = 0; t < T; t++)
+        if (tokens[t] >= s->b->m->cfg.vocab) return hq_internal_fail("%s: token %u out of range", who, tokens[t]);
+    *n_tokens = T;
     return 0;
 }
 
@@ -1046,23 +1064,14 @@ extern "C" int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, 
     if (!s) return hq_internal_fail("%s: null argument", who);
     HipBackend *b = s->b;
     const hq_ref_config_t &c = b->m->cfg;
-    if (n_seqs < 0 || n_seqs > s->max_seqs) return hq_internal_fail("%s: %d sequences (the batch takes %d)", who, n_seqs, s->max_seqs);
-    if (n_seqs && (!n_new || !n_pos)) return hq_internal_fail("%s: null argument", who);
     if (n_ids < 0 || n_ids > MAX_IDS || (n_ids && logp && !ids)) return hq_internal_fail("%s: %d ids (0 .. %d)", who, n_ids, MAX_IDS);
     if (top_k < 0 || top_k > HQ_LOGPROBS_MAX_TOP || (uint32_t)top_k > c.vocab)
         return hq_internal_fail("%s: top_k %d (0 .. %d, at most the vocabulary's %u)", who, top_k, HQ_LOGPROBS_MAX_TOP, c.vocab);
     if (!logp) n_ids = 0;
     if (!top_ids && !top_logp) top_k = 0;
-    int64_t T = 0;
-    int rows = 0;
-    for (int i = 0; i < n_seqs; i++) {
-        if (n_new[i] < 0 || n_new[i] > n_pos[i]) return hq_internal_fail("%s: sequence %d has %d new tokens of %d positions", who, i, n_new[i], n_pos[i]);
-        T += n_new[i], rows += n_new[i] > 0;
-    }
-    if (T > s->max_tokens) return hq_internal_fail("%s: %lld new tokens (the batch takes %d)", who, (long long)T, s->max_tokens);
-    if (T && !tokens) return hq_internal_fail("%s: null argument", who);
-    for (int64_t t = 0; t < T; t++)
-        if (tokens[t] >= c.vocab) return hq_internal_fail("%s: token %u out of range", who, tokens[t]);
+    int64_t T;
+    int rows;
+    if (batch_tokens(who, s, n_seqs, tokens, n_new, n_pos, &T, &rows)) return -1;
     for (size_t i = 0; i < (size_t)n_seqs * (size_t)n_ids; i++)
         if (ids[i] >= c.vocab) return hq_internal_fail("%s: id %u out of range", who, ids[i]);
     BCK(hipSetDevice(b->device));
@@ -1081,7 +1090,11 @@ extern "C" int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, 
     }
     float *const o_lp = (float *)s->h_out, *const o_en = o_lp + n_lp, *const o_top = o_en + rows;
     uint32_t *const o_ids = (uint32_t *)(o_top + n_top);
-    if (batch_run(s, (size_t)T + rows + n_lp, (int)T, rows, n_ids, top_k, n_ids ? o_lp : nullptr, entropy ? o_en : nullptr, top_ids ? o_ids : nullptr, top_logp ? o_top : nullptr)) {
+    if (!entropy && !n_ids && !top_k) rows = 0;
+    if (batch_run(s, (size_t)T + rows + n_lp, (int)T) ||
+        (rows && (batch_logits(s, (int)T, rows) ||
+                  hq_logprobs(s->logits, 1, rows, c.vocab, c.vocab, n_ids ? s->d_in + T + rows : nullptr, n_ids, top_k, n_ids ? o_lp : nullptr,
+                              entropy ? o_en : nullptr, top_ids ? o_ids : nullptr, top_logp ? o_top : nullptr, b->st)))) {
         // what was queued before the failure still reads h_in, which the next step rewrites
         (void)hipStreamSynchronize(b->st);
         return -1;
@@ -1095,6 +1108,66 @@ extern "C" int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, 
         if (top_k && top_logp) memcpy(top_logp + (size_t)i * top_k, o_top + (size_t)r * top_k, (size_t)top_k * 4);
         r++;
     }
+    return 0;
+}
+
+extern "C" int hip_batch_copy(hip_batch *s, const uint32_t *src, const uint32_t *dst, const int32_t *n_pos, int n) {
+    const char *const who = "hip_batch_copy";
+    if (!s) return hq_internal_fail("%s: null argument", who);
+    BCK(hipSetDevice(s->b->device));
+    try {
+        std::vector<hq_kv_t> kv(s->k.size(), s->kv);
+        for (size_t l = 0; l < kv.size(); l++) {
+            kv[l].k = s->k[l].first, kv[l].k_scale = (uint16_t *)s->k[l].second;
+            kv[l].v = s->v[l].first, kv[l].v_scale = (uint16_t *)s->v[l].second;
+        }
+        return hq_kv_copy(kv.data(), (int)kv.size(), src, dst, n_pos, n, s->b->st);
+    } catch (const std::exception &) {
+        return hq_internal_fail("%s: out of memory", who);
+    }
+}
+
+extern "C" int hip_batch_beam(hip_batch *s, int n_groups, int n_beams, const uint32_t *tokens, const int32_t *n_new, const int32_t *n_pos,
+                              const uint32_t *pages, int pages_ld, const float *score, const uint8_t *done, uint32_t done_token, int k,
+                              float *out_score, uint32_t *out_token, int32_t *out_beam) {
+    const char *const who = "hip_batch_beam";
+    if (!s) return hq_internal_fail("%s: null argument", who);
+    HipBackend *b = s->b;
+    const uint32_t V = b->m->cfg.vocab;
+    if (n_beams < 1 || n_beams > HQ_BEAM_MAX || n_groups < 0 || n_groups > s->max_seqs / n_beams)
+        return hq_internal_fail("%s: %d groups of %d beams (1 .. %d beams; the batch takes %d sequences)", who, n_groups, n_beams, HQ_BEAM_MAX, s->max_seqs);
+    if (k < 1 || k > HQ_BEAM_MAX) return hq_internal_fail("%s: k %d (1 .. %d)", who, k, HQ_BEAM_MAX);
+    const int n = n_groups * n_beams;
+    if (n && (!score || !out_score || !out_token || !out_beam)) return hq_internal_fail("%s: null argument", who);
+    int64_t T;
+    int rows;
+    if (batch_tokens(who, s, n, tokens, n_new, n_pos, &T, &rows)) return -1;
+    for (int i = 0; i < n; i++)
+        if (!n_new[i] && !(done && done[i]) && score[i] > -INFINITY)
+            return hq_internal_fail("%s: beam %d of group %d has no new tokens, but a score of %g", who, i % n_beams, i / n_beams, (double)score[i]);
+    BCK(hipSetDevice(b->device));
+    // in: tokens, then the row that each sequence's logits are of (any, where it has no new tokens: nothing reads them), scores, done
+    const size_t n_out = (size_t)n_groups * (size_t)k, words = (size_t)T + 2 * (size_t)n + ((size_t)n + 3) / 4;
+    if (batch_room(s, words + 4, (3 * n_out + 4) * 4)) return -1;
+    if (hq_batch_set(s->step, &s->kv, (int)b->m->cfg.n_heads, n, n_new, n_pos, pages, pages_ld, b->st)) return -1;
+    if (!n) return 0;
+    uint32_t *const last = s->h_in + T, *const in_score = last + n, *const in_done = in_score + n;
+    if (T) memcpy(s->h_in, tokens, (size_t)T * 4);
+    for (int64_t i = 0, t = 0; i < n; i++) t += n_new[i], last[i] = (uint32_t)(n_new[i] ? t - 1 : 0);
+    memcpy(in_score, score, (size_t)n * 4);
+    if (done) memcpy(in_done, done, (size_t)n);
+    else memset(in_done, 0, (size_t)n);
+    float *const o_score = (float *)s->h_out;
+    uint32_t *const o_token = (uint32_t *)(o_score + n_out);
+    int32_t *const o_beam = (int32_t *)(o_token + n_out);
+    uint32_t *const d = s->d_in + T + n;
+    if (batch_run(s, words, (int)T) || (T && batch_logits(s, (int)T, n)) ||
+        hq_beam(s->logits, 1, n_groups, n_beams, V, V, (const float *)d, (const uint8_t *)(d + n), done_token, k, o_score, o_token, o_beam, b->st)) {
+        (void)hipStreamSynchronize(b->st);  // (what was queued reads h_in)
+        return -1;
+    }
+    BCK(hipStreamSynchronize(b->st));
+    memcpy(out_score, o_score, n_out * 4), memcpy(out_token, o_token, n_out * 4), memcpy(out_beam, o_beam, n_out * 4);
     return 0;
 }
 

@@ -32,7 +32,7 @@ EXPORTS = (
     "hq_pages_fork", "hq_pages_compact", "hq_pages_copies", "hq_pages_table", "hq_pages_count", "hq_kv_copy", "hq_beam",
 )
 # include/hq_backend.h (no hq_ prefix: the names of the reference entry points they replace)
-BACKEND_EXPORTS = ("hip_backend_create", "hip_selftest", "hip_batch_create", "hip_batch_free", "hip_batch_step")
+BACKEND_EXPORTS = ("hip_backend_create", "hip_selftest", "hip_batch_create", "hip_batch_free", "hip_batch_step", "hip_batch_copy", "hip_batch_beam")
 
 
 class WMat(C.Structure):
@@ -226,6 +226,8 @@ def load(path=LIB_PATH):
         "hip_batch_create": (i, [C.POINTER(RefBackend), i, i, C.c_uint32, i, i, i, C.POINTER(vp)]),
         "hip_batch_free": (None, [vp]),
         "hip_batch_step": (i, [vp, i, vp, vp, vp, vp, i, vp, i, i, vp, vp, vp, vp]),
+        "hip_batch_copy": (i, [vp, vp, vp, vp, i]),
+        "hip_batch_beam": (i, [vp, i, i, vp, vp, vp, vp, i, vp, vp, u32, i, vp, vp, vp]),
         "hip_backend_create": (C.POINTER(RefBackend), [C.POINTER(RefModel), sz, i, C.c_bool]),
         "hip_selftest": (i, [C.POINTER(RefModel), i, sz, i]),
         "hq_gemm_workspace_bytes": (i, [i, i, u32, u32, i, C.POINTER(sz), C.POINTER(sz), C.POINTER(sz),
@@ -927,6 +929,32 @@ class HipBatch:
         _check(_lib.hip_batch_step(self.h, n, _ptr(tokens), _ptr(n_new), _ptr(n_pos), _ptr(pages), pages.shape[1], _ptr(ids), ids.shape[1],
                                    top_k, _ptr(logp), _ptr(entropy), _ptr(top_ids), _ptr(top_logp)))
         return logp, entropy, top_ids, top_logp
+
+    def copy(self, src, dst, n_pos=None):
+        """hip_batch_copy: pages src to pages dst (their first n_pos positions) in every layer."""
+        src, dst = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
+        n_pos = None if n_pos is None else np.ascontiguousarray(n_pos, np.int32)
+        if src.ndim != 1 or dst.shape != src.shape or (n_pos is not None and n_pos.shape != src.shape):
+            raise HQError(f"HipBatch.copy: src {src.shape}, dst {dst.shape}, n_pos {None if n_pos is None else n_pos.shape}")
+        _check(_lib.hip_batch_copy(self.h, _ptr(src), _ptr(dst), None if n_pos is None else _ptr(n_pos), len(src)))
+
+    def beam(self, tokens, n_new, n_pos, pages, score, k, done=None, done_token=0):
+        """hip_batch_beam: a step of the sequences [groups, beams] that score [groups, beams] belongs to. Returns (score, token, beam)
+        [groups, k]."""
+        tokens, pages = np.ascontiguousarray(tokens, np.uint32), np.ascontiguousarray(pages, np.uint32)
+        n_new, n_pos = np.ascontiguousarray(n_new, np.int32), np.ascontiguousarray(n_pos, np.int32)
+        score = np.ascontiguousarray(score, np.float32)
+        n = score.size
+        done = None if done is None else np.ascontiguousarray(done, np.uint8)
+        if (score.ndim != 2 or n_new.shape != (n,) or n_pos.shape != (n,) or pages.ndim != 2 or len(pages) != n or
+                tokens.shape != (int(n_new.sum()),) or (done is not None and done.shape != score.shape)):
+            raise HQError(f"HipBatch.beam: tokens {tokens.shape}, n_new {n_new.shape}, n_pos {n_pos.shape}, pages {pages.shape}, "
+                          f"score {score.shape}, done {None if done is None else done.shape}")
+        g = len(score)
+        out = np.empty((g, max(k, 0)), np.float32), np.empty((g, max(k, 0)), np.uint32), np.empty((g, max(k, 0)), np.int32)
+        _check(_lib.hip_batch_beam(self.h, g, score.shape[1], _ptr(tokens), _ptr(n_new), _ptr(n_pos), _ptr(pages), pages.shape[1], _ptr(score),
+                                   None if done is None else _ptr(done), done_token, k, *(_ptr(o) for o in out)))
+        return out
 
     def free(self):
         if self.h:

@@ -130,6 +130,18 @@ int hip_batch_step(hip_batch *s, int n_seqs, const uint32_t *tokens, const int32
                    const uint32_t *pages, int pages_ld, const uint32_t *ids, int n_ids, int top_k, float *logp, float *entropy,
                    uint32_t *top_ids, float *top_logp);
 
+/* hq_kv_copy in the caches of all layers: the first n_pos[i] positions (NULL: all) of page src[i] to page dst[i], for i of 0 .. n - 1
+ * (what hq_pages_copies gives). Queued: the batch's steps come behind it. */
+int hip_batch_copy(hip_batch *s, const uint32_t *src, const uint32_t *dst, const int32_t *n_pos, int n);
+
+/* One step of a beam search: as hip_batch_step for n_groups * n_beams sequences, beam j of group i being sequence i * n_beams + j,
+ * and from the logits of their last new tokens the k best continuations of each group, as hq_beam gives them (score, done, done_token
+ * and the outputs as there, but the host's). A beam without new tokens must be done or have a score of -inf. Synchronous. What the
+ * beams come from next is the caller's to say: hq_pages_fork and hip_batch_copy. */
+int hip_batch_beam(hip_batch *s, int n_groups, int n_beams, const uint32_t *tokens, const int32_t *n_new, const int32_t *n_pos,
+                   const uint32_t *pages, int pages_ld, const float *score, const uint8_t *done, uint32_t done_token, int k,
+                   float *out_score, uint32_t *out_token, int32_t *out_beam);
+
 #ifdef __cplusplus
 }
 #endif
