@@ -212,7 +212,7 @@ struct ChunkArgs {
     const HqRun *runs;
     int n_runs, n_chunks;
     char *work;
-    float *carry;
+    float *places;  // states of the workspace
     float one;  // 1: a factor that the compiler does not know, so that a difference is one fused instruction
 };
 
@@ -462,21 +462,28 @@ DEV float column_max(const f4 (&x)[N]) {
             __builtin_amdgcn_sched_group_barrier(what, M, 0);    \
         }                                                        \
     }
-template <int KS, int W>
+// OUT: outputs are formed. Without: a part's effect on states, Q from zeros or, from I and without values, P (a chunk takes some 1.8 us
+// either way: it is the way from state to state that bounds both).
+template <int KS, int W, bool OUT>
 __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
+    constexpr int LW = 4;  // waves that load
     constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS;
     constexpr int KB = CPR, VB = 2 * W;    // KB of a chunk's keys or queries (64 rows of CPR pieces of 16 bytes) and of its values
     constexpr int BUFS = KS <= 4 ? 2 : 1;  // (two chunks of wider keys do not fit: the next one's wait until this one is done)
     constexpr int AHEAD = 2;               // steps of K or Q that are read before their use
-    constexpr int AT_F = 2 * KB, AT_VEC = AT_F + FRAG_VEC, AT_V = AT_VEC + 1, SIZE = AT_V + VB;
-    static_assert(KB % 4 == 0, "whole rounds of loads");
+    constexpr int FRAGS = OUT ? FRAG_VEC : FRAG_M;
+    constexpr int AT_F = OUT ? 2 * KB : KB, AT_VEC = AT_F + FRAGS, AT_V = AT_VEC + 1, SIZE = AT_V + VB;
+    static_assert(KB % LW == 0, "whole rounds of loads");
     __shared__ alignas(1024) char lds[BUFS * SIZE * 1024];
     const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim;
-    const int groups = (dv + 16 * W - 1) / (16 * W);
+    const int groups = ((OUT ? dv : max(dk, dv)) + 16 * W - 1) / (16 * W);
     // workgroup i runs on XCD i % 8: the groups of one head on one, where they share its keys
     const int head = blockIdx.x / (8 * groups) * 8 + blockIdx.x % 8, group = blockIdx.x / 8 % groups;
     if (head >= g.n_runs * nv) return;
     const HqRun run = g.runs[head / nv];
+    const bool eye = !OUT && run.from == HQ_IDENTITY;
+    const int cols = eye ? dk : dv;
+    if (!OUT && group * 16 * W >= cols) return;
     const int h = head % nv, hk = h / (nv / nk);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
     const int chunks = (run.n + HQ_CHUNK - 1) / HQ_CHUNK;
@@ -488,33 +495,35 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
     if (w >= W) {
         const int lw = w - W;
         const uint32_t row_bytes = (uint32_t)g.d.qk_stride * 2u, v_bytes = (uint32_t)g.d.v_stride * 2u;
-        uint32_t k_off[KB / 4], v_off[(VB + 3) / 4];
+        uint32_t k_off[KB / LW], v_off[(VB + LW - 1) / LW];
 #pragma unroll
-        for (int i = 0; i < KB / 4; i++) {
-            const int slot = 64 * (4 * i + lw) + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
+        for (int i = 0; i < KB / LW; i++) {
+            const int slot = 64 * (LW * i + lw) + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
             k_off[i] = 8 * x < dk ? (uint32_t)row * row_bytes + 16u * (uint32_t)x : 0x80000000u;
         }
 #pragma unroll
-        for (int i = 0; i < (VB + 3) / 4; i++) {
-            const int slot = 64 * (4 * i + lw) + lane, row = slot / VB, x = 8 * (2 * W * group + v_piece(row, slot % VB));
+        for (int i = 0; i < (VB + LW - 1) / LW; i++) {
+            const int slot = 64 * (LW * i + lw) + lane, row = slot / VB, x = 8 * (2 * W * group + v_piece(row, slot % VB));
             v_off[i] = x < dv ? (uint32_t)row * v_bytes + 2u * (uint32_t)x : 0x80000000u;
         }
         const auto load = [&](int c) {
             const size_t tok = (size_t)(run.tok0 + c * HQ_CHUNK);
             const uint32_t range = (rows_of(c) - 1u) * row_bytes + (uint32_t)dk * 2u, to = buffer(c) + 1024u * (uint32_t)lw;
             const rsrc_t rk = make_rsrc(g.d.k + tok * g.d.qk_stride + hk * dk, range), rq = make_rsrc(g.d.q + tok * g.d.qk_stride + hk * dk, range);
-            const rsrc_t rv = make_rsrc(g.d.v + tok * g.d.v_stride + (size_t)h * dv, (rows_of(c) - 1u) * v_bytes + (uint32_t)dv * 2u);
+            const rsrc_t rv = make_rsrc(g.d.v + tok * g.d.v_stride + (size_t)h * dv, eye ? 0u : (rows_of(c) - 1u) * v_bytes + (uint32_t)dv * 2u);
             const rsrc_t rw = make_rsrc(g.work + ((size_t)(run.chunk0 + c) * nv + h) * HQ_CHUNK_BYTES, (uint32_t)HQ_CHUNK_BYTES);
 #pragma unroll
-            for (int i = 0; i < KB; i += 4) dma16_untracked(rk, to + 1024u * (uint32_t)i, k_off[i / 4]);
+            for (int i = 0; i < KB; i += LW) dma16_untracked(rk, to + 1024u * (uint32_t)i, k_off[i / LW]);
 #pragma unroll
-            for (int i = 0; i < VB; i += 4)
-                if (VB % 4 == 0 || i + lw < VB) dma16_untracked(rv, to + 1024u * (uint32_t)(AT_V + i), v_off[i / 4]);
+            for (int i = 0; i < VB; i += LW)
+                if (VB % LW == 0 || i + lw < VB) dma16_untracked(rv, to + 1024u * (uint32_t)(AT_V + i), v_off[i / LW]);
 #pragma unroll
-            for (int i = 0; i < 20; i += 4)
-                if (i < 16 || lw < 3) dma16_untracked(rw, to + 1024u * (uint32_t)(AT_F + i), 1024u * (uint32_t)(i + lw) + 16u * (uint32_t)lane);
+            for (int i = 0; i <= FRAGS; i += LW)
+                if (i + LW <= FRAGS + 1 || i + lw <= FRAGS)
+                    dma16_untracked(rw, to + 1024u * (uint32_t)(AT_F + i), 1024u * (uint32_t)(i + lw == FRAGS ? FRAG_VEC : i + lw) + 16u * (uint32_t)lane);
+            if (OUT)
 #pragma unroll
-            for (int i = 0; i < KB; i += 4) dma16_untracked(rq, to + 1024u * (uint32_t)(KB + i), k_off[i / 4]);
+                for (int i = 0; i < KB; i += LW) dma16_untracked(rq, to + 1024u * (uint32_t)(KB + i), k_off[i / LW]);
         };
         if (BUFS == 2) load(0);
         for (int c = 0; c < chunks; c++) {
@@ -529,13 +538,18 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         return;
     }
     const int col = 16 * (group * W + w) + n;
-    const bool on = 16 * (group * W + w) < dv;  // (of a wave as a whole)
-    const size_t size = (size_t)dk * dv;
+    const bool on = 16 * (group * W + w) < cols;  // (of a wave as a whole)
+    const size_t size = (size_t)dk * dv, place = (size_t)dk * max(dk, dv);
     f4 S[2 * KS];
 #pragma unroll
     for (int t = 0; t < 2 * KS; t++) S[t] = f4{0.f, 0.f, 0.f, 0.f};
-    if (on && run.from != -1) {
-        const float *s = (run.from >= 0 ? g.st.s + ((size_t)run.from * nv + h) * size : g.carry + ((size_t)(-2 - run.from) * nv + h) * size) + col;
+    if (eye) {
+#pragma unroll
+        for (int t = 0; t < 2 * KS; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) S[t][r] = 32 * (t >> 1) + 8 * q + r + 4 * (t & 1) == col ? 1.f : 0.f;
+    } else if (on && run.from != -1) {
+        const float *s = (run.from >= 0 ? g.st.s + ((size_t)run.from * nv + h) * size : g.places + ((size_t)(-2 - run.from) * nv + h) * place) + col;
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++)
 #pragma unroll
@@ -569,7 +583,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
         for (int s = 0; s < KS; s++) k_at[s] = base + k_in[s], t_at[s] = base + t_in[s];
         const auto rows4 = [&](int which, int b) { return __builtin_bit_cast(f4, read16(vec_at + 256u * (uint32_t)which + 4u * (uint32_t)token_of(b, 0))); };
-        const float keep = *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 63u), m_unit = *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 128u);
+        const float keep = *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 63u), m_unit = OUT ? *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 128u) : 0.f;
         // Reads of LDS are issued a stage ahead of their use (STAGE: nothing moves past it), and what the outputs need is put between the
         // steps of the state.
         const auto read_rows = [&](int what, int s, h8(&x)[4]) {
@@ -591,7 +605,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             if (s + AHEAD < KS) read_rows(0, s + AHEAD, K[s + AHEAD]);
-            else read_rows(1, s + AHEAD - KS, Q[s + AHEAD - KS]);
+            else if (OUT) read_rows(1, s + AHEAD - KS, Q[s + AHEAD - KS]);
             if (s == KS - 1) {
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
@@ -607,27 +621,30 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
             MIX(8, 0x100, 3);
             STAGE;
         }
+        if (OUT) {
 #pragma unroll
-        for (int s = AHEAD; s < KS; s++) read_rows(1, s, Q[s]);
+            for (int s = AHEAD; s < KS; s++) read_rows(1, s, Q[s]);
 #pragma unroll
-        for (int s = 0; s < AHEAD; s++)
+            for (int s = 0; s < AHEAD; s++)
 #pragma unroll
-            for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+                for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+        }
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             eg[b] = eg[b] * back;
 #pragma unroll
             for (int r = 0; r < 4; r++) X[b][r] = fmaf(-eg[b][r], X[b][r], (float)V[4 * b + r]);
         }
-        MIX(4 * AHEAD, 2, 4);
+        if (OUT) MIX(4 * AHEAD, 2, 4);
         STAGE;
         h8 T[6], Tl[6];
 #pragma unroll
         for (int i = 0; i < 6; i++) T[i] = read16(f_at + 1024u * (uint32_t)(FRAG_T + i)), Tl[i] = read16(f_at + 1024u * (uint32_t)(FRAG_T_LO + i));
+        if (OUT)
 #pragma unroll
-        for (int s = AHEAD; s < KS; s++)
+            for (int s = AHEAD; s < KS; s++)
 #pragma unroll
-            for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+                for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
         const int ex = exponent(column_max(X));
         h8 Xh[2], Xl[2];
 #pragma unroll
@@ -636,7 +653,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         const int uu = ex - 14 - T_BITS;
 #pragma unroll
         for (int b = 0; b < 4; b++) U[b] = f4{0.f, 0.f, 0.f, 0.f};
-        MIX(4 * (KS - AHEAD), 2, 6);
+        if (OUT) MIX(4 * (KS - AHEAD), 2, 6);
         STAGE;
         // lane i of a group of 16 hands over 4 values of k_dim of row i / 4, and gets one of k_dim of 4 rows
         s4v Kt[2][2 * KS][2];
@@ -661,8 +678,9 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         MIX(18, 0x100, 1);
         STAGE;
         h8 M[6];
+        if (OUT)
 #pragma unroll
-        for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i));
+            for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i));
         read_columns(1);
         const float mu = column_max(U);
         bound = fmaf(bound, keep, 64.f * mu * pow2(in_range(uu)));
@@ -686,10 +704,11 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(0, t), Dl[0], S[t]);
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(0, t), Dh[0], S[t]);
+        if (OUT)
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+            for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int b = 2 * s; b < 4; b++) y[b] = mfma(M[frag_of(b, s)], Uh[s], y[b]);
+                for (int b = 2 * s; b < 4; b++) y[b] = mfma(M[frag_of(b, s)], Uh[s], y[b]);
         MIX(4 * KS, 2, 2);
         STAGE;
         const float bu = pow2(next) * m_unit;
@@ -698,23 +717,86 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dl[1], S[t]);
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dh[1], S[t]);
+        if (OUT)
 #pragma unroll
-        for (int b = 0; b < 4; b++)
+            for (int b = 0; b < 4; b++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)fmaf(bu, y[b][r], eg[b][r] * g.d.scale * O[b][r])), ro, o_off[4 * b + r], 0u, 0);
-        MIX(4 * KS, 2, 3);
+                for (int r = 0; r < 4; r++)
+                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)fmaf(bu, y[b][r], eg[b][r] * g.d.scale * O[b][r])), ro, o_off[4 * b + r], 0u, 0);
+        if (OUT) MIX(4 * KS, 2, 3);
         if ((c & 15) == 15) bound = column_max(S) * pow2(unit);
     }
     if (on && run.to != -1) {
-        float *s = (run.to >= 0 ? g.st.s + ((size_t)run.to * nv + h) * size : g.carry + ((size_t)(-2 - run.to) * nv + h) * size) + col;
+        float *s = (run.to >= 0 ? g.st.s + ((size_t)run.to * nv + h) * size : g.places + ((size_t)(-2 - run.to) * nv + h) * place) + col;
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int d = 32 * (t >> 1) + 8 * q + r + 4 * (t & 1);
-                if (d < dk) s[(size_t)d * dv] = S[t][r] * pow2(unit);
+                if (d < dk) s[(size_t)d * cols] = S[t][r] * pow2(unit);
             }
+    }
+}
+
+// The states between the parts of a sequence: S of the first part's end, then P S + Q of one after another, in place of Q. A workgroup has
+// 16 columns of a head, wave w the rows 16 w .. (and 128 on). The products are of 32 bits: an accumulator's four rows of block m are what
+// lane group q has of the contraction's steps 4 m .. 4 m + 3, so that a state's blocks lie in LDS as they come.
+template <int KS>
+__global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *joins) {
+    constexpr int RT = KS > 4 ? 2 : 1, KT = 8 * RT;
+    __shared__ alignas(16) f4 at[2][KT][64];
+    const int nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim, tiles = dv / 16, kt = dk / 16;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+    const int h = blockIdx.x / tiles % nv, col = 16 * (int)(blockIdx.x % tiles) + n;
+    const HqJoin jn = joins[blockIdx.x / tiles / nv];
+    const size_t size = (size_t)dk * dv, place = (size_t)dk * max(dk, dv);
+    const auto state = [&](int i) { return g.places + ((size_t)i * nv + h) * place; };
+    f4 x[RT], P[RT][KT];
+    const auto load = [&](const float *s, int t) {
+        const float *const p = s + (size_t)(16 * (w + 8 * t) + 4 * q) * dv + col;
+        return f4{p[0], p[dv], p[2 * dv], p[3 * dv]};
+    };
+    const auto store = [&](float *s, int t, f4 v) {
+        float *const p = s + (size_t)(16 * (w + 8 * t) + 4 * q) * dv + col;
+        p[0] = v[0], p[dv] = v[1], p[2 * dv] = v[2], p[3 * dv] = v[3];
+    };
+    const auto load_p = [&](int j) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int m = 0; m < KT; m++)
+                if (w + 8 * t < kt && m < kt) P[t][m] = *(const f4 *)(state(jn.place + jn.n + j - 1) + (size_t)(16 * (w + 8 * t) + n) * dk + 16 * m + 4 * q);
+    };
+    if (jn.n > 2) load_p(1);
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        if (w + 8 * t >= kt) continue;
+        if (jn.from != -1) store(state(jn.place), t, load(jn.from >= 0 ? g.st.s + ((size_t)jn.from * nv + h) * size : state(-2 - jn.from), t));
+        x[t] = load(state(jn.place + 1), t);
+    }
+    for (int j = 1; j < jn.n - 1; j++) {
+        f4 y[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if (w + 8 * t < kt) {
+                y[t] = load(state(jn.place + 1 + j), t);
+                at[j & 1][w + 8 * t][lane] = x[t];
+            }
+        __syncthreads();  // (and the other half is free again: its readers have all come here)
+#pragma unroll
+        for (int m = 0; m < KT; m++) {
+            if (m >= kt) continue;
+            const f4 s = at[j & 1][m][lane];
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+                if (w + 8 * t < kt)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) y[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(P[t][m][r], s[r], y[t], 0, 0, 0);
+        }
+        if (j + 2 < jn.n) load_p(j + 1);
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if (w + 8 * t < kt) store(state(jn.place + 1 + j), t, x[t] = y[t]);
     }
 }
 
@@ -760,12 +842,18 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
 }
 
 template <int KS>
-void launch_chunks(const ChunkArgs &g, hipStream_t s) {
-    k_delta_prep<KS><<<((unsigned)g.n_chunks * (unsigned)g.st.n_k_heads + 7) / 8 * 8 * (unsigned)(g.st.n_v_heads / g.st.n_k_heads), 256, 0, s>>>(g);
-    const unsigned heads = ((unsigned)g.n_runs * (unsigned)g.st.n_v_heads + 7) / 8 * 8;
-    const auto grid = [&](int W) { return heads * (unsigned)((g.st.v_dim + 16 * W - 1) / (16 * W)); };
-    constexpr int W = KS == 8 ? 2 : 4;
-    k_delta_scan<KS, W><<<grid(W), 64 * (W + 4), 0, s>>>(g);
+void launch_chunks(ChunkArgs g, const HqPass &p, const HqRun *runs, const HqJoin *joins, hipStream_t s) {
+    constexpr int W = hq_scan_columns(32 * KS) / 16;
+    const int nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim;
+    k_delta_prep<KS><<<((unsigned)g.n_chunks * (unsigned)g.st.n_k_heads + 7) / 8 * 8 * (unsigned)(nv / g.st.n_k_heads), 256, 0, s>>>(g);
+    const auto grid = [&](int n, int cols) { return ((unsigned)n * (unsigned)nv + 7) / 8 * 8 * (unsigned)((cols + 16 * W - 1) / (16 * W)); };
+    if (p.n_parts) {
+        g.runs = runs + p.part0, g.n_runs = p.n_parts;
+        k_delta_scan<KS, W, false><<<grid(p.n_parts, std::max(dk, dv)), 64 * (W + 4), 0, s>>>(g);
+        k_delta_join<KS><<<(unsigned)p.n_joins * (unsigned)nv * (unsigned)(dv / 16), 512, 0, s>>>(g, joins + p.join0);
+    }
+    g.runs = runs + p.run0, g.n_runs = p.n_runs;
+    k_delta_scan<KS, W, true><<<grid(p.n_runs, dv), 64 * (W + 4), 0, s>>>(g);
 }
 
 }  // namespace
@@ -802,10 +890,10 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     if (cur != c->device) SCK(hipSetDevice(c->device));
     hipStream_t s = (hipStream_t)stream;
     for (const HqPass &p : c->passes) {
-        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, c->runs + p.run0, p.n_runs, p.n_chunks, c->work, (float *)(c->work + c->carry_at), 1.0f};
-        if (st->k_dim <= 64) launch_chunks<2>(g, s);
-        else if (st->k_dim <= 128) launch_chunks<4>(g, s);
-        else launch_chunks<8>(g, s);
+        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), 1.0f};
+        if (st->k_dim <= 64) launch_chunks<2>(g, p, c->runs, c->joins, s);
+        else if (st->k_dim <= 128) launch_chunks<4>(g, p, c->runs, c->joins, s);
+        else launch_chunks<8>(g, p, c->runs, c->joins, s);
         if (d->norm) {
             const int lanes = st->v_dim <= 64 ? 8 : st->v_dim <= 128 ? 16 : 32;
             const dim3 grid((unsigned)p.n_chunks, 16);

@@ -28,16 +28,26 @@ constexpr size_t HQ_CHUNK_BYTES = 19 * 1024;
 struct HqChunk {
     int tok0, n;
 };
-// A sequence, or the part of one that a pass has: its tokens, its first chunk in the pass, slots as in HqSeq; a state on its way from
-// one pass to the next lies in one of two places of the workspace, -2 and -3.
+// A sequence, or a part of one: its tokens, its first chunk in the pass, slots as in HqSeq, or places of the workspace for states: -2 - i
+// is place i. Places 0 and 1 have states on their way from one pass to the next.
+constexpr int HQ_IDENTITY = -0x7fffffff;  // from: S = I, and the values are zeros
 struct HqRun {
     int tok0, n, chunk0;
     int from, to;
 };
+// A sequence that a pass takes in `n` parts at a time. What a part does to a state is S' = P S + Q. Places of the workspace: `place` a copy
+// of the sequence's state, from there on the states behind parts 0 .. n - 2 (at first Q), then P of parts 1 .. n - 2.
+struct HqJoin {
+    int from, place, n;
+};
 struct HqPass {
     int chunk0, n_chunks;  // of hq_scan::chunks
     int run0, n_runs;      // of hq_scan::runs
+    int part0, n_parts;    // of hq_scan::runs: those that only lead to states, before
+    int join0, n_joins;    // of hq_scan::joins: and what makes the parts' first states of them
 };
+// columns of a head's state that one workgroup takes through a run
+constexpr int hq_scan_columns(int k_dim) { return k_dim > 128 ? 32 : 64; }
 
 struct hq_scan {
     int device, n_cu;
@@ -54,9 +64,10 @@ struct hq_scan {
     int n_steps;
     const HqChunk *chunks;  // and those that it takes by chunks
     const HqRun *runs;      // (a pass's longest first)
+    const HqJoin *joins;
     std::vector<HqPass> passes;
-    char *work;             // chunks of a pass, then two states
-    size_t work_bytes, carry_at;
+    char *work;             // chunks of a pass, then places for states, each n_v_heads * k_dim * max(k_dim, v_dim) long
+    size_t work_bytes, places_at;
     // storage: one pinned copy of `dev`, which the next set waits for
     int *host, *dev;
     size_t words;

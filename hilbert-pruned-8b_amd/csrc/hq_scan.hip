@@ -34,6 +34,65 @@ int check_geometry(const char *who, const hq_state_t *st) {
     return 0;
 }
 
+// Few long runs leave most of the chip idle, each a chain of chunks. Cut into parts that fill it, a workgroup a CU, first every part's
+// effect on a state is formed (P and Q, all parts side by side, without outputs), then the states between them, then the outputs of all
+// parts side by side: two chains of a part's length and a product a part instead of one. It costs two launches, the states' way through
+// memory and the products, some 17 us, as much as 8 or 9 chunks: one sequence of 1000 tokens, 32 heads of 128, 47 us with it or without,
+// 2048: 82 without, 77 with, 6001: 215 and 173, 16000: 555 and 428. (Two workgroups a CU and so shorter parts: 90, 190, 467.)
+constexpr int JOIN_CHUNKS = 9, LEAST_PART = 4;
+void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std::vector<HqRun> *runs, std::vector<HqJoin> *joins, int *places) {
+    const int cols = hq_scan_columns(st->k_dim);
+    const int64_t units = (int64_t)st->n_v_heads * ((st->v_dim + cols - 1) / cols), p_units = (int64_t)st->n_v_heads * ((st->k_dim + cols - 1) / cols);
+    std::vector<HqRun> all, parts;
+    const auto chunks_of = [](int n) { return (n + HQ_CHUNK - 1) / HQ_CHUNK; };
+    for (HqPass &p : *passes) {
+        int longest = 0;
+        for (int i = 0; i < p.n_runs; i++) longest = std::max(longest, chunks_of((*runs)[p.run0 + i].n));
+        const auto fits = [&](int part) {  // a workgroup a CU
+            int64_t outputs = 0, effects = 0;
+            for (int i = 0; i < p.n_runs; i++) {
+                const int64_t n = (chunks_of((*runs)[p.run0 + i].n) + part - 1) / part;
+                outputs += n * units, effects += n > 1 ? (n - 1) * units + (n - 2) * p_units : 0;
+            }
+            return outputs <= n_cu && effects <= n_cu;
+        };
+        int part = LEAST_PART;
+        while (part < longest && !fits(part)) part++;
+        const bool split = longest > 2 * part + JOIN_CHUNKS;
+        const int run0 = (int)all.size();
+        parts.clear();
+        p.join0 = (int)joins->size();
+        for (int i = 0; i < p.n_runs; i++) {
+            const HqRun r = (*runs)[p.run0 + i];
+            const int chunks = chunks_of(r.n), n = split ? (chunks + part - 1) / part : 1;
+            if (n == 1) {
+                all.push_back(r);
+                continue;
+            }
+            const int each = (chunks + n - 1) / n, m = (chunks + each - 1) / each;  // (m: with parts of one length, as many as there are)
+            const int first = std::max(*places, 2), place = -2 - first;             // (2: those between passes)
+            *places = first + 2 * m - 2;
+            joins->push_back({r.from, first, m});
+            for (int j = 0; j < m; j++) {
+                HqRun q = {r.tok0 + j * each * HQ_CHUNK, std::min(each * HQ_CHUNK, r.n - j * each * HQ_CHUNK), r.chunk0 + j * each, j ? place - j : r.from == -1 ? -1 : place,
+                           j == m - 1 ? r.to : -1};
+                all.push_back(q);
+                if (j == m - 1) break;
+                q.from = j ? -1 : r.from, q.to = place - 1 - j;
+                parts.push_back(q);
+                if (!j) continue;
+                q.from = HQ_IDENTITY, q.to = place - m - j + 1;
+                parts.push_back(q);
+            }
+        }
+        p.run0 = run0, p.n_runs = (int)all.size() - run0;
+        p.part0 = (int)all.size(), p.n_parts = (int)parts.size();
+        all.insert(all.end(), parts.begin(), parts.end());
+        p.n_joins = (int)joins->size() - p.join0;
+    }
+    runs->swap(all);
+}
+
 }  // namespace
 
 int hq_state_check(const char *who, const hq_state_t *st, const hq_scan *c) {
@@ -97,10 +156,11 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     std::vector<HqChunk> chunks;
     std::vector<HqRun> runs;
     std::vector<HqPass> passes;
+    std::vector<HqJoin> joins;
     // chunks of a pass: what fits MOST_WORK, and 64 at least
     const size_t per_chunk = (size_t)st->n_v_heads * HQ_CHUNK_BYTES;
     const int most_chunks = (int)std::max<size_t>(64, MOST_WORK / per_chunk);
-    bool carries = false;
+    int places = 0;  // for states
     try {
         // slots that are written: each by one sequence, and read by no other
         std::vector<std::pair<int, int>> w, r;
@@ -130,7 +190,7 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
         for (const auto &l : long_seqs) {
             int from_now = from[l.first];
             for (int t = 0; t < n_new[l.first];) {
-                if (passes.empty() || passes.back().n_chunks == most_chunks) passes.push_back({(int)chunks.size(), 0, (int)runs.size(), 0});
+                if (passes.empty() || passes.back().n_chunks == most_chunks) passes.push_back({(int)chunks.size(), 0, (int)runs.size(), 0, 0, 0, 0, 0});
                 HqPass &p = passes.back();
                 const int n = std::min<int64_t>((int64_t)n_new[l.first] - t, (int64_t)(most_chunks - p.n_chunks) * HQ_CHUNK);
                 const bool cut = t + n < n_new[l.first];
@@ -138,10 +198,12 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
                 runs.push_back({l.second + t, n, p.n_chunks, from_now, cut ? carry : to[l.first]});
                 for (int j = 0; j < n; j += HQ_CHUNK) chunks.push_back({l.second + t + j, std::min(HQ_CHUNK, n - j)}), p.n_chunks++;
                 p.n_runs++;
-                from_now = carry, carries |= cut;
+                from_now = carry;
+                if (cut) places = 2;
                 t += n;
             }
         }
+        split_runs(st, c->n_cu, &passes, &runs, &joins, &places);
         for (const HqPass &p : passes)
             std::stable_sort(runs.begin() + p.run0, runs.begin() + p.run0 + p.n_runs, [](const HqRun &a, const HqRun &b) { return a.n > b.n; });
         std::stable_sort(steps.begin(), steps.end(), [&](int a, int b) { return n_new[a] > n_new[b]; });
@@ -155,7 +217,7 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
         c->sending = false;
     }
     const size_t words = (size_t)n_seqs * (sizeof(HqSeq) / 4) + tiles.size() * (sizeof(HqTile) / 4) + steps.size() + chunks.size() * (sizeof(HqChunk) / 4) +
-                         runs.size() * (sizeof(HqRun) / 4) + 16;
+                         runs.size() * (sizeof(HqRun) / 4) + joins.size() * (sizeof(HqJoin) / 4) + 16;
     if (words > c->words) {
         const size_t want = words + words / 2;
         SCK(hipDeviceSynchronize());
@@ -170,8 +232,8 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     }
     size_t work = 0;
     for (const HqPass &p : passes) work = std::max(work, (size_t)p.n_chunks * per_chunk);
-    c->carry_at = work;
-    if (carries) work += 2 * (size_t)st->n_v_heads * st->k_dim * st->v_dim * 4;
+    c->places_at = work;
+    work += (size_t)places * st->n_v_heads * st->k_dim * std::max(st->k_dim, st->v_dim) * 4;
     if (work > c->work_bytes) {
         SCK(hipDeviceSynchronize());
         if (c->work) SCK(hipFree(c->work));
@@ -199,6 +261,9 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     c->runs = (const HqRun *)dev();
     if (!runs.empty()) memcpy(w, runs.data(), runs.size() * sizeof(HqRun));
     w += runs.size() * (sizeof(HqRun) / 4);
+    c->joins = (const HqJoin *)dev();
+    if (!joins.empty()) memcpy(w, joins.data(), joins.size() * sizeof(HqJoin));
+    w += joins.size() * (sizeof(HqJoin) / 4);
     c->passes.swap(passes);
     const size_t used = (size_t)(w - c->host);
     if (used) {

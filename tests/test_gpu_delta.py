@@ -220,3 +220,55 @@ def test_refusals(hqlib):
         with pytest.raises(hqlib.HQError, match=text):
             hqlib.delta(**{**ok, **kw})
     scan.free()
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv,seqs,gate", [
+    (2, 2, 64, 64, [(1500, 0, 0)], None),                                   # one long sequence, its state in its place
+    (1, 2, 128, 128, [(1601, 1, 3)], np.float32),
+    (1, 1, 128, 32, [(1000, -1, -1), (900, -1, 0), (40, 1, 1), (3, 2, 2)], np.float16),  # beginnings, nothing kept, short ones beside it
+    (1, 2, 32, 128, [(1100, 0, 0), (0, 1, 2), (1025, 3, 4)], None),
+    (1, 1, 256, 48, [(900, 0, 1)], None), (1, 1, 48, 256, [(1217, 0, 0)], np.float32),
+    (3, 3, 16, 16, [(2100, -1, 0), (17, 2, 2)], None)])
+def test_long_sequences_in_parts(hqlib, hk, hv, dk, dv, seqs, gate):
+    """Few heads and long sequences: parts of a sequence side by side, with the states between them formed of their effects."""
+    check(hqlib, 40 + hv + dk + dv, hk, hv, dk, dv, seqs, gate)
+
+
+def test_parts_keep_what_is_not_a_number_apart(hqlib):
+    """A value that is not a number, in the first part's state and in a middle part's values, stays in its column through the parts."""
+    hk, hv, dk, dv, n = 1, 1, 64, 64, 1200
+    rng = np.random.default_rng(9)
+    x, g, beta = inputs(rng, n, hk, hv, dk, dv)
+    states = np.zeros((2, hv, dk, dv), np.float32)
+    states[0] = rng.normal(0, 0.5, (hv, dk, dv))
+    print("[gpu] delta parts with NaN", flush=True)
+    want, sw = go(hqlib, x, g, beta, states, [n], [0], [1], hk, hv, dk, dv)
+    x[500, 2 * hk * dk + 7] = np.nan
+    states[0, 0, 3, 50] = np.inf
+    got, sg = go(hqlib, x, g, beta, states, [n], [0], [1], hk, hv, dk, dv)
+    fine = [i for i in range(dv) if i not in (7, 50)]
+    assert np.array_equal(got[:, :, fine], want[:, :, fine]) and np.array_equal(sg[1][:, :, fine], sw[1][:, :, fine])
+    assert np.isnan(got[563:, 0, 7]).all() and np.isnan(got[63:, 0, 50]).all() and np.isnan(sg[1][0][:, [7, 50]]).all()
+    assert np.array_equal(got[:448, 0, 7], want[:448, 0, 7])
+
+
+@pytest.mark.parametrize("hk,hv,d,seqs,heads", [
+    (64, 512, 16, [(300, 0, 0), (4500, 1, 2), (100, -1, 3)], (0, 8, 504)),  # 68 chunks of 512 heads to a pass of the workspace
+    (8, 64, 16, [(36000, 0, 0)], (0,))])                                     # 538 of 64, and parts within each
+def test_more_chunks_than_a_pass_has(hqlib, hk, hv, d, seqs, heads):
+    """A sequence whose chunks do not fit the workspace together: its state goes on from pass to pass. (Heads are independent of each
+    other: some of them are compared, two of one key head each.)"""
+    n_new, src, dst = [list(a) for a in zip(*seqs)]
+    rng = np.random.default_rng(hv)
+    x, g, beta = inputs(rng, sum(n_new), hk, hv, d, d)
+    states = rng.normal(0, 0.5, (max(dst) + 2, hv, d, d)).astype(np.float32)
+    print(f"[gpu] delta passes {hk}/{hv} x {d} {seqs}", flush=True)
+    y, s = go(hqlib, x, g, beta, states, n_new, src, dst, hk, hv, d, d)
+    q, k, v = split(x, hk, hv, d, d)
+    for h in heads:
+        two, kh = slice(h, h + 2), slice(h // (hv // hk), h // (hv // hk) + 1)
+        before = [states[i][two] if i >= 0 else np.zeros((2, d, d), np.float32) for i in src]
+        want, bound, after, e = delta(q[:, kh], k[:, kh], v[:, two], g[:, two], beta[:, two], before, n_new, d ** -0.5)
+        assert (np.abs(y[:, two] - want) <= bound).all()
+        for i, a, b in zip(dst, after, e):
+            assert (np.abs(s[i][two] - a) <= b + U_MIN).all() and np.sqrt(((s[i][two] - a) ** 2).mean()) <= 2.0 ** -19 * np.sqrt((a * a).mean())
