@@ -180,9 +180,10 @@ __global__ void __launch_bounds__(512, ROWS <= 16 ? 4 : 2) k_delta_step(DeltaArg
 // and 2 s + 1 together hold, lane group by lane group, the 8 consecutive contraction indices that an operand takes. Tiles of S
 // likewise.
 //
-// Precision: K, Q and V are exact. S, U and T enter products as two fp16 terms each, scaled by a power of two of their column's largest
-// (T: of the matrix), good to 2^-22 of it; only for the outputs, which end in fp16, one term of S, M and U does.
-constexpr int FRAG_T = 0, FRAG_T_LO = 6, FRAG_M = 12, FRAG_VEC = 18;  // of a chunk's workspace, in KB; fragments (block, half) in the order below
+// Precision: K, Q and V are exact. S, U, T and M enter products as two fp16 terms each, scaled by a power of two of their column's largest
+// (T and M: of the matrix), good to 2^-22 of it. (One term of S, M and U for the outputs, which end in fp16, made them 1.6 to 1.8 times
+// as inexact as their own rounding does.)
+constexpr int FRAG_T = 0, FRAG_T_LO = 6, FRAG_M = 12, FRAG_M_LO = 18, FRAG_VEC = 24;  // of a chunk's workspace, in KB; fragments (block, half) in the order below
 constexpr int T_BITS = 12;  // T is held 2^12 times as large
 constexpr float T_SCALE = 1 << T_BITS;
 DEV int frag_of(int b, int s) { return b < 2 ? b : 2 * b - 2 + s; }
@@ -229,8 +230,10 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
         u4v kq[2][64 * CPR];
         struct {
             uint32_t t[64 * LD];  // T: its two terms
-            _Float16 m[64 * LD];  // M
-            float At[64 * LA];    // A transposed
+            union {
+                uint32_t m[64 * LD];  // M likewise
+                float At[64 * LA];    // A transposed
+            };
         };
     } sh;
     __shared__ alignas(16) float Td[4][16 * LT];
@@ -360,18 +363,19 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
     const float scale = T_SCALE * bet[16 * w + n];
     const int em = exponent(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
     const float to_m = pow2(268 - em);
+    const auto terms = [](float v) { return __builtin_bit_cast(uint32_t, h2{(_Float16)v, (_Float16)(v - (float)(_Float16)v)}); };
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (i >= (w & ~1)) {  // (above the diagonal: the half of a fragment that is zero)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float v = T[i][r] * scale;
-                sh.t[(16 * i + 4 * q + r) * LD + 16 * w + n] = __builtin_bit_cast(uint32_t, h2{(_Float16)v, (_Float16)(v - (float)(_Float16)v)});
+                sh.t[(16 * i + 4 * q + r) * LD + 16 * w + n] = terms(T[i][r] * scale);
             }
         }
         if (i <= (w | 1)) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) sh.m[(i0 + r) * LD + 16 * i + n] = (_Float16)(M[i][r] * to_m);
+            for (int r = 0; r < 4; r++) sh.m[(i0 + r) * LD + 16 * i + n] = terms(M[i][r] * to_m);
         }
     }
     __syncthreads();
@@ -379,17 +383,14 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
 #pragma unroll
     for (int p0 = 0; p0 < 12; p0 += 4) {
         const int p = p0 + wave, k = p % 6, b = k < 2 ? k : k / 2 + 1, s = k < 2 ? 0 : k & 1;
-        if (p < 6) {
-            const u4v *const x = (const u4v *)(sh.t + token_of(b, n) * LD + 32 * s + 8 * q);
-            const u4v u = x[0], v = x[1];
-            // (the terms of neighbouring values lie side by side)
-            *(u4v *)(to + (FRAG_T + k) * 1024) = u4v{__builtin_amdgcn_perm(u.y, u.x, 0x05040100u), __builtin_amdgcn_perm(u.w, u.z, 0x05040100u),
-                                                     __builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x05040100u)};
-            *(u4v *)(to + (FRAG_T_LO + k) * 1024) = u4v{__builtin_amdgcn_perm(u.y, u.x, 0x07060302u), __builtin_amdgcn_perm(u.w, u.z, 0x07060302u),
-                                                        __builtin_amdgcn_perm(v.y, v.x, 0x07060302u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u)};
-        } else {
-            *(u4v *)(to + (FRAG_M + k) * 1024) = *(const u4v *)(sh.m + token_of(b, n) * LD + 32 * s + 8 * q);
-        }
+        const u4v *const x = (const u4v *)((p < 6 ? sh.t : sh.m) + token_of(b, n) * LD + 32 * s + 8 * q);
+        const u4v u = x[0], v = x[1];
+        // (the terms of neighbouring values lie side by side)
+        char *const o = to + ((p < 6 ? FRAG_T : FRAG_M) + k) * 1024;
+        *(u4v *)o = u4v{__builtin_amdgcn_perm(u.y, u.x, 0x05040100u), __builtin_amdgcn_perm(u.w, u.z, 0x05040100u),
+                        __builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x05040100u)};
+        *(u4v *)(o + 6 * 1024) = u4v{__builtin_amdgcn_perm(u.y, u.x, 0x07060302u), __builtin_amdgcn_perm(u.w, u.z, 0x07060302u),
+                                     __builtin_amdgcn_perm(v.y, v.x, 0x07060302u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u)};
     }
     if (wave == 3) {
         float *const v = (float *)(g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES + FRAG_VEC * 1024);
@@ -621,13 +622,17 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
             MIX(8, 0x100, 3);
             STAGE;
         }
+        const auto old = [&](int s) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sl[s], O[b]);
+#pragma unroll
+            for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+        };
         if (OUT) {
 #pragma unroll
             for (int s = AHEAD; s < KS; s++) read_rows(1, s, Q[s]);
 #pragma unroll
-            for (int s = 0; s < AHEAD; s++)
-#pragma unroll
-                for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+            for (int s = 0; s < AHEAD; s++) old(s);
         }
 #pragma unroll
         for (int b = 0; b < 4; b++) {
@@ -635,16 +640,14 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
             for (int r = 0; r < 4; r++) X[b][r] = fmaf(-eg[b][r], X[b][r], (float)V[4 * b + r]);
         }
-        if (OUT) MIX(4 * AHEAD, 2, 4);
+        if (OUT) MIX(8 * AHEAD, 2, 2);
         STAGE;
         h8 T[6], Tl[6];
 #pragma unroll
         for (int i = 0; i < 6; i++) T[i] = read16(f_at + 1024u * (uint32_t)(FRAG_T + i)), Tl[i] = read16(f_at + 1024u * (uint32_t)(FRAG_T_LO + i));
         if (OUT)
 #pragma unroll
-            for (int s = AHEAD; s < KS; s++)
-#pragma unroll
-                for (int b = 0; b < 4; b++) O[b] = mfma(Q[s][b], Sh[s], O[b]);
+            for (int s = AHEAD; s < KS; s++) old(s);
         const int ex = exponent(column_max(X));
         h8 Xh[2], Xl[2];
 #pragma unroll
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         const int uu = ex - 14 - T_BITS;
 #pragma unroll
         for (int b = 0; b < 4; b++) U[b] = f4{0.f, 0.f, 0.f, 0.f};
-        if (OUT) MIX(4 * (KS - AHEAD), 2, 6);
+        if (OUT) MIX(8 * (KS - AHEAD), 2, 3);
         STAGE;
         // lane i of a group of 16 hands over 4 values of k_dim of row i / 4, and gets one of k_dim of 4 rows
         s4v Kt[2][2 * KS][2];
@@ -677,21 +680,22 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
                 for (int b = 2 * s; b < 4; b++) U[b] = mfma(i == 0 ? Tl[frag_of(b, s)] : T[frag_of(b, s)], i == 1 ? Xl[s] : Xh[s], U[b]);
         MIX(18, 0x100, 1);
         STAGE;
-        h8 M[6];
+        h8 M[6], Ml[6];
         if (OUT)
 #pragma unroll
-            for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i));
+            for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i)), Ml[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M_LO + i));
         read_columns(1);
         const float mu = column_max(U);
         bound = fmaf(bound, keep, 64.f * mu * pow2(in_range(uu)));
         const int next = exponent(bound) - 14;
         const float sd = pow2(in_range(uu - next + 127)), ratio = keep * pow2(in_range(unit - next + 127));
         unit = next;
-        h8 Uh[2], Dh[2], Dl[2];
+        h8 Uh[2], Ul[2], Dh[2], Dl[2];
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const f4 x = U[2 * s] * sd, y = U[2 * s + 1] * sd, xd = x * dec[2 * s], yd = y * dec[2 * s + 1];
             Uh[s] = halves(x, y);
+            if (OUT) Ul[s] = second_term(x, y, g.one, Uh[s]);
             Dh[s] = halves(xd, yd), Dl[s] = second_term(xd, yd, g.one, Dh[s]);
         }
 #pragma unroll
@@ -708,7 +712,9 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
             for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int b = 2 * s; b < 4; b++) y[b] = mfma(M[frag_of(b, s)], Uh[s], y[b]);
+                for (int i = 0; i < 3; i++)
+#pragma unroll
+                    for (int b = 2 * s; b < 4; b++) y[b] = mfma(i == 0 ? Ml[frag_of(b, s)] : M[frag_of(b, s)], i == 1 ? Ul[s] : Uh[s], y[b]);
         MIX(4 * KS, 2, 2);
         STAGE;
         const float bu = pow2(next) * m_unit;

@@ -21,10 +21,10 @@ struct HqTile {
 constexpr int HQ_CONV_TILE = 8;  // most tokens of a tile of hq_delta_append
 
 // hq_delta by chunks of 64 tokens. A chunk's operands that depend on its value head but not on the state are formed first, for many
-// chunks at a time (a pass), into HQ_CHUNK_BYTES of workspace each: 18 fragments and a vector of 1 KB (hq_delta.hip).
+// chunks at a time (a pass), into HQ_CHUNK_BYTES of workspace each: 24 fragments and a vector of 1 KB (hq_delta.hip).
 constexpr int HQ_STEP_TOKENS = 16;  // most new tokens of a sequence that it takes token by token
 constexpr int HQ_CHUNK = 64;
-constexpr size_t HQ_CHUNK_BYTES = 19 * 1024;
+constexpr size_t HQ_CHUNK_BYTES = 25 * 1024;
 struct HqChunk {
     int tok0, n;
 };

@@ -38,7 +38,8 @@ int check_geometry(const char *who, const hq_state_t *st) {
 // effect on a state is formed (P and Q, all parts side by side, without outputs), then the states between them, then the outputs of all
 // parts side by side: two chains of a part's length and a product a part instead of one. It costs two launches, the states' way through
 // memory and the products, some 17 us, as much as 8 or 9 chunks: one sequence of 1000 tokens, 32 heads of 128, 47 us with it or without,
-// 2048: 82 without, 77 with, 6001: 215 and 173, 16000: 555 and 428. (Two workgroups a CU and so shorter parts: 90, 190, 467.)
+// 2048: 82 without, 77 with, 6001: 215 and 173, 16000: 555 and 428. (Two workgroups a CU and so shorter parts: 90, 190, 467. All before
+// M and U had a second term in the outputs, which is 4 to 7 % more.)
 constexpr int JOIN_CHUNKS = 9, LEAST_PART = 4;
 void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std::vector<HqRun> *runs, std::vector<HqJoin> *joins, int *places) {
     const int cols = hq_scan_columns(st->k_dim);

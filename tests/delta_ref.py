@@ -5,9 +5,9 @@ and a <= 1 is a contraction, so errors add up and never grow: e <- a e + c. A to
 over k_dim products, (k_dim + 8) 2^-24 of |k| |S| at most; operands that are held as two fp16 terms are off by 2^-22 of their
 column's largest; a chunked form has sums over up to 64 tokens beside them. c = 4 (k_dim + 80) 2^-24 (|a S| + |v|) covers both.
 
-Outputs end in fp16, and the chunked form rounds the operands of their products to it: of o = scale (e^G q S0 + sum_j M_j u_j) with S0
-the state before the chunk (of 64 tokens from the sequence's first), S0 once and M and u once each, so 2^-11 of sum |e^G q S0| and 2
-2^-11 of sum |M_j u_j| are added to the state's error and the rounding of the result."""
+Outputs are the state's products with a query of norm 1, so their error is e |q|, and end in fp16; with the norm, those of chunks are
+rounded to it before the norm too. (Products of the chunked form besides the state's are of operands of two terms as well, 2^-22 of
+the largest of up to 64 tokens' magnitudes: within what c has for each of these tokens.)"""
 import numpy as np
 
 U16, U32 = 2.0 ** -11, 2.0 ** -24
@@ -60,10 +60,6 @@ def delta(q, k, v, decay, beta, states, n_new, scale, norm=None, gate=None, eps=
     for s0, n in zip(states, n_new):
         S, e = s0.astype(np.float64), np.zeros((hv, 1, dv))
         for i in range(n):
-            if i % 64 == 0:  # a chunk: the state before it, what its tokens have written, the logarithm of the decay since
-                S0, first, G, us = np.abs(S), t, np.zeros((hv, 0)), np.zeros((0, hv, dv))
-            g_t = np.maximum(decay[t].astype(np.float64), -1e4)
-            G = np.concatenate([G + g_t[:, None], np.zeros((hv, 1))], 1)  # [hv, tokens of the chunk]: to now from each of them
             keep = np.exp(decay[t].astype(np.float64))[:, None, None]
             # (a decay's exponential is off by 2^-22 of itself: its argument's sums and the function)
             S = S * keep
@@ -72,11 +68,7 @@ def delta(q, k, v, decay, beta, states, n_new, scale, norm=None, gate=None, eps=
             u = (v[t] - (k[t][:, :, None] * S).sum(1)) * beta[t].astype(np.float64)[:, None]
             S = S + k[t][:, :, None] * u[:, None]
             o = scale * (S * q[t][:, :, None]).sum(1)
-            us = np.concatenate([us, np.abs(u)[None]])
-            with np.errstate(under="ignore"):
-                M = np.exp(G) * np.abs((k[first:t + 1] * q[t]).sum(-1)).T
-                old = np.exp(G[:, :1] + (np.maximum(decay[first].astype(np.float64), -1e4)[:, None])) * (S0 * np.abs(q[t])[:, :, None]).sum(1)
-            b = abs(scale) * (U16 * old + 2 * U16 * (M.T[:, :, None] * us).sum(0) + e[:, 0] * np.linalg.norm(q[t], axis=-1)[:, None])
+            b = abs(scale) * e[:, 0] * np.linalg.norm(q[t], axis=-1)[:, None]
             if norm is not None:
                 z = silu(gate[t].astype(np.float64)) * norm.astype(np.float64)
                 ms = (o * o).mean(-1, keepdims=True) + eps
