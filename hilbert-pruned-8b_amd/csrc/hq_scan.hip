@@ -50,12 +50,13 @@ void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std
         int longest = 0;
         for (int i = 0; i < p.n_runs; i++) longest = std::max(longest, chunks_of((*runs)[p.run0 + i].n));
         const auto fits = [&](int part) {  // a workgroup a CU
-            int64_t outputs = 0, effects = 0;
+            int64_t outputs = 0, effects = 0, rest = 0;  // (runs shorter than a part: one after another in its time)
             for (int i = 0; i < p.n_runs; i++) {
-                const int64_t n = (chunks_of((*runs)[p.run0 + i].n) + part - 1) / part;
-                outputs += n * units, effects += n > 1 ? (n - 1) * units + (n - 2) * p_units : 0;
+                const int64_t chunks = chunks_of((*runs)[p.run0 + i].n), n = (chunks + part - 1) / part;
+                if (n == 1) rest += chunks;
+                else outputs += n * units, effects += (n - 1) * units + (n - 2) * p_units;
             }
-            return outputs <= n_cu && effects <= n_cu;
+            return outputs + (rest + part - 1) / part * units <= n_cu && effects <= n_cu;
         };
         int part = LEAST_PART;
         while (part < longest && !fits(part)) part++;
@@ -179,10 +180,13 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
                 if (r[k].second != w[i].second) return hq_internal_fail("%s: sequence %d goes on from slot %d, where sequence %d leaves its state", who, r[k].second, w[i].first, w[i].second);
         }
         std::vector<std::pair<int, int>> long_seqs;
+        int64_t few = 0, many = 0;
+        for (int i = 0; i < n_seqs; i++) few += n_new[i] > HQ_STEP_BESIDE && n_new[i] <= HQ_STEP_TOKENS, many += n_new[i] > HQ_STEP_TOKENS;
+        const int by_steps = many && few * st->n_v_heads <= 4 * c->n_cu ? HQ_STEP_BESIDE : HQ_STEP_TOKENS;
         for (int i = 0, tok = 0; i < n_seqs; tok += n_new[i], i++) {
             if (n_new[i] == 0 && (to[i] < 0 || to[i] == from[i])) continue;
             for (int t = 0; t == 0 || t < n_new[i]; t += HQ_CONV_TILE) tiles.push_back({i, t, std::min(HQ_CONV_TILE, n_new[i] - t)});
-            if (n_new[i] <= HQ_STEP_TOKENS) {
+            if (n_new[i] <= by_steps) {
                 steps.push_back(i);
                 continue;
             }
