@@ -217,15 +217,32 @@ struct ChunkArgs {
     float one;  // 1: a factor that the compiler does not know, so that a difference is one fused instruction
 };
 
-// T and M of a chunk and value head. Wave w forms rows 16 w .. of K K^T and Q K^T, then inverts the 16 x 16 block (w, w) of I + A by
-// substitution, a column a lane, and last computes block column w of the inverse from the top down, T_ij = -T_ii sum_l A_il T_lj, on
+// The largest of a wave's magnitudes, in rows of 16 lanes and across them
+DEV float largest(float x) {
+    uint32_t v = __builtin_bit_cast(uint32_t, x);
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // (rows turned by 8, 4, 2, 1 lanes)
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_bit_cast(float, max(b[0], b[1]));
+}
+
+// T and M of a chunk and value head. Wave w forms rows 16 w .. of K K^T and Q K^T, one inverts the 16 x 16 blocks of I + A on the diagonal by
+// substitution, a column a lane, and last each computes block column w of the inverse from the top down, T_ij = -T_ii sum_l A_il T_lj, on
 // the fp32 matrix cores: each block of the column is the next one's operand.
 // e^(G_i - G_j) of a block left of the diagonal is a factor of the row, from the block's first row, times one of the column, to it:
 // neither exceeds 1. Sums of logarithms are formed in 64 bits and held as a multiple of 2^-9 and a rest, so that their differences
 // lose nothing; below -150 a decay is 0 in 32 bits.
+// Bound: a chain of some 9 us (loads, products, substitution, blocks, stores), hidden by four workgroups a CU: 1024 of them (32 chunks of
+// 32 heads of 128) 14 us; 8352 of 16384 tokens 86, 56 of which would be their bytes'. (With every wave substituting in a block of its own, a
+// fourth of the lanes' work new, and rows of 72 words, three fit a CU: 18 and 109. The wave with the sums of logarithms loads nothing by
+// DMA: it would wait for that too.)
 template <int KS>
-__global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g) {
-    constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS, LD = 72, LA = 68, LT = 20;
+__global__ void __launch_bounds__(256, KS <= 4 ? 4 : 2) k_delta_prep(ChunkArgs g) {
+    constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS, LD = 68, LA = 68, LT = 20;
     __shared__ union {
         u4v kq[2][64 * CPR];
         struct {
@@ -248,17 +265,6 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
     // (the waves' shares are unlike: turned from workgroup to workgroup, so that no SIMD has all the long ones)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = (wave + (int)(blockIdx.x / 8)) & 3;
     const int lane = tid & 63, n = lane & 15, q = lane >> 4;
-    {
-        const uint32_t row_bytes = (uint32_t)g.d.qk_stride * 2u, range = (uint32_t)(ch.n - 1) * row_bytes + (uint32_t)dk * 2u;
-        const rsrc_t rk = make_rsrc(g.d.k + (size_t)ch.tok0 * g.d.qk_stride + hk * dk, range), rq = make_rsrc(g.d.q + (size_t)ch.tok0 * g.d.qk_stride + hk * dk, range);
-#pragma unroll
-        for (int i = 0; i < CPR; i += 4) {
-            const int slot = 64 * (i + wave) + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
-            const uint32_t off = 8 * x < dk ? (uint32_t)row * row_bytes + 16u * (uint32_t)x : 0x80000000u, to = (uint32_t)(uintptr_t)sh.kq + 1024u * (uint32_t)(i + wave);
-            dma16_untracked(rk, to, off);
-            dma16_untracked(rq, to + 1024u * CPR, off);
-        }
-    }
     if (w == 0) {
         const float gl = lane < ch.n ? g.d.decay[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
         bet[lane] = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
@@ -270,6 +276,19 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
         }
         const double top = rint(sum * 512.0) * (1.0 / 512.0);
         gam[lane] = f2{(float)top, (float)(sum - top)};
+    } else {
+        // (a wave that loads by DMA and waits for a register's load waits for both)
+        const uint32_t row_bytes = (uint32_t)g.d.qk_stride * 2u, range = (uint32_t)(ch.n - 1) * row_bytes + (uint32_t)dk * 2u;
+        const rsrc_t rk = make_rsrc(g.d.k + (size_t)ch.tok0 * g.d.qk_stride + hk * dk, range), rq = make_rsrc(g.d.q + (size_t)ch.tok0 * g.d.qk_stride + hk * dk, range);
+#pragma unroll
+        for (int c = 0; c < CPR; c += 3) {
+            const int i = c + w - 1;
+            if (i >= CPR) break;
+            const int slot = 64 * i + lane, row = slot / CPR, x = piece_at<CPR>(row, slot % CPR) - row * CPR;  // (its own inverse)
+            const uint32_t off = 8 * x < dk ? (uint32_t)row * row_bytes + 16u * (uint32_t)x : 0x80000000u, to = (uint32_t)(uintptr_t)sh.kq + 1024u * (uint32_t)i;
+            dma16_untracked(rk, to, off);
+            dma16_untracked(rq, to + 1024u * CPR, off);
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -316,11 +335,10 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
         mx = fmaxf(fmaxf(mx, fabsf(M[b][2])), fabsf(M[b][3]));
         *(f4 *)(sh.At + (16 * b + n) * LA + i0) = A[b];
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    mx = largest(mx);
     if (lane == 0) ms[w] = mx;
     __syncthreads();
-    {
+    if (w == 0) {  // (it had the least to do before)
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = i == n ? 1.f : 0.f;
@@ -328,14 +346,13 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 3 : 2) k_delta_prep(ChunkArgs g
         for (int j = 0; j < 15; j++)
 #pragma unroll
             for (int i4 = (j + 1) / 4; i4 < 4; i4++) {
-                const f4 a = *(const f4 *)(sh.At + (16 * w + j) * LA + 16 * w + 4 * i4);
+                const f4 a = *(const f4 *)(sh.At + (16 * q + j) * LA + 16 * q + 4 * i4);
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (4 * i4 + r > j) x[4 * i4 + r] = fmaf(-a[r], x[j], x[4 * i4 + r]);
             }
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (i / 4 == q) Td[w][i * LT + n] = x[i];
+        for (int i = 0; i < 16; i++) Td[q][i * LT + n] = x[i];
     }
     __syncthreads();
     f4 T[4];
