@@ -486,7 +486,7 @@ DEV float value_of(unsigned long long o) {
 
 template <bool F32>
 __global__ void __launch_bounds__(NT) k_beam(BeamArgs a) {
-    extern __shared__ unsigned long long lds[];  // the row's Shared, then the group's lists
+    alignas(16) extern __shared__ unsigned long long lds[];  // the row's Shared, then the group's lists
     __shared__ struct {
         float m[WAVES];
         double s[WAVES];

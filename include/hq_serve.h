@@ -53,8 +53,8 @@ void hq_batch_free(hq_batch *b);
  * counts may be 0. With n_new > n_pos the first n_new - n_pos tokens are padding before position 0: they see nothing, are
  * not stored, and give zeros. kv: the cache's geometry (its pointers may differ in each call that follows); n_heads: query
  * heads, a multiple of the kv heads (head h reads kv head h / (n_heads / n_kv_heads)). Page numbers are checked here.
- * Also plans hq_attention's work and grows its workspace: the only call of this header, with hq_batch_create and the
- * growing of hq_logprobs' workspace, that allocates. It waits until the last set's transfer is done, and with growing for
+ * Also plans hq_attention's work and grows its workspace: the only call on device memory of this header, with hq_batch_create,
+ * hq_scan_create and hq_scan_set, and the growing of hq_logprobs' and hq_beam's workspaces, that allocates. It waits until the last set's transfer is done, and with growing for
  * the device. Calls that use the batch must be ordered after it on the device, and the next set after them; calls that
  * overlap in time need batches of their own. */
 int hq_batch_set(hq_batch *b, const hq_kv_t *kv, int n_heads, int n_seqs, const int32_t *n_new, const int32_t *n_pos,
@@ -151,7 +151,8 @@ void hq_scan_free(hq_scan *c);
  * after sequence), goes on from the state in slot from[i] (-1: begins, all zeros) and leaves the state behind them in slot to[i]
  * (-1: nowhere). Without new tokens the state is copied. Several sequences may go on from one slot. No two leave theirs in one
  * slot, nor in a slot that another goes on from. st: the geometry (its pointers may differ in each call that follows). Plans the
- * work and grows the workspace: allocation, waiting and order as with hq_batch_set. */
+ * work and grows the workspace: allocation, waiting and order as with hq_batch_set (steps that overlap in time need descriptions of
+ * their own; a captured graph of a step's calls is good until the next hq_scan_set). */
 int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const int32_t *n_new, const int32_t *from, const int32_t *to, void *stream);
 
 typedef struct {
