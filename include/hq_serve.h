@@ -171,7 +171,7 @@ typedef struct {
 /* For every new token: y = silu(sum_j conv_w[j] x[t - (conv_taps - 1) + j]) over the sequence's inputs (the slot's before its
  * first new one), heads of queries and keys divided by sqrt(sum y^2 + eps), to qkv; decay = -e^a_log softplus(a + dt_bias), the
  * logarithm of the state's decay; beta = 1 / (1 + e^-b). Each sequence's last conv_taps - 1 inputs to its slot. fp32 arithmetic,
- * results rounded once. One kernel. */
+ * results rounded once. Outputs must not overlap inputs. One kernel. */
 int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_delta_in_t *r, void *stream);
 
 typedef struct {
@@ -200,7 +200,7 @@ typedef struct {
  * such, of more than 4) are taken in chunks of 64 tokens from their first, as products on the matrix cores whose operands are two fp16
  * terms each (2^-22 of a column's largest). Outputs are rounded once; with norm, those of chunks to fp16 before it too. A value that is
  * not a number stays in its value column (and head, with the norm), but there it may reach outputs of its chunk's earlier tokens. The
- * same step gives the same bits. Kernels in a row, no allocation. */
+ * same step gives the same bits. out must not overlap what is read. Kernels in a row, no allocation. */
 int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t *d, void *stream);
 
 /* ---- pages of sequences that branch and end */

@@ -64,3 +64,7 @@ def test_on_a_stream(hqlib):
     got = cs[0][2].keep[0].download((6, ps), np.uint16)
     assert (got == cs[0][0][0].reshape(6, ps)[0]).all()
     s.destroy()
+
+
+def test_more_caches_and_copies_than_a_launch_has(hqlib):
+    test_kv_copy(hqlib, False, 45, 700, 16, 1, 16, "pos", 300, True)
