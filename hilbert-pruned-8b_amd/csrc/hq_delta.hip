@@ -482,6 +482,15 @@ DEV float column_max(const f4 (&x)[N]) {
     }
 // OUT: outputs are formed. Without: a part's effect on states, Q from zeros or, from I and without values, P (a chunk takes some 1.8 us
 // either way: it is the way from state to state that bounds both).
+// N times a product, D reads of LDS and V arithmetic instructions
+#define MIX2(N, D, V)                                            \
+    if (KS <= 4) {                                               \
+        _Pragma("unroll") for (int i_ = 0; i_ < (N); i_++) {     \
+            __builtin_amdgcn_sched_group_barrier(8, 1, 0);       \
+            __builtin_amdgcn_sched_group_barrier(0x100, D, 0);   \
+            __builtin_amdgcn_sched_group_barrier(2, V, 0);       \
+        }                                                        \
+    }
 template <int KS, int W, bool OUT>
 __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
     constexpr int LW = 4;  // waves that load
@@ -697,27 +706,32 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
                 for (int b = 2 * s; b < 4; b++) U[b] = mfma(i == 0 ? Tl[frag_of(b, s)] : T[frag_of(b, s)], i == 1 ? Xl[s] : Xh[s], U[b]);
         MIX(18, 0x100, 1);
         STAGE;
-        h8 M[6], Ml[6];
-        if (OUT)
-#pragma unroll
-            for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i)), Ml[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M_LO + i));
-        read_columns(1);
+        // the state's products of the chunk's first half start while the second's operands and the outputs' are formed
         const float mu = column_max(U);
         bound = fmaf(bound, keep, 64.f * mu * pow2(in_range(uu)));
         const int next = exponent(bound) - 14;
         const float sd = pow2(in_range(uu - next + 127)), ratio = keep * pow2(in_range(unit - next + 127));
         unit = next;
         h8 Uh[2], Ul[2], Dh[2], Dl[2];
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const f4 x = U[2 * s] * sd, y = U[2 * s + 1] * sd, xd = x * dec[2 * s], yd = y * dec[2 * s + 1];
-            Uh[s] = halves(x, y);
-            if (OUT) Ul[s] = second_term(x, y, g.one, Uh[s]);
+        const auto written = [&](int s) {
+            const f4 xd = U[2 * s] * dec[2 * s], yd = U[2 * s + 1] * dec[2 * s + 1];
             Dh[s] = halves(xd, yd), Dl[s] = second_term(xd, yd, g.one, Dh[s]);
-        }
+        };
+        U[0] = U[0] * sd, U[1] = U[1] * sd;
+        written(0);
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = S[t] * ratio;
         STAGE;
+        h8 M[6], Ml[6];
+        if (OUT)
+#pragma unroll
+            for (int i = 0; i < 6; i++) M[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M + i)), Ml[i] = read16(f_at + 1024u * (uint32_t)(FRAG_M_LO + i));
+        read_columns(1);
+        U[2] = U[2] * sd, U[3] = U[3] * sd;
+        written(1);
+        if (OUT)
+#pragma unroll
+            for (int s = 0; s < 2; s++) Uh[s] = halves(U[2 * s], U[2 * s + 1]), Ul[s] = second_term(U[2 * s], U[2 * s + 1], g.one, Uh[s]);
         f4 y[4];
 #pragma unroll
         for (int b = 0; b < 4; b++) y[b] = f4{0.f, 0.f, 0.f, 0.f};
@@ -725,6 +739,8 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(0, t), Dl[0], S[t]);
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(0, t), Dh[0], S[t]);
+        MIX2(4 * KS, 2, 5);
+        STAGE;
         if (OUT)
 #pragma unroll
             for (int s = 0; s < 2; s++)
@@ -732,7 +748,10 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
                 for (int i = 0; i < 3; i++)
 #pragma unroll
                     for (int b = 2 * s; b < 4; b++) y[b] = mfma(i == 0 ? Ml[frag_of(b, s)] : M[frag_of(b, s)], i == 1 ? Ul[s] : Uh[s], y[b]);
-        MIX(4 * KS, 2, 2);
+        if (OUT)
+#pragma unroll
+            for (int b = 0; b < 4; b++) O[b] = eg[b] * g.d.scale * O[b];
+        if (OUT) MIX(18, 2, 2);
         STAGE;
         const float bu = pow2(next) * m_unit;
         const rsrc_t ro = make_rsrc(g.d.out + (size_t)(run.tok0 + c * HQ_CHUNK) * g.d.out_stride + (size_t)h * dv, (rows_of(c) - 1u) * o_bytes + (uint32_t)dv * 2u);
@@ -745,7 +764,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
             for (int b = 0; b < 4; b++)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)fmaf(bu, y[b][r], eg[b][r] * g.d.scale * O[b][r])), ro, o_off[4 * b + r], 0u, 0);
+                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)fmaf(bu, y[b][r], O[b][r])), ro, o_off[4 * b + r], 0u, 0);
         if (OUT) MIX(4 * KS, 2, 3);
         if ((c & 15) == 15) bound = column_max(S) * pow2(unit);
     }
