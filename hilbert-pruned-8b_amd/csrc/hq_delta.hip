@@ -599,7 +599,12 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
     // what a lane reads of K and Q, of K transposed and of V, as offsets into a chunk's buffer
 #pragma unroll
     for (int s = 0; s < KS; s++) k_in[s] = 16u * (uint32_t)piece_at<CPR>(token_of(0, n), 4 * s + q), t_in[s] = 16u * (uint32_t)piece_at<CPR>(8 * q + (n >> 2), 4 * s + (n & 3));
-    const uint32_t v_in = 1024u * AT_V + 16u * (uint32_t)(8 * q * VB + v_piece(8 * q, 2 * w + (n >> 3))) + 2u * (uint32_t)(n & 7);
+    // (wider keys: values one by one, since by columns, 12 instructions less, the kernel spills and takes 10 % longer)
+    constexpr bool BY_COLUMN = KS <= 4;
+    const uint32_t v_in = 1024u * AT_V + (BY_COLUMN ? 16u * (uint32_t)((8 * q + (n >> 2)) * VB + v_piece(8 * q, 2 * w + (n >> 1 & 1))) + 8u * (uint32_t)(n & 1)
+                                                    : 16u * (uint32_t)(8 * q * VB + v_piece(8 * q, 2 * w + (n >> 3))) + 2u * (uint32_t)(n & 7));
+    // lane i of a group of 16 hands over 4 values of row i / 4, and gets one column's of 4 rows
+    const auto read_tr = [](uint32_t at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(uintptr_t)at); };
     const auto read16 = [](uint32_t at) { return __builtin_bit_cast(h8, *(lds_u4 *)(uintptr_t)at); };
     for (int c = 0; c < chunks; c++) {
         if (BUFS == 1) __syncthreads();
@@ -625,7 +630,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int s = 0; s < KS; s++) Sh[s] = halves(S[2 * s], S[2 * s + 1]), Sl[s] = second_term(S[2 * s], S[2 * s + 1], g.one, Sh[s]);
         const float back = pow2(unit);
         f4 X[4], O[4], eg[4];
-        _Float16 V[16];
+        h4 V[4];
 #pragma unroll
         for (int b = 0; b < 4; b++) X[b] = O[b] = f4{0.f, 0.f, 0.f, 0.f};
         STAGE;
@@ -637,8 +642,10 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
                     eg[b] = rows4(0, b);
+                    if (BY_COLUMN) V[b] = __builtin_bit_cast(h4, read_tr(base + v_in + 16u * VB * (uint32_t)token_of(b, 0)));
+                    else
 #pragma unroll
-                    for (int r = 0; r < 4; r++) V[4 * b + r] = *(lds_h *)(uintptr_t)(base + v_in + 16u * VB * (uint32_t)token_of(b, r));
+                        for (int r = 0; r < 4; r++) V[b][r] = *(lds_h *)(uintptr_t)(base + v_in + 16u * VB * (uint32_t)token_of(b, r));
                 }
             }
 #pragma unroll
@@ -664,7 +671,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int b = 0; b < 4; b++) {
             eg[b] = eg[b] * back;
 #pragma unroll
-            for (int r = 0; r < 4; r++) X[b][r] = fmaf(-eg[b][r], X[b][r], (float)V[4 * b + r]);
+            for (int r = 0; r < 4; r++) X[b][r] = fmaf(-eg[b][r], X[b][r], (float)V[b][r]);
         }
         if (OUT) MIX(8 * AHEAD, 2, 2);
         STAGE;
@@ -684,14 +691,13 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int b = 0; b < 4; b++) U[b] = f4{0.f, 0.f, 0.f, 0.f};
         if (OUT) MIX(8 * (KS - AHEAD), 2, 3);
         STAGE;
-        // lane i of a group of 16 hands over 4 values of k_dim of row i / 4, and gets one of k_dim of 4 rows
         s4v Kt[2][2 * KS][2];
         const auto read_columns = [&](int s) {
 #pragma unroll
             for (int t = 0; t < 2 * KS; t++)
 #pragma unroll
                 for (int e = 0; e < 2; e++)
-                    Kt[s][t][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(uintptr_t)(t_at[t >> 1] + 8u * (uint32_t)(t & 1) + 16u * CPR * (uint32_t)(32 * s + 4 * e)));
+                    Kt[s][t][e] = read_tr(t_at[t >> 1] + 8u * (uint32_t)(t & 1) + 16u * CPR * (uint32_t)(32 * s + 4 * e));
         };
         const auto column = [&](int s, int t) { return __builtin_bit_cast(h8, __builtin_shufflevector(Kt[s][t][0], Kt[s][t][1], 0, 1, 2, 3, 4, 5, 6, 7)); };
         f4 dec[4];
