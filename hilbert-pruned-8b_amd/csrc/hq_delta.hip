@@ -789,17 +789,20 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 // The states between the parts of a sequence: S of the first part's end, then P S + Q of one after another, in place of Q. A workgroup has
 // 16 columns of a head, wave w the rows 16 w .. (and 128 on). The products are of 32 bits: an accumulator's four rows of block m are what
 // lane group q has of the contraction's steps 4 m .. 4 m + 3, so that a state's blocks lie in LDS as they come.
+// Bound: one way through memory and a chain of products: 32 heads of 128, three parts: 5.9 us (8.8 with a head's columns on eight XCDs).
 template <int KS>
-__global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *joins) {
+__global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *joins, int n_joins) {
     constexpr int RT = KS > 4 ? 2 : 1, KT = 8 * RT;
     __shared__ alignas(16) f4 at[2][KT][64];
     const int nv = g.st.n_v_heads, dk = g.st.k_dim, dv = g.st.v_dim, tiles = dv / 16, kt = dk / 16;
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
-    const int h = blockIdx.x / tiles % nv, col = 16 * (int)(blockIdx.x % tiles) + n;
-    const HqJoin jn = joins[blockIdx.x / tiles / nv];
+    // workgroup i runs on XCD i % 8: a head's on one, where they share its P
+    const int head = blockIdx.x / (8 * tiles) * 8 + blockIdx.x % 8, h = head % nv, col = 16 * (int)(blockIdx.x / 8 % tiles) + n;
+    if (head >= n_joins * nv) return;
+    const HqJoin jn = joins[head / nv];
     const size_t size = (size_t)dk * dv, place = (size_t)dk * max(dk, dv);
     const auto state = [&](int i) { return g.places + ((size_t)i * nv + h) * place; };
-    f4 x[RT], P[RT][KT];
+    f4 x[RT], y[RT], first[RT], P[RT][KT];
     const auto load = [&](const float *s, int t) {
         const float *const p = s + (size_t)(16 * (w + 8 * t) + 4 * q) * dv + col;
         return f4{p[0], p[dv], p[2 * dv], p[3 * dv]};
@@ -808,28 +811,29 @@ __global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *j
         float *const p = s + (size_t)(16 * (w + 8 * t) + 4 * q) * dv + col;
         p[0] = v[0], p[dv] = v[1], p[2 * dv] = v[2], p[3 * dv] = v[3];
     };
-    const auto load_p = [&](int j) {
+    const auto part = [&](int j) {  // its P and Q
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int t = 0; t < RT; t++) {
+            if (w + 8 * t >= kt) continue;
+            y[t] = load(state(jn.place + 1 + j), t);
 #pragma unroll
             for (int m = 0; m < KT; m++)
-                if (w + 8 * t < kt && m < kt) P[t][m] = *(const f4 *)(state(jn.place + jn.n + j - 1) + (size_t)(16 * (w + 8 * t) + n) * dk + 16 * m + 4 * q);
+                if (m < kt) P[t][m] = *(const f4 *)(state(jn.place + jn.n + j - 1) + (size_t)(16 * (w + 8 * t) + n) * dk + 16 * m + 4 * q);
+        }
     };
-    if (jn.n > 2) load_p(1);
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        if (w + 8 * t >= kt) continue;
-        if (jn.from != -1) store(state(jn.place), t, load(jn.from >= 0 ? g.st.s + ((size_t)jn.from * nv + h) * size : state(-2 - jn.from), t));
-        x[t] = load(state(jn.place + 1), t);
-    }
-    for (int j = 1; j < jn.n - 1; j++) {
-        f4 y[RT];
+    for (int t = 0; t < RT; t++)
+        if (w + 8 * t < kt) x[t] = load(state(jn.place + 1), t);
+    if (jn.n > 2) part(1);
+    if (jn.from != -1) {
 #pragma unroll
         for (int t = 0; t < RT; t++)
-            if (w + 8 * t < kt) {
-                y[t] = load(state(jn.place + 1 + j), t);
-                at[j & 1][w + 8 * t][lane] = x[t];
-            }
+            if (w + 8 * t < kt) first[t] = load(jn.from >= 0 ? g.st.s + ((size_t)jn.from * nv + h) * size : state(-2 - jn.from), t);
+    }
+    for (int j = 1; j < jn.n - 1; j++) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if (w + 8 * t < kt) at[j & 1][w + 8 * t][lane] = x[t];
         __syncthreads();  // (and the other half is free again: its readers have all come here)
 #pragma unroll
         for (int m = 0; m < KT; m++) {
@@ -841,10 +845,15 @@ __global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *j
 #pragma unroll
                     for (int r = 0; r < 4; r++) y[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(P[t][m][r], s[r], y[t], 0, 0, 0);
         }
-        if (j + 2 < jn.n) load_p(j + 1);
 #pragma unroll
         for (int t = 0; t < RT; t++)
             if (w + 8 * t < kt) store(state(jn.place + 1 + j), t, x[t] = y[t]);
+        if (j + 2 < jn.n) part(j + 1);
+    }
+    if (jn.from != -1) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if (w + 8 * t < kt) store(state(jn.place), t, first[t]);
     }
 }
 
@@ -898,7 +907,7 @@ void launch_chunks(ChunkArgs g, const HqPass &p, const HqRun *runs, const HqJoin
     if (p.n_parts) {
         g.runs = runs + p.part0, g.n_runs = p.n_parts;
         k_delta_scan<KS, W, false><<<grid(p.n_parts, std::max(dk, dv)), 64 * (W + 4), 0, s>>>(g);
-        k_delta_join<KS><<<(unsigned)p.n_joins * (unsigned)nv * (unsigned)(dv / 16), 512, 0, s>>>(g, joins + p.join0);
+        k_delta_join<KS><<<((unsigned)p.n_joins * (unsigned)nv + 7) / 8 * 8 * (unsigned)(dv / 16), 512, 0, s>>>(g, joins + p.join0, p.n_joins);
     }
     g.runs = runs + p.run0, g.n_runs = p.n_runs;
     k_delta_scan<KS, W, true><<<grid(p.n_runs, dv), 64 * (W + 4), 0, s>>>(g);
