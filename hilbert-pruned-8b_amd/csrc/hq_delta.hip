@@ -470,6 +470,11 @@ DEV float column_max(const f4 (&x)[N]) {
 // A column of S is held in units of a power of two, taken from a bound of its magnitudes (the bound before, decayed, and what a chunk can
 // add, 64 times its largest U as no key's element exceeds 1; every 16 chunks the largest itself): so S can enter products without a
 // look over it, and fp16's range leaves what the bound is too large by.
+//
+// Bound: the way from one state to the next, some 750 instructions of one wave in order, which its SIMD has for itself: 4400 clocks a chunk
+// (32 heads of 128), the products in them 2100; the outputs' work fills what the state's leaves. Products are started as soon as half of
+// their operands are there (both halves first: 3.5 % more). W columns' waves read the same operands from LDS: 4 waves; with 2 (1), one
+// sequence of 2048 tokens took 76 (74) us in place of 79, ten prompts of 16384 473 (679) in place of 411; with 8 a chunk takes twice as long.
 // (wider keys' operands do not all fit the registers: they are read where they are used)
 #define STAGE if (KS <= 4) __builtin_amdgcn_sched_barrier(0)
 // N times a product and M other instructions (what: 2 arithmetic, 0x100 reads of LDS), in the order of issue
@@ -859,7 +864,7 @@ __global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *j
 
 // The outputs' norm and gate of chunks, in place: G lanes a head, eight columns a lane. (The outputs have been rounded to fp16 by
 // then, 2^-11 of each beside the rounding of the result.)
-// Bound: bytes.
+// Bound: bytes. 16384 tokens of 32 heads of 128, gates in fp32: 537 MB in 100 us, 5.4 TB/s.
 template <int G, bool F32>
 __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
     const int nv = g.st.n_v_heads, dv = g.st.v_dim, u = threadIdx.x % G;
@@ -968,9 +973,10 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     }
     if (c->n_steps == 0) return 0;
     const DeltaArgs g = {*st, *d, c->seqs, c->steps};
-    // a head's waves in one workgroup; few heads without a norm, for which they would have to meet, a wave each
+    // A head's waves in one workgroup; few heads with one token and no norm, for which they would have to meet, a wave each: 32 heads 5.0
+    // us (in one workgroup 5.2), 128 6.5 (7.0), but of five tokens, whose keys each wave then fetches itself, 9.7 (9.4) and 13.1 (11.8).
     const int waves = (st->v_dim + 31) / 32, heads = c->n_steps * st->n_v_heads;
-    const bool apart = !d->norm && heads * waves <= 2 * c->n_cu;
+    const bool apart = !d->norm && c->longest_step <= 1 && heads * waves <= 2 * c->n_cu;
     const dim3 grid((unsigned)heads, apart ? (unsigned)waves : 1u);
     const unsigned threads = apart ? 64u : 64u * (unsigned)waves;
     if (st->k_dim == 64) k_delta_step<8, true><<<grid, threads, 0, s>>>(g);

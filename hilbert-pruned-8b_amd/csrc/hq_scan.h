@@ -65,7 +65,7 @@ struct hq_scan {
     const HqTile *tiles;  // of hq_delta_append: every sequence's first tile, which has its convolution's state, is there
     int n_tiles;
     const int *steps;  // the sequences that hq_delta takes token by token, longest first
-    int n_steps;
+    int n_steps, longest_step;  // (its tokens)
     const HqChunk *chunks;  // and those that it takes by chunks
     const HqRun *runs;      // (a pass's longest first)
     const HqJoin *joins;

@@ -38,8 +38,8 @@ int check_geometry(const char *who, const hq_state_t *st) {
 // effect on a state is formed (P and Q, all parts side by side, without outputs), then the states between them, then the outputs of all
 // parts side by side: two chains of a part's length and a product a part instead of one. It costs two launches, the states' way through
 // memory and the products, some 17 us, as much as 8 or 9 chunks: one sequence of 1000 tokens, 32 heads of 128, 47 us with it or without,
-// 2048: 82 without, 77 with, 6001: 215 and 173, 16000: 555 and 428. (Two workgroups a CU and so shorter parts: 90, 190, 467. All before
-// M and U had a second term in the outputs, which is 4 to 7 % more.)
+// 2048: 82 without, 77 with, 6001: 215 and 173, 16000: 555 and 428. (Two workgroups a CU and so shorter parts: 90, 190, 467. With what
+// followed, in parts: 2048 74, 6001 171, 16000 432.)
 constexpr int JOIN_CHUNKS = 9, LEAST_PART = 4;
 void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std::vector<HqRun> *runs, std::vector<HqJoin> *joins, int *places) {
     const int cols = hq_scan_columns(st->k_dim);
@@ -257,7 +257,7 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     c->tiles = (const HqTile *)dev(), c->n_tiles = (int)tiles.size();
     if (!tiles.empty()) memcpy(w, tiles.data(), tiles.size() * sizeof(HqTile));
     w += tiles.size() * (sizeof(HqTile) / 4);
-    c->steps = dev(), c->n_steps = (int)steps.size();
+    c->steps = dev(), c->n_steps = (int)steps.size(), c->longest_step = steps.empty() ? 0 : n_new[steps[0]];
     if (!steps.empty()) memcpy(w, steps.data(), steps.size() * 4);
     w += steps.size();
     c->chunks = (const HqChunk *)dev();
@@ -314,6 +314,8 @@ DEV float silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdg
 // input is read once for a tile and taps - 1 times more at its border, four tokens ahead of its use. The tile with a sequence's first
 // token reads the slot's inputs and writes those that the sequence leaves: the same lane the same channels, so one slot may be both.
 // TAPS: conv_taps, or with EXACT false more: taps beyond it have no input and no weight.
+// Bound: bytes. 2048 tokens of 8192 channels, fp32: 100 MB in 26.5 us, 3.8 TB/s, a few us of them the launch and its ends (57 with a load
+// a token waited for, and weights one by one); 16 single tokens 5.1 us, launch and two loads that wait for each other.
 template <bool F32, int G, int TAPS, bool EXACT>
 __global__ void __launch_bounds__(256) k_delta_append(AppendArgs g) {
     const HqTile tile = g.tiles[blockIdx.x];
