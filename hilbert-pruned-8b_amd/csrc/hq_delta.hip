@@ -944,7 +944,7 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
         // a chunk's rows are addressed by 32 bits
         if (!c->passes.empty())
             for (int64_t s : {d->qk_stride, d->v_stride, d->out_stride})
-                if (s > MOST_CHUNK_STRIDE) return hq_internal_fail("%s: stride %lld (with more than %d new tokens of a sequence at most %lld)", who, (long long)s, HQ_STEP_TOKENS, (long long)MOST_CHUNK_STRIDE);
+                if (s > MOST_CHUNK_STRIDE) return hq_internal_fail("%s: stride %lld (with more than %d new tokens of a sequence at most %lld)", who, (long long)s, HQ_STEP_ALONE, (long long)MOST_CHUNK_STRIDE);
         if (!(fabsf(d->scale) <= 1e20f)) return hq_internal_fail("%s: scale %g", who, (double)d->scale);
     }
     int cur = -1;

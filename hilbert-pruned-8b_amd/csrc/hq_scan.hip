@@ -180,9 +180,13 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
                 if (r[k].second != w[i].second) return hq_internal_fail("%s: sequence %d goes on from slot %d, where sequence %d leaves its state", who, r[k].second, w[i].first, w[i].second);
         }
         std::vector<std::pair<int, int>> long_seqs;
-        int64_t few = 0, many = 0;
-        for (int i = 0; i < n_seqs; i++) few += n_new[i] > HQ_STEP_BESIDE && n_new[i] <= HQ_STEP_TOKENS, many += n_new[i] > HQ_STEP_TOKENS;
-        const int by_steps = many && few * st->n_v_heads <= 4 * c->n_cu ? HQ_STEP_BESIDE : HQ_STEP_TOKENS;
+        int64_t all = 0, few = 0;
+        int longest = 0;
+        for (int i = 0; i < n_seqs; i++) all += n_new[i] > 0, few += n_new[i] > HQ_STEP_BESIDE && n_new[i] <= HQ_STEP_TOKENS, longest = std::max(longest, n_new[i]);
+        const int cols = hq_scan_columns(st->k_dim);
+        int by_steps = HQ_STEP_TOKENS;
+        if (longest > HQ_STEP_ALONE && all * st->n_v_heads * ((st->v_dim + cols - 1) / cols) <= c->n_cu) by_steps = 0;
+        else if (longest > HQ_STEP_TOKENS && few * st->n_v_heads <= 4 * c->n_cu) by_steps = HQ_STEP_BESIDE;
         for (int i = 0, tok = 0; i < n_seqs; tok += n_new[i], i++) {
             if (n_new[i] == 0 && (to[i] < 0 || to[i] == from[i])) continue;
             for (int t = 0; t == 0 || t < n_new[i]; t += HQ_CONV_TILE) tiles.push_back({i, t, std::min(HQ_CONV_TILE, n_new[i] - t)});

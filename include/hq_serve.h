@@ -176,7 +176,7 @@ int hq_delta_append(const hq_scan *c, const hq_state_t *st, const hq_delta_in_t 
 
 typedef struct {
     /* fp16: head h of token t at q and k + t * qk_stride + h * k_dim, v + t * v_stride + h * v_dim; 16-byte aligned, strides
-     * multiples of 8, those and out_stride no less than the heads of a token (and at most 2^22 where a sequence has more than 16
+     * multiples of 8, those and out_stride no less than the heads of a token (and at most 2^22 where a sequence has more than 8
      * new tokens) */
     const uint16_t *q, *k, *v;
     int64_t qk_stride, v_stride;
@@ -196,9 +196,9 @@ typedef struct {
 
 /* For every new token, value head and its key head, from the sequence's state: S' = e^decay S; S = S' + k (beta (v - S'^T k))^T;
  * o = scale S^T q. States to their slots. Keys are to have a norm of at most 1 and beta to lie in 0 .. 1 (as hq_delta_append gives
- * them): the recurrence itself grows without bound otherwise. States and sums are fp32; sequences of more than 16 new tokens (beside
- * such, of more than 4) are taken in chunks of 64 tokens from their first, as products on the matrix cores whose operands are two fp16
- * terms each (2^-22 of a column's largest). Outputs are rounded once; with norm, those of chunks to fp16 before it too. A value that is
+ * them): the recurrence itself grows without bound otherwise. States and sums are fp32; sequences of more than 16 new tokens (fewer,
+ * where it is the faster way) are taken in chunks of 64 tokens from their first, as products on the matrix cores whose operands are two
+ * fp16 terms each (2^-22 of a column's largest). Outputs are rounded once; with norm, those of chunks to fp16 before it too. A value that is
  * not a number stays in its value column (and head, with the norm), but there it may reach outputs of its chunk's earlier tokens. The
  * same step gives the same bits. out must not overlap what is read. Kernels in a row, no allocation. */
 int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t *d, void *stream);

@@ -272,3 +272,14 @@ def test_more_chunks_than_a_pass_has(hqlib, hk, hv, d, seqs, heads):
         assert (np.abs(y[:, two] - want) <= bound).all()
         for i, a, b in zip(dst, after, e):
             assert (np.abs(s[i][two] - a) <= b + U_MIN).all() and np.sqrt(((s[i][two] - a) ** 2).mean()) <= 2.0 ** -19 * np.sqrt((a * a).mean())
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv,gate", [(4, 64, 64, 32, np.float32), (32, 64, 128, 64, None), (8, 72, 256, 48, np.float16), (5, 65, 48, 16, None)])
+def test_some_tokens_of_many_heads(hqlib, hk, hv, dk, dv, gate):
+    """Enough heads for sequences of up to 16 tokens to go token by token, eight at a time."""
+    check(hqlib, 60 + hv, hk, hv, dk, dv, [(16, 0, 0), (9, 1, 6), (0, 2, 2), (1, -1, 3), (13, 3 + 1, -1), (8, 5, 7)], gate)
+
+
+def test_some_tokens_of_few_heads(hqlib):
+    """The same by chunks, a sequence of one token among them."""
+    check(hqlib, 61, 1, 2, 128, 128, [(16, 0, 0), (9, 1, 6), (0, 2, 2), (1, -1, 3), (13, 3 + 1, -1), (8, 5, 7)], np.float32)
