@@ -58,8 +58,12 @@ void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std
             }
             return outputs + (rest + part - 1) / part * units <= n_cu && effects <= n_cu;
         };
-        int part = LEAST_PART;
-        while (part < longest && !fits(part)) part++;
+        int part = LEAST_PART, above = longest;  // the shortest that fits: `above` does, or is the whole
+        while (part < above) {
+            const int mid = (part + above) / 2;
+            if (fits(mid)) above = mid;
+            else part = mid + 1;
+        }
         const bool split = longest > 2 * part + JOIN_CHUNKS;
         const int run0 = (int)all.size();
         parts.clear();
