@@ -214,6 +214,7 @@ struct ChunkArgs {
     int n_runs, n_chunks;
     char *work;
     float *places;  // states of the workspace
+    float *outs;    // outputs ahead of their norm, 64 rows of v_dim for each chunk of the pass and value head
     float one;  // 1: a factor that the compiler does not know, so that a difference is one fused instruction
 };
 
@@ -485,8 +486,10 @@ DEV float column_max(const f4 (&x)[N]) {
             __builtin_amdgcn_sched_group_barrier(what, M, 0);    \
         }                                                        \
     }
-// OUT: outputs are formed. Without: a part's effect on states, Q from zeros or, from I and without values, P (a chunk takes some 1.8 us
-// either way: it is the way from state to state that bounds both).
+// OUT: outputs are formed, in fp16 where they belong or, ahead of their norm, in fp32 (in fp16 they would be rounded twice, and the norm
+// takes sizes that fp16 has not). Without: a part's effect on states, Q from zeros or, from I and without values, P (a chunk takes some
+// 1.8 us either way: it is the way from state to state that bounds both).
+enum { STATES_ONLY, TO_OUT, TO_NORM };
 // N times a product, D reads of LDS and V arithmetic instructions
 #define MIX2(N, D, V)                                            \
     if (KS <= 4) {                                               \
@@ -496,7 +499,7 @@ DEV float column_max(const f4 (&x)[N]) {
             __builtin_amdgcn_sched_group_barrier(2, V, 0);       \
         }                                                        \
     }
-template <int KS, int W, bool OUT>
+template <int KS, int W, int OUT>
 __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
     constexpr int LW = 4;  // waves that load
     constexpr int CPR = 4 * KS < 8 ? 8 : 4 * KS;
@@ -597,10 +600,11 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = S[t] * to_unit;
     }
-    const uint32_t o_bytes = (uint32_t)g.d.out_stride * 2u;
+    constexpr uint32_t O_SIZE = OUT == TO_NORM ? 4 : 2;
+    const uint32_t o_bytes = OUT == TO_NORM ? (uint32_t)dv * 4u : (uint32_t)g.d.out_stride * 2u;
     uint32_t o_off[16], k_in[KS], t_in[KS];
 #pragma unroll
-    for (int i = 0; i < 16; i++) o_off[i] = (uint32_t)token_of(i >> 2, 4 * q + (i & 3)) * o_bytes + 2u * (uint32_t)col;
+    for (int i = 0; i < 16; i++) o_off[i] = (uint32_t)token_of(i >> 2, 4 * q + (i & 3)) * o_bytes + O_SIZE * (uint32_t)col;
     // what a lane reads of K and Q, of K transposed and of V, as offsets into a chunk's buffer
 #pragma unroll
     for (int s = 0; s < KS; s++) k_in[s] = 16u * (uint32_t)piece_at<CPR>(token_of(0, n), 4 * s + q), t_in[s] = 16u * (uint32_t)piece_at<CPR>(8 * q + (n >> 2), 4 * s + (n & 3));
@@ -765,7 +769,8 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         if (OUT) MIX(18, 2, 2);
         STAGE;
         const float bu = pow2(next) * m_unit;
-        const rsrc_t ro = make_rsrc(g.d.out + (size_t)(run.tok0 + c * HQ_CHUNK) * g.d.out_stride + (size_t)h * dv, (rows_of(c) - 1u) * o_bytes + (uint32_t)dv * 2u);
+        const rsrc_t ro = OUT == TO_NORM ? make_rsrc(g.outs + ((size_t)(run.chunk0 + c) * nv + h) * HQ_CHUNK * dv, rows_of(c) * o_bytes)
+                                         : make_rsrc(g.d.out + (size_t)(run.tok0 + c * HQ_CHUNK) * g.d.out_stride + (size_t)h * dv, (rows_of(c) - 1u) * o_bytes + (uint32_t)dv * 2u);
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dl[1], S[t]);
 #pragma unroll
@@ -774,8 +779,11 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
             for (int b = 0; b < 4; b++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)fmaf(bu, y[b][r], O[b][r])), ro, o_off[4 * b + r], 0u, 0);
+                for (int r = 0; r < 4; r++) {
+                    const float o = fmaf(bu, y[b][r], O[b][r]);
+                    if (OUT == TO_NORM) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, o), ro, o_off[4 * b + r], 0u, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)o), ro, o_off[4 * b + r], 0u, 0);
+                }
         if (OUT) MIX(4 * KS, 2, 3);
         if ((c & 15) == 15) bound = column_max(S) * pow2(unit);
     }
@@ -862,9 +870,8 @@ __global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *j
     }
 }
 
-// The outputs' norm and gate of chunks, in place: G lanes a head, eight columns a lane. (The outputs have been rounded to fp16 by
-// then, 2^-11 of each beside the rounding of the result.)
-// Bound: bytes. 16384 tokens of 32 heads of 128, gates in fp32: 537 MB in 100 us, 5.4 TB/s.
+// The norm and gate of chunks' outputs, from the workspace to where they belong: G lanes a head, eight columns a lane.
+// Bound: bytes. 16384 tokens of 32 heads of 128, gates in fp32: 671 MB in 134 us, 5.0 TB/s (from fp16 outputs 537 MB in 101).
 template <int G, bool F32>
 __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
     const int nv = g.st.n_v_heads, dv = g.st.v_dim, u = threadIdx.x % G;
@@ -876,8 +883,8 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
         const size_t in = (size_t)h * dv + (on ? 8 * u : 0);
         for (int t = blockIdx.y; t < ch.n; t += gridDim.y) {
             const size_t tok = (size_t)(ch.tok0 + t), zat = tok * g.d.gate_stride + in;
-            _Float16 *const at = (_Float16 *)g.d.out + tok * g.d.out_stride + in;
-            const h8 x = *(const h8 *)at;
+            const float *const from = g.outs + (((size_t)blockIdx.x * nv + h) * HQ_CHUNK + t) * dv + (on ? 8 * u : 0);
+            const f4 xa = *(const f4 *)from, xb = *(const f4 *)(from + 4);
             float z[8];
             if (F32) {
                 const f4 a = *(const f4 *)((const float *)g.d.gate + zat), b = *(const f4 *)((const float *)g.d.gate + zat + 4);
@@ -890,15 +897,15 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
             }
             float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) ss = fmaf((float)x[e], (float)x[e], ss);
+            for (int e = 0; e < 4; e++) ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
             if (!on) ss = 0.f;
 #pragma unroll
             for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
             const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
             h8 y;
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = (_Float16)((float)x[e] * inv * (e < 4 ? wa[e & 3] : wb[e & 3]) * silu(z[e]));
-            if (on) *(h8 *)at = y;
+            for (int e = 0; e < 4; e++) y[e] = (_Float16)(xa[e] * inv * wa[e] * silu(z[e])), y[4 + e] = (_Float16)(xb[e] * inv * wb[e] * silu(z[4 + e]));
+            if (on) *(h8 *)((_Float16 *)g.d.out + tok * g.d.out_stride + in) = y;
         }
     }
 }
@@ -911,11 +918,12 @@ void launch_chunks(ChunkArgs g, const HqPass &p, const HqRun *runs, const HqJoin
     const auto grid = [&](int n, int cols) { return ((unsigned)n * (unsigned)nv + 7) / 8 * 8 * (unsigned)((cols + 16 * W - 1) / (16 * W)); };
     if (p.n_parts) {
         g.runs = runs + p.part0, g.n_runs = p.n_parts;
-        k_delta_scan<KS, W, false><<<grid(p.n_parts, std::max(dk, dv)), 64 * (W + 4), 0, s>>>(g);
+        k_delta_scan<KS, W, STATES_ONLY><<<grid(p.n_parts, std::max(dk, dv)), 64 * (W + 4), 0, s>>>(g);
         k_delta_join<KS><<<((unsigned)p.n_joins * (unsigned)nv + 7) / 8 * 8 * (unsigned)(dv / 16), 512, 0, s>>>(g, joins + p.join0, p.n_joins);
     }
     g.runs = runs + p.run0, g.n_runs = p.n_runs;
-    k_delta_scan<KS, W, true><<<grid(p.n_runs, dv), 64 * (W + 4), 0, s>>>(g);
+    if (g.d.norm) k_delta_scan<KS, W, TO_NORM><<<grid(p.n_runs, dv), 64 * (W + 4), 0, s>>>(g);
+    else k_delta_scan<KS, W, TO_OUT><<<grid(p.n_runs, dv), 64 * (W + 4), 0, s>>>(g);
 }
 
 }  // namespace
@@ -952,7 +960,7 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     if (cur != c->device) SCK(hipSetDevice(c->device));
     hipStream_t s = (hipStream_t)stream;
     for (const HqPass &p : c->passes) {
-        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), 1.0f};
+        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), (float *)(c->work + c->outs_at), 1.0f};
         if (st->k_dim <= 64) launch_chunks<2>(g, p, c->runs, c->joins, s);
         else if (st->k_dim <= 128) launch_chunks<4>(g, p, c->runs, c->joins, s);
         else launch_chunks<8>(g, p, c->runs, c->joins, s);

@@ -72,8 +72,9 @@ struct hq_scan {
     const HqRun *runs;      // (a pass's longest first)
     const HqJoin *joins;
     std::vector<HqPass> passes;
-    char *work;             // chunks of a pass, then places for states, each n_v_heads * k_dim * max(k_dim, v_dim) long
-    size_t work_bytes, places_at;
+    char *work;             // chunks of a pass, then their outputs ahead of a norm (fp32: 64 rows of n_v_heads * v_dim a chunk), then places for
+                            // states, each n_v_heads * k_dim * max(k_dim, v_dim) long
+    size_t work_bytes, outs_at, places_at;
     // storage: one pinned copy of `dev`, which the next set waits for
     int *host, *dev;
     size_t words;

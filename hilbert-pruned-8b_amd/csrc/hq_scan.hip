@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr size_t MOST_WORK = (size_t)640 << 20;  // of the chunks of a pass
+constexpr size_t MOST_WORK = (size_t)640 << 20;  // of the chunks of a pass (their outputs ahead of a norm are beside it, 2.6 times as much at most)
 
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
@@ -243,9 +243,10 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
         SCK(hipHostMalloc((void **)&c->host, want * 4, hipHostMallocDefault));
         c->words = want;
     }
-    size_t work = 0;
-    for (const HqPass &p : passes) work = std::max(work, (size_t)p.n_chunks * per_chunk);
-    c->places_at = work;
+    size_t most = 0;  // chunks of a pass
+    for (const HqPass &p : passes) most = std::max(most, (size_t)p.n_chunks);
+    const size_t outs_at = most * per_chunk, places_at = outs_at + most * HQ_CHUNK * (size_t)st->n_v_heads * (size_t)st->v_dim * 4;
+    size_t work = places_at;
     work += (size_t)places * st->n_v_heads * st->k_dim * std::max(st->k_dim, st->v_dim) * 4;
     if (work > c->work_bytes) {
         SCK(hipDeviceSynchronize());
@@ -278,6 +279,7 @@ extern "C" int hq_scan_set(hq_scan *c, const hq_state_t *st, int n_seqs, const i
     if (!joins.empty()) memcpy(w, joins.data(), joins.size() * sizeof(HqJoin));
     w += joins.size() * (sizeof(HqJoin) / 4);
     c->passes.swap(passes);
+    c->outs_at = outs_at, c->places_at = places_at;
     const size_t used = (size_t)(w - c->host);
     if (used) {
         SCK(hipMemcpyAsync(c->dev, c->host, used * 4, hipMemcpyHostToDevice, (hipStream_t)stream));
