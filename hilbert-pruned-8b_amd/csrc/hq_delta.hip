@@ -16,11 +16,42 @@ constexpr int64_t MOST_CHUNK_STRIDE = 1 << 22;  // 64 rows of it stay below 2^29
 // z / (1 + e^-z) with the hardware's exponential and reciprocal (2^-22 of the result together; -inf gives NaN, as the formula)
 DEV float silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
 
+// x 2^e / sqrt(mean (x 2^e)^2 + eps) of a head's dv values, N of them in each of G neighbouring lanes (zeros behind dv). e is that of the
+// scale, which outputs ahead of their norm are formed without, as it goes up to 1e20 and the norm takes it out again. The squares of values that
+// are far from 1 leave fp32's range all the same: where their mean is not well inside it, of values over a power of two of the largest.
+template <int N, int G>
+DEV void normalise(float (&x)[N], int dv, float eps, int e) {
+    const auto mean = [&](int by) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        return ss / (float)dv + ldexpf(eps, 2 * by);
+    };
+    float ms = mean(-e);
+    if (!(ms > 1e-30f && ms < INFINITY)) {  // (all of a head's lanes, or none)
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) m = max(m, __builtin_bit_cast(uint32_t, fabsf(x[i])));  // (magnitudes: their order as integers)
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+        const int to_1 = min(max(127 - (int)(m >> 23), -126), 126);
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = ldexpf(x[i], to_1);
+        ms = mean(to_1 - e);
+    }
+    const float inv = 1.0f / sqrtf(ms);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] *= inv;
+}
+
 struct DeltaArgs {
     hq_state_t st;
     hq_delta_t d;
     const HqSeq *seqs;
     const int *steps;
+    int scale_exp;  // with a norm: of the scale, whose rest d.scale is
 };
 
 // The sum of x over the lane groups of eight: all lanes have it. (Elements are bit-cast from plain scalars.)
@@ -144,17 +175,15 @@ __global__ void __launch_bounds__(512, ROWS <= 16 ? 4 : 2) k_delta_step(DeltaArg
         __syncthreads();
         for (int t = tid >> 6; t < m; t += nt >> 6) {
             const int d = 4 * lane;
-            f4 y = {0.f, 0.f, 0.f, 0.f};
-            if (d < dv) y = *(const f4 *)(o[t] + d);
-            float ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
-#pragma unroll
-            for (int i = 32; i > 0; i >>= 1) ss += __shfl_xor(ss, i, 64);
-            const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
+            f4 at = {0.f, 0.f, 0.f, 0.f};
+            if (d < dv) at = *(const f4 *)(o[t] + d);
+            float y[4] = {at[0], at[1], at[2], at[3]};
+            normalise<4, 64>(y, dv, g.d.eps, g.scale_exp);
             if (d >= dv) continue;
             const f4 zz = *(const f4 *)(z[t] + d), nw = *(const f4 *)(g.d.norm + d);
             h4 w;
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = (_Float16)(y[e] * inv * nw[e] * silu(zz[e]));
+            for (int e = 0; e < 4; e++) w[e] = (_Float16)(y[e] * nw[e] * silu(zz[e]));
             *(h4 *)((_Float16 *)g.d.out + (tok0 + t) * g.d.out_stride + (size_t)h * dv + d) = w;
         }
     }
@@ -215,6 +244,7 @@ struct ChunkArgs {
     char *work;
     float *places;  // states of the workspace
     float *outs;    // outputs ahead of their norm, 64 rows of v_dim for each chunk of the pass and value head
+    int scale_exp;  // with a norm: of the scale, whose rest d.scale is
     float one;  // 1: a factor that the compiler does not know, so that a difference is one fused instruction
 };
 
@@ -884,7 +914,10 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
         for (int t = blockIdx.y; t < ch.n; t += gridDim.y) {
             const size_t tok = (size_t)(ch.tok0 + t), zat = tok * g.d.gate_stride + in;
             const float *const from = g.outs + (((size_t)blockIdx.x * nv + h) * HQ_CHUNK + t) * dv + (on ? 8 * u : 0);
+            float x[8];
             const f4 xa = *(const f4 *)from, xb = *(const f4 *)(from + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = on ? xa[e] : 0.f, x[4 + e] = on ? xb[e] : 0.f;
             float z[8];
             if (F32) {
                 const f4 a = *(const f4 *)((const float *)g.d.gate + zat), b = *(const f4 *)((const float *)g.d.gate + zat + 4);
@@ -895,16 +928,10 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) z[e] = (float)a[e];
             }
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; e++) ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
-            if (!on) ss = 0.f;
-#pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const float inv = 1.0f / sqrtf(ss / (float)dv + g.d.eps);
+            normalise<8, G>(x, dv, g.d.eps, g.scale_exp);
             h8 y;
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = (_Float16)(xa[e] * inv * wa[e] * silu(z[e])), y[4 + e] = (_Float16)(xb[e] * inv * wb[e] * silu(z[4 + e]));
+            for (int e = 0; e < 8; e++) y[e] = (_Float16)(x[e] * (e < 4 ? wa[e & 3] : wb[e & 3]) * silu(z[e]));
             if (on) *(h8 *)((_Float16 *)g.d.out + tok * g.d.out_stride + in) = y;
         }
     }
@@ -959,8 +986,11 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     SCK(hipGetDevice(&cur));
     if (cur != c->device) SCK(hipSetDevice(c->device));
     hipStream_t s = (hipStream_t)stream;
+    hq_delta_t in = *d;
+    int scale_exp = 0;
+    if (in.norm) in.scale = frexpf(in.scale, &scale_exp);
     for (const HqPass &p : c->passes) {
-        const ChunkArgs g = {*st, *d, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), (float *)(c->work + c->outs_at), 1.0f};
+        const ChunkArgs g = {*st, in, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), (float *)(c->work + c->outs_at), scale_exp, 1.0f};
         if (st->k_dim <= 64) launch_chunks<2>(g, p, c->runs, c->joins, s);
         else if (st->k_dim <= 128) launch_chunks<4>(g, p, c->runs, c->joins, s);
         else launch_chunks<8>(g, p, c->runs, c->joins, s);
@@ -980,7 +1010,7 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
         SCK(hipGetLastError());
     }
     if (c->n_steps == 0) return 0;
-    const DeltaArgs g = {*st, *d, c->seqs, c->steps};
+    const DeltaArgs g = {*st, in, c->seqs, c->steps, scale_exp};
     // A head's waves in one workgroup; few heads with one token and no norm, for which they would have to meet, a wave each: 32 heads 5.0
     // us (in one workgroup 5.2), 128 6.5 (7.0), but of five tokens, whose keys each wave then fetches itself, 9.7 (9.4) and 13.1 (11.8).
     const int waves = (st->v_dim + 31) / 32, heads = c->n_steps * st->n_v_heads;

@@ -99,3 +99,52 @@ def test_the_company_of_other_sequences(hqlib):
             m = len(parts)
             y, _ = go(hqlib, x[:T], g[:T], beta[:T], states, parts, [0] + [-1] * (m - 1), [-1] * m, hk, hv, dk, dv, gate[:T], norm, eps=1e-6, scale=10.0)
         assert (np.abs(y[:n] - want) <= bound).all(), parts[:3]
+
+
+@pytest.mark.parametrize("seqs", [STEPS, CHUNKS], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 32), (96, 192)])
+@pytest.mark.parametrize("size,eps", [(4e18, 1e-6), (3e19, 0.0), (1e-16, 0.0), (1e-25, 0.0), (1e-30, 1e-38)])
+def test_squares_beyond_fp32(hqlib, seqs, dk, dv, size, eps):
+    """Outputs whose squares pass fp32's range, or vanish in it, through the scale that hq_delta takes."""
+    hk, hv = 1, 2
+    rng = np.random.default_rng(5)
+    n_new, src, dst = [list(a) for a in zip(*seqs)]
+    x, g, beta = inputs(rng, sum(n_new), hk, hv, dk, dv)
+    x[1, 2 * hk * dk:] = 0
+    beta[1] = 0
+    states = rng.normal(0, 4, (max(src + dst) + 2, hv, dk, dv)).astype(np.float32)
+    before = [states[i] if i >= 0 else np.zeros((hv, dk, dv), np.float32) for i in src]
+    o, b, after, e = delta(*split(x, hk, hv, dk, dv), g, beta, before, n_new, 1.0)
+    b = b - U16 * np.abs(o) - 2.0 ** -25
+    scale = float(np.float32(min(size / np.sqrt((o * o).mean()), 1e20)))
+    gate, norm = rng.normal(0, 2, (sum(n_new), hv, dv)).astype(np.float32), rng.normal(1, 0.2, dv).astype(np.float32)
+    print(f"[gpu] delta norm {dk}, {dv} {seqs} outputs of {size} eps={eps}", flush=True)
+    y, _ = go(hqlib, x, g, beta, states, n_new, src, dst, hk, hv, dk, dv, gate, norm, eps=eps, scale=scale)
+    want, bound = normed(scale * o, scale * b, gate, norm, float(np.float32(eps)))
+    assert (np.abs(y - want) <= bound).all()
+    once = np.sqrt(((want.astype(np.float16).astype(np.float64) - want) ** 2).mean())
+    assert np.sqrt(((y - want) ** 2).mean()) <= 1.1 * once
+
+
+@pytest.mark.parametrize("seqs", [STEPS, CHUNKS], ids=["tokens", "chunks"])
+def test_outputs_beyond_fp32(hqlib, seqs):
+    """Outputs that the scale would take beyond fp32 (one column of 1e45 and more: it has the head's norm, and the others are nothing beside it);
+    rows of zeros, which are 0 for eps above 0."""
+    hk, hv, dk, dv = 1, 1, 64, 64
+    rng = np.random.default_rng(6)
+    n_new, src, dst = [list(a) for a in zip(*seqs)]
+    T = sum(n_new)
+    x, g, beta = inputs(rng, T, hk, hv, dk, dv)
+    states = rng.normal(0, 4, (max(src + dst) + 2, hv, dk, dv)).astype(np.float32)
+    x[2, :hk * dk] = 0  # a query of zeros
+    states[0, 0, :, 5] = 1e30
+    x[:, :2 * hk * dk] = np.abs(x[:, :2 * hk * dk])  # (queries and keys of one sign: nothing cancels in the column)
+    g[:3], beta[:3] = 0, 0
+    gate, norm = rng.normal(0, 2, (T, hv, dv)).astype(np.float32), np.ones(dv, np.float32)
+    print(f"[gpu] delta norm beyond fp32 {seqs}", flush=True)
+    y, _ = go(hqlib, x, g, beta, states, n_new, src, [-1] * len(dst), hk, hv, dk, dv, gate, norm, eps=1e-6, scale=1e15)
+    before = [states[i] if i >= 0 else np.zeros((hv, dk, dv), np.float32) for i in src]
+    o, b, *_ = delta(*split(x, hk, hv, dk, dv), g, beta, before, n_new, 1.0)
+    want, bound = normed(1e15 * o, 1e15 * (b - U16 * np.abs(o) - 2.0 ** -25), gate, norm, 1e-6)
+    assert (np.abs(want[:2, 0, 5] / silu(gate[:2, 0, 5].astype(np.float64)) - 8) < 1e-6).all() and (want[2] == 0).all()
+    assert (np.abs(y[:3] - want[:3]) <= bound[:3]).all()
