@@ -210,11 +210,10 @@ __global__ void __launch_bounds__(512, ROWS <= 16 ? 4 : 2) k_delta_step(DeltaArg
 // likewise.
 //
 // Precision: K, Q and V are exact. S, U, T and M enter products as two fp16 terms each, scaled by a power of two of their column's largest
-// (T and M: of the matrix), good to 2^-22 of it. (One term of S, M and U for the outputs, which end in fp16, made them 1.6 to 1.8 times
+// (T and M: of the matrix; T's is the largest beta, which stands on its diagonal), good to 2^-22 of it. (One term of S, M and U for the outputs, which end in fp16, made them 1.6 to 1.8 times
 // as inexact as their own rounding does.)
 constexpr int FRAG_T = 0, FRAG_T_LO = 6, FRAG_M = 12, FRAG_M_LO = 18, FRAG_VEC = 24;  // of a chunk's workspace, in KB; fragments (block, half) in the order below
-constexpr int T_BITS = 12;  // T is held 2^12 times as large
-constexpr float T_SCALE = 1 << T_BITS;
+constexpr int T_EXP = 265;  // T's largest entry has an exponent e, and is held as pow2(T_EXP - e) times it, 2^11 .. 2^12
 DEV int frag_of(int b, int s) { return b < 2 ? b : 2 * b - 2 + s; }
 DEV int token_of(int b, int row) { return 32 * (b >> 1) + 8 * (row >> 2) + (row & 3) + 4 * (b & 1); }
 // A row's 16-byte pieces lie in LDS in an order of the row's own, so that what is read together falls into different banks: a piece of
@@ -287,6 +286,7 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 4 : 2) k_delta_prep(ChunkArgs g
     __shared__ alignas(16) float Td[4][16 * LT];
     __shared__ alignas(16) f2 gam[64];
     __shared__ alignas(16) float bet[64], ms[4];
+    __shared__ int t_exp;
     // workgroup i runs on XCD i % 8: the value heads of a key head on one
     const int nk = g.st.n_k_heads, nv = g.st.n_v_heads, dk = g.st.k_dim, rep = nv / nk;
     const int unit = blockIdx.x / (8 * rep) * 8 + blockIdx.x % 8;
@@ -298,7 +298,10 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 4 : 2) k_delta_prep(ChunkArgs g
     const int lane = tid & 63, n = lane & 15, q = lane >> 4;
     if (w == 0) {
         const float gl = lane < ch.n ? g.d.decay[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
-        bet[lane] = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
+        const float bl = lane < ch.n ? g.d.beta[(size_t)(ch.tok0 + lane) * nv + h] : 0.f;
+        bet[lane] = bl;
+        const float most = largest(fabsf(bl));
+        if (lane == 0) t_exp = exponent(most);
         double sum = (double)(gl < -150.f ? -150.f : gl) * 1.4426950408889634074;  // to base 2
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 4 : 2) k_delta_prep(ChunkArgs g
         for (int r = 0; r < 4; r++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(t[r], y[r], z, 0, 0, 0);
         T[i] = -z;
     }
-    const float scale = T_SCALE * bet[16 * w + n];
+    const float scale = pow2(T_EXP - t_exp) * bet[16 * w + n];
     const int em = exponent(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
     const float to_m = pow2(268 - em);
     const auto terms = [](float v) { return __builtin_bit_cast(uint32_t, h2{(_Float16)v, (_Float16)(v - (float)(_Float16)v)}); };
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(256, KS <= 4 ? 4 : 2) k_delta_prep(ChunkArgs g
         float *const v = (float *)(g.work + ((size_t)at * nv + h) * HQ_CHUNK_BYTES + FRAG_VEC * 1024);
         v[lane] = decay(gam[lane], f2{0.f, 0.f});
         v[64 + lane] = decay(gam[63], gam[lane]);
-        if (lane == 0) v[128] = g.d.scale * pow2(em - 14);
+        if (lane == 0) v[128] = g.d.scale * pow2(em - 14), ((int *)v)[129] = t_exp;
     }
 }
 
@@ -452,6 +455,7 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4v lds_s4v;
 typedef const __attribute__((address_space(3))) u4v lds_u4;
 typedef const __attribute__((address_space(3))) float lds_f;
+typedef const __attribute__((address_space(3))) int lds_i;
 typedef const __attribute__((address_space(3))) _Float16 lds_h;
 
 // Two fp16 terms of 8 values scaled by sc: accumulator blocks a and b as an operand. Scaling and conversion stay two instructions:
@@ -655,6 +659,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int s = 0; s < KS; s++) k_at[s] = base + k_in[s], t_at[s] = base + t_in[s];
         const auto rows4 = [&](int which, int b) { return __builtin_bit_cast(f4, read16(vec_at + 256u * (uint32_t)which + 4u * (uint32_t)token_of(b, 0))); };
         const float keep = *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 63u), m_unit = OUT ? *(lds_f *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 128u) : 0.f;
+        const int t_exp = *(lds_i *)(uintptr_t)(base + 1024u * AT_VEC + 4u * 129u);
         // Reads of LDS are issued a stage ahead of their use (STAGE: nothing moves past it), and what the outputs need is put between the
         // steps of the state.
         const auto read_rows = [&](int what, int s, h8(&x)[4]) {
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
 #pragma unroll
         for (int s = 0; s < 2; s++) Xh[s] = first_term(X[2 * s], X[2 * s + 1], pow2(268 - ex)), Xl[s] = second_term(X[2 * s], X[2 * s + 1], pow2(268 - ex), Xh[s]);
         f4 U[4];  // in units of 2^(uu - 127)
-        const int uu = ex - 14 - T_BITS;
+        const int uu = ex - 14 - (T_EXP - 127 - t_exp);
 #pragma unroll
         for (int b = 0; b < 4; b++) U[b] = f4{0.f, 0.f, 0.f, 0.f};
         if (OUT) MIX(8 * (KS - AHEAD), 2, 3);
