@@ -47,7 +47,7 @@ void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std
     std::vector<HqRun> all, parts;
     const auto chunks_of = [](int n) { return (n + HQ_CHUNK - 1) / HQ_CHUNK; };
     for (HqPass &p : *passes) {
-        int longest = 0;
+        int longest = 0, used = 2;  // (passes follow one another: their parts' places are the same, behind the 2 between passes)
         for (int i = 0; i < p.n_runs; i++) longest = std::max(longest, chunks_of((*runs)[p.run0 + i].n));
         const auto fits = [&](int part) {  // a workgroup a CU
             int64_t outputs = 0, effects = 0, rest = 0;  // (runs shorter than a part: one after another in its time)
@@ -76,8 +76,8 @@ void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std
                 continue;
             }
             const int each = (chunks + n - 1) / n, m = (chunks + each - 1) / each;  // (m: with parts of one length, as many as there are)
-            const int first = std::max(*places, 2), place = -2 - first;             // (2: those between passes)
-            *places = first + 2 * m - 2;
+            const int first = used, place = -2 - first;
+            used += 2 * m - 2, *places = std::max(*places, used);
             joins->push_back({r.from, first, m});
             for (int j = 0; j < m; j++) {
                 HqRun q = {r.tok0 + j * each * HQ_CHUNK, std::min(each * HQ_CHUNK, r.n - j * each * HQ_CHUNK), r.chunk0 + j * each, j ? place - j : r.from == -1 ? -1 : place,
