@@ -1014,20 +1014,23 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
         }
         SCK(hipGetLastError());
     }
-    if (c->n_steps == 0) return 0;
-    const DeltaArgs g = {*st, in, c->seqs, c->steps, scale_exp};
     // A head's waves in one workgroup; few heads with one token and no norm, for which they would have to meet, a wave each: 32 heads 5.0
     // us (in one workgroup 5.2), 128 6.5 (7.0), but of five tokens, whose keys each wave then fetches itself, 9.7 (9.4) and 13.1 (11.8).
-    const int waves = (st->v_dim + 31) / 32, heads = c->n_steps * st->n_v_heads;
-    const bool apart = !d->norm && c->longest_step <= 1 && heads * waves <= 2 * c->n_cu;
-    const dim3 grid((unsigned)heads, apart ? (unsigned)waves : 1u);
+    const int waves = (st->v_dim + 31) / 32;
+    const bool apart = !d->norm && c->longest_step <= 1 && (int64_t)c->n_steps * st->n_v_heads * waves <= 2 * c->n_cu;
     const unsigned threads = apart ? 64u : 64u * (unsigned)waves;
-    if (st->k_dim == 64) k_delta_step<8, true><<<grid, threads, 0, s>>>(g);
-    else if (st->k_dim < 64) k_delta_step<8, false><<<grid, threads, 0, s>>>(g);
-    else if (st->k_dim == 128) k_delta_step<16, true><<<grid, threads, 0, s>>>(g);
-    else if (st->k_dim < 128) k_delta_step<16, false><<<grid, threads, 0, s>>>(g);
-    else if (st->k_dim == 256) k_delta_step<32, true><<<grid, threads, 0, s>>>(g);
-    else k_delta_step<32, false><<<grid, threads, 0, s>>>(g);
-    SCK(hipGetLastError());
+    // (a launch has fewer than 2^32 threads)
+    const int most = std::max(1, (int)((((int64_t)1 << 32) - 1) / ((int64_t)st->n_v_heads * threads)));
+    for (int i = 0; i < c->n_steps; i += most) {
+        const DeltaArgs g = {*st, in, c->seqs, c->steps + i, scale_exp};
+        const dim3 grid((unsigned)std::min(most, c->n_steps - i) * (unsigned)st->n_v_heads, apart ? (unsigned)waves : 1u);
+        if (st->k_dim == 64) k_delta_step<8, true><<<grid, threads, 0, s>>>(g);
+        else if (st->k_dim < 64) k_delta_step<8, false><<<grid, threads, 0, s>>>(g);
+        else if (st->k_dim == 128) k_delta_step<16, true><<<grid, threads, 0, s>>>(g);
+        else if (st->k_dim < 128) k_delta_step<16, false><<<grid, threads, 0, s>>>(g);
+        else if (st->k_dim == 256) k_delta_step<32, true><<<grid, threads, 0, s>>>(g);
+        else k_delta_step<32, false><<<grid, threads, 0, s>>>(g);
+        SCK(hipGetLastError());
+    }
     return 0;
 }
