@@ -19,17 +19,22 @@ DEV float silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdg
 // x 2^e / sqrt(mean (x 2^e)^2 + eps) of a head's dv values, N of them in each of G neighbouring lanes (zeros behind dv). e is that of the
 // scale, which outputs ahead of their norm are formed without, as it goes up to 1e20 and the norm takes it out again. The squares of values that
 // are far from 1 leave fp32's range all the same: where their mean is not well inside it, of values over a power of two of the largest.
+// (eps 2^-2e comes from the host: formed here it cost k_delta_step registers, 64 single tokens 56.4 us in place of 54.8)
+struct Eps {
+    float eps, unit;  // unit: eps 2^-2e
+    int e;
+};
 template <int N, int G>
-DEV void normalise(float (&x)[N], int dv, float eps, int e) {
-    const auto mean = [&](int by) {
+DEV void normalise(float (&x)[N], int dv, const Eps &at) {
+    const auto mean = [&](float eps) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < N; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        return ss / (float)dv + ldexpf(eps, 2 * by);
+        return ss / (float)dv + eps;
     };
-    float ms = mean(-e);
+    float ms = mean(at.unit);
     if (!(ms > 1e-30f && ms < INFINITY)) {  // (all of a head's lanes, or none)
         uint32_t m = 0;
 #pragma unroll
@@ -39,7 +44,7 @@ DEV void normalise(float (&x)[N], int dv, float eps, int e) {
         const int to_1 = min(max(127 - (int)(m >> 23), -126), 126);
 #pragma unroll
         for (int i = 0; i < N; i++) x[i] = ldexpf(x[i], to_1);
-        ms = mean(to_1 - e);
+        ms = mean(ldexpf(at.eps, 2 * (to_1 - at.e)));
     }
     const float inv = 1.0f / sqrtf(ms);
 #pragma unroll
@@ -51,7 +56,7 @@ struct DeltaArgs {
     hq_delta_t d;
     const HqSeq *seqs;
     const int *steps;
-    int scale_exp;  // with a norm: of the scale, whose rest d.scale is
+    Eps eps;  // with a norm: e is the scale's exponent, whose rest d.scale is
 };
 
 // The sum of x over the lane groups of eight: all lanes have it. (Elements are bit-cast from plain scalars.)
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(512, ROWS <= 16 ? 4 : 2) k_delta_step(DeltaArg
             f4 at = {0.f, 0.f, 0.f, 0.f};
             if (d < dv) at = *(const f4 *)(o[t] + d);
             float y[4] = {at[0], at[1], at[2], at[3]};
-            normalise<4, 64>(y, dv, g.d.eps, g.scale_exp);
+            normalise<4, 64>(y, dv, g.eps);
             if (d >= dv) continue;
             const f4 zz = *(const f4 *)(z[t] + d), nw = *(const f4 *)(g.d.norm + d);
             h4 w;
@@ -243,7 +248,7 @@ struct ChunkArgs {
     char *work;
     float *places;  // states of the workspace
     float *outs;    // outputs ahead of their norm, 64 rows of v_dim for each chunk of the pass and value head
-    int scale_exp;  // with a norm: of the scale, whose rest d.scale is
+    Eps eps;        // as in DeltaArgs
     float one;  // 1: a factor that the compiler does not know, so that a difference is one fused instruction
 };
 
@@ -933,7 +938,7 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) z[e] = (float)a[e];
             }
-            normalise<8, G>(x, dv, g.d.eps, g.scale_exp);
+            normalise<8, G>(x, dv, g.eps);
             h8 y;
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = (_Float16)(x[e] * (e < 4 ? wa[e & 3] : wb[e & 3]) * silu(z[e]));
@@ -992,10 +997,10 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     if (cur != c->device) SCK(hipSetDevice(c->device));
     hipStream_t s = (hipStream_t)stream;
     hq_delta_t in = *d;
-    int scale_exp = 0;
-    if (in.norm) in.scale = frexpf(in.scale, &scale_exp);
+    Eps eps = {in.eps, in.eps, 0};
+    if (in.norm) in.scale = frexpf(in.scale, &eps.e), eps.unit = ldexpf(eps.eps, -2 * eps.e);
     for (const HqPass &p : c->passes) {
-        const ChunkArgs g = {*st, in, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), (float *)(c->work + c->outs_at), scale_exp, 1.0f};
+        const ChunkArgs g = {*st, in, c->chunks + p.chunk0, nullptr, 0, p.n_chunks, c->work, (float *)(c->work + c->places_at), (float *)(c->work + c->outs_at), eps, 1.0f};
         if (st->k_dim <= 64) launch_chunks<2>(g, p, c->runs, c->joins, s);
         else if (st->k_dim <= 128) launch_chunks<4>(g, p, c->runs, c->joins, s);
         else launch_chunks<8>(g, p, c->runs, c->joins, s);
@@ -1022,7 +1027,7 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
     // (a launch has fewer than 2^32 threads)
     const int most = std::max(1, (int)((((int64_t)1 << 32) - 1) / ((int64_t)st->n_v_heads * threads)));
     for (int i = 0; i < c->n_steps; i += most) {
-        const DeltaArgs g = {*st, in, c->seqs, c->steps + i, scale_exp};
+        const DeltaArgs g = {*st, in, c->seqs, c->steps + i, eps};
         const dim3 grid((unsigned)std::min(most, c->n_steps - i) * (unsigned)st->n_v_heads, apart ? (unsigned)waves : 1u);
         if (st->k_dim == 64) k_delta_step<8, true><<<grid, threads, 0, s>>>(g);
         else if (st->k_dim < 64) k_delta_step<8, false><<<grid, threads, 0, s>>>(g);
