@@ -660,6 +660,9 @@ void split_rows(LpArgs *g, int M, bool f32, int n_cu) {
     g->per = (pieces + (uint32_t)g->parts - 1) / (uint32_t)g->parts;
 }
 
+// Rows of a launch, which has fewer than 2^32 threads: half of what 512 a row leave. (Rows that are split are far fewer.)
+constexpr int LAUNCH_ROWS = 1 << 22;
+
 }  // namespace
 
 extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64_t stride, const uint32_t *ids, int n_ids, int top_k,
@@ -692,10 +695,19 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
         }
         g.work = (float *)work, g.counters = (int *)cnt;
     }
-    const unsigned grid = (unsigned)M * (unsigned)g.parts;
-    if (f32) k_logprobs<true><<<grid, NT, 0, (hipStream_t)stream>>>(g);
-    else k_logprobs<false><<<grid, NT, 0, (hipStream_t)stream>>>(g);
-    SCK(hipGetLastError());
+    for (int r = 0; r < M; r += LAUNCH_ROWS) {
+        const size_t at = (size_t)r;
+        LpArgs l = g;
+        l.x = (const char *)logits + at * (size_t)stride * (f32 ? 4 : 2);
+        if (logp) l.ids = ids + at * n_ids, l.logp = logp + at * n_ids;
+        if (entropy) l.entropy = entropy + at;
+        if (top_ids) l.top_ids = top_ids + at * top_k;
+        if (top_logp) l.top_logp = top_logp + at * top_k;
+        const unsigned grid = (unsigned)std::min(LAUNCH_ROWS, M - r) * (unsigned)g.parts;
+        if (f32) k_logprobs<true><<<grid, NT, 0, (hipStream_t)stream>>>(l);
+        else k_logprobs<false><<<grid, NT, 0, (hipStream_t)stream>>>(l);
+        SCK(hipGetLastError());
+    }
     return 0;
 }
 
@@ -714,16 +726,16 @@ extern "C" int hq_beam(const void *logits, int f32, int n_groups, int n_beams, u
     const int M = n_groups * n_beams;
     BeamArgs a = {};
     LpArgs &g = a.lp;
-    g.x = logits, g.stride = stride, g.V = V, g.k = (int)std::min((uint32_t)k, V), g.parts = g.group = 1;
+    g.stride = stride, g.V = V, g.k = (int)std::min((uint32_t)k, V), g.parts = g.group = 1;
     int device, n_cu;
     if (hq_internal_device(&device, &n_cu)) return -1;
     split_rows(&g, M, f32, n_cu);
-    a.score = score, a.done = done, a.done_token = done_token, a.n_beams = n_beams, a.k = k;
-    a.out_score = out_score, a.out_token = out_token, a.out_beam = out_beam;
-    // the rows' results, and behind them the sums of split rows; counters of rows and groups
+    a.done_token = done_token, a.n_beams = n_beams, a.k = k;
+    // the rows' results, and behind them the sums of split rows; counters of rows and groups (of a launch: they follow one another)
     a.row_bytes = 16u + 8u * (uint32_t)((g.k + 1) & ~1);
-    const size_t each = 4 + NT / (size_t)g.group, rows = (size_t)M * a.row_bytes, sums = g.parts > 1 ? (size_t)M * g.parts * each * 4 : 0;
-    const int n_count = M + n_groups;
+    const int groups = std::min(n_groups, LAUNCH_ROWS / n_beams), most = groups * n_beams;
+    const size_t each = 4 + NT / (size_t)g.group, rows = (size_t)most * a.row_bytes, sums = g.parts > 1 ? (size_t)most * g.parts * each * 4 : 0;
+    const int n_count = most + groups;
     void *work, *cnt;
     int grew;
     if (hq_internal_staging(device, stream, HQ_STAGE_BEAM, rows + sums, &work, &grew) ||
@@ -734,11 +746,17 @@ extern "C" int hq_beam(const void *logits, int f32, int n_groups, int n_beams, u
         SCK(hipGetLastError());
     }
     a.rows = (char *)work, g.work = (float *)((char *)work + rows);
-    a.group_counters = (int *)cnt, g.counters = (int *)cnt + n_groups;
-    const unsigned grid = (unsigned)M * (unsigned)g.parts;
+    a.group_counters = (int *)cnt, g.counters = (int *)cnt + groups;
     const size_t lds = std::max(sizeof(Shared), beam_lists(n_beams, k));
-    if (f32) k_beam<true><<<grid, NT, lds, (hipStream_t)stream>>>(a);
-    else k_beam<false><<<grid, NT, lds, (hipStream_t)stream>>>(a);
-    SCK(hipGetLastError());
+    for (int i = 0; i < n_groups; i += groups) {
+        const size_t r = (size_t)i * n_beams, o = (size_t)i * k;
+        g.x = (const char *)logits + r * (size_t)stride * (f32 ? 4 : 2);
+        a.score = score + r, a.done = done ? done + r : nullptr;
+        a.out_score = out_score + o, a.out_token = out_token + o, a.out_beam = out_beam + o;
+        const unsigned grid = (unsigned)(std::min(groups, n_groups - i) * n_beams) * (unsigned)g.parts;
+        if (f32) k_beam<true><<<grid, NT, lds, (hipStream_t)stream>>>(a);
+        else k_beam<false><<<grid, NT, lds, (hipStream_t)stream>>>(a);
+        SCK(hipGetLastError());
+    }
     return 0;
 }

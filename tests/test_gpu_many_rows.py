@@ -41,3 +41,65 @@ def test_delta_single_tokens_of_many_sequences(hqlib):
         # (sums of 16 products and three more operations in 32 bits, then fp16)
         assert (np.abs(y - kq[t] * u) <= (20 * 2.0 ** -24 * mag[t] + 2.0 ** -11 * abs(kq[t])) * np.abs(u) + 2.0 ** -25).all(), t
     scan.free()
+
+
+ROWS = (1 << 23) + 5  # of 512 threads: 2^32 and more
+
+
+def logits(V):
+    """Multiples of 1/8 in falling and rising order, unlike from row to row."""
+    r = np.arange(ROWS, dtype=np.int64)[:, None]
+    return (((r * 7 + np.arange(V) * 5 * (1 + r % 3)) % 64) / 8.0).astype(np.float32)
+
+
+def test_logprobs_of_many_rows(hqlib):
+    print(f"[gpu] logprobs of {ROWS} rows", flush=True)
+    V = 3
+    x = logits(V)
+    d = hqlib.DevBuf.from_array(x)
+    ids = hqlib.DevBuf.from_array((np.arange(ROWS) % V).astype(np.uint32))
+    out = [hqlib.DevBuf.from_array(np.full(ROWS + 1, 77, np.uint32)) for _ in range(4)]
+    hqlib.logprobs(d, ROWS, V, f32=True, ids=ids, n_ids=1, top_k=1, logp=out[0], entropy=out[1], top_ids=out[2], top_logp=out[3])
+    hqlib.synchronize()
+    got = [o.download(ROWS + 1, t) for o, t in zip(out, (np.float32, np.float32, np.uint32, np.float32))]
+    assert all(g.view(np.uint32)[-1] == 77 for g in got)
+    e = x.astype(np.float64) - x.max(-1, keepdims=True)
+    lp = e - np.log(np.exp(e).sum(-1, keepdims=True))
+    r = np.arange(ROWS)
+    # (three exponentials and a logarithm in 32 bits, of values up to 8 + log 3)
+    assert np.abs(got[0][:-1] - lp[r, r % V]).max() <= 2.0 ** -18 and np.abs(got[3][:-1] - lp.max(-1)).max() <= 2.0 ** -18
+    assert np.abs(got[1][:-1] + (np.exp(lp) * lp).sum(-1)).max() <= 2.0 ** -18
+    assert np.array_equal(got[2][:-1], x.argmax(-1))
+
+
+@pytest.mark.parametrize("beams", [1, 3])
+def test_beams_of_many_groups(hqlib, beams):
+    print(f"[gpu] beams of {ROWS} rows in groups of {beams}", flush=True)
+    V, k, G = 3, 2, ROWS // beams
+    x = logits(V)[:G * beams]
+    rng = np.random.default_rng(beams)
+    score = rng.integers(-40, 0, G * beams).astype(np.float32) / 16
+    done = (rng.random(G * beams) < 0.1).astype(np.uint8)
+    d = [hqlib.DevBuf.from_array(a) for a in (x, score, done)]
+    out = [hqlib.DevBuf.from_array(np.full(G * k + 1, 77, np.uint32)) for _ in range(3)]
+    hqlib.beam(d[0], G, beams, V, d[1], k, *out, f32=True, done=d[2], done_token=9)
+    hqlib.synchronize()
+    got = [o.download(G * k + 1, t) for o, t in zip(out, (np.float32, np.uint32, np.int32))]
+    assert all(g.view(np.uint32)[-1] == 77 for g in got)
+    e = x.astype(np.float64) - x.max(-1, keepdims=True)
+    val = score[:, None].astype(np.float64) + (e - np.log(np.exp(e).sum(-1, keepdims=True)))
+    tok = np.broadcast_to(np.arange(V), val.shape).copy()
+    val[done != 0, 1:], val[done != 0, 0], tok[done != 0] = -np.inf, score[done != 0], 9
+    val, tok = val.reshape(G, beams * V), tok.reshape(G, beams * V)
+    at = np.argsort(-val, axis=1, kind="stable")[:, :k + 1]
+    best = np.take_along_axis(val, at, 1)
+    score_got, token_got, beam_got = (g[:-1].reshape(G, k) for g in got)
+    some = np.isfinite(best[:, :k])
+    with np.errstate(invalid="ignore"):
+        assert (np.where(some, np.abs(score_got - best[:, :k]), 0) <= 2.0 ** -19).all() and (score_got[~some] == -np.inf).all()
+        # choices where no other value is near (values of unlike rows are off by 2^-20 each)
+        clear = some & (np.nan_to_num(best[:, :k] - best[:, 1:], posinf=1) > 2.0 ** -19)
+    clear = np.logical_and.accumulate(clear, 1)
+    assert clear.mean() > 0.5
+    assert (token_got == np.take_along_axis(tok, at, 1)[:, :k])[clear].all() and (beam_got == at[:, :k] // V)[clear].all()
+    assert (beam_got[~some] == -1).all() and (token_got[~some] == 0xffffffff).all()
