@@ -338,7 +338,7 @@ struct RopeArgs {
     hq_kv_t kv;
     hq_rope_t r;
     const int *tok_pos, *tok_slot;
-    int nh, n_tokens;
+    int nh, n_tokens, first;  // first: of the launch's tokens
     uint8_t axis[128];  // of each frequency
 };
 
@@ -364,7 +364,7 @@ DEV void store4(_Float16 *p, f4 x) { *(h4 *)p = h4{(_Float16)x[0], (_Float16)x[1
 // .. 58), the next head's values read ahead (50).
 template <bool F32, int G>
 __global__ void __launch_bounds__(256, 8) k_rope_append(RopeArgs g) {
-    const int t = blockIdx.x, hd = g.kv.head_dim, nkv = g.kv.n_kv_heads, half = g.r.rot_dim / 2;
+    const int t = g.first + (int)blockIdx.x, hd = g.kv.head_dim, nkv = g.kv.n_kv_heads, half = g.r.rot_dim / 2;
     const int u = threadIdx.x % G, first = threadIdx.x / G;
     const int d0 = 4 * u < half ? 4 * u : 2 * half + 8 * (u - half / 4), d1 = 4 * u < half ? half + 4 * u : d0 + 4;
     const bool on = 8 * u < hd, turn = 4 * u < half;
@@ -507,19 +507,21 @@ extern "C" int hq_rope_append(const hq_batch *b, const hq_kv_t *kv, const hq_rop
     const int lanes = kv->head_dim <= 64 ? 8 : kv->head_dim <= 128 ? 16 : 32, heads = b->n_heads + 2 * kv->n_kv_heads, per = 256 / lanes;
     // few tokens: their heads over several workgroups, while there are fewer than 8 per CU
     const int y = std::min((heads + per - 1) / per, std::max(8 * b->n_cu / b->n_tokens, 1));
-    const dim3 grid((unsigned)b->n_tokens, (unsigned)y);
     hipStream_t st = (hipStream_t)stream;
+    for (g.first = 0; g.first < b->n_tokens; g.first += 1 << 23) {  // (a launch has fewer than 2^32 threads)
+        const dim3 grid((unsigned)std::min(1 << 23, b->n_tokens - g.first), (unsigned)y);
 #define HQ_ROPE(F, G) k_rope_append<F, G><<<grid, 256, 0, st>>>(g)
-    if (r->f32) {
-        if (lanes == 8) HQ_ROPE(true, 8);
-        else if (lanes == 16) HQ_ROPE(true, 16);
-        else HQ_ROPE(true, 32);
-    } else {
-        if (lanes == 8) HQ_ROPE(false, 8);
-        else if (lanes == 16) HQ_ROPE(false, 16);
-        else HQ_ROPE(false, 32);
+        if (r->f32) {
+            if (lanes == 8) HQ_ROPE(true, 8);
+            else if (lanes == 16) HQ_ROPE(true, 16);
+            else HQ_ROPE(true, 32);
+        } else {
+            if (lanes == 8) HQ_ROPE(false, 8);
+            else if (lanes == 16) HQ_ROPE(false, 16);
+            else HQ_ROPE(false, 32);
+        }
+        SCK(hipGetLastError());
     }
 #undef HQ_ROPE
-    SCK(hipGetLastError());
     return 0;
 }

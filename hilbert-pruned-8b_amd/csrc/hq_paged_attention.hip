@@ -1188,9 +1188,13 @@ extern "C" int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_
     g.slack = kv->type == HQ_KV_Q8 ? SLACK : SLACK / g.sc;
     for (int body = 0; body < HQ_BODIES; body++) {
         if (!b->n_items[body]) continue;
-        g.items = b->items[body];
-        const int width = hq_attn_width(body, kv->head_dim);
-        SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, b->stream_rows, g, (unsigned)b->n_items[body], b->joins[body], (unsigned)b->n_joins[body], (hipStream_t)stream));
+        const int width = hq_attn_width(body, kv->head_dim), n = b->n_items[body];
+        constexpr int MOST = 1 << 22;  // items of a launch, which has fewer than 2^32 threads
+        for (int i = 0; i < n; i += MOST) {
+            g.items = b->items[body] + i;
+            const unsigned joins = n - i <= MOST ? (unsigned)b->n_joins[body] : 0u;
+            SCK((kv->type == HQ_KV_Q8 ? launch<true> : launch<false>)(body, width, b->stream_rows, g, (unsigned)std::min(MOST, n - i), b->joins[body], joins, (hipStream_t)stream));
+        }
     }
     return 0;
 }

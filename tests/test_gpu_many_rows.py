@@ -103,3 +103,49 @@ def test_beams_of_many_groups(hqlib, beams):
     assert clear.mean() > 0.5
     assert (token_got == np.take_along_axis(tok, at, 1)[:, :k])[clear].all() and (beam_got == at[:, :k] // V)[clear].all()
     assert (beam_got[~some] == -1).all() and (token_got[~some] == 0xffffffff).all()
+
+
+def test_append_of_many_tokens(hqlib):
+    """2^24 tokens of one sequence, not rotated: the cache's pages have the keys and values, the queries are as they were."""
+    n, d, page = 1 << 24, 16, 4096
+    print(f"[gpu] append of {n} tokens", flush=True)
+    rng = np.random.default_rng(2)
+    block = rng.normal(0, 1, (3, 1 << 13, d)).astype(np.float16)  # (the values repeat every 2^13 tokens)
+    q, k, v = (hqlib.DevBuf(n * d * 2) for _ in range(3))
+    for buf, b in zip((q, k, v), block):
+        fill(hqlib, buf, b)
+    q_out, ck, cv = (hqlib.DevBuf(n * d * 2) for _ in range(3))
+    for buf in (q_out, ck, cv):
+        fill(hqlib, buf, np.full(1 << 16, np.nan, np.float16))
+    kv = hqlib.KvCache(hqlib.KV_F16, n // page, page, 1, d, ck, cv, (page * d, d, d))
+    pages = rng.permutation(n // page).astype(np.uint32)
+    batch = hqlib.Batch(1, n, n // page)
+    batch.set(kv, 1, [n], [n], pages[None])
+    hqlib.rope_append(batch, kv, q, k, v, q_out, None, 0, 0, f32=False, q_stride=d, kv_stride=d)
+    hqlib.synchronize()
+    for p in (*range(0, n // page, 97), n // page // 2 - 1, n // page // 2, n // page - 1):
+        want = block[:, p * page % (1 << 13):][:, :page]
+        at = int(pages[p]) * page * d * 2
+        assert np.array_equal(q_out.download((page, d), np.float16, offset=p * page * d * 2), want[0]), p
+        assert np.array_equal(ck.download((page, d), np.float16, offset=at), want[1]) and np.array_equal(cv.download((page, d), np.float16, offset=at), want[2]), p
+    batch.free()
+
+
+def test_attention_of_many_sequences(hqlib):
+    """2^20 sequences of one token and 16 heads, which all read one page: each has the values of its one position."""
+    n, heads, d, page = 1 << 20, 16, 16, 16
+    print(f"[gpu] attention of {n} sequences", flush=True)
+    rng = np.random.default_rng(3)
+    c = rng.normal(0, 1, (2, page, heads, d)).astype(np.float16)
+    c[:, 1:] = np.nan
+    kv = hqlib.KvCache(hqlib.KV_F16, 1, page, heads, d, *(hqlib.DevBuf.from_array(a) for a in c), (page * heads * d, heads * d, d))
+    q, out = hqlib.DevBuf(n * heads * d * 2), hqlib.DevBuf(n * heads * d * 2)
+    fill(hqlib, q, rng.normal(0, 1, (1 << 10, heads, d)).astype(np.float16))
+    fill(hqlib, out, np.full(1 << 16, np.nan, np.float16))
+    batch = hqlib.Batch(n, n, 1)
+    batch.set(kv, heads, np.ones(n, np.int32), np.ones(n, np.int32), np.zeros((n, 1), np.uint32))
+    hqlib.attention(batch, kv, q, out, 0.25)
+    hqlib.synchronize()
+    y = out.download((n, heads, d), np.float16)
+    assert (y == c[1, 0]).all()
+    batch.free()
