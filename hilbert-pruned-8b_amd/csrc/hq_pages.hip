@@ -24,6 +24,7 @@ struct hq_pages {
     std::vector<uint32_t> free;  // a heap, the lowest page first
     std::vector<uint32_t> src, dst;  // waiting copies
     std::vector<int32_t> n;
+    std::vector<int> waits;      // the one into each page, or -1
     std::vector<uint32_t> out_src, out_dst;  // those handed to the caller
     std::vector<int32_t> out_n;
 
@@ -38,17 +39,20 @@ struct hq_pages {
         holders[p] = 1;
         return p;
     }
+    void push(uint32_t from, uint32_t to, int32_t m) {  // (there is room)
+        waits[to] = (int)dst.size();
+        src.push_back(from), dst.push_back(to), n.push_back(m);
+        readers[from]++;
+    }
     void drop(uint32_t p) {
         if (--holders[p]) return;
-        // a copy into a page that nobody holds any more is not wanted
-        for (size_t i = 0; i < dst.size(); i++)
-            if (dst[i] == p) {
-                const uint32_t s = src[i];
-                src[i] = src.back(), dst[i] = dst.back(), n[i] = n.back();
-                src.pop_back(), dst.pop_back(), n.pop_back();
-                if (--readers[s] == 0 && holders[s] == 0) put(s);
-                break;
-            }
+        if (const int i = waits[p]; i >= 0) {  // a copy into a page that nobody holds any more is not wanted
+            const uint32_t s = src[(size_t)i];
+            src[(size_t)i] = src.back(), dst[(size_t)i] = dst.back(), n[(size_t)i] = n.back();
+            waits[dst[(size_t)i]] = i, waits[p] = -1;
+            src.pop_back(), dst.pop_back(), n.pop_back();
+            if (--readers[s] == 0 && holders[s] == 0) put(s);
+        }
         if (readers[p] == 0) put(p);
     }
 };
@@ -78,6 +82,7 @@ extern "C" int hq_pages_create(uint32_t n_pages, int page_size, int max_seqs, hq
         p->seqs.resize((size_t)max_seqs);
         p->holders.assign(n_pages, 0);
         p->readers.assign(n_pages, 0);
+        p->waits.assign(n_pages, -1);
         p->free.resize(n_pages);
         for (uint32_t i = 0; i < n_pages; i++) p->free[i] = i;  // in order: a heap
     } catch (const std::exception &) {
@@ -105,7 +110,10 @@ extern "C" int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos) {
     if (want > p->free.size()) return hq_internal_fail("%s: sequence %d needs %zu pages more (%zu are free)", who, seq, want, p->free.size());
     try {
         s.pages.reserve(need);
-        p->src.reserve(p->src.size() + 1), p->dst.reserve(p->dst.size() + 1), p->n.reserve(p->n.size() + 1);
+        if (p->src.size() == std::min({p->src.capacity(), p->dst.capacity(), p->n.capacity()})) {  // (twice the room: not a new place for all of them at each call)
+            const size_t room = std::max<size_t>(16, 2 * p->src.size());
+            p->src.reserve(room), p->dst.reserve(room), p->n.reserve(room);
+        }
     } catch (const std::exception &) {
         return hq_internal_fail("%s: out of memory", who);
     }
@@ -118,10 +126,8 @@ extern "C" int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos) {
             // what the old page is itself still waiting for comes from there
             uint32_t from = old;
             int n = kept;
-            for (size_t j = 0; j < p->dst.size(); j++)
-                if (p->dst[j] == old) from = p->src[j], n = std::min(n, (int)p->n[j]);
-            p->src.push_back(from), p->dst.push_back(page), p->n.push_back(n);
-            p->readers[from]++;
+            if (const int j = p->waits[old]; j >= 0) from = p->src[(size_t)j], n = std::min(n, (int)p->n[(size_t)j]);
+            p->push(from, page, n);
         }
         p->drop(old);
     }
@@ -158,7 +164,6 @@ extern "C" int hq_pages_compact(hq_pages *p) {
     if (!p->dst.empty()) return hq_internal_fail("%s: %zu copies wait (hq_pages_copies)", who, p->dst.size());
     const uint32_t used = p->n_pages - (uint32_t)p->free.size();
     std::vector<uint32_t> to;
-    std::vector<uint8_t> seen;
     try {
         to.resize(p->n_pages);
         size_t moves = 0;
@@ -174,8 +179,7 @@ extern "C" int hq_pages_compact(hq_pages *p) {
         while (p->holders[hole]) hole++;  // (as many free pages lie below `used` as held ones above)
         to[i] = hole;
         p->holders[hole] = p->holders[i];
-        p->src.push_back(i), p->dst.push_back(hole), p->n.push_back(p->page_size);
-        p->readers[i]++;
+        p->push(i, hole, p->page_size);
     }
     for (uint32_t i : p->src) p->holders[i] = 0;
     for (hq_pages::Seq &s : p->seqs)
@@ -191,6 +195,7 @@ extern "C" int hq_pages_copies(hq_pages *p, const uint32_t **src, const uint32_t
     if (!p || !src || !dst || !n_pos || !n) return hq_internal_fail("%s: null argument", who);
     p->out_src.swap(p->src), p->out_dst.swap(p->dst), p->out_n.swap(p->n);
     p->src.clear(), p->dst.clear(), p->n.clear();
+    for (uint32_t d : p->out_dst) p->waits[d] = -1;
     for (uint32_t s : p->out_src)
         if (--p->readers[s] == 0 && p->holders[s] == 0) p->put(s);
     *src = p->out_src.data(), *dst = p->out_dst.data(), *n_pos = p->out_n.data(), *n = (int)p->out_src.size();
