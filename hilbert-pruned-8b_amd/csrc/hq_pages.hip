@@ -44,6 +44,13 @@ struct hq_pages {
         src.push_back(from), dst.push_back(to), n.push_back(m);
         readers[from]++;
     }
+    // The pages that go back to the pool with one of p's holders: itself, and one that only a copy into it still reads. (Of the pages of
+    // one sequence no two wait for one page's copy: each is another part of what they are copied from.)
+    size_t returns(uint32_t p) const {
+        if (holders[p] > 1) return 0;
+        const int i = waits[p];
+        return (readers[p] == 0) + (i >= 0 && readers[src[(size_t)i]] == 1 && holders[src[(size_t)i]] == 0);
+    }
     void drop(uint32_t p) {
         if (--holders[p]) return;
         if (const int i = waits[p]; i >= 0) {  // a copy into a page that nobody holds any more is not wanted
@@ -107,7 +114,13 @@ extern "C" int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos) {
     const size_t first = n_pos > n_keep ? (size_t)n_keep / ps : need, stay = std::min(have, need);
     size_t want = need > have ? need - have : 0;
     for (size_t i = first; i < stay; i++) want += p->holders[s.pages[i]] > 1;
-    if (want > p->free.size()) return hq_internal_fail("%s: sequence %d needs %zu pages more (%zu are free)", who, seq, want, p->free.size());
+    // too few in the pool: those that the sequence itself gives back come first
+    const bool give_first = want > p->free.size();
+    if (give_first) {
+        size_t given = 0;
+        for (size_t i = need; i < have; i++) given += p->returns(s.pages[i]);
+        if (want > p->free.size() + given) return hq_internal_fail("%s: sequence %d needs %zu pages more (%zu are free)", who, seq, want, p->free.size() + given);
+    }
     try {
         s.pages.reserve(need);
         if (p->src.size() == std::min({p->src.capacity(), p->dst.capacity(), p->n.capacity()})) {  // (twice the room: not a new place for all of them at each call)
@@ -117,6 +130,10 @@ extern "C" int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos) {
     } catch (const std::exception &) {
         return hq_internal_fail("%s: out of memory", who);
     }
+    const auto give = [&]() {
+        for (; s.pages.size() > need; s.pages.pop_back()) p->drop(s.pages.back());
+    };
+    if (give_first) give();
     for (size_t i = first; i < stay; i++) {
         const uint32_t old = s.pages[i];
         if (p->holders[old] == 1) continue;
@@ -131,10 +148,7 @@ extern "C" int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos) {
         }
         p->drop(old);
     }
-    while (s.pages.size() > need) {
-        p->drop(s.pages.back());
-        s.pages.pop_back();
-    }
+    give();
     while (s.pages.size() < need) s.pages.push_back(p->take());
     s.n_pos = n_pos;
     return 0;

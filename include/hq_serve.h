@@ -212,7 +212,7 @@ void hq_pages_free(hq_pages *p);
 /* Sequence seq has n_pos positions from now on, of which it keeps the first n_keep (at most n_pos and those it has): pages are
  * taken from the pool, the lowest first, or go back to it (0, 0: all of them). Where positions behind n_keep lie in a page that
  * others hold too, the sequence gets one of its own in its place, with a copy of what it keeps there (hq_pages_copies). Too few
- * pages in the pool: -1, and nothing is changed. */
+ * pages in the pool, with those that it gives back itself: -1, and nothing is changed. */
 int hq_pages_resize(hq_pages *p, int seq, int n_keep, int n_pos);
 /* child, which must have no positions, gets the first n_pos of parent's and shares their pages. */
 int hq_pages_fork(hq_pages *p, int parent, int child, int n_pos);
