@@ -400,21 +400,39 @@ __global__ void __launch_bounds__(256) k_delta_append(AppendArgs g) {
         if (t >= tile.n) break;
         fetch(t + AHEAD < HQ_CONV_TILE ? t + AHEAD : HQ_CONV_TILE);
         f8 y;
-        float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < TAPS; i++) s = fmaf(w[i][e], x[t + i][e], s);
             y[e] = silu(s);
-            ss = fmaf(y[e], y[e], ss);
         }
-        if (!on) ss = 0.f;
+        float inv = 1.0f;
         if (!is_v) {  // (not the same for all lanes of a wave, but for those that exchange)
+            const auto sum = [&]() {
+                float ss = 0.f;
 #pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+                for (int e = 0; e < 8; e++) ss = fmaf(y[e], y[e], ss);
+                if (!on) ss = 0.f;
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+                return ss;
+            };
+            float ss = sum() + g.r.eps;
+            if (!(ss > 1e-30f && ss < INFINITY)) {  // squares beyond fp32's range: of values over a power of two of the largest
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = max(m, __builtin_bit_cast(uint32_t, fabsf(y[e])));  // (magnitudes: their order as integers)
+                if (!on) m = 0;
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+                const int to_1 = min(max(127 - (int)(m >> 23), -126), 126);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = ldexpf(y[e], to_1);
+                ss = sum() + ldexpf(g.r.eps, 2 * to_1);
+            }
+            inv = 1.0f / sqrtf(ss);
         }
-        const float inv = is_v ? 1.0f : 1.0f / sqrtf(ss + g.r.eps);
         h8 o;
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] = (_Float16)(y[e] * inv);
