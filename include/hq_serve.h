@@ -237,8 +237,8 @@ int hq_kv_copy(const hq_kv_t *kv, int n_kv, const uint32_t *src, const uint32_t 
 /* The k best continuations of each of n_groups groups of n_beams beams. Row i * n_beams + j of the logits (fp16, or fp32 with f32;
  * V each, row m at logits + m * stride) and score[i * n_beams + j] belong to beam j of group i; its candidates are the tokens v
  * with the value score + log softmax(row)[v]. A beam with done != 0 (done may be NULL) has the one candidate done_token, with its
- * score as the value. To out_score, out_token and out_beam [n_groups, k], best first, equal values by the lower beam, then the
- * lower token; candidates of -inf (barred tokens, beams with a score of -inf) are none, and places beyond the last candidate get
+ * score as the value. To out_score, out_token and out_beam [n_groups, k], best first, equal values by the lower beam; of one
+ * beam's, whose values may be equal where its logits are not (next to a score of -1e30, say), the larger logit, then the lower token; candidates of -inf (barred tokens, beams with a score of -inf) are none, and places beyond the last candidate get
  * -inf, UINT32_MAX and -1. Rows of done beams and of those with a score of -inf are not read. A NaN or +inf in a group's scores or
  * in a row that is read: NaN, UINT32_MAX and -1 in all of the group's places. Values are formed and compared in 64 bits from 32-bit
  * exponentials. Its workspace belongs to (device, stream) as hq_logprobs' does. score and
