@@ -641,9 +641,12 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
     }
     constexpr uint32_t O_SIZE = OUT == TO_NORM ? 4 : 2;
     const uint32_t o_bytes = OUT == TO_NORM ? (uint32_t)dv * 4u : (uint32_t)g.d.out_stride * 2u;
-    uint32_t o_off[16], k_in[KS], t_in[KS];
+    // where a lane's outputs go (wider keys: but the first is formed anew for each chunk, since the kernel spills; 2048 tokens of 16 heads of 256
+    // 161 us in place of 165)
+    constexpr int PLACES = KS <= 4 ? 16 : 1;
+    uint32_t o_off[PLACES], k_in[KS], t_in[KS];
 #pragma unroll
-    for (int i = 0; i < 16; i++) o_off[i] = (uint32_t)token_of(i >> 2, 4 * q + (i & 3)) * o_bytes + O_SIZE * (uint32_t)col;
+    for (int i = 0; i < PLACES; i++) o_off[i] = (uint32_t)token_of(i >> 2, 4 * q + (i & 3)) * o_bytes + O_SIZE * (uint32_t)col;
     // what a lane reads of K and Q, of K transposed and of V, as offsets into a chunk's buffer
 #pragma unroll
     for (int s = 0; s < KS; s++) k_in[s] = 16u * (uint32_t)piece_at<CPR>(token_of(0, n), 4 * s + q), t_in[s] = 16u * (uint32_t)piece_at<CPR>(8 * q + (n >> 2), 4 * s + (n & 3));
@@ -815,14 +818,17 @@ __global__ void __launch_bounds__(64 * (W + 4), 1) k_delta_scan(ChunkArgs g) {
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dl[1], S[t]);
 #pragma unroll
         for (int t = 0; t < 2 * KS; t++) S[t] = mfma(column(1, t), Dh[1], S[t]);
+        uint32_t o_at = o_off[0];
+        asm("" : "+v"(o_at));  // (not held from chunk to chunk)
         if (OUT)
 #pragma unroll
             for (int b = 0; b < 4; b++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float o = fmaf(bu, y[b][r], O[b][r]);
-                    if (OUT == TO_NORM) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, o), ro, o_off[4 * b + r], 0u, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)o), ro, o_off[4 * b + r], 0u, 0);
+                    const uint32_t to = PLACES == 16 ? o_off[(4 * b + r) % PLACES] : o_at + (uint32_t)token_of(b, r) * o_bytes;
+                    if (OUT == TO_NORM) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, o), ro, to, 0u, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (_Float16)o), ro, to, 0u, 0);
                 }
         if (OUT) MIX(4 * KS, 2, 3);
         if ((c & 15) == 15) bound = column_max(S) * pow2(unit);
