@@ -454,23 +454,33 @@ struct Staging {  // slots: 0 x fp32, 1 x fp16, 2 y fp32 (hq_matmul_host), 3 emb
                   // 11 rows and 12 counters (kept zero) of hq_beam
     void *buf[13] = {};
     size_t cap[13] = {};
+    std::vector<void *> former;  // of slots that graphs may have been captured with (9 and up)
 };
 std::mutex g_staging_mu;
 std::map<std::pair<int, void *>, Staging> g_staging;
 std::map<int, int> g_n_cu;
 
-// The slot's buffer of at least `bytes` for (device, stream); *grew = 1 when it was (re)allocated.
-int staging(int device, void *stream, int slot, size_t bytes, void **p, int *grew = nullptr) {
+// The slot's buffer of at least `bytes` for (device, stream); *grew: its size when it was (re)allocated, else 0.
+int staging(int device, void *stream, int slot, size_t bytes, void **p, size_t *grew = nullptr) {
     std::lock_guard<std::mutex> lk(g_staging_mu);
     Staging &s = g_staging[std::make_pair(device, stream)];
     if (grew) *grew = 0;
     if (s.cap[slot] < bytes) {
-        if (s.buf[slot]) HIPCK(hipFree(s.buf[slot]));
+        if (slot >= HQ_STAGE_LOGPROBS) {
+            // a captured call goes on with the buffer it was captured with, until the stream goes; powers of two, so that those kept are
+            // less than the last
+            size_t all = 4096;
+            while (all < bytes) all *= 2;
+            bytes = all;
+            if (s.buf[slot]) s.former.push_back(s.buf[slot]);
+        } else if (s.buf[slot]) {
+            HIPCK(hipFree(s.buf[slot]));
+        }
         s.buf[slot] = nullptr;
         s.cap[slot] = 0;
         HIPCK(hipMalloc(&s.buf[slot], bytes));
         s.cap[slot] = bytes;
-        if (grew) *grew = 1;
+        if (grew) *grew = bytes;
     }
     *p = s.buf[slot];
     return 0;
@@ -488,6 +498,7 @@ void staging_release(void *stream) {
         if (hipGetDevice(&cur) == hipSuccess && cur != it->first.first) (void)hipSetDevice(it->first.first);
         for (void *b : it->second.buf)
             if (b) (void)hipFree(b);
+        for (void *b : it->second.former) (void)hipFree(b);
         if (cur >= 0 && cur != it->first.first) (void)hipSetDevice(cur);
         it = g_staging.erase(it);
     }
@@ -511,8 +522,12 @@ extern "C" int hq_internal_device(int *device, int *n_cu) {
     HIPCK(hipGetDevice(device));
     return device_cus(*device, n_cu);
 }
-extern "C" int hq_internal_staging(int device, void *stream, int slot, size_t bytes, void **p, int *grew) {
-    return staging(device, stream, slot, bytes, p, grew);
+extern "C" int hq_internal_staging(int device, void *stream, int slot, size_t bytes, void **p, size_t *grew) {
+    try {
+        return staging(device, stream, slot, bytes, p, grew);
+    } catch (const std::exception &) {
+        return fail("out of memory");
+    }
 }
 
 namespace {
@@ -525,7 +540,7 @@ int gemm_work(const hq_mat *W, int M, void *stream, HqGemmWork *wk, bool swiglu 
     hq_gemm_work_bytes(&W->m, M, n_cu, &pb, &cb, &sb);
     if (swiglu) sb = std::max(sb, hq_swiglu_sums_bytes(&W->m, M, n_cu));
     void *part, *cnt, *sums = nullptr;
-    int grew = 0;
+    size_t grew = 0;
     if (staging(W->device, stream, 5, pb, &part) || staging(W->device, stream, 6, cb, &cnt, &grew)) return -1;
     if (sb && staging(W->device, stream, 7, sb, &sums)) return -1;
     if (grew && cb) HIPCK(hipMemset(cnt, 0, cb));

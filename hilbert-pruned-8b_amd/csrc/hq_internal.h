@@ -26,11 +26,11 @@ int hq_internal_swiglu_small(int ggml_type, int M, uint32_t rows, uint32_t K, in
 /* Tokens of the backend's layer-loop pass, for activations of bytes_per_token. */
 int hq_internal_pass_tokens(size_t max_seq, size_t bytes_per_token, size_t free_bytes);
 
-/* The current device and its CUs; and a library buffer of at least `bytes` for (device, stream), grown on first need
- * (*grew = 1 then; contents are not kept), freed by hq_stream_destroy. */
+/* The current device and its CUs; and a library buffer of at least `bytes` for (device, stream), another one on first need
+ * (*grew its size then, else 0; contents are not kept), all of them freed by hq_stream_destroy. */
 enum { HQ_STAGE_LOGPROBS = 9, HQ_STAGE_LOGPROBS_COUNT = 10, HQ_STAGE_BEAM = 11, HQ_STAGE_BEAM_COUNT = 12 };
 int hq_internal_device(int *device, int *n_cu);
-int hq_internal_staging(int device, void *stream, int slot, size_t bytes, void **p, int *grew);
+int hq_internal_staging(int device, void *stream, int slot, size_t bytes, void **p, size_t *grew);
 
 /* The rows of n matrices of one type and width (Hugging Face order, one after the other) as one resident matrix. */
 int hq_internal_upload_cat(const hq_wmat_t *const *w, int n, int device, hq_mat **out);

@@ -685,12 +685,12 @@ extern "C" int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64
     if (g.parts > 1) {
         const size_t each = 4 + NT / (size_t)g.group, sums = (size_t)M * g.parts * each * 4;
         void *work, *cnt;
-        int grew;
+        size_t grew;
         if (hq_internal_staging(device, stream, HQ_STAGE_LOGPROBS, sums, &work, &grew) ||
             hq_internal_staging(device, stream, HQ_STAGE_LOGPROBS_COUNT, (size_t)M * 4, &cnt, &grew))
             return -1;
         if (grew) {
-            k_zero<<<1, 256, 0, (hipStream_t)stream>>>((int *)cnt, M);
+            k_zero<<<(unsigned)std::min<size_t>(grew / 1024, 1024), 256, 0, (hipStream_t)stream>>>((int *)cnt, (int)(grew / 4));
             SCK(hipGetLastError());
         }
         g.work = (float *)work, g.counters = (int *)cnt;
@@ -737,12 +737,12 @@ extern "C" int hq_beam(const void *logits, int f32, int n_groups, int n_beams, u
     const size_t each = 4 + NT / (size_t)g.group, rows = (size_t)most * a.row_bytes, sums = g.parts > 1 ? (size_t)most * g.parts * each * 4 : 0;
     const int n_count = most + groups;
     void *work, *cnt;
-    int grew;
+    size_t grew;
     if (hq_internal_staging(device, stream, HQ_STAGE_BEAM, rows + sums, &work, &grew) ||
         hq_internal_staging(device, stream, HQ_STAGE_BEAM_COUNT, (size_t)n_count * 4, &cnt, &grew))
         return -1;
     if (grew) {
-        k_zero<<<1, 256, 0, (hipStream_t)stream>>>((int *)cnt, n_count);
+        k_zero<<<(unsigned)std::min<size_t>(grew / 1024, 1024), 256, 0, (hipStream_t)stream>>>((int *)cnt, (int)(grew / 4));
         SCK(hipGetLastError());
     }
     a.rows = (char *)work, g.work = (float *)((char *)work + rows);

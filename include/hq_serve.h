@@ -123,7 +123,9 @@ int hq_attention(const hq_batch *b, const hq_kv_t *kv, const hq_attn_t *a, void 
  * token. logp, entropy, top_ids and top_logp may each be NULL (top_ids and top_logp as they are wanted). fp32 throughout.
  * A barred token has the logit -inf: log probability -inf, no part in the entropy. A row of nothing but -inf gives -inf
  * everywhere and entropy 0; a row with a NaN or +inf gives NaN everywhere (its top_ids put NaN first, then +inf).
- * Its workspace belongs to (device, stream), grows on first use of a larger shape, and goes with hq_stream_destroy. */
+ * Its workspace belongs to (device, stream), grows on first use of a larger shape, and goes with hq_stream_destroy; a captured call keeps the
+ * one that it was captured with until then (capture after an eager call of the shape on the stream; graphs captured on one stream run one at
+ * a time). */
 int hq_logprobs(const void *logits, int f32, int M, uint32_t V, int64_t stride, const uint32_t *ids, int n_ids, int top_k,
                 float *logp, float *entropy, uint32_t *top_ids, float *top_logp, void *stream);
 
