@@ -514,7 +514,8 @@ DEV float column_max(const f4 (&x)[N]) {
 // Bound: the way from one state to the next, some 750 instructions of one wave in order, which its SIMD has for itself: 4400 clocks a chunk
 // (32 heads of 128), the products in them 2100; the outputs' work fills what the state's leaves. Products are started as soon as half of
 // their operands are there (both halves first: 3.5 % more). W columns' waves read the same operands from LDS: 4 waves; with 2 (1), one
-// sequence of 2048 tokens took 76 (74) us in place of 79, ten prompts of 16384 473 (679) in place of 411; with 8 a chunk takes twice as long.
+// sequence of 2048 tokens takes 76 (75) us in place of 80 (in parts 71, for which narrower groups leave no CUs), ten prompts of 16384 354
+// (585) in place of 290; with 8 a chunk takes twice as long.
 // (wider keys' operands do not all fit the registers: they are read where they are used)
 #define STAGE if (KS <= 4) __builtin_amdgcn_sched_barrier(0)
 // N times a product and M other instructions (what: 2 arithmetic, 0x100 reads of LDS), in the order of issue

@@ -23,10 +23,10 @@ constexpr int HQ_CONV_TILE = 8;  // most tokens of a tile of hq_delta_append
 // hq_delta by chunks of 64 tokens. A chunk's operands that depend on its value head but not on the state are formed first, for many
 // chunks at a time (a pass), into HQ_CHUNK_BYTES of workspace each: 24 fragments and a vector of 1 KB (hq_delta.hip).
 // Most new tokens of a sequence that it takes token by token. Alone (32 heads of 128, us, by chunks behind the stroke): 16 sequences of 5
-// tokens, 21 / 38, of 12, 33 / 39, of 16, 39 / 40; 64 of 16, 117 / 139. Where all sequences' workgroups by chunks find a CU each, a
-// chain of tokens is the longer one sooner: one sequence of 8, 12.4 / 14.0, of 12, 17.2 / 14.0; 4 of 8, 14.9 / 16.5, of 12, 20.0 / 16.5; so there
-// all go by chunks as soon as one has more than 8. Beside sequences of more than 16 it is a launch more: a chunk of 2048 and 8 of 5 tokens, 96 / 92,
-// and 32 of 5, 123 / 112, and 32 of 16, 153 / 112; but 64 of 5, 150 / 173, and 64 of one, 139 / 173; so there those of more than 4 tokens go by
+// tokens, 21 / 39, of 12, 34 / 39, of 16, 39 / 39; 64 of 16, 117 / 139. Where all sequences' workgroups by chunks find a CU each, a
+// chain of tokens is the longer one sooner: one sequence of 8, 12.4 / 13.8, of 12, 17.2 / 14.0; 4 of 8, 15.1 / 16.5, of 12, 20.2 / 16.5; so there
+// all go by chunks as soon as one has more than 8. Beside sequences of more than 16 it is a launch more: a chunk of 2048 and 8 of 5 tokens, 87 / 85,
+// and 32 of 5, 107 / 100, and 32 of 16, 141 / 102; but 64 of 5, 138 / 162, and 64 of one, 128 / 160; so there those of more than 4 tokens go by
 // chunks where they have four heads a CU at most.
 constexpr int HQ_STEP_TOKENS = 16, HQ_STEP_ALONE = 8, HQ_STEP_BESIDE = 4;
 constexpr int HQ_CHUNK = 64;

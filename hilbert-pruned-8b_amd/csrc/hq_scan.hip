@@ -37,9 +37,9 @@ int check_geometry(const char *who, const hq_state_t *st) {
 // Few long runs leave most of the chip idle, each a chain of chunks. Cut into parts that fill it, a workgroup a CU, first every part's
 // effect on a state is formed (P and Q, all parts side by side, without outputs), then the states between them, then the outputs of all
 // parts side by side: two chains of a part's length and a product a part instead of one. It costs two launches, the states' way through
-// memory and the products, some 17 us, as much as 8 or 9 chunks: one sequence of 1000 tokens, 32 heads of 128, 47 us with it or without,
-// 2048: 82 without, 77 with, 6001: 215 and 173, 16000: 555 and 428. (Two workgroups a CU and so shorter parts: 90, 190, 467. With what
-// followed, in parts: 2048 74, 6001 171, 16000 432.)
+// memory and the products. One sequence, 32 heads of 128, us, in one chain / in parts: 1000 tokens 46.5 / 48.5, 1300 57.5 / 54, 2048 80 / 71, 4096
+// 153 / 118, 6001 219 / 161, 16000 562 / 395; 2048 of 8 heads of 128 74 / 54, of 32 heads of 64 67 / 46. JOIN_CHUNKS chunks are more than it
+// costs here (some 6), on the side of the one chain.
 constexpr int JOIN_CHUNKS = 9, LEAST_PART = 4;
 void split_runs(const hq_state_t *st, int n_cu, std::vector<HqPass> *passes, std::vector<HqRun> *runs, std::vector<HqJoin> *joins, int *places) {
     const int cols = hq_scan_columns(st->k_dim);
