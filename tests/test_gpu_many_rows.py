@@ -149,3 +149,30 @@ def test_attention_of_many_sequences(hqlib):
     y = out.download((n, heads, d), np.float16)
     assert (y == c[1, 0]).all()
     batch.free()
+
+
+@pytest.mark.parametrize("f32", [True, False])
+def test_longest_rows(hqlib, f32):
+    """One row of 2^30 logits, the likeliest at its ends and on both sides of 4 GB: hq_beam's values to 2^-20, hq_logprobs' to what sums of 2^16
+    terms in 32 bits each lose (2^-24 a sum, at most 2^16 of them in a row: 2^-8)."""
+    V, t = 1 << 30, np.float32 if f32 else np.float16
+    print(f"[gpu] rows of {V}, f32={f32}", flush=True)
+    block = (np.random.default_rng(4).integers(-64, 0, 1 << 20) / 16.0).astype(t)
+    row = hqlib.DevBuf(V * block.itemsize)
+    fill(hqlib, row, block)
+    top = {V - 1: 5.0, 0: 4.0, V // 2: 3.0, V // 2 - 1: 3.0, (1 << 29) + 12345: 2.0, V - 2: 1.5, 777: 1.0, V - 100000: 0.5}
+    total = np.exp(block.astype(np.float64)).sum() * (V / len(block))
+    for i, x in top.items():
+        row.upload(np.array([x], t), offset=i * block.itemsize)
+        total += np.exp(x) - np.exp(float(block[i % len(block)]))
+    order = sorted(top, key=lambda i: (-top[i], i))
+    k = len(order)
+    want = np.array([top[i] for i in order]) - np.log(total)
+    score = hqlib.DevBuf.from_array(np.array([-0.5], np.float32))
+    out = [hqlib.DevBuf(k * 4) for _ in range(5)]
+    hqlib.beam(row, 1, 1, V, score, k, *out[:3], f32=f32)
+    hqlib.logprobs(row, 1, V, f32=f32, top_k=k, top_ids=out[3], top_logp=out[4])
+    hqlib.synchronize()
+    assert out[1].download(k, np.uint32).tolist() == order and out[3].download(k, np.uint32).tolist() == order
+    assert np.abs(out[0].download(k, np.float32) - (want - 0.5)).max() <= 2.0 ** -19 + 2.0 ** -24 * 32
+    assert np.abs(out[4].download(k, np.float32) - want).max() <= 2.0 ** -8
