@@ -918,7 +918,9 @@ __global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *j
 }
 
 // The norm and gate of chunks' outputs, from the workspace to where they belong: G lanes a head, eight columns a lane.
-// Bound: bytes. 16384 tokens of 32 heads of 128, gates in fp32: 671 MB in 134 us, 5.0 TB/s (from fp16 outputs 537 MB in 101).
+// Bound: bytes. 16384 tokens of 32 heads of 128, gates in fp32: 671 MB in 127 us, 5.3 TB/s (from fp16 outputs 537 MB in 101), a
+// workgroup a token of a chunk, gates past the caches that hold the outputs (four tokens and without that: 134; 800 tokens of 16 heads of 256 72 us in
+// all in place of 79).
 template <int G, bool F32>
 __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
     const int nv = g.st.n_v_heads, dv = g.st.v_dim, u = threadIdx.x % G;
@@ -928,7 +930,7 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
     if (on) wa = *(const f4 *)(g.d.norm + 8 * u), wb = *(const f4 *)(g.d.norm + 8 * u + 4);
     for (int h = threadIdx.x / G; h < nv; h += 256 / G) {
         const size_t in = (size_t)h * dv + (on ? 8 * u : 0);
-        for (int t = blockIdx.y; t < ch.n; t += gridDim.y) {
+        if (const int t = blockIdx.y; t < ch.n) {
             const size_t tok = (size_t)(ch.tok0 + t), zat = tok * g.d.gate_stride + in;
             const float *const from = g.outs + (((size_t)blockIdx.x * nv + h) * HQ_CHUNK + t) * dv + (on ? 8 * u : 0);
             float x[8];
@@ -937,7 +939,7 @@ __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
             for (int e = 0; e < 4; e++) x[e] = on ? xa[e] : 0.f, x[4 + e] = on ? xb[e] : 0.f;
             float z[8];
             if (F32) {
-                const f4 a = *(const f4 *)((const float *)g.d.gate + zat), b = *(const f4 *)((const float *)g.d.gate + zat + 4);
+                const f4 a = __builtin_nontemporal_load((const f4 *)((const float *)g.d.gate + zat)), b = __builtin_nontemporal_load((const f4 *)((const float *)g.d.gate + zat + 4));
 #pragma unroll
                 for (int e = 0; e < 4; e++) z[e] = a[e], z[4 + e] = b[e];
             } else {
@@ -1013,7 +1015,7 @@ extern "C" int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t
         else launch_chunks<8>(g, p, c->runs, c->joins, s);
         if (d->norm) {
             const int lanes = st->v_dim <= 64 ? 8 : st->v_dim <= 128 ? 16 : 32;
-            const dim3 grid((unsigned)p.n_chunks, 16);
+            const dim3 grid((unsigned)p.n_chunks, HQ_CHUNK);
 #define HQ_NORM(G)                                                          \
     do {                                                                    \
         if (d->gate_f32) k_delta_norm<G, true><<<grid, 256, 0, s>>>(g);     \
