@@ -919,40 +919,40 @@ __global__ void __launch_bounds__(512) k_delta_join(ChunkArgs g, const HqJoin *j
 
 // The norm and gate of chunks' outputs, from the workspace to where they belong: G lanes a head, eight columns a lane.
 // Bound: bytes. 16384 tokens of 32 heads of 128, gates in fp32: 671 MB in 127 us, 5.3 TB/s (from fp16 outputs 537 MB in 101), a
-// workgroup a token of a chunk, gates past the caches that hold the outputs (four tokens and without that: 134; 800 tokens of 16 heads of 256 72 us in
+// workgroup a token of a chunk, gates past the caches that hold the outputs (four tokens and without that: 134; 1100 tokens of 16 heads of 256 72 us in
 // all in place of 79).
 template <int G, bool F32>
 __global__ void __launch_bounds__(256) k_delta_norm(ChunkArgs g) {
     const int nv = g.st.n_v_heads, dv = g.st.v_dim, u = threadIdx.x % G;
     const bool on = 8 * u < dv;
     const HqChunk ch = g.chunks[blockIdx.x];
+    const int t = blockIdx.y;
+    if (t >= ch.n) return;
     f4 wa = {0.f, 0.f, 0.f, 0.f}, wb = wa;
     if (on) wa = *(const f4 *)(g.d.norm + 8 * u), wb = *(const f4 *)(g.d.norm + 8 * u + 4);
     for (int h = threadIdx.x / G; h < nv; h += 256 / G) {
         const size_t in = (size_t)h * dv + (on ? 8 * u : 0);
-        if (const int t = blockIdx.y; t < ch.n) {
-            const size_t tok = (size_t)(ch.tok0 + t), zat = tok * g.d.gate_stride + in;
-            const float *const from = g.outs + (((size_t)blockIdx.x * nv + h) * HQ_CHUNK + t) * dv + (on ? 8 * u : 0);
-            float x[8];
-            const f4 xa = *(const f4 *)from, xb = *(const f4 *)(from + 4);
+        const size_t tok = (size_t)(ch.tok0 + t), zat = tok * g.d.gate_stride + in;
+        const float *const from = g.outs + (((size_t)blockIdx.x * nv + h) * HQ_CHUNK + t) * dv + (on ? 8 * u : 0);
+        float x[8];
+        const f4 xa = *(const f4 *)from, xb = *(const f4 *)(from + 4);
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = on ? xa[e] : 0.f, x[4 + e] = on ? xb[e] : 0.f;
-            float z[8];
-            if (F32) {
-                const f4 a = __builtin_nontemporal_load((const f4 *)((const float *)g.d.gate + zat)), b = __builtin_nontemporal_load((const f4 *)((const float *)g.d.gate + zat + 4));
+        for (int e = 0; e < 4; e++) x[e] = on ? xa[e] : 0.f, x[4 + e] = on ? xb[e] : 0.f;
+        float z[8];
+        if (F32) {
+            const f4 a = __builtin_nontemporal_load((const f4 *)((const float *)g.d.gate + zat)), b = __builtin_nontemporal_load((const f4 *)((const float *)g.d.gate + zat + 4));
 #pragma unroll
-                for (int e = 0; e < 4; e++) z[e] = a[e], z[4 + e] = b[e];
-            } else {
-                const h8 a = *(const h8 *)((const _Float16 *)g.d.gate + zat);
+            for (int e = 0; e < 4; e++) z[e] = a[e], z[4 + e] = b[e];
+        } else {
+            const h8 a = *(const h8 *)((const _Float16 *)g.d.gate + zat);
 #pragma unroll
-                for (int e = 0; e < 8; e++) z[e] = (float)a[e];
-            }
-            normalise<8, G>(x, dv, g.eps);
-            h8 y;
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = (_Float16)(x[e] * (e < 4 ? wa[e & 3] : wb[e & 3]) * silu(z[e]));
-            if (on) *(h8 *)((_Float16 *)g.d.out + tok * g.d.out_stride + in) = y;
+            for (int e = 0; e < 8; e++) z[e] = (float)a[e];
         }
+        normalise<8, G>(x, dv, g.eps);
+        h8 y;
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = (_Float16)(x[e] * (e < 4 ? wa[e & 3] : wb[e & 3]) * silu(z[e]));
+        if (on) *(h8 *)((_Float16 *)g.d.out + tok * g.d.out_stride + in) = y;
     }
 }
 
