@@ -200,7 +200,7 @@ typedef struct {
  * o = scale S^T q. States to their slots. Keys are to have a norm of at most 1 and beta to lie in 0 .. 1 (as hq_delta_append gives
  * them): the recurrence itself grows without bound otherwise. States and sums are fp32; sequences of more than 16 new tokens (fewer,
  * where it is the faster way) are taken in chunks of 64 tokens from their first, as products on the matrix cores whose operands are two
- * fp16 terms each (2^-22 of a column's largest). Outputs are rounded once, behind the norm. A value that is
+ * fp16 terms each (2^-22 of a column's largest, of a chunk's strengths of the chunk's largest). Outputs are rounded once, behind the norm. A value that is
  * not a number stays in its value column (and head, with the norm), but there it may reach outputs of its chunk's earlier tokens. The
  * same step gives the same bits. out must not overlap what is read. Kernels in a row, no allocation. */
 int hq_delta(const hq_scan *c, const hq_state_t *st, const hq_delta_t *d, void *stream);
